@@ -24,7 +24,8 @@ OBJ = HERE / "_build"
 SOURCES = ["prepare.hip", "plain.hip", "attention.hip", "attention_hm.hip", "attention_split.hip",
            "noalloc.hip", "gemm.hip",
            "abi.cpp", "stack.cpp",
-           "tables.cpp", "vsa.hip", "vsa_host.cpp", "fp6.hip"]
+           "tables.cpp", "vsa.hip", "vsa_host.cpp", "fp6.hip",
+           "kv4.hip", "attention_kv4.hip"]
 ARCH = "gfx950"
 
 

@@ -5,6 +5,7 @@
 // kernel's config.decl ranges bound its specialisation (kernels/*.loom). A failing check
 // returns its status, records a message for h3_last_error(), and launches nothing.
 #include <algorithm>
+#include <cmath>
 #include <cstdarg>
 #include <initializer_list>
 #include <cstdio>
@@ -340,6 +341,86 @@ int attention_common(const char* stage, const h3_attention_cfg* cfg, uint32_t to
                                           static_cast<const uint16_t*>(vt.ptr),
                                           static_cast<uint16_t*>(out.ptr), workspace.ptr,
                                           stream));
+}
+
+// The cache's ranges (h3attn.h); no reference counterpart.
+int check_kv4_cfg(const char* stage, const h3_kv4_cfg* cfg) {
+  if (!cfg) return set_error(H3_ERR_ARGUMENT, "%s: null config", stage);
+  if (!in_range(cfg->kv_heads, 1, 256))
+    return set_error(H3_ERR_CONFIG, "%s: kv_heads %u outside [1, 256]", stage, cfg->kv_heads);
+  if (cfg->head_dim != 64 && cfg->head_dim != 128)
+    return set_error(H3_ERR_CONFIG, "%s: head_dim %u is neither 64 nor 128", stage, cfg->head_dim);
+  if (!in_range(cfg->page_tokens, 16, 1024) || (cfg->page_tokens & (cfg->page_tokens - 1)) != 0)
+    return set_error(H3_ERR_CONFIG, "%s: page_tokens %u is no power of two in [16, 1024]", stage,
+                     cfg->page_tokens);
+  if (cfg->pages < 1 || (uint64_t)cfg->pages * cfg->page_tokens > 0x7fffffffull)
+    return set_error(H3_ERR_CONFIG, "%s: %u pages of %u tokens outside [1, 2^31 - 1] tokens", stage,
+                     cfg->pages, cfg->page_tokens);
+  if (cfg->elem != H3_ELEM_F16 && cfg->elem != H3_ELEM_BF16)
+    return set_error(H3_ERR_CONFIG, "%s: unknown element format %u", stage, cfg->elem);
+  return H3_OK;
+}
+
+size_t kv4_cache_bytes(const h3_kv4_cfg& cfg) {
+  return (size_t)cfg.pages * cfg.kv_heads * cfg.page_tokens * (cfg.head_dim + 8);
+}
+
+// Rows of K and V (bindings k, v) and their slots: the checks h3_kv4_write and _read share.
+int check_kv4_rows(const char* stage, const h3_kv4_cfg* cfg, uint32_t tokens, uint32_t k_stride,
+                   uint32_t v_stride) {
+  int st = check_kv4_cfg(stage, cfg);
+  if (st) return st;
+  if (!in_range(tokens, 1, 16777216))
+    return set_error(H3_ERR_ARGUMENT, "%s: tokens %u outside [1, 16777216]", stage, tokens);
+  const uint32_t width = cfg->kv_heads * cfg->head_dim;
+  if (!in_range(k_stride, width, 1048576, 8) || !in_range(v_stride, width, 1048576, 8))
+    return set_error(H3_ERR_ARGUMENT, "%s: strides %u and %u outside [%u, 1048576] step 8", stage,
+                     k_stride, v_stride, width);
+  return H3_OK;
+}
+
+// Binding i is aligned to align[i] bytes (rows move 16 bytes at a time).
+int check_alignments(const char* stage, const h3_view* views, std::initializer_list<uint32_t> align) {
+  int i = 0;
+  for (const uint32_t bytes : align) {
+    if (reinterpret_cast<uintptr_t>(views[i].ptr) % bytes != 0)
+      return set_error(H3_ERR_ARGUMENT, "%s: binding %d is not %u-byte aligned", stage, i, bytes);
+    ++i;
+  }
+  return H3_OK;
+}
+
+// The last row ends with its heads' channels.
+size_t kv4_rows_bytes(uint32_t rows, uint32_t stride, uint32_t width) {
+  return ((size_t)(rows - 1) * stride + width) * 2;
+}
+
+int check_kv4_attention(const char* stage, const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* acfg,
+                        uint32_t batch, uint32_t q_rows, uint32_t max_q) {
+  int st = check_kv4_cfg(stage, cfg);
+  if (st) return st;
+  if (!acfg) return set_error(H3_ERR_ARGUMENT, "%s: null attention config", stage);
+  if (!in_range(acfg->heads, 1, 4096, cfg->kv_heads))
+    return set_error(H3_ERR_CONFIG, "%s: heads %u outside [1, 4096] or no multiple of kv_heads %u",
+                     stage, acfg->heads, cfg->kv_heads);
+  const uint32_t width = acfg->heads * cfg->head_dim;
+  if (!in_range(acfg->q_stride, width, 1048576, 8) || !in_range(acfg->out_stride, width, 1048576, 8))
+    return set_error(H3_ERR_CONFIG, "%s: q_stride %u, out_stride %u outside [%u, 1048576] step 8",
+                     stage, acfg->q_stride, acfg->out_stride, width);
+  if (acfg->table_stride < 1 || (uint64_t)acfg->table_stride * cfg->page_tokens > 16777216)
+    return set_error(H3_ERR_CONFIG, "%s: table_stride %u of %u-token pages outside [1, 2^24] tokens",
+                     stage, acfg->table_stride, cfg->page_tokens);
+  if (acfg->causal > 1 || (acfg->window && !acfg->causal) || acfg->window > 0x7fffffffu)
+    return set_error(H3_ERR_CONFIG, "%s: causal %u with window %u", stage, acfg->causal,
+                     acfg->window);
+  if (!std::isfinite(acfg->scale))
+    return set_error(H3_ERR_CONFIG, "%s: scale is not finite", stage);
+  if (!in_range(batch, 1, 65535))
+    return set_error(H3_ERR_ARGUMENT, "%s: batch %u outside [1, 65535]", stage, batch);
+  if (!in_range(q_rows, 1, 16777216) || !in_range(max_q, 1, q_rows))
+    return set_error(H3_ERR_ARGUMENT, "%s: q_rows %u outside [1, 2^24] or max_q %u outside [1, q_rows]",
+                     stage, q_rows, max_q);
+  return H3_OK;
 }
 
 // kernels/vsa_ops.loom:3-9 (h3.vsa.*), plus the relations src/vsa/device.rs:63-77 builds the
@@ -1022,6 +1103,80 @@ int h3_attention_i8qkhm_cross(const h3_cross_cfg* cfg, h3_view qi, h3_view qs, h
                                                 static_cast<const uint8_t*>(key_mask.ptr),
                                                 static_cast<uint16_t*>(out.ptr),
                                                 reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t h3_kv4_cache_bytes(const h3_kv4_cfg* cfg) {
+  return check_kv4_cfg("kv4_cache_bytes", cfg) ? 0 : (ok(), kv4_cache_bytes(*cfg));
+}
+
+int h3_kv4_write(const h3_kv4_cfg* cfg, uint32_t tokens, uint32_t k_stride, uint32_t v_stride,
+                 h3_view k, h3_view v, h3_view slots, h3_view cache, h3_stream stream) {
+  const char* stage = "kv4_write";
+  int st = check_kv4_rows(stage, cfg, tokens, k_stride, v_stride);
+  if (st) return st;
+  const uint32_t width = cfg->kv_heads * cfg->head_dim;
+  h3_view views[4] = {k, v, slots, cache};
+  size_t need[4] = {kv4_rows_bytes(tokens, k_stride, width), kv4_rows_bytes(tokens, v_stride, width),
+                    (size_t)tokens * 4, kv4_cache_bytes(*cfg)};
+  if ((st = check_bindings(stage, views, need, 4))) return st;
+  if ((st = check_alignments(stage, views, {16, 16, 4, 16}))) return st;
+  if ((st = device_ready(stage))) return st;
+  return launched(stage, launch_kv4_write(*cfg, tokens, k_stride, v_stride, k.ptr, v.ptr,
+                                          static_cast<const int32_t*>(slots.ptr), cache.ptr,
+                                          reinterpret_cast<hipStream_t>(stream)));
+}
+
+int h3_kv4_read(const h3_kv4_cfg* cfg, uint32_t tokens, uint32_t k_stride, uint32_t v_stride,
+                h3_view slots, h3_view cache, h3_view k, h3_view v, h3_stream stream) {
+  const char* stage = "kv4_read";
+  int st = check_kv4_rows(stage, cfg, tokens, k_stride, v_stride);
+  if (st) return st;
+  const uint32_t width = cfg->kv_heads * cfg->head_dim;
+  h3_view views[4] = {slots, cache, k, v};
+  size_t need[4] = {(size_t)tokens * 4, kv4_cache_bytes(*cfg),
+                    kv4_rows_bytes(tokens, k_stride, width), kv4_rows_bytes(tokens, v_stride, width)};
+  if ((st = check_bindings(stage, views, need, 4))) return st;
+  if ((st = check_alignments(stage, views, {4, 16, 16, 16}))) return st;
+  if ((st = device_ready(stage))) return st;
+  return launched(stage, launch_kv4_read(*cfg, tokens, k_stride, v_stride,
+                                         static_cast<const int32_t*>(slots.ptr), cache.ptr, k.ptr,
+                                         v.ptr, reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t h3_kv4_workspace_bytes(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attention,
+                              uint32_t batch, uint32_t q_rows, uint32_t max_q) {
+  if (check_kv4_attention("kv4_workspace_bytes", cfg, attention, batch, q_rows, max_q)) return 0;
+  ok();
+  return kv4_workspace_bytes(*cfg, *attention, q_rows,
+                             kv4_plan(*cfg, *attention, batch, max_q, device_cus()));
+}
+
+int h3_attention_kv4(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attention, uint32_t batch,
+                     uint32_t q_rows, uint32_t max_q, h3_view q, h3_view cache, h3_view table,
+                     h3_view lengths, h3_view q_starts, h3_view out, h3_view lse, h3_view workspace,
+                     h3_stream stream) {
+  const char* stage = "attention_kv4";
+  int st = check_kv4_attention(stage, cfg, attention, batch, q_rows, max_q);
+  if (st) return st;
+  const uint32_t width = attention->heads * cfg->head_dim;
+  const size_t ws = workspace.ptr
+                        ? kv4_workspace_bytes(*cfg, *attention, q_rows,
+                                              kv4_plan(*cfg, *attention, batch, max_q, device_cus()))
+                        : 0;
+  h3_view views[8] = {q, cache, table, lengths, q_starts, out, lse, workspace};
+  size_t need[8] = {kv4_rows_bytes(q_rows, attention->q_stride, width), kv4_cache_bytes(*cfg),
+                    (size_t)batch * attention->table_stride * 4, (size_t)batch * 4,
+                    ((size_t)batch + 1) * 4, kv4_rows_bytes(q_rows, attention->out_stride, width),
+                    lse.ptr ? (size_t)q_rows * attention->heads * 4 : 0, ws};
+  if ((st = check_bindings(stage, views, need, 8))) return st;
+  if ((st = check_alignments(stage, views, {16, 16, 4, 4, 4, 16, 4, 16}))) return st;
+  if ((st = device_ready(stage))) return st;
+  return launched(stage, launch_attention_kv4(*cfg, *attention, batch, q_rows, max_q, q.ptr,
+                                              cache.ptr, static_cast<const int32_t*>(table.ptr),
+                                              static_cast<const int32_t*>(lengths.ptr),
+                                              static_cast<const int32_t*>(q_starts.ptr), out.ptr,
+                                              static_cast<float*>(lse.ptr), workspace.ptr,
+                                              reinterpret_cast<hipStream_t>(stream)));
 }
 
 int h3_vsa_attention_i8(const h3_attention_cfg* cfg, uint32_t token_count, uint32_t heads,

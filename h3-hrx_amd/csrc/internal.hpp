@@ -223,6 +223,27 @@ int vsa_attention_i8_ws(const h3_attention_cfg* cfg, uint32_t token_count, uint3
 int attention_i8qk_static_ws(const h3_attention_cfg* cfg, uint32_t token_count, uint32_t heads,
                              h3_view qi, h3_view qs, h3_view ki, h3_view ks, h3_view vt,
                              h3_view out, h3_view workspace, hipStream_t stream);
+// The 4-bit key/value cache (kv4.hip): rows of K and V into their slots, and back from them.
+hipError_t launch_kv4_write(const h3_kv4_cfg& cfg, uint32_t tokens, uint32_t k_stride,
+                            uint32_t v_stride, const void* k, const void* v, const int32_t* slots,
+                            void* cache, hipStream_t stream);
+hipError_t launch_kv4_read(const h3_kv4_cfg& cfg, uint32_t tokens, uint32_t k_stride,
+                           uint32_t v_stride, const int32_t* slots, const void* cache, void* k,
+                           void* v, hipStream_t stream);
+// Attention over it (attention_kv4.hip). How a call is cut: tiles of `tile_rows` rows (a row is a
+// token's query head) and the keys of each in `parts`, which need a workspace to be joined.
+struct Kv4Plan {
+  uint32_t tile_rows, row_tiles, parts;
+};
+Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
+                 uint32_t max_q, uint32_t cus);
+size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t q_rows,
+                           const Kv4Plan& plan);
+hipError_t launch_attention_kv4(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
+                                uint32_t batch, uint32_t q_rows, uint32_t max_q, const void* q,
+                                const void* cache, const int32_t* table, const int32_t* lengths,
+                                const int32_t* q_starts, void* out, float* lse, void* workspace,
+                                hipStream_t stream);
 // VSA operations (vsa.hip)
 hipError_t launch_vsa_gather(uint32_t tokens, uint32_t padded, uint32_t width, const int32_t* src,
                              const uint16_t* x, uint16_t* y, hipStream_t stream);

@@ -123,6 +123,30 @@ pub struct H3CrossCfg {
     pub out_stride: u32,
 }
 
+/// A paged cache of keys and values in 4 bits.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct H3Kv4Cfg {
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub page_tokens: u32,
+    pub pages: u32,
+    pub elem: u32,
+}
+
+/// Attention over it.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct H3Kv4AttentionCfg {
+    pub heads: u32,
+    pub q_stride: u32,
+    pub out_stride: u32,
+    pub table_stride: u32,
+    pub causal: u32,
+    pub window: u32,
+    pub scale: f32,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
 pub struct H3VsaCfg {
@@ -290,6 +314,20 @@ extern "C" {
     pub fn h3_attention_i8qkhm_cross(cfg: *const H3CrossCfg, qi: H3View, qs: H3View, ki: H3View,
                                      ks: H3View, vt: H3View, key_mask: H3View, out: H3View,
                                      stream: H3Stream) -> c_int;
+
+    // 4-bit key/value cache
+    pub fn h3_kv4_cache_bytes(cfg: *const H3Kv4Cfg) -> usize;
+    pub fn h3_kv4_write(cfg: *const H3Kv4Cfg, tokens: u32, k_stride: u32, v_stride: u32, k: H3View,
+                        v: H3View, slots: H3View, cache: H3View, stream: H3Stream) -> c_int;
+    pub fn h3_kv4_read(cfg: *const H3Kv4Cfg, tokens: u32, k_stride: u32, v_stride: u32,
+                       slots: H3View, cache: H3View, k: H3View, v: H3View,
+                       stream: H3Stream) -> c_int;
+    pub fn h3_kv4_workspace_bytes(cfg: *const H3Kv4Cfg, attention: *const H3Kv4AttentionCfg,
+                                  batch: u32, q_rows: u32, max_q: u32) -> usize;
+    pub fn h3_attention_kv4(cfg: *const H3Kv4Cfg, attention: *const H3Kv4AttentionCfg, batch: u32,
+                            q_rows: u32, max_q: u32, q: H3View, cache: H3View, table: H3View,
+                            lengths: H3View, q_starts: H3View, out: H3View, lse: H3View,
+                            workspace: H3View, stream: H3Stream) -> c_int;
 
     // VSA block-sparse attention
     pub fn h3_vsa_gather(cfg: *const H3VsaCfg, src: H3View, x: H3View, y: H3View,

@@ -133,6 +133,18 @@ class CrossCfg(ctypes.Structure):
         "out_stride")]
 
 
+class Kv4Cfg(ctypes.Structure):
+    """A paged cache of keys and values in 4 bits (h3_kv4_cfg)."""
+    _fields_ = [(name, ctypes.c_uint32) for name in (
+        "kv_heads", "head_dim", "page_tokens", "pages", "elem")]
+
+
+class Kv4AttentionCfg(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_uint32) for name in (
+        "heads", "q_stride", "out_stride", "table_stride", "causal", "window")] + [
+        ("scale", ctypes.c_float)]
+
+
 class VsaCfg(ctypes.Structure):
     """h3.vsa.* (kernels/vsa_ops.loom:3-9)."""
     _fields_ = [
@@ -207,6 +219,19 @@ SIGNATURES = {
          _S], ctypes.c_int),
     "h3_attention_i8qkhm_cross": (
         [_P(CrossCfg), View, View, View, View, View, View, View, _S], ctypes.c_int),
+    "h3_kv4_cache_bytes": ([_P(Kv4Cfg)], ctypes.c_size_t),
+    "h3_kv4_write": (
+        [_P(Kv4Cfg), ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, View, View, View, View, _S],
+        ctypes.c_int),
+    "h3_kv4_read": (
+        [_P(Kv4Cfg), ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, View, View, View, View, _S],
+        ctypes.c_int),
+    "h3_kv4_workspace_bytes": (
+        [_P(Kv4Cfg), _P(Kv4AttentionCfg), ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32],
+        ctypes.c_size_t),
+    "h3_attention_kv4": (
+        [_P(Kv4Cfg), _P(Kv4AttentionCfg), ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, View,
+         View, View, View, View, View, View, View, _S], ctypes.c_int),
     "h3_vsa_gather": ([_P(VsaCfg), View, View, View, _S], ctypes.c_int),
     "h3_vsa_scatter": ([_P(VsaCfg), View, View, View, _S], ctypes.c_int),
     "h3_vsa_pool": ([_P(VsaCfg), View, View, View, _S], ctypes.c_int),
@@ -544,6 +569,47 @@ def attention_i8qkhm_cross(cfg: CrossCfg, qi, qs, ki, ks, vt, key_mask, out, str
     check(lib().h3_attention_i8qkhm_cross(ctypes.byref(cfg), view(qi), view(qs), view(ki),
                                           view(ks), view(vt), view(key_mask), view(out),
                                           stream_ptr(stream)))
+
+
+# ------------------------------------------------------------------------- 4-bit key/value cache
+
+def kv4_cache_bytes(cfg: Kv4Cfg) -> int:
+    """Bytes of the cache `cfg` describes (0 for a config outside its ranges)."""
+    return int(lib().h3_kv4_cache_bytes(ctypes.byref(cfg)))
+
+
+def kv4_write(cfg: Kv4Cfg, tokens: int, k_stride: int, v_stride: int, k, v, slots, cache,
+              stream=None) -> None:
+    """Rows of k and v quantized into the cache's slots (a slot outside it: not written). Strides
+    are in elements, so a fused projection's columns are passed as flat views from their first
+    channel on: qkv.view(-1)[heads * dim:]."""
+    check(lib().h3_kv4_write(ctypes.byref(cfg), tokens, k_stride, v_stride, view(k), view(v),
+                             view(slots), view(cache), stream_ptr(stream)))
+
+
+def kv4_read(cfg: Kv4Cfg, tokens: int, k_stride: int, v_stride: int, slots, cache, k, v,
+             stream=None) -> None:
+    """The rows that the cache's slots stand for, into k and v (a slot outside it: zeros)."""
+    check(lib().h3_kv4_read(ctypes.byref(cfg), tokens, k_stride, v_stride, view(slots),
+                            view(cache), view(k), view(v), stream_ptr(stream)))
+
+
+def kv4_workspace_bytes(cfg: Kv4Cfg, acfg: Kv4AttentionCfg, batch: int, q_rows: int,
+                        max_q: int) -> int:
+    """Bytes of the workspace with which attention_kv4 divides such a call's keys (0: it would
+    not)."""
+    return int(lib().h3_kv4_workspace_bytes(ctypes.byref(cfg), ctypes.byref(acfg), batch, q_rows,
+                                            max_q))
+
+
+def attention_kv4(cfg: Kv4Cfg, acfg: Kv4AttentionCfg, batch: int, q_rows: int, max_q: int, q,
+                  cache, table, lengths, q_starts, out, lse=None, workspace=None,
+                  stream=None) -> None:
+    """Grouped-query attention of `batch` sequences over the cache, for decoding steps, drafted
+    tokens, prompts and any mix of them."""
+    check(lib().h3_attention_kv4(ctypes.byref(cfg), ctypes.byref(acfg), batch, q_rows, max_q,
+                                 view(q), view(cache), view(table), view(lengths), view(q_starts),
+                                 view(out), view(lse), view(workspace), stream_ptr(stream)))
 
 
 # ------------------------------------------------------------------------- VSA (src/vsa.rs)

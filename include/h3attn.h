@@ -387,6 +387,99 @@ int h3_attention_i8qkhm_cross(const h3_cross_cfg *cfg, h3_view qi, h3_view qs, h
                               h3_view ks, h3_view vt, h3_view key_mask, h3_view out,
                               h3_stream stream);
 
+/* ------------------------------------------------------------------ 4-bit key/value cache */
+
+/* A paged cache of keys and values in 4 bits, for sequences that grow a token at a time: rows are
+ * quantized as they are written, and attention reads the codes. No counterpart in the reference,
+ * which keeps no cache.
+ *   kv_heads     [1, 256]
+ *   head_dim     64 or 128
+ *   page_tokens  a power of two in [16, 1024]
+ *   pages        >= 1, pages * page_tokens <= 2^31 - 1
+ *   elem         H3_ELEM_F16 or H3_ELEM_BF16: the rows' type and the parameters'
+ * A row is one token's head_dim channels of one head, of K or of V. It is held as m = min x, s =
+ * (max x - m) / 15 rounded toward zero to the element type, and 4-bit codes u = clamp(rne((x - m) /
+ * s), 0, 15) (0 where s is 0), and stands for m + s * u, which never leaves [min x, max x]. A row
+ * that holds a NaN or an infinity stands for NaN throughout.
+ * Layout: per page, per head, one block of page_tokens * (head_dim + 8) bytes: K codes
+ * [page_tokens][head_dim / 2] (low nibble first), V codes the same, K words [page_tokens] and V words
+ * [page_tokens], 32 bits each with m low and s high. Slot t is token t % page_tokens of page
+ * t / page_tokens. Rows of channels that differ much in size lose least when K and the queries
+ * (or V) are rotated by an orthogonal matrix first, which leaves every score as it was. */
+typedef struct {
+  uint32_t kv_heads;
+  uint32_t head_dim;
+  uint32_t page_tokens;
+  uint32_t pages;
+  uint32_t elem;
+} h3_kv4_cfg;
+
+/* Bytes of a cache: pages * kv_heads * page_tokens * (head_dim + 8); 0 for a config outside its
+ * ranges. A new cache needs no particular contents. */
+size_t h3_kv4_cache_bytes(const h3_kv4_cfg *cfg);
+
+/* h3_kv4_write: row i of k and v, for i < tokens, quantized into slot slots[i]. A slot outside
+ * [0, pages * page_tokens) names no row: nothing is written (padding rows carry -1). Slots that are
+ * not named keep their bytes. The slots of one call must differ from each other: of two rows with
+ * one slot each of the slot's bytes holds either's.
+ *   k [tokens][k_stride], v [tokens][v_stride] (elem; kv_heads * head_dim channels used, strides
+ *   multiples of 8 from that to 2^20, so the K and V columns of a fused projection are views into
+ *   its rows), slots [tokens] i32, cache (h3_kv4_cache_bytes). k, v and cache 16-byte aligned.
+ *   tokens in [1, 16777216]. */
+int h3_kv4_write(const h3_kv4_cfg *cfg, uint32_t tokens, uint32_t k_stride, uint32_t v_stride,
+                 h3_view k, h3_view v, h3_view slots, h3_view cache, h3_stream stream);
+
+/* h3_kv4_read: the rows that slots[i] stand for, rounded to the element type, into k and v (laid
+ * out as above; columns past the heads are left as they were). A slot outside the cache gives
+ * zeros. */
+int h3_kv4_read(const h3_kv4_cfg *cfg, uint32_t tokens, uint32_t k_stride, uint32_t v_stride,
+                h3_view slots, h3_view cache, h3_view k, h3_view v, h3_stream stream);
+
+/* Config of h3_attention_kv4:
+ *   heads        query heads, a multiple of kv_heads in [1, 4096]; head h reads cache head
+ *                h / (heads / kv_heads)
+ *   q_stride     elements per row of q, a multiple of 8 in [heads * head_dim, 2^20]
+ *   out_stride   the same for out
+ *   table_stride pages a sequence's row of the table holds; table_stride * page_tokens <= 2^24
+ *   causal       1: row i of a sequence's n sits at position p = length - n + i and sees the keys
+ *                j <= p (its own key included, written before the call); 0: every row sees all
+ *   window       causal only: a row sees j > p - window alone; 0: no lower end
+ *   scale        the softmax scale, finite */
+typedef struct {
+  uint32_t heads;
+  uint32_t q_stride;
+  uint32_t out_stride;
+  uint32_t table_stride;
+  uint32_t causal;
+  uint32_t window;
+  float scale;
+} h3_kv4_attention_cfg;
+
+/* h3_attention_kv4: grouped-query attention of `batch` sequences over the cache. Sequence b has the
+ * query rows q_starts[b] .. q_starts[b + 1] - 1 and lengths[b] keys, key j in slot
+ * table[b][j / page_tokens] * page_tokens + j % page_tokens:
+ *   out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j,  lse[r][h] = ln sum_j exp(scale * q . k_j)
+ * over the keys that row r sees, k and v as they stand in the cache (not rounded to 16 bits but where
+ * noted in the kernels), probabilities and sums in f32. A row that sees no key gets zeros, and -inf
+ * as its lse. Rows of q that belong to no sequence are left as they were in out and lse.
+ *   q [q_rows][q_stride], out [q_rows][out_stride] (elem, 16-byte aligned), cache, table
+ *   [batch][table_stride] i32, lengths [batch] i32, q_starts [batch + 1] i32, lse [q_rows][heads] f32
+ *   or an empty view. q_rows in [1, 2^24], batch in [1, 65535], max_q in [1, q_rows]: no sequence
+ *   has more rows (of one that has, the rows from max_q on are left as they were).
+ * The device arrays are read on the device: a call can be captured in a graph and replayed with
+ * other lengths, tables and rows. Values outside their ranges read and write nothing out of bounds:
+ * a table entry that is no page of the cache hides its keys, a length is cut to table_stride *
+ * page_tokens, q_starts to [0, q_rows].
+ * With a workspace of h3_kv4_workspace_bytes bytes (16-byte aligned) the keys of a call that leaves
+ * the chip idle are divided and the parts joined by a second launch; without one (an empty view)
+ * each row's keys are one workgroup's. Calls that share a workspace must not overlap. */
+size_t h3_kv4_workspace_bytes(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention,
+                              uint32_t batch, uint32_t q_rows, uint32_t max_q);
+int h3_attention_kv4(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention, uint32_t batch,
+                     uint32_t q_rows, uint32_t max_q, h3_view q, h3_view cache, h3_view table,
+                     h3_view lengths, h3_view q_starts, h3_view out, h3_view lse, h3_view workspace,
+                     h3_stream stream);
+
 /* ------------------------------------------------------------------ VSA (video sparse attention) */
 
 /* Config of h3.vsa.* (kernels/vsa_ops.loom:3-9), as src/vsa/device.rs:63-77 builds it:
