@@ -230,10 +230,14 @@ hipError_t launch_kv4_write(const h3_kv4_cfg& cfg, uint32_t tokens, uint32_t k_s
 hipError_t launch_kv4_read(const h3_kv4_cfg& cfg, uint32_t tokens, uint32_t k_stride,
                            uint32_t v_stride, const int32_t* slots, const void* cache, void* k,
                            void* v, hipStream_t stream);
-// Attention over it (attention_kv4.hip). How a call is cut: tiles of `tile_rows` rows (a row is a
-// token's query head) and the keys of each in `parts`, which need a workspace to be joined.
+// Attention over it (attention_kv4.hip). How a call is cut: a launch for the sequences of many rows
+// and one for those of few (row_tiles 0: none), each in tiles of `tile_rows` rows (a row is a token's
+// query head) with the keys of a tile in `parts`, which need a workspace to be joined.
+struct Kv4Launch {
+  uint32_t tile_rows, row_tiles, parts, rows_from, rows_to;
+};
 struct Kv4Plan {
-  uint32_t tile_rows, row_tiles, parts;
+  Kv4Launch many, few;
 };
 Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
                  uint32_t max_q, uint32_t cus);
