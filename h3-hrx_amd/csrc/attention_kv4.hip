@@ -26,7 +26,6 @@ typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kKeys = 32;  // keys of a wave's step: two 16-key score tiles, one PV step
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_inff();
@@ -95,6 +94,12 @@ __device__ __forceinline__ float widen(uint32_t bits) {
   if constexpr (kBf16) return __uint_as_float(bits << 16);
   return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
+// Whether either half of a parameter word is a NaN or an infinity.
+template <bool kBf16>
+__device__ __forceinline__ bool has_nan(uint32_t word) {
+  constexpr uint32_t kTop = kBf16 ? 0x7f80u : 0x7c00u;
+  return (word & kTop) == kTop || ((word >> 16) & kTop) == kTop;
+}
 template <bool kBf16>
 __device__ __forceinline__ uint32_t narrow(float v) {
   if constexpr (kBf16) return __builtin_bit_cast(uint16_t, (__bf16)v);
@@ -123,111 +128,149 @@ __device__ __forceinline__ v4f mfma16(uint4 a, uint4 b, v4f c) {
                                                 __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// What one lane loads of a wave's 32 keys: lane (n = lane % 16, h = lane / 16) the K codes of key n
-// of either 16-key half, channels D/4 h and on; the V codes of keys 4h + e of either half, channels
-// D/16 n and on; and those keys' K and V words.
-template <int D>
-struct Tile {
-  uint32_t k[2][D / 32];
-  uint32_t v[8];
-  uint4 kw[2], vw[2];
+__device__ __forceinline__ int page_of(const Args& a, const int32_t* table, int key) {
+  const uint32_t col = (uint32_t)key >> a.page_shift;
+  const int id = col < a.table_stride ? table[col] : -1;
+  return (uint32_t)id < a.pages ? id : -1;
+}
+
+// Few rows: a workgroup's four waves hold the same R * QT rows of one cache head and take every
+// fourth 64 keys; their results are joined in LDS. Loads of the next 64 keys are in flight over the
+// work on these, so the kernel is bound by HBM as long as that work is short, and most of it is
+// vector instructions: the unpacking of the codes (one shift and one AND-OR a pair, fixed), then the
+// softmax. A 16 x 16 x 32 score tile S = Q K^T of R < 16 rows would leave 16 - R of its rows idle in
+// every softmax instruction, so T = 16 / R groups of 16 keys share one: group t meets a copy of Q
+// that holds its R rows at rows R t .. and zeros elsewhere, all accumulating into the same tile. A
+// lane (n = lane % 16, h = lane / 16) then has rows (4 h + i) % R of key 16 ((4 h) / R) + n: its
+// own key's factors, and no copies. Probabilities pass through LDS, [key][R] in 16 bits, and come
+// back through the transposed read as the operand of O^T = V^T P^T.
+constexpr int kStepKeys = 64;
+constexpr float kRaise = 7.0f;     // scores may pass m by this (p up to 2^7) before m is raised
+constexpr float kHeld = 256.0f;    // f16: p s is held times this over the largest scale
+
+template <int D, int R>
+struct Step {
+  uint32_t k[4][D / 32];          // key n of each 16: channels D/4 h and on
+  uint32_t v[16];                 // keys 32 (e / 8) + 8 h + e % 8: channels D/16 n and on
+  uint32_t kw[R / 4], vw[R / 4];  // the words of the lane's key in each score tile
+  uint32_t hidden;                // a bit per 16 keys: their page is none of the cache's
 };
 
-template <int D>
-__device__ __forceinline__ void load_half(const uint8_t* block, uint32_t in_page,
-                                          uint32_t page_tokens, int half, int n, int h,
-                                          Tile<D>& t) {
-  const uint8_t* kc = block + in_page * (D / 2);
-  const uint8_t* vc = kc + page_tokens * (D / 2);
-  const uint8_t* kw = block + page_tokens * D + in_page * 4;
-  const uint8_t* vw = kw + page_tokens * 4;
-  if constexpr (D == 128) {
-    const uint4 k = *reinterpret_cast<const uint4*>(kc + n * 64 + 16 * h);
-    t.k[half][0] = k.x, t.k[half][1] = k.y, t.k[half][2] = k.z, t.k[half][3] = k.w;
+// `ids`: lane l's is the page of key `key` + l.
+template <int D, int R>
+__device__ __forceinline__ void load_step(const Args& a, int ids, uint32_t head, int key, int n,
+                                          int h, Step<D, R>& s) {
+  const uint32_t page_tokens = 1u << a.page_shift, mask = page_tokens - 1;
+  const uint32_t block = page_tokens * (D + 8), page_bytes = block * a.kv_heads;
+  const uint8_t* base = a.cache + (uint64_t)head * block;
+  int id[4];
+  s.hidden = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      t.v[4 * half + e] = *reinterpret_cast<const uint32_t*>(vc + (4 * h + e) * 64 + 4 * n);
-  } else {
-    const uint2 k = *reinterpret_cast<const uint2*>(kc + n * 32 + 8 * h);
-    t.k[half][0] = k.x, t.k[half][1] = k.y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      t.v[4 * half + e] = *reinterpret_cast<const uint16_t*>(vc + (4 * h + e) * 32 + 2 * n);
+  for (int t = 0; t < 4; ++t) {
+    id[t] = __builtin_amdgcn_readlane(ids, 16 * t);
+    s.hidden |= id[t] < 0 ? 1u << t : 0u;
+    id[t] = max(id[t], 0);  // keys of no page are masked; page 0 is there to read
   }
-  t.kw[half] = *reinterpret_cast<const uint4*>(kw + 16 * h);
-  t.vw[half] = *reinterpret_cast<const uint4*>(vw + 16 * h);
-}
-
-// The pages of a step's two halves; -1 where the table names none that the cache has.
-struct Pages {
-  int id[2];
-};
-__device__ __forceinline__ Pages pages_of(const Args& a, const int32_t* table, int key) {
-  Pages p;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const uint32_t col = (uint32_t)(key + 16 * half) >> a.page_shift;
-    const int id = col < a.table_stride ? table[col] : -1;
-    p.id[half] = (uint32_t)id < a.pages ? id : -1;
+  for (int t = 0; t < 4; ++t) {
+    const uint8_t* kc = base + (uint64_t)(uint32_t)id[t] * page_bytes +
+                        (((uint32_t)key + 16 * t) & mask) * (D / 2);
+    if constexpr (D == 128) {
+      const uint4 k = *reinterpret_cast<const uint4*>(kc + (n * 64 + 16 * h));
+      s.k[t][0] = k.x, s.k[t][1] = k.y, s.k[t][2] = k.z, s.k[t][3] = k.w;
+    } else {
+      const uint2 k = *reinterpret_cast<const uint2*>(kc + (n * 32 + 8 * h));
+      s.k[t][0] = k.x, s.k[t][1] = k.y;
+    }
   }
-  return p;
-}
-
-template <int D>
-__device__ __forceinline__ void load_tile(const Args& a, const Pages& p, uint32_t head, int key,
-                                          int n, int h, Tile<D>& t) {
-  const uint32_t page_tokens = 1u << a.page_shift;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
-    const uint64_t page = max(p.id[half], 0);  // keys of no page are masked; page 0 is there to read
-    const uint8_t* block =
-        a.cache + (page * a.kv_heads + head) * ((uint64_t)page_tokens * (D + 8));
-    load_half<D>(block, (uint32_t)(key + 16 * half) & (page_tokens - 1), page_tokens, half, n, h, t);
+  for (int c = 0; c < R / 4; ++c) {
+    const int at = 16 * (c * (16 / R) + 4 * h / R);
+    int page;
+    if constexpr (R == 4) page = max(ids, 0);
+    if constexpr (R == 8) {
+      const int even = id[2 * c], odd = id[2 * c + 1];
+      page = h >> 1 ? odd : even;
+    }
+    if constexpr (R == 16) page = id[c];
+    const uint8_t* kw = base + (uint64_t)(uint32_t)page * page_bytes + page_tokens * D +
+                        (((uint32_t)key + at + n) & mask) * 4;
+    s.kw[c] = *reinterpret_cast<const uint32_t*>(kw);
+    s.vw[c] = *reinterpret_cast<const uint32_t*>(kw + page_tokens * 4);
+  }
+#pragma unroll
+  for (int st = 0; st < 2; ++st) {
+    const int even = id[2 * st], odd = id[2 * st + 1];
+    const int page = h >> 1 ? odd : even;
+    const uint8_t* vc = base + (uint64_t)(uint32_t)page * page_bytes + page_tokens * (D / 2) +
+                        (((uint32_t)key + 32 * st + 8 * h) & mask) * (D / 2) + n * (D / 32);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (D == 128)
+        s.v[8 * st + e] = *reinterpret_cast<const uint32_t*>(vc + e * 64);
+      else
+        s.v[8 * st + e] = *reinterpret_cast<const uint16_t*>(vc + e * 32);
+    }
   }
 }
 
-__device__ __forceinline__ float quarter_max(float v) {  // over the lanes with the same lane % 16
-  v = fmaxf(v, __shfl_xor(v, 16));
-  return fmaxf(v, __shfl_xor(v, 32));
-}
-__device__ __forceinline__ float quarter_sum(float v) {
-  v += __shfl_xor(v, 16);
-  return v + __shfl_xor(v, 32);
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+// Maximum or sum over the lanes that hold the same rows: the 16 of a group, and the groups whose
+// 4 h % R is the same.
+template <int R, bool kMax>
+__device__ __forceinline__ float row_lanes(float v) {
+  auto op = [](float x, float y) { return kMax ? fmaxf(x, y) : x + y; };
+#pragma unroll
+  for (int x = 1; x <= 8; x <<= 1) v = op(v, __shfl_xor(v, x));
+  if constexpr (R == 4) v = op(v, __shfl_xor(v, 16));
+  if constexpr (R <= 8) v = op(v, __shfl_xor(v, 32));
+  return v;
 }
 
-// Few rows: a workgroup's four waves hold the same QT * 16 rows of one cache head and take every
-// fourth step of its keys; their results are joined in LDS. S^T = K Q^T and O^T = V^T P^T, both
-// 16 x 16 x 32: a lane's score registers are four keys of one row, and they are the lane's own part
-// of the next product's operand, so no probability crosses lanes.
-template <int D, bool kBf16, int QT>
-__global__ __launch_bounds__(kThreads) void k_attention_kv4_few(Args a) {
-  constexpr int kRows = 16 * QT, kSteps = D / 32, kDimTiles = D / 16;
+template <int D, bool kBf16, int R, int QT>
+__global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few(Args a) {
+  static_assert(QT == 1 || R == 16, "row tiles of 16");
+  constexpr int T = 16 / R, kTiles = R / 4, kSteps = D / 32, kDimTiles = D / 16, kRows = R * QT;
+  __shared__ __attribute__((aligned(16))) uint16_t lds_p[kWaves][QT][kStepKeys * R];
+  __shared__ __attribute__((aligned(16))) float lds_o[kWaves][R][D + 4];
+  __shared__ float lds_row[kWaves][kRows];    // a factor per row, from its lanes to its column
+  __shared__ float2 lds_ml[kWaves][kRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, h = lane >> 4;
-  const uint32_t head = blockIdx.y, b = blockIdx.z;
-  const uint32_t part = blockIdx.x % a.parts;
+  const uint32_t head = blockIdx.y, b = blockIdx.z, part = blockIdx.x;
   const Sequence seq = sequence(a, b);
-  const int rows = seq.rows * (int)a.group;
-  const int row0 = (int)(blockIdx.x / a.parts) * kRows;
-  if (row0 >= rows || !takes(a, rows)) return;
-  const int token0 = row0 / (int)a.group;
-  const int token1 = min(row0 + kRows, rows) - 1;
-  const int2 first_span = span(a, seq, token0), last_span = span(a, seq, token1 / (int)a.group);
-  const int key_lo = first_span.x, key_hi = last_span.y;     // seen by some row
-  const int all_lo = last_span.x, all_hi = first_span.y;     // seen by every row
-  const Steps st = steps(key_lo, key_hi, a.parts, part, kKeys);
+  const int group = (int)a.group, rows = seq.rows * group;
+  if (rows == 0 || !takes(a, rows)) return;
+  const int2 first_span = span(a, seq, 0), last_span = span(a, seq, (rows - 1) / group);
+  const int key_lo = first_span.x, key_hi = last_span.y;  // seen by some row
+  const int all_lo = last_span.x, all_hi = first_span.y;  // seen by every row
+  const Steps st = steps(key_lo, key_hi, a.parts, part, kStepKeys);
   const uint32_t heads = a.kv_heads * a.group;
+  if (a.parts > 1 && st.first >= st.last && part > 0) {  // no keys: part 0 stands for an empty row
+    if ((int)threadIdx.x < rows) {
+      const int token = threadIdx.x / group, g = threadIdx.x - token * group;
+      a.part_ml[((size_t)part * a.q_rows + seq.start + token) * heads + head * group + g] = {-kInf, 0};
+    }
+    return;
+  }
+  const int32_t* table = a.table + (size_t)b * a.table_stride;
+  int step = st.first + wave;
+  int ids = page_of(a, table, step * kStepKeys + lane);
+  Step<D, R> next;
+  if (step < st.last) load_step<D, R>(a, ids, head, step * kStepKeys, n, h, next);
+  ids = page_of(a, table, (step + kWaves) * kStepKeys + lane);
 
-  // Q^T operands: channel D/4 h + 8 s + {0,4,1,5,2,6,3,7} in k slot 8 h + 0..7 of step s, the order
-  // in which the codes of a K word come out in pairs. Rows past the last are zeros.
-  uint4 qf[QT][kSteps];
-  float q_sum[QT];
-  int2 seen[QT];
+  // Q operands: channel D/4 h + 8 s + {0,4,1,5,2,6,3,7} in k slot 8 h + 0..7 of step s, the order in
+  // which the codes of a word come out in pairs. Rows past the last are zeros.
+  uint4 qf[QT][T][kSteps];
+  float q_sum[QT][4], m[QT][4], l[QT][4], mid[QT][4];  // row (4 h + i) % R; mid: sum p (m + 8 s)
+  v4f o[QT][kDimTiles], ones[QT];
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    const int row = row0 + 16 * t + n;
-    const int token = row / (int)a.group, g = row - token * (int)a.group;
-    seen[t] = row < rows ? span(a, seq, token) : int2{0, 0};
+    const int row = 16 * t + n % R;
+    const int token = row / group, g = row - token * group;
     float sum = 0.0f;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -235,227 +278,280 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_few(Args a) {
       if (row < rows)
         x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
                                             (size_t)(seq.start + token) * a.q_stride +
-                                            (head * a.group + g) * D + (D / 4) * h + 8 * s);
+                                            (head * group + g) * D + (D / 4) * h + 8 * s);
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum += widen<kBf16>(w[i] & 0xffffu) + widen<kBf16>(w[i] >> 16);
-      qf[t][s] = {(x.x & 0xffffu) | (x.z << 16), (x.x >> 16) | (x.z & 0xffff0000u),
-                  (x.y & 0xffffu) | (x.w << 16), (x.y >> 16) | (x.w & 0xffff0000u)};
-    }
-    q_sum[t] = quarter_sum(sum);
-  }
-
-  v4f o[QT][kDimTiles], ones[QT];
-  float m[QT], base[QT], l[QT], mid[QT];  // base: m, or 0 while no key was seen; mid: sum p (m + 8 s)
+      x = {(x.x & 0xffffu) | (x.z << 16), (x.x >> 16) | (x.z & 0xffff0000u),
+           (x.y & 0xffffu) | (x.w << 16), (x.y >> 16) | (x.w & 0xffff0000u)};
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
+      for (int u = 0; u < T; ++u) qf[t][u][s] = n / R == u ? x : uint4{0, 0, 0, 0};
+    }
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      q_sum[t][i] = __shfl(sum, (4 * h + i) % R);
+      m[t][i] = -kInf;
+      l[t][i] = mid[t][i] = 0.0f;
+    }
 #pragma unroll
     for (int d = 0; d < kDimTiles; ++d) o[t][d] = {0, 0, 0, 0};
     ones[t] = {0, 0, 0, 0};
-    m[t] = -kInf;
-    base[t] = l[t] = mid[t] = 0.0f;
   }
-  float s_top = 0.0f;            // f16: the power of two that p s is held relative to
-  float s_factor = 1.0f;         // what p is multiplied by beside s
+  float s_top = 0.0f, s_factor = 0.0f;  // f16: a power of two no scale passes, and kHeld over it
   const uint32_t one2 = kBf16 ? 0x3F803F80u : 0x3C003C00u;
   const uint4 one8 = {one2, one2, one2, one2};
-  const int32_t* table = a.table + (size_t)b * a.table_stride;
 
-  Tile<D> tile;
-  int step = st.first + wave;
-  Pages pg{{-1, -1}};
-  if (step < st.last) {
-    pg = pages_of(a, table, step * kKeys);
-    load_tile<D>(a, pg, head, step * kKeys, n, h, tile);
-  }
   for (; step < st.last; step += kWaves) {
-    const Tile<D> cur = tile;
-    const Pages at = pg;
-    const int key0 = step * kKeys;
+    const Step<D, R> cur = next;
+    const int key0 = step * kStepKeys;
     if (step + kWaves < st.last) {
-      pg = pages_of(a, table, key0 + kKeys * kWaves);
-      load_tile<D>(a, pg, head, key0 + kKeys * kWaves, n, h, tile);
+      const int now = ids;
+      ids = page_of(a, table, key0 + 2 * kStepKeys * kWaves + lane);
+      load_step<D, R>(a, now, head, key0 + kStepKeys * kWaves, n, h, next);
     }
     // Scores.
-    v4f acc[QT][2];
+    v4f acc[QT][kTiles];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
+    for (int c = 0; c < kTiles; ++c) {
 #pragma unroll
-      for (int t = 0; t < QT; ++t) acc[t][half] = {0, 0, 0, 0};
+      for (int t = 0; t < QT; ++t) acc[t][c] = {0, 0, 0, 0};
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
-        const uint32_t w = cur.k[half][s];
-        const uint4 kf = {code_pair<kBf16>(w, 0), code_pair<kBf16>(w, 1), code_pair<kBf16>(w, 2),
-                          code_pair<kBf16>(w, 3)};
+      for (int u = 0; u < T; ++u)
 #pragma unroll
-        for (int t = 0; t < QT; ++t) acc[t][half] = mfma16<kBf16>(kf, qf[t][s], acc[t][half]);
-      }
-    }
-    // This lane's eight keys: score factors and value factors.
-    float ks[8], km[8], vs[8], vm[8], s_max = 0.0f;
+        for (int s = 0; s < kSteps; ++s) {
+          const uint32_t w = cur.k[c * T + u][s];
+          const uint4 kf = {code_pair<kBf16>(w, 0), code_pair<kBf16>(w, 1), code_pair<kBf16>(w, 2),
+                            code_pair<kBf16>(w, 3)};
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint4 kw4 = cur.kw[e / 4], vw4 = cur.vw[e / 4];
-      const uint32_t kw = e % 4 == 0 ? kw4.x : e % 4 == 1 ? kw4.y : e % 4 == 2 ? kw4.z : kw4.w;
-      const uint32_t vw = e % 4 == 0 ? vw4.x : e % 4 == 1 ? vw4.y : e % 4 == 2 ? vw4.z : vw4.w;
-      const float s = widen<kBf16>(kw >> 16) * a.scale;
-      ks[e] = s;
-      km[e] = fmaf(-16.0f, s, widen<kBf16>(kw & 0xffffu) * a.scale);
-      vs[e] = widen<kBf16>(vw >> 16);
-      vm[e] = fmaf(8.0f, vs[e], widen<kBf16>(vw & 0xffffu));
-    }
-    const bool whole = key0 >= all_lo && key0 + kKeys <= all_hi && at.id[0] >= 0 && at.id[1] >= 0;
-    float x[QT][8];
-    bool raise = false;
-#pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      float top = -kInf;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[t][e] = fmaf(ks[e], acc[t][e / 4][e % 4], km[e] * q_sum[t]);
-        if (!whole) {
-          const int key = key0 + 16 * (e / 4) + 4 * h + e % 4;
-          if (key < seen[t].x || key >= seen[t].y || at.id[e / 4] < 0) x[t][e] = -kInf;
+          for (int t = 0; t < QT; ++t) acc[t][c] = mfma16<kBf16>(qf[t][u][s], kf, acc[t][c]);
         }
-        top = fmaxf(top, x[t][e]);
-      }
-      raise |= top > m[t];
     }
+    float ks[kTiles], km[kTiles], vs[kTiles], vm[kTiles];
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c) {
+      ks[c] = widen<kBf16>(cur.kw[c] >> 16) * a.scale;
+      km[c] = fmaf(-16.0f, ks[c], widen<kBf16>(cur.kw[c] & 0xffffu) * a.scale);
+      vs[c] = widen<kBf16>(cur.vw[c] >> 16);
+      vm[c] = fmaf(8.0f, vs[c], widen<kBf16>(cur.vw[c] & 0xffffu));
+    }
+    const bool whole = key0 >= all_lo && key0 + kStepKeys <= all_hi && cur.hidden == 0;
+    if (!whole) {
+      // A key whose V words hold a NaN gives NaN through its score, where only the rows that see it
+      // look; the words of keys that no row sees may hold anything.
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c) {
+        const int sub = c * T + 4 * h / R, key = key0 + 16 * sub + n;
+        const bool none = key < key_lo || key >= key_hi || (cur.hidden >> sub) & 1;
+        const bool nan = has_nan<kBf16>(cur.vw[c]);
+        if (nan) km[c] = __uint_as_float(0x7fc00000u);
+        if (none || nan) vs[c] = vm[c] = 0.0f;
+      }
+    }
+    bool raise = false;
+    float x[QT][kTiles][4];  // scores less m, base 2
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          x[t][c][i] = fmaf(ks[c], acc[t][c][i], fmaf(km[c], q_sum[t][i], -m[t][i]));
+    if (!whole) {
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c) {
+        const int sub = c * T + 4 * h / R, key = key0 + 16 * sub + n;
+        const bool hidden = (cur.hidden >> sub) & 1;
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = 16 * t + (4 * h + i) % R;
+            const int2 seen = row < rows ? span(a, seq, row / group) : int2{0, 0};
+            if (hidden || key < seen.x || key >= seen.y) x[t][c][i] = -kInf;
+          }
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c)
+        raise |= fmaxf(fmaxf(x[t][c][0], x[t][c][1]), fmaxf(x[t][c][2], x[t][c][3])) > kRaise;
     if constexpr (!kBf16) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int key = key0 + 16 * (e / 4) + 4 * h + e % 4;
-        if (whole || (key >= key_lo && key < key_hi && at.id[e / 4] >= 0)) s_max = fmaxf(s_max, vs[e]);
-      }
-      raise |= s_max > s_top;
+      for (int c = 0; c < kTiles; ++c) raise |= vs[c] > s_top;
     }
     if (__any(raise)) {
       float ratio = 1.0f;
       if constexpr (!kBf16) {
-        // The least power of two that no scale so far passes; s_top stays 0 while all are 0.
-        float s = s_max;
+        float s = vs[0];
 #pragma unroll
-        for (int x2 = 32; x2 >= 1; x2 >>= 1) s = fmaxf(s, __shfl_xor(s, x2));
+        for (int c = 1; c < kTiles; ++c) s = fmaxf(s, vs[c]);
+#pragma unroll
+        for (int w = 32; w >= 1; w >>= 1) s = fmaxf(s, __shfl_xor(s, w));
         if (s > s_top) {
           const float up = __uint_as_float((__float_as_uint(s) + 0x7fffffu) & 0x7f800000u);
           ratio = s_top / up;
           s_top = up;
-          s_factor = 16384.0f / up;
+          s_factor = kHeld / up;
         }
       }
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
-        float top = x[t][0];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) top = fmaxf(top, x[t][e]);
-        const float up = fmaxf(m[t], quarter_max(top));
-        const float at0 = up == -kInf ? 0.0f : up;
-        const float alpha = __builtin_amdgcn_exp2f(m[t] - at0);
-        m[t] = up;
-        base[t] = at0;
-        l[t] *= alpha;
-        mid[t] *= alpha;
-        const float both = alpha * ratio;
+        for (int i = 0; i < 4; ++i) {
+          // The scores themselves again: x is infinite while m is.
+          float y[kTiles], top = -kInf;
+#pragma unroll
+          for (int c = 0; c < kTiles; ++c) {
+            y[c] = fmaf(ks[c], acc[t][c][i], km[c] * q_sum[t][i]);
+            if (!whole && x[t][c][i] == -kInf) y[c] = -kInf;
+            top = fmaxf(top, y[c]);
+          }
+          const float up = fmaxf(m[t][i], row_lanes<R, true>(top));
+          const float base = up == -kInf ? 0.0f : up;
+          const float alpha = __builtin_amdgcn_exp2f(m[t][i] - base);
+          m[t][i] = up;
+          l[t][i] *= alpha;
+          mid[t][i] *= alpha;
+          if (n == 0 && 4 * h < R) lds_row[wave][16 * t + 4 * h + i] = alpha * ratio;
+#pragma unroll
+          for (int c = 0; c < kTiles; ++c) x[t][c][i] = y[c] - base;
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        const float both = lds_row[wave][16 * t + n % R];
 #pragma unroll
         for (int d = 0; d < kDimTiles; ++d) o[t][d] *= both;
         ones[t] *= both;
       }
     }
-    // Probabilities, and the operand p s in 16 bits (f16: relative to s_top, times 2^14; one
-    // rounding, of a weight of u - 8).
-    uint4 pf[QT];
+    // Probabilities, and p s in 16 bits (one rounding, of a weight of u - 8) on their way to columns.
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      float ps[8];
+    for (int c = 0; c < kTiles; ++c) {
+      const float f = kBf16 ? vs[c] : vs[c] * s_factor;
+      const int key = 16 * (c * T + 4 * h / R) + n;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = __builtin_amdgcn_exp2f(x[t][e] - base[t]);
-        const bool off = !whole && x[t][e] == -kInf;  // its words may hold anything
-        l[t] += p;
-        mid[t] += off ? 0.0f : p * vm[e];
-        ps[e] = off ? 0.0f : p * (kBf16 ? vs[e] : vs[e] * s_factor);
+      for (int t = 0; t < QT; ++t) {
+        float ps[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = __builtin_amdgcn_exp2f(x[t][c][i]);
+          l[t][i] += p;
+          mid[t][i] = fmaf(p, vm[c], mid[t][i]);
+          ps[i] = p * f;
+        }
+        *reinterpret_cast<uint2*>(&lds_p[wave][t][key * R + 4 * h % R]) = {
+            narrow2<kBf16>(ps[0], ps[1]), narrow2<kBf16>(ps[2], ps[3])};
       }
-      pf[t] = {narrow2<kBf16>(ps[0], ps[1]), narrow2<kBf16>(ps[2], ps[3]),
-               narrow2<kBf16>(ps[4], ps[5]), narrow2<kBf16>(ps[6], ps[7])};
-      ones[t] = mfma16<kBf16>(one8, pf[t], ones[t]);
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     // O^T: dim tile d holds channel D/16 n + d in row n; keys pair up across words.
-    uint32_t lo[4], hi[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      lo[i] = (cur.v[2 * i] & 0xffffu) | (cur.v[2 * i + 1] << 16);
-      hi[i] = (cur.v[2 * i] >> 16) | (cur.v[2 * i + 1] & 0xffff0000u);
+    for (int s = 0; s < 2; ++s) {
+      uint4 pf[QT];
+      const int at = (32 * s + 8 * h + (n >> 2)) * R + 4 * (n & 3) % R;
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        uint16_t* p = &lds_p[wave][t][at];
+        const v4s p0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p);
+        const v4s p1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 4 * R));
+        const uint2 w0 = __builtin_bit_cast(uint2, p0), w1 = __builtin_bit_cast(uint2, p1);
+        pf[t] = {w0.x, w0.y, w1.x, w1.y};
+        ones[t] = mfma16<kBf16>(one8, pf[t], ones[t]);
+      }
+      uint32_t lo[4], hi[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t v0 = cur.v[8 * s + 2 * i], v1 = cur.v[8 * s + 2 * i + 1];
+        lo[i] = (v0 & 0xffffu) | (v1 << 16);
+        hi[i] = (v0 >> 16) | (v1 & 0xffff0000u);
+      }
+#pragma unroll
+      for (int d = 0; d < kDimTiles; ++d) {
+        const uint32_t* w = d < 4 ? lo : hi;
+        const uint4 vf = {code_pair<kBf16>(w[0], d & 3), code_pair<kBf16>(w[1], d & 3),
+                          code_pair<kBf16>(w[2], d & 3), code_pair<kBf16>(w[3], d & 3)};
+#pragma unroll
+        for (int t = 0; t < QT; ++t) o[t][d] = mfma16<kBf16>(vf, pf[t], o[t][d]);
+      }
     }
-#pragma unroll
-    for (int d = 0; d < kDimTiles; ++d) {
-      const uint32_t* w = d < 4 ? lo : hi;
-      const uint4 vf = {code_pair<kBf16>(w[0], d & 3), code_pair<kBf16>(w[1], d & 3),
-                        code_pair<kBf16>(w[2], d & 3), code_pair<kBf16>(w[3], d & 3)};
-#pragma unroll
-      for (int t = 0; t < QT; ++t) o[t][d] = mfma16<kBf16>(vf, pf[t], o[t][d]);
-    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 
-  // Join the four waves: per 16-row tile, every wave's sums relative to the common maximum.
-  __shared__ float lds_o[kWaves][16][D + 4];
-  __shared__ float2 lds_ml[kWaves][16];
+  // Join the four waves: every wave's sums relative to the common maximum.
+  const float unit = kBf16 ? 1.0f : s_top * (1.0f / kHeld);
 #pragma unroll
   for (int t = 0; t < QT; ++t) {
-    const float lsum = quarter_sum(l[t]), msum = quarter_sum(mid[t]);
-    const float unit = kBf16 ? 1.0f : s_top * (1.0f / 16384.0f);
-    if (t) __syncthreads();
-    if (h == 0) lds_ml[wave][n] = {m[t], lsum};
-    // Row i of dim tile d: channel (D/16) (4h + i) + d.
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int d = 0; d < kDimTiles; d += 4) {
-        float4 f;
-        f.x = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d][i]), msum);
-        f.y = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d + 1][i]), msum);
-        f.z = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d + 2][i]), msum);
-        f.w = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d + 3][i]), msum);
-        *reinterpret_cast<float4*>(&lds_o[wave][n][kDimTiles * (4 * h + i) + d]) = f;
+    for (int i = 0; i < 4; ++i) {
+      const float ls = row_lanes<R, false>(l[t][i]), ms = row_lanes<R, false>(mid[t][i]);
+      if (n == 0 && 4 * h < R) {
+        lds_ml[wave][16 * t + 4 * h + i] = {m[t][i], ls};
+        lds_row[wave][16 * t + 4 * h + i] = ms;
       }
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+  for (int t = 0; t < QT; ++t) {
+    const float ms = lds_row[wave][16 * t + n % R];
+    if (t) __syncthreads();
+    if (n < R) {
+      // Row i of dim tile d: channel (D/16) (4h + i) + d.
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int d = 0; d < kDimTiles; d += 4) {
+          float4 f;
+          f.x = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d][i]), ms);
+          f.y = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d + 1][i]), ms);
+          f.z = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d + 2][i]), ms);
+          f.w = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d + 3][i]), ms);
+          *reinterpret_cast<float4*>(&lds_o[wave][n][kDimTiles * (4 * h + i) + d]) = f;
+        }
+    }
     __syncthreads();
-    // 16 threads a row, D/16 channels each.
-    const int r = threadIdx.x >> 4, c = (threadIdx.x & 15) * (D / 16);
-    const int row = row0 + 16 * t + r;
+    constexpr int kPer = R * D / kThreads;  // channels a thread; 256 / R threads a row
+    const int r = threadIdx.x / (kThreads / R), ch = (threadIdx.x % (kThreads / R)) * kPer;
+    const int row = 16 * t + r;
     if (row < rows) {
       float2 ml[kWaves];
       float top = -kInf;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        ml[w] = lds_ml[w][r];
+        ml[w] = lds_ml[w][row];
         top = fmaxf(top, ml[w].x);
       }
-      const float at0 = top == -kInf ? 0.0f : top;
-      float total = 0.0f, sum[D / 16];
+      const float base = top == -kInf ? 0.0f : top;
+      float total = 0.0f, sum[kPer];
 #pragma unroll
-      for (int d = 0; d < D / 16; ++d) sum[d] = 0.0f;
+      for (int d = 0; d < kPer; ++d) sum[d] = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(ml[w].x - at0);
+        const float f = __builtin_amdgcn_exp2f(ml[w].x - base);
         total = fmaf(f, ml[w].y, total);
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) sum[d] = fmaf(f, lds_o[w][r][c + d], sum[d]);
+        for (int d = 0; d < kPer; ++d) sum[d] = fmaf(f, lds_o[w][r][ch + d], sum[d]);
       }
-      const int token = row / (int)a.group, g = row - token * (int)a.group;
+      const int token = row / group, g = row - token * group;
       const size_t q_row = (size_t)(seq.start + token);
-      const uint32_t q_head = head * a.group + g;
+      const uint32_t q_head = head * group + g;
       if (a.parts > 1) {
-        const size_t at = ((size_t)part * a.q_rows + q_row) * heads + q_head;
+        const size_t place = ((size_t)part * a.q_rows + q_row) * heads + q_head;
 #pragma unroll
-        for (int d = 0; d < D / 16; ++d) a.part_o[at * D + c + d] = sum[d];
-        if (c == 0) a.part_ml[at] = {top, total};
+        for (int d = 0; d < kPer; ++d) a.part_o[place * D + ch + d] = sum[d];
+        if (ch == 0) a.part_ml[place] = {top, total};
       } else {
         const bool none = total == 0.0f;  // a NaN among the scores leaves total NaN
         const float inv = none ? 0.0f : 1.0f / total;
-        uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + c;
+        uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + ch;
 #pragma unroll
-        for (int d = 0; d < D / 16; d += 2)
-          *reinterpret_cast<uint32_t*>(out + d) = narrow2<kBf16>(sum[d] * inv, sum[d + 1] * inv);
-        if (a.lse && c == 0)
+        for (int d = 0; d < kPer; ++d) out[d] = (uint16_t)narrow<kBf16>(sum[d] * inv);
+        if (a.lse && ch == 0)
           a.lse[q_row * heads + q_head] = none ? -kInf : (top + __log2f(total)) * kLn2;
       }
     }
@@ -472,9 +568,6 @@ constexpr int kRowsThreads = 512;
 constexpr int kTileKeys = 64;
 constexpr float kPTop = 32768.0f;  // a lane's probabilities of 32 keys sum to no more, or m is raised
 constexpr float kPLog = 7.0f;      // the largest score gives p = 2^7: f16 stays normal to 2^-21 of it
-
-typedef short v4s __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4s lds_v4s;
 
 __device__ __forceinline__ uint32_t swap23(uint32_t m) {
   return (m & ~12u) | ((m & 4) << 1) | ((m & 8) >> 1);
@@ -529,12 +622,6 @@ __device__ __forceinline__ void fetch(const Args& a, uint32_t head, int key, int
   s.page = page;
 }
 
-__device__ __forceinline__ int page_of(const Args& a, const int32_t* table, int key) {
-  const uint32_t col = (uint32_t)key >> a.page_shift;
-  const int id = col < a.table_stride ? table[col] : -1;
-  return (uint32_t)id < a.pages ? id : -1;
-}
-
 // A pair of values m + s u, u as 16 + u in `code`, in the element type. f16: (u - 8) s + (m + 8 s) in
 // packed f16, exact but for the midpoint's rounding and the result's.
 template <bool kBf16>
@@ -561,12 +648,11 @@ __device__ __forceinline__ void unpack(const Args& a, RowsLds<D>& lds, int buf, 
   const uint32_t at = threadIdx.x >> 3, part = threadIdx.x & 7;
   const uint32_t m = (at & 32) + swap23(at & 31);
   const int key = key0 + (int)at;
-  constexpr uint32_t kNan = kBf16 ? 0x7f80u : 0x7c00u;
   const bool live = s.page >= 0;
   const bool seen = live && key >= key_lo && key < key_hi;
   // A key whose V words hold a NaN gives NaN through its score, where only the rows that see it
   // look; its V rows, and those of keys that no row sees, are zeros.
-  const bool nan = (s.vw & 0x7fffu) >= kNan || ((s.vw >> 16) & 0x7fffu) >= kNan;
+  const bool nan = has_nan<kBf16>(s.vw);
   const bool keep = seen && !nan;
   const float vs = keep ? widen<kBf16>(s.vw >> 16) : 0.0f;
   const float vm = keep ? widen<kBf16>(s.vw & 0xffffu) : 0.0f;
@@ -822,39 +908,78 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
     a.lse[q_row * heads + q_head] = none ? -kInf : (m + __log2f(total)) * kLn2;
 }
 
-// Joins the parts of a row: one wave per (row, query head), D/64 channels a lane.
-template <int D, bool kBf16>
+// Joins the parts of a row: W waves per (row, query head), wave w the parts w, w + W, ..; lane p of a
+// wave holds part p's weight (kMaxParts lanes at most). A part without keys has no sums to read.
+constexpr uint32_t kMaxParts = 64;
+
+template <int D, bool kBf16, int W>
 __global__ __launch_bounds__(kThreads) void k_attention_kv4_join(Args a) {
+  constexpr int kPer = D / 64;
+  __shared__ float lds_sum[W == 1 ? 1 : W][D];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t heads = a.kv_heads * a.group;
   const Sequence seq = sequence(a, blockIdx.z);
-  const uint32_t row = blockIdx.x * kWaves + wave;
+  const uint32_t row = blockIdx.x * (kWaves / W) + wave / W;
   const uint32_t token = row / a.group, g = row - token * a.group;
   if ((int)token >= seq.rows || !takes(a, seq.rows * (int)a.group)) return;
   const size_t q_row = (size_t)(seq.start + token);
   const uint32_t q_head = blockIdx.y * a.group + g;
-  float top = -kInf;
-  for (uint32_t p = 0; p < a.parts; ++p)
-    top = fmaxf(top, a.part_ml[((size_t)p * a.q_rows + q_row) * heads + q_head].x);
-  const float at0 = top == -kInf ? 0.0f : top;
-  float total = 0.0f, sum[D / 64];
+  const size_t place = q_row * heads + q_head, pitch = (size_t)a.q_rows * heads;
+  const float2 ml = lane < (int)a.parts ? a.part_ml[lane * pitch + place] : float2{-kInf, 0.0f};
+  float top = ml.x;
 #pragma unroll
-  for (int d = 0; d < D / 64; ++d) sum[d] = 0.0f;
-  for (uint32_t p = 0; p < a.parts; ++p) {
-    const size_t at = ((size_t)p * a.q_rows + q_row) * heads + q_head;
-    const float2 ml = a.part_ml[at];
-    const float f = __builtin_amdgcn_exp2f(ml.x - at0);
-    total = fmaf(f, ml.y, total);
+  for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+  const float f = __builtin_amdgcn_exp2f(ml.x - (top == -kInf ? 0.0f : top));
+  float total = f * ml.y;
 #pragma unroll
-    for (int d = 0; d < D / 64; ++d) sum[d] = fmaf(f, a.part_o[at * D + lane * (D / 64) + d], sum[d]);
+  for (int x = 32; x >= 1; x >>= 1) total += __shfl_xor(total, x);
+  // The parts with sums: those with a weight or a NaN.
+  uint64_t todo = __ballot(!(ml.y == 0.0f));
+  if constexpr (W > 1) {
+    uint64_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 64; i += W) mine |= 1ull << i;
+    todo &= mine << (wave % W);
+  }
+  float sum[kPer];
+#pragma unroll
+  for (int d = 0; d < kPer; ++d) sum[d] = 0.0f;
+  const float* from = a.part_o + place * D + lane * kPer;
+  while (todo) {
+    float x[4][kPer], w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // four loads in flight
+      const int p = todo ? __builtin_ctzll(todo) : 0;
+      w[i] = todo ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), p)) : 0.0f;
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) x[i][d] = todo ? from[p * pitch * D + d] : 0.0f;
+      todo &= todo - 1;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) sum[d] = fmaf(w[i], x[i][d], sum[d]);
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) lds_sum[wave][lane * kPer + d] = sum[d];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) {
+      sum[d] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) sum[d] += lds_sum[w][lane * kPer + d];
+    }
   }
   const bool none = total == 0.0f;
   const float inv = none ? 0.0f : 1.0f / total;
-  uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + lane * (D / 64);
-#pragma unroll
-  for (int d = 0; d < D / 64; ++d) out[d] = (uint16_t)narrow<kBf16>(sum[d] * inv);
-  if (a.lse && lane == 0)
-    a.lse[q_row * heads + q_head] = none ? -kInf : (top + __log2f(total)) * kLn2;
+  uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + lane * kPer;
+  if constexpr (kPer == 2)
+    *reinterpret_cast<uint32_t*>(out) = narrow2<kBf16>(sum[0] * inv, sum[1] * inv);
+  else
+    *out = (uint16_t)narrow<kBf16>(sum[0] * inv);
+  if (a.lse && lane == 0) a.lse[place] = none ? -kInf : (top + __log2f(total)) * kLn2;
 }
 
 // One launch over the sequences of `plan`'s row counts, and the join of its parts.
@@ -869,18 +994,27 @@ hipError_t launch(Args a, uint32_t batch, const Kv4Launch& plan, hipStream_t str
                                                        a.group * D);
   const uint32_t tiles = plan.row_tiles * plan.parts;
   const dim3 few(tiles, a.kv_heads, batch);
-  if (plan.tile_rows == 16)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 1>), few, dim3(kThreads), 0, stream, a);
+  if (plan.tile_rows == 4)
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 4, 1>), few, dim3(kThreads), 0, stream, a);
+  else if (plan.tile_rows == 8)
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 8, 1>), few, dim3(kThreads), 0, stream, a);
+  else if (plan.tile_rows == 16)
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16, 1>), few, dim3(kThreads), 0, stream, a);
   else if (plan.tile_rows == 32)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 2>), few, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16, 2>), few, dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL((k_attention_kv4_rows<D, kBf16>), dim3(a.kv_heads, tiles, batch),
                        dim3(kRowsThreads), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || plan.parts == 1) return e;
   const uint32_t rows = std::min(a.max_q * a.group, plan.rows_to);
-  const dim3 join((rows + kWaves - 1) / kWaves, a.kv_heads, batch);
-  hipLaunchKernelGGL((k_attention_kv4_join<D, kBf16>), join, dim3(kThreads), 0, stream, a);
+  if (plan.parts > 8)
+    hipLaunchKernelGGL((k_attention_kv4_join<D, kBf16, kWaves>), dim3(rows, a.kv_heads, batch),
+                       dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((k_attention_kv4_join<D, kBf16, 1>),
+                       dim3((rows + kWaves - 1) / kWaves, a.kv_heads, batch), dim3(kThreads), 0,
+                       stream, a);
   return hipGetLastError();
 }
 
@@ -906,7 +1040,7 @@ Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32
   auto parts = [&](uint32_t row_tiles, uint32_t resident) {
     const uint64_t groups = (uint64_t)batch * cfg.kv_heads * row_tiles;
     const uint64_t room = ((uint64_t)resident * cus + groups - 1) / groups;
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({room, most, 128}));
+    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({room, most, kMaxParts}));
   };
   if (rows > kFewRows) {
     p.many = {256, (rows + 255) / 256, 1, kFewRows + 1, rows};
@@ -914,7 +1048,7 @@ Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32
   }
   if (rows <= kFewRows || batch > 1) {
     const uint32_t few = std::min(rows, kFewRows);
-    p.few = {few <= 16 ? 16u : 32u, 1, 1, 0, few};
+    p.few = {few <= 4 ? 4u : few <= 8 ? 8u : few <= 16 ? 16u : 32u, 1, 1, 0, few};
     p.few.parts = parts(1, 4);
   }
   return p;
