@@ -106,17 +106,32 @@ __device__ __forceinline__ uint32_t narrow(float v) {
   return __builtin_bit_cast(uint16_t, (_Float16)v);
 }
 template <bool kBf16>
-__device__ __forceinline__ uint32_t narrow2(float lo, float hi) {
-  return narrow<kBf16>(lo) | (narrow<kBf16>(hi) << 16);
+__device__ __forceinline__ uint32_t narrow2(float lo, float hi) {  // one v_cvt_pk
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+  if constexpr (kBf16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{lo, hi}, v2bf));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{lo, hi}, v2h));
+}
+
+// The constants that make 16-bit floats of codes, the mask in a scalar and the exponent of 16 in a
+// vector register: as literals they would split every AND-OR in two.
+struct Codes {
+  uint32_t mask, bias;
+};
+template <bool kBf16>
+__device__ __forceinline__ Codes make_codes() {
+  Codes c{kBf16 ? 0x00780078u : 0x03C003C0u, kBf16 ? 0x41804180u : 0x4C004C00u};
+  asm("" : "+s"(c.mask));
+  asm("" : "+v"(c.bias));
+  return c;
 }
 
 // Nibble n of both halves of w as a pair of 16 + u.
 template <bool kBf16>
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int n) {
-  constexpr int kAt = kBf16 ? 3 : 6;  // the code's lowest bit in the mantissa
-  const int shift = kAt - 4 * n;
-  const uint32_t at = shift >= 0 ? w << shift : w >> -shift;
-  return (at & (kBf16 ? 0x00780078u : 0x03C003C0u)) | (kBf16 ? 0x41804180u : 0x4C004C00u);
+__device__ __forceinline__ uint32_t code_pair(uint32_t w, int n, const Codes& c) {
+  const int shift = (kBf16 ? 3 : 6) - 4 * n;  // to the top of the mantissa
+  return ((shift >= 0 ? w << shift : w >> -shift) & c.mask) | c.bias;
 }
 
 template <bool kBf16>
@@ -302,6 +317,7 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
   float s_top = 0.0f, s_factor = 0.0f;  // f16: a power of two no scale passes, and kHeld over it
   const uint32_t one2 = kBf16 ? 0x3F803F80u : 0x3C003C00u;
   const uint4 one8 = {one2, one2, one2, one2};
+  const Codes codes = make_codes<kBf16>();
 
   for (; step < st.last; step += kWaves) {
     const Step<D, R> cur = next;
@@ -322,8 +338,8 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
           const uint32_t w = cur.k[c * T + u][s];
-          const uint4 kf = {code_pair<kBf16>(w, 0), code_pair<kBf16>(w, 1), code_pair<kBf16>(w, 2),
-                            code_pair<kBf16>(w, 3)};
+          const uint4 kf = {code_pair<kBf16>(w, 0, codes), code_pair<kBf16>(w, 1, codes), code_pair<kBf16>(w, 2, codes),
+                            code_pair<kBf16>(w, 3, codes)};
 #pragma unroll
           for (int t = 0; t < QT; ++t) acc[t][c] = mfma16<kBf16>(qf[t][u][s], kf, acc[t][c]);
         }
@@ -473,8 +489,8 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
 #pragma unroll
       for (int d = 0; d < kDimTiles; ++d) {
         const uint32_t* w = d < 4 ? lo : hi;
-        const uint4 vf = {code_pair<kBf16>(w[0], d & 3), code_pair<kBf16>(w[1], d & 3),
-                          code_pair<kBf16>(w[2], d & 3), code_pair<kBf16>(w[3], d & 3)};
+        const uint4 vf = {code_pair<kBf16>(w[0], d & 3, codes), code_pair<kBf16>(w[1], d & 3, codes),
+                          code_pair<kBf16>(w[2], d & 3, codes), code_pair<kBf16>(w[3], d & 3, codes)};
 #pragma unroll
         for (int t = 0; t < QT; ++t) o[t][d] = mfma16<kBf16>(vf, pf[t], o[t][d]);
       }
@@ -589,10 +605,15 @@ __device__ __forceinline__ float spread(float v) {
       __builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + kLane, 0xF, 0xF, true));
 }
 
+// Row pitches in LDS. The rows that a K read of eight lanes takes start 16 bytes apart modulo 256, the
+// four keys of a transposed V read 64 apart, so that no two fall on the same banks.
+template <int D> constexpr int kKPitch = 2 * D + 16;
+template <int D> constexpr int kVPitch = 2 * D + 64;
+
 template <int D>
 struct RowsLds {
-  uint8_t k[2][kTileKeys * D * 2];
-  uint8_t v[2][kTileKeys * D * 2];
+  uint8_t k[2][kTileKeys * kKPitch<D>];
+  uint8_t v[2][kTileKeys * kVPitch<D>];
   float ks[2][kTileKeys], km[2][kTileKeys];  // times the scale: s, and m - 16 s
   uint8_t live[2][8];                        // a bit per key: its page is one
 };
@@ -635,16 +656,9 @@ __device__ __forceinline__ uint32_t value_pair(uint32_t code, float s, float m16
                                                                 __builtin_bit_cast(v2h, mid2)));
 }
 
-// Chunk (16 bytes) swizzles of the LDS rows of 2 D bytes, which spread the rows that one read takes
-// over the banks.
-template <int D>
-__device__ __forceinline__ uint32_t v_swizzle(uint32_t key) {
-  return (D == 128 ? 4 : 2) * (key & 3);
-}
-
 template <int D, bool kBf16>
 __device__ __forceinline__ void unpack(const Args& a, RowsLds<D>& lds, int buf, int key0, int key_lo,
-                                       int key_hi, const Staged<D>& s) {
+                                       int key_hi, const Codes& codes, const Staged<D>& s) {
   const uint32_t at = threadIdx.x >> 3, part = threadIdx.x & 7;
   const uint32_t m = (at & 32) + swap23(at & 31);
   const int key = key0 + (int)at;
@@ -663,14 +677,14 @@ __device__ __forceinline__ void unpack(const Args& a, RowsLds<D>& lds, int buf, 
   for (int i = 0; i < D / 64; ++i) {
     const uint32_t chunk = part * (D / 64) + i;
     uint4 x;
-    x.x = code_pair<kBf16>(s.k[i], 0), x.y = code_pair<kBf16>(s.k[i], 1);
-    x.z = code_pair<kBf16>(s.k[i], 2), x.w = code_pair<kBf16>(s.k[i], 3);
-    *reinterpret_cast<uint4*>(&lds.k[buf][m * (2 * D) + 16 * (chunk ^ (m & (D / 8 - 1)))]) = x;
-    x.x = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 0), vs, m16, s2, mid2);
-    x.y = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 1), vs, m16, s2, mid2);
-    x.z = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 2), vs, m16, s2, mid2);
-    x.w = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 3), vs, m16, s2, mid2);
-    *reinterpret_cast<uint4*>(&lds.v[buf][at * (2 * D) + 16 * (chunk ^ v_swizzle<D>(at))]) = x;
+    x.x = code_pair<kBf16>(s.k[i], 0, codes), x.y = code_pair<kBf16>(s.k[i], 1, codes);
+    x.z = code_pair<kBf16>(s.k[i], 2, codes), x.w = code_pair<kBf16>(s.k[i], 3, codes);
+    *reinterpret_cast<uint4*>(&lds.k[buf][m * kKPitch<D> + 16 * chunk]) = x;
+    x.x = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 0, codes), vs, m16, s2, mid2);
+    x.y = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 1, codes), vs, m16, s2, mid2);
+    x.z = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 2, codes), vs, m16, s2, mid2);
+    x.w = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 3, codes), vs, m16, s2, mid2);
+    *reinterpret_cast<uint4*>(&lds.v[buf][at * kVPitch<D> + 16 * chunk]) = x;
   }
   if (part == 0) {
     const float ks = widen<kBf16>(s.kw >> 16) * a.scale;
@@ -694,6 +708,95 @@ __device__ __forceinline__ void scores(float ks, const v16f& acc, const v16f& c,
   if constexpr (R < 16) {
     y[R] = spread<R>(ks) * acc[R] + c[R];
     scores<R + 1>(ks, acc, c, y);
+  }
+}
+
+// A wave's sums over the keys so far: O^T, and per lane (of its row) l, relative to m.
+template <int D>
+struct RowSums {
+  v16f o[D / 32];
+  float m, l;
+};
+
+// 32 keys of a tile (block blk of buffer buf) for a wave's 32 rows. Not `whole`: some key is hidden
+// from some row, by `live`, the tile's pages, or by `seen`, the row's keys counted from the tile's
+// first.
+template <int D, bool kBf16>
+__device__ __forceinline__ void attend_block(const RowsLds<D>& lds, int buf, int blk,
+                                             const uint4 (&qf)[D / 16], float q_sum, int lane,
+                                             bool whole, uint64_t live, int2 seen, RowSums<D>& r) {
+  const int n = lane & 31, half = lane >> 5;
+  const float ks = lds.ks[buf][32 * blk + (lane & 7) + 8 * half + 2 * (lane & 8)];
+  const float km = half ? -1.0f : lds.km[buf][32 * blk + swap23(n)];
+  // c = (m - 16 s) sum(q) - m of the row, in f32 on the matrix unit.
+  const v16f c = __builtin_amdgcn_mfma_f32_32x32x2f32(km, half ? r.m : q_sum, v16f{}, 0, 0, 0);
+  v16f acc = v16f{};
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    const uint4 kf = *reinterpret_cast<const uint4*>(
+        &lds.k[buf][(32 * blk + n) * kKPitch<D> + 16 * (2 * s + half)]);
+    acc = mfma32<kBf16>(kf, qf[s], acc);
+  }
+  float y[16], p[16], ts = 0.0f;
+  scores(ks, acc, c, y);
+  if (!whole) {
+    asm volatile("");  // a branch, not 16 selects in every block
+    const uint32_t mine = (uint32_t)(live >> (32 * blk)) >> (8 * half);
+    const int lo = seen.x - (32 * blk + 8 * half), hi = seen.y - (32 * blk + 8 * half);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int k = (i & 7) + 2 * (i & 8);
+      if (k < lo || k >= hi || !((mine >> k) & 1)) y[i] = -kInf;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    p[i] = __builtin_amdgcn_exp2f(y[i]);
+    ts += p[i];
+  }
+  if (__builtin_expect(__any(!(ts <= kPTop)), 0)) {
+    // The first keys, or scores far past m: the block's maximum, and everything relative to it.
+    const v16f c0 = __builtin_amdgcn_mfma_f32_32x32x2f32(km, half ? 0.0f : q_sum, v16f{}, 0, 0, 0);
+    float x[16], top = -kInf;
+    scores(ks, acc, c0, x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (!whole && y[i] == -kInf) x[i] = -kInf;
+      top = fmaxf(top, x[i]);
+    }
+    top = fmaxf(top, __shfl_xor(top, 32)) - kPLog;
+    const float up = fmaxf(r.m, top), base = up == -kInf ? 0.0f : up;
+    const float alpha = __builtin_amdgcn_exp2f(r.m - base);
+    r.m = up;
+    r.l *= alpha;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) r.o[d] *= alpha;
+    ts = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(x[i] - base);
+      ts += p[i];
+    }
+  }
+  r.l += ts;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const uint4 pf = {narrow2<kBf16>(p[8 * s], p[8 * s + 1]), narrow2<kBf16>(p[8 * s + 2], p[8 * s + 3]),
+                      narrow2<kBf16>(p[8 * s + 4], p[8 * s + 5]),
+                      narrow2<kBf16>(p[8 * s + 6], p[8 * s + 7])};
+    // V^T operand: row 32 d + n, keys 8 half + 0..7 of the step. Lane j of 16 points at key j / 4,
+    // channels 4 (j % 4) and on, and receives channel j of four keys.
+    const int j = lane & 15, quad = lane >> 4;
+    const int key = 32 * blk + 16 * s + 8 * (quad >> 1) + (j >> 2);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+      const uint32_t chunk = 4 * d + 2 * (quad & 1) + ((j & 3) >> 1);
+      const uint8_t* v = &lds.v[buf][key * kVPitch<D> + 16 * chunk + 8 * (j & 1)];
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)v);
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(v + 4 * kVPitch<D>));
+      const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+      r.o[d] = mfma32<kBf16>(uint4{l2.x, l2.y, h2.x, h2.y}, pf, r.o[d]);
+    }
   }
 }
 
@@ -743,18 +846,20 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   }
   const float q_sum = sum + __shfl_xor(sum, 32);
 
-  v16f o[kBlocks];
+  RowSums<D> sums;
 #pragma unroll
-  for (int d = 0; d < kBlocks; ++d) o[d] = v16f{};
-  float m = -kInf, l = 0.0f;  // m: what exponents are relative to, the largest score less kPLog
+  for (int d = 0; d < kBlocks; ++d) sums.o[d] = v16f{};
+  sums.m = -kInf;  // what exponents are relative to: the largest score less kPLog
+  sums.l = 0.0f;
   const int32_t* table = a.table + (size_t)b * a.table_stride;
   const int at = (int)(threadIdx.x >> 3);
+  const Codes codes = make_codes<kBf16>();
 
   Staged<D> staged;
   int page = -1;
   if (st.first < st.last) {
     fetch<D>(a, head, st.first * kTileKeys + at, page_of(a, table, st.first * kTileKeys + at), staged);
-    unpack<D, kBf16>(a, lds, 0, st.first * kTileKeys, key_lo, key_hi, staged);
+    unpack<D, kBf16>(a, lds, 0, st.first * kTileKeys, key_lo, key_hi, codes, staged);
     if (st.first + 1 < st.last) {
       const int key = (st.first + 1) * kTileKeys + at;
       fetch<D>(a, head, key, page_of(a, table, key), staged);
@@ -765,7 +870,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   for (int step = st.first; step < st.last; ++step) {
     const int buf = (step - st.first) & 1, key0 = step * kTileKeys;
     if (step + 1 < st.last) {
-      unpack<D, kBf16>(a, lds, buf ^ 1, key0 + kTileKeys, key_lo, key_hi, staged);
+      unpack<D, kBf16>(a, lds, buf ^ 1, key0 + kTileKeys, key_lo, key_hi, codes, staged);
       if (step + 2 < st.last) {
         const int key = key0 + 2 * kTileKeys + at;
         fetch<D>(a, head, key, page, staged);
@@ -775,90 +880,17 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
     if (active && key0 < wave_last.y && key0 + kTileKeys > wave_first.x) {
       const uint64_t live = *reinterpret_cast<const uint64_t*>(lds.live[buf]);
       const bool whole = key0 >= wave_last.x && key0 + kTileKeys <= wave_first.y && live == ~0ull;
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
-        const float ks = lds.ks[buf][32 * blk + (lane & 7) + 8 * half + 2 * (lane & 8)];
-        const float km = half ? -1.0f : lds.km[buf][32 * blk + swap23(n)];
-        // c = (m - 16 s) sum(q) - m of the row, in f32 on the matrix unit.
-        const v16f c = __builtin_amdgcn_mfma_f32_32x32x2f32(km, half ? m : q_sum, v16f{}, 0, 0, 0);
-        v16f acc = v16f{};
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const uint4 kf = *reinterpret_cast<const uint4*>(
-              &lds.k[buf][(32 * blk + n) * (2 * D) + 16 * ((2 * s + half) ^ (n & (D / 8 - 1)))]);
-          acc = mfma32<kBf16>(kf, qf[s], acc);
-        }
-        float y[16], ts = 0.0f;
-        scores(ks, acc, c, y);
-        if (!whole) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int k = 32 * blk + 8 * half + (r & 7) + 2 * (r & 8);
-            if (key0 + k < seen.x || key0 + k >= seen.y || !((live >> k) & 1)) y[r] = -kInf;
-          }
-        }
-        float p[16];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          p[r] = __builtin_amdgcn_exp2f(y[r]);
-          ts += p[r];
-        }
-        if (__any(!(ts <= kPTop))) {
-          // The first keys, or scores far past m: the block's maximum, and everything relative to it.
-          float top = -kInf;
-          const v16f c0 =
-              __builtin_amdgcn_mfma_f32_32x32x2f32(km, half ? 0.0f : q_sum, v16f{}, 0, 0, 0);
-          float x[16];
-          scores(ks, acc, c0, x);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            if (!whole && y[r] == -kInf) x[r] = -kInf;
-            top = fmaxf(top, x[r]);
-          }
-          top = fmaxf(top, __shfl_xor(top, 32)) - kPLog;
-          const float up = fmaxf(m, top), base = up == -kInf ? 0.0f : up;
-          const float alpha = __builtin_amdgcn_exp2f(m - base);
-          m = up;
-          l *= alpha;
-#pragma unroll
-          for (int d = 0; d < kBlocks; ++d) o[d] *= alpha;
-          ts = 0.0f;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            p[r] = __builtin_amdgcn_exp2f(x[r] - base);
-            ts += p[r];
-          }
-        }
-        l += ts;
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const uint4 pf = {narrow2<kBf16>(p[8 * s], p[8 * s + 1]),
-                            narrow2<kBf16>(p[8 * s + 2], p[8 * s + 3]),
-                            narrow2<kBf16>(p[8 * s + 4], p[8 * s + 5]),
-                            narrow2<kBf16>(p[8 * s + 6], p[8 * s + 7])};
-          // V^T operand: row 32 d + n, keys 8 half + 0..7 of the step. Lane j of 16 points at key j / 4,
-          // channels 4 (j % 4) and on, and receives channel j of four keys.
-          const int j = lane & 15, quad = lane >> 4;
-          const int key = 32 * blk + 16 * s + 8 * (quad >> 1) + (j >> 2);
-#pragma unroll
-          for (int d = 0; d < kBlocks; ++d) {
-            const uint32_t chunk = 4 * d + 2 * (quad & 1) + ((j & 3) >> 1);
-            const uint8_t* v =
-                &lds.v[buf][key * (2 * D) + 16 * (chunk ^ v_swizzle<D>(j >> 2)) + 8 * (j & 1)];
-            const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)v);
-            const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(v + 4 * 2 * D));
-            const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-            o[d] = mfma32<kBf16>(uint4{l2.x, l2.y, h2.x, h2.y}, pf, o[d]);
-          }
-        }
-      }
+      const int2 here = {seen.x - key0, seen.y - key0};
+      attend_block<D, kBf16>(lds, buf, 0, qf, q_sum, lane, whole, live, here, sums);
+      attend_block<D, kBf16>(lds, buf, 1, qf, q_sum, lane, whole, live, here, sums);
     }
     __syncthreads();
   }
 
   // Register 4 i + b of block d holds channel 32 d + 8 i + 2 half + {0, 4, 1, 5}[b] of the lane's row.
   if (!active) return;
-  const float total = l + __shfl_xor(l, 32);
+  const v16f(&o)[kBlocks] = sums.o;
+  const float m = sums.m, total = sums.l + __shfl_xor(sums.l, 32);
   const bool none = total == 0.0f;
   const size_t q_row = (size_t)(seq.start + token);
   const uint32_t q_head = head * a.group + g;
@@ -879,8 +911,10 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   }
   const float inv = none ? 0.0f : 1.0f / total;
   // Through LDS (each wave its own 32 rows; the tiles are done) so that whole rows leave together.
-  uint8_t* rows_lds = &lds.k[0][0] + wave * 32 * 2 * D;
-  static_assert(sizeof(lds.k) + sizeof(lds.v) >= 8 * 32 * 2 * D, "the tiles hold the rows");
+  uint8_t* rows_lds = reinterpret_cast<uint8_t*>(&lds) + wave * 32 * 2 * D;
+  static_assert(sizeof(lds.k) + sizeof(lds.v) >= 8 * 32 * 2 * D && offsetof(RowsLds<D>, k) == 0 &&
+                    offsetof(RowsLds<D>, v) == sizeof(lds.k),
+                "the tiles hold the rows");
 #pragma unroll
   for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
