@@ -612,10 +612,10 @@ template <int D> constexpr int kVPitch = 2 * D + 64;
 
 template <int D>
 struct RowsLds {
-  uint8_t k[2][kTileKeys * kKPitch<D>];
-  uint8_t v[2][kTileKeys * kVPitch<D>];
-  float ks[2][kTileKeys], km[2][kTileKeys];  // times the scale: s, and m - 16 s
-  uint8_t live[2][8];                        // a bit per key: its page is one
+  uint8_t k[3][kTileKeys * kKPitch<D>];
+  uint8_t v[3][kTileKeys * kVPitch<D>];
+  float ks[3][kTileKeys], km[3][kTileKeys];  // times the scale: s, and m - 16 s
+  uint8_t live[3][8];                        // a bit per key: its page is one
 };
 
 // A thread's share of a tile on the way to LDS: key tid / 8, channels D/8 (tid % 8) and on.
@@ -701,92 +701,119 @@ __device__ __forceinline__ void unpack(const Args& a, RowsLds<D>& lds, int buf, 
   }
 }
 
-// The 16 scores of a lane in a 32-key block, less m (base 2): acc times the keys' factors (lane r of
-// 16 holds register r's) plus c.
+// acc times the keys' factors: lane r of 16 holds register r's.
 template <int R = 0>
-__device__ __forceinline__ void scores(float ks, const v16f& acc, const v16f& c, float (&y)[16]) {
+__device__ __forceinline__ void scale_scores(float ks, v16f& acc) {
   if constexpr (R < 16) {
-    y[R] = spread<R>(ks) * acc[R] + c[R];
-    scores<R + 1>(ks, acc, c, y);
+    acc[R] *= spread<R>(ks);
+    scale_scores<R + 1>(ks, acc);
   }
 }
 
-// A wave's sums over the keys so far: O^T, and per lane (of its row) l, relative to m.
+// A wave's sums over the keys so far: O^T, and per lane (of its row) l, relative to m; m is -inf until
+// the row has met a key, and exponents are relative to 0 until then.
 template <int D>
 struct RowSums {
   v16f o[D / 32];
   float m, l;
+  __device__ __forceinline__ float base() const { return m == -kInf ? 0.0f : m; }
 };
 
-// 32 keys of a tile (block blk of buffer buf) for a wave's 32 rows. Not `whole`: some key is hidden
-// from some row, by `live`, the tile's pages, or by `seen`, the row's keys counted from the tile's
-// first.
-template <int D, bool kBf16>
-__device__ __forceinline__ void attend_block(const RowsLds<D>& lds, int buf, int blk,
-                                             const uint4 (&qf)[D / 16], float q_sum, int lane,
-                                             bool whole, uint64_t live, int2 seen, RowSums<D>& r) {
+// Steps kFrom .. kTo - 1 of the products q (16 + u) for the 32 keys of block blk of buffer buf.
+template <int D, bool kBf16, int kFrom, int kTo>
+__device__ __forceinline__ void add_products(const RowsLds<D>& lds, int buf, int blk,
+                                             const uint4 (&qf)[D / 16], int lane, v16f& acc) {
   const int n = lane & 31, half = lane >> 5;
-  const float ks = lds.ks[buf][32 * blk + (lane & 7) + 8 * half + 2 * (lane & 8)];
-  const float km = half ? -1.0f : lds.km[buf][32 * blk + swap23(n)];
-  // c = (m - 16 s) sum(q) - m of the row, in f32 on the matrix unit.
-  const v16f c = __builtin_amdgcn_mfma_f32_32x32x2f32(km, half ? r.m : q_sum, v16f{}, 0, 0, 0);
-  v16f acc = v16f{};
 #pragma unroll
-  for (int s = 0; s < D / 16; ++s) {
+  for (int s = kFrom; s < kTo; ++s) {
     const uint4 kf = *reinterpret_cast<const uint4*>(
         &lds.k[buf][(32 * blk + n) * kKPitch<D> + 16 * (2 * s + half)]);
     acc = mfma32<kBf16>(kf, qf[s], acc);
   }
-  float y[16], p[16], ts = 0.0f;
-  scores(ks, acc, c, y);
+}
+
+// Which keys of a 32-key block a lane's row sees: [lo, hi) counted from its first key (8 half), and
+// a bit per key whose page is one.
+struct Seen {
+  int lo, hi;
+  uint32_t live;
+};
+
+// The probabilities of a block as the operands of its two PV steps, from its products x. s_k x +
+// (m_k - 16 s_k) sum(q) - m is a multiplication on the vector unit and two products added to it in f32 on
+// the matrix unit (km, 1) (sum(q), -m). Where a row meets its first keys, or a lane's probabilities pass
+// kPTop, m is raised. The products of the next block (next_blk of next_buf) are under way meanwhile:
+// they are returned.
+template <int D, bool kBf16>
+__device__ __forceinline__ v16f probabilities(const RowsLds<D>& lds, int buf, int blk, int next_buf,
+                                              int next_blk, v16f x, const uint4 (&qf)[D / 16],
+                                              bool whole, const Seen& seen, float q_sum, int lane,
+                                              RowSums<D>& r, uint4 (&pf)[2]) {
+  const int n = lane & 31, half = lane >> 5;
+  const float ks = lds.ks[buf][32 * blk + (lane & 7) + 8 * half + 2 * (lane & 8)];
+  const float km = half ? -1.0f : lds.km[buf][32 * blk + swap23(n)];
+  scale_scores(ks, x);
+  v16f y = __builtin_amdgcn_mfma_f32_32x32x2f32(km, half ? r.base() : q_sum, x, 0, 0, 0);
+  v16f next = v16f{};
+  add_products<D, kBf16, 0, D / 32>(lds, next_buf, next_blk, qf, lane, next);
   if (!whole) {
     asm volatile("");  // a branch, not 16 selects in every block
-    const uint32_t mine = (uint32_t)(live >> (32 * blk)) >> (8 * half);
-    const int lo = seen.x - (32 * blk + 8 * half), hi = seen.y - (32 * blk + 8 * half);
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int k = (i & 7) + 2 * (i & 8);
-      if (k < lo || k >= hi || !((mine >> k) & 1)) y[i] = -kInf;
+      if (k < seen.lo || k >= seen.hi || !((seen.live >> k) & 1)) y[i] = -kInf;
     }
   }
+  float p[16], ts = 0.0f;
+  add_products<D, kBf16, D / 32, D / 16>(lds, next_buf, next_blk, qf, lane, next);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     p[i] = __builtin_amdgcn_exp2f(y[i]);
     ts += p[i];
   }
-  if (__builtin_expect(__any(!(ts <= kPTop)), 0)) {
-    // The first keys, or scores far past m: the block's maximum, and everything relative to it.
-    const v16f c0 = __builtin_amdgcn_mfma_f32_32x32x2f32(km, half ? 0.0f : q_sum, v16f{}, 0, 0, 0);
-    float x[16], top = -kInf;
-    scores(ks, acc, c0, x);
+  // Matrix and vector instructions in turn, so that the matrix unit works under the vector ones
+  // whatever the SIMD's other wave is at.
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if (!whole && y[i] == -kInf) x[i] = -kInf;
-      top = fmaxf(top, x[i]);
-    }
-    top = fmaxf(top, __shfl_xor(top, 32)) - kPLog;
-    const float up = fmaxf(r.m, top), base = up == -kInf ? 0.0f : up;
-    const float alpha = __builtin_amdgcn_exp2f(r.m - base);
+  for (int i = 0; i < D / 32; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, 32 / (D / 32), 0);
+  }
+  if (__builtin_expect(__any(!(ts <= kPTop) || r.m == -kInf), 0)) {
+    const float was = r.base();
+    float top = y[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) top = fmaxf(top, y[i]);
+    top = fmaxf(top, __shfl_xor(top, 32)) + (was - kPLog);
+    const float up = fmaxf(r.m, top);
+    const float alpha = __builtin_amdgcn_exp2f(r.m - (up == -kInf ? 0.0f : up));
     r.m = up;
+    const float by = was - r.base();
     r.l *= alpha;
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) r.o[d] *= alpha;
     ts = 0.0f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(x[i] - base);
+      p[i] = __builtin_amdgcn_exp2f(y[i] + by);
       ts += p[i];
     }
   }
   r.l += ts;
 #pragma unroll
+  for (int s = 0; s < 2; ++s)
+    pf[s] = {narrow2<kBf16>(p[8 * s], p[8 * s + 1]), narrow2<kBf16>(p[8 * s + 2], p[8 * s + 3]),
+             narrow2<kBf16>(p[8 * s + 4], p[8 * s + 5]), narrow2<kBf16>(p[8 * s + 6], p[8 * s + 7])};
+  return next;
+}
+
+// O^T += V^T P^T for a block. V^T operand of step s and channels 32 d + n: keys 8 half + 0..7 of the
+// step. Lane j of 16 points at key j / 4, channels 4 (j % 4) and on, and receives channel j of four keys.
+template <int D, bool kBf16>
+__device__ __forceinline__ void add_values(const RowsLds<D>& lds, int buf, int blk,
+                                           const uint4 (&pf)[2], int lane, RowSums<D>& r) {
+  const int j = lane & 15, quad = lane >> 4;
+#pragma unroll
   for (int s = 0; s < 2; ++s) {
-    const uint4 pf = {narrow2<kBf16>(p[8 * s], p[8 * s + 1]), narrow2<kBf16>(p[8 * s + 2], p[8 * s + 3]),
-                      narrow2<kBf16>(p[8 * s + 4], p[8 * s + 5]),
-                      narrow2<kBf16>(p[8 * s + 6], p[8 * s + 7])};
-    // V^T operand: row 32 d + n, keys 8 half + 0..7 of the step. Lane j of 16 points at key j / 4,
-    // channels 4 (j % 4) and on, and receives channel j of four keys.
-    const int j = lane & 15, quad = lane >> 4;
     const int key = 32 * blk + 16 * s + 8 * (quad >> 1) + (j >> 2);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d) {
@@ -795,7 +822,7 @@ __device__ __forceinline__ void attend_block(const RowsLds<D>& lds, int buf, int
       const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)v);
       const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(v + 4 * kVPitch<D>));
       const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-      r.o[d] = mfma32<kBf16>(uint4{l2.x, l2.y, h2.x, h2.y}, pf, r.o[d]);
+      r.o[d] = mfma32<kBf16>(uint4{l2.x, l2.y, h2.x, h2.y}, pf[s], r.o[d]);
     }
   }
 }
@@ -820,13 +847,15 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   const Steps st = steps(key_lo, key_hi, a.parts, part, kTileKeys);
   const uint32_t heads = a.kv_heads * a.group;
 
-  // The wave's rows, and the keys that some and that all of them see.
+  // The wave's rows, the keys that some and that all of them see, and the tiles it takes.
   const int wave_row0 = row0 + 32 * wave, row = wave_row0 + n;
-  const bool active = wave_row0 < rows;
   const int2 wave_first = span(a, seq, min(wave_row0, rows - 1) / group);
   const int2 wave_last = span(a, seq, min(wave_row0 + 31, rows - 1) / group);
   const int token = row / group, g = row - token * group;
   const int2 seen = row < rows ? span(a, seq, token) : int2{0, 0};
+  const bool active = wave_row0 < rows;
+  const int from = max(st.first, wave_first.x / kTileKeys);
+  const int to = active ? min(st.last, (wave_last.y + kTileKeys - 1) / kTileKeys) : from;
 
   // Q^T operands: channels 8 (2 s + half) + {0,4,1,5,2,6,3,7}, the order of the codes' pairs.
   uint4 qf[kSteps];
@@ -849,7 +878,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   RowSums<D> sums;
 #pragma unroll
   for (int d = 0; d < kBlocks; ++d) sums.o[d] = v16f{};
-  sums.m = -kInf;  // what exponents are relative to: the largest score less kPLog
+  sums.m = row < rows ? -kInf : 0.0f;
   sums.l = 0.0f;
   const int32_t* table = a.table + (size_t)b * a.table_stride;
   const int at = (int)(threadIdx.x >> 3);
@@ -860,33 +889,43 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   if (st.first < st.last) {
     fetch<D>(a, head, st.first * kTileKeys + at, page_of(a, table, st.first * kTileKeys + at), staged);
     unpack<D, kBf16>(a, lds, 0, st.first * kTileKeys, key_lo, key_hi, codes, staged);
-    if (st.first + 1 < st.last) {
-      const int key = (st.first + 1) * kTileKeys + at;
-      fetch<D>(a, head, key, page_of(a, table, key), staged);
-      page = page_of(a, table, key + kTileKeys);
-    }
+    const int key = (st.first + 1) * kTileKeys + at;
+    fetch<D>(a, head, key, page_of(a, table, key), staged);
+    page = page_of(a, table, key + kTileKeys);
     __syncthreads();
   }
+  // Three buffers and one barrier a tile: while a wave is at tile t, another may still read t - 1's
+  // values, and the tile written is t + 1. Tiles past the last are fetched and unpacked like the
+  // others (their keys are seen by no row, and page -1 reads page 0), so that the loop has no tail.
+  v16f x = v16f{};
+  int buf = 0;
   for (int step = st.first; step < st.last; ++step) {
-    const int buf = (step - st.first) & 1, key0 = step * kTileKeys;
-    if (step + 1 < st.last) {
-      unpack<D, kBf16>(a, lds, buf ^ 1, key0 + kTileKeys, key_lo, key_hi, codes, staged);
-      if (step + 2 < st.last) {
-        const int key = key0 + 2 * kTileKeys + at;
-        fetch<D>(a, head, key, page, staged);
-        page = page_of(a, table, key + kTileKeys);
-      }
-    }
-    if (active && key0 < wave_last.y && key0 + kTileKeys > wave_first.x) {
+    const int next = buf == 2 ? 0 : buf + 1, key0 = step * kTileKeys;
+    if (step >= from && step < to) {
       const uint64_t live = *reinterpret_cast<const uint64_t*>(lds.live[buf]);
       const bool whole = key0 >= wave_last.x && key0 + kTileKeys <= wave_first.y && live == ~0ull;
-      const int2 here = {seen.x - key0, seen.y - key0};
-      attend_block<D, kBf16>(lds, buf, 0, qf, q_sum, lane, whole, live, here, sums);
-      attend_block<D, kBf16>(lds, buf, 1, qf, q_sum, lane, whole, live, here, sums);
+      if (step == from) add_products<D, kBf16, 0, kSteps>(lds, buf, 0, qf, lane, x);
+      Seen see = {seen.x - key0 - 8 * half, seen.y - key0 - 8 * half, (uint32_t)live >> (8 * half)};
+      uint4 pf[2];
+      x = probabilities<D, kBf16>(lds, buf, 0, buf, 1, x, qf, whole, see, q_sum, lane, sums, pf);
+      add_values<D, kBf16>(lds, buf, 0, pf, lane, sums);
+      unpack<D, kBf16>(a, lds, next, key0 + kTileKeys, key_lo, key_hi, codes, staged);
+      fetch<D>(a, head, key0 + 2 * kTileKeys + at, page, staged);
+      page = page_of(a, table, key0 + 3 * kTileKeys + at);
+      __syncthreads();
+      see = {see.lo - 32, see.hi - 32, (uint32_t)(live >> 32) >> (8 * half)};
+      x = probabilities<D, kBf16>(lds, buf, 1, next, 0, x, qf, whole, see, q_sum, lane, sums, pf);
+      add_values<D, kBf16>(lds, buf, 1, pf, lane, sums);
+    } else {
+      unpack<D, kBf16>(a, lds, next, key0 + kTileKeys, key_lo, key_hi, codes, staged);
+      fetch<D>(a, head, key0 + 2 * kTileKeys + at, page, staged);
+      page = page_of(a, table, key0 + 3 * kTileKeys + at);
+      __syncthreads();
     }
-    __syncthreads();
+    buf = next;
   }
 
+  __syncthreads();  // the tiles are done with: LDS is free for the results
   // Register 4 i + b of block d holds channel 32 d + 8 i + 2 half + {0, 4, 1, 5}[b] of the lane's row.
   if (!active) return;
   const v16f(&o)[kBlocks] = sums.o;
@@ -910,7 +949,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
     return;
   }
   const float inv = none ? 0.0f : 1.0f / total;
-  // Through LDS (each wave its own 32 rows; the tiles are done) so that whole rows leave together.
+  // Through LDS (each wave its own 32 rows) so that whole rows leave together.
   uint8_t* rows_lds = reinterpret_cast<uint8_t*>(&lds) + wave * 32 * 2 * D;
   static_assert(sizeof(lds.k) + sizeof(lds.v) >= 8 * 32 * 2 * D && offsetof(RowsLds<D>, k) == 0 &&
                     offsetof(RowsLds<D>, v) == sizeof(lds.k),
