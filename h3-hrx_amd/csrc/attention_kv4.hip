@@ -615,31 +615,41 @@ struct RowsLds {
   uint8_t k[3][kTileKeys * kKPitch<D>];
   uint8_t v[3][kTileKeys * kVPitch<D>];
   float ks[3][kTileKeys], km[3][kTileKeys];  // times the scale: s, and m - 16 s
-  uint8_t live[3][8];                        // a bit per key: its page is one
+  float vn[3][kTileKeys];                    // NaN for a key whose V words hold one, else 0
+  uint8_t dead[3][kTileKeys];                // the key's page is none of the cache's
 };
 
-// A thread's share of a tile on the way to LDS: key tid / 8, channels D/8 (tid % 8) and on.
+// Waves 0..3 bring a tile's keys to LDS, waves 4..7 its values: a thread one key's (tid / 4 % 64)
+// channels D/4 (tid % 4) and on. Their D/32 words go to 16-byte chunks 4 i + tid % 4, so that the
+// lanes of a store lie side by side: chunk c of an LDS row holds channels 8 chunk_word(c) and on, an
+// order that Q is read in and the results are written in.
 template <int D>
 struct Staged {
-  uint32_t k[D / 64], v[D / 64];
-  uint32_t kw, vw;
+  uint32_t codes[D / 32];
+  uint32_t word;
   int page;
 };
+template <int D>
+__device__ __forceinline__ constexpr int chunk_word(int c) {
+  return (D / 32) * (c & 3) + (c >> 2);
+}
 
 template <int D>
 __device__ __forceinline__ void fetch(const Args& a, uint32_t head, int key, int page, Staged<D>& s) {
   const uint32_t page_tokens = 1u << a.page_shift, in_page = (uint32_t)key & (page_tokens - 1);
-  const uint8_t* block = a.cache + ((uint64_t)max(page, 0) * a.kv_heads + head) *
-                                       ((uint64_t)page_tokens * (D + 8));
-  const uint8_t* kc = block + in_page * (D / 2) + (threadIdx.x & 7) * (D / 16);
-  const uint8_t* kw = block + page_tokens * D + in_page * 4;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    s.k[i] = reinterpret_cast<const uint32_t*>(kc)[i];
-    s.v[i] = reinterpret_cast<const uint32_t*>(kc + page_tokens * (D / 2))[i];
+  const uint32_t block = page_tokens * (D + 8), v = threadIdx.x >> 8;
+  const uint8_t* at = a.cache + (uint64_t)head * block +
+                      (uint64_t)(uint32_t)max(page, 0) * (block * a.kv_heads);
+  const uint8_t* codes = at + (v * page_tokens * (D / 2) + in_page * (D / 2) + (threadIdx.x & 3) * (D / 8));
+  const uint8_t* word = at + (page_tokens * D + v * page_tokens * 4 + in_page * 4);
+  if constexpr (D == 128) {
+    const uint4 x = *reinterpret_cast<const uint4*>(codes);
+    s.codes[0] = x.x, s.codes[1] = x.y, s.codes[2] = x.z, s.codes[3] = x.w;
+  } else {
+    const uint2 x = *reinterpret_cast<const uint2*>(codes);
+    s.codes[0] = x.x, s.codes[1] = x.y;
   }
-  s.kw = *reinterpret_cast<const uint32_t*>(kw);
-  s.vw = *reinterpret_cast<const uint32_t*>(kw + page_tokens * 4);
+  s.word = *reinterpret_cast<const uint32_t*>(word);
   s.page = page;
 }
 
@@ -659,46 +669,42 @@ __device__ __forceinline__ uint32_t value_pair(uint32_t code, float s, float m16
 template <int D, bool kBf16>
 __device__ __forceinline__ void unpack(const Args& a, RowsLds<D>& lds, int buf, int key0, int key_lo,
                                        int key_hi, const Codes& codes, const Staged<D>& s) {
-  const uint32_t at = threadIdx.x >> 3, part = threadIdx.x & 7;
-  const uint32_t m = (at & 32) + swap23(at & 31);
-  const int key = key0 + (int)at;
-  const bool live = s.page >= 0;
-  const bool seen = live && key >= key_lo && key < key_hi;
+  const uint32_t at = (threadIdx.x >> 2) & 63, part = threadIdx.x & 3;
+  if (__builtin_amdgcn_readfirstlane(threadIdx.x >> 8) == 0) {
+    const uint32_t m = (at & 32) + swap23(at & 31);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i)
+      *reinterpret_cast<uint4*>(&lds.k[buf][m * kKPitch<D> + 16 * (4 * i + part)]) = {
+          code_pair<kBf16>(s.codes[i], 0, codes), code_pair<kBf16>(s.codes[i], 1, codes),
+          code_pair<kBf16>(s.codes[i], 2, codes), code_pair<kBf16>(s.codes[i], 3, codes)};
+    if (part == 0) {
+      const float ks = widen<kBf16>(s.word >> 16) * a.scale;
+      lds.ks[buf][at] = ks;
+      lds.km[buf][at] = fmaf(-16.0f, ks, widen<kBf16>(s.word & 0xffffu) * a.scale);
+      lds.dead[buf][at] = s.page < 0;
+    }
+    return;
+  }
   // A key whose V words hold a NaN gives NaN through its score, where only the rows that see it
   // look; its V rows, and those of keys that no row sees, are zeros.
-  const bool nan = has_nan<kBf16>(s.vw);
-  const bool keep = seen && !nan;
-  const float vs = keep ? widen<kBf16>(s.vw >> 16) : 0.0f;
-  const float vm = keep ? widen<kBf16>(s.vw & 0xffffu) : 0.0f;
+  const int key = key0 + (int)at;
+  const bool nan = has_nan<kBf16>(s.word);
+  const bool keep = s.page >= 0 && key >= key_lo && key < key_hi && !nan;
+  const uint32_t word = keep ? s.word : 0u;
+  const float vs = widen<kBf16>(word >> 16), vm = widen<kBf16>(word & 0xffffu);
   const float m16 = fmaf(-16.0f, vs, vm);
   const uint32_t s2 = narrow2<kBf16>(vs, vs), mid = narrow<kBf16>(fmaf(8.0f, vs, vm));
   const uint32_t mid2 = mid | (mid << 16);
 #pragma unroll
-  for (int i = 0; i < D / 64; ++i) {
-    const uint32_t chunk = part * (D / 64) + i;
+  for (int i = 0; i < D / 32; ++i) {
     uint4 x;
-    x.x = code_pair<kBf16>(s.k[i], 0, codes), x.y = code_pair<kBf16>(s.k[i], 1, codes);
-    x.z = code_pair<kBf16>(s.k[i], 2, codes), x.w = code_pair<kBf16>(s.k[i], 3, codes);
-    *reinterpret_cast<uint4*>(&lds.k[buf][m * kKPitch<D> + 16 * chunk]) = x;
-    x.x = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 0, codes), vs, m16, s2, mid2);
-    x.y = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 1, codes), vs, m16, s2, mid2);
-    x.z = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 2, codes), vs, m16, s2, mid2);
-    x.w = value_pair<kBf16>(code_pair<kBf16>(s.v[i], 3, codes), vs, m16, s2, mid2);
-    *reinterpret_cast<uint4*>(&lds.v[buf][at * kVPitch<D> + 16 * chunk]) = x;
+    x.x = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 0, codes), vs, m16, s2, mid2);
+    x.y = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 1, codes), vs, m16, s2, mid2);
+    x.z = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 2, codes), vs, m16, s2, mid2);
+    x.w = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 3, codes), vs, m16, s2, mid2);
+    *reinterpret_cast<uint4*>(&lds.v[buf][at * kVPitch<D> + 16 * (4 * i + part)]) = x;
   }
-  if (part == 0) {
-    const float ks = widen<kBf16>(s.kw >> 16) * a.scale;
-    const float km = fmaf(-16.0f, ks, widen<kBf16>(s.kw & 0xffffu) * a.scale);
-    lds.ks[buf][at] = ks;
-    lds.km[buf][at] = seen && nan ? __uint_as_float(0x7fc00000u) : km;
-  }
-  const uint64_t bits = __ballot(live && part == 0);  // key 8 w + i of wave w at bit 8 i
-  if ((threadIdx.x & 63) == 0) {
-    uint32_t byte = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) byte |= (uint32_t)((bits >> (8 * i)) & 1) << i;
-    lds.live[buf][threadIdx.x >> 6] = (uint8_t)byte;
-  }
+  if (part == 0) lds.vn[buf][at] = nan ? __uint_as_float(0x7fc00000u) : 0.0f;
 }
 
 // acc times the keys' factors: lane r of 16 holds register r's.
@@ -719,53 +725,93 @@ struct RowSums {
   __device__ __forceinline__ float base() const { return m == -kInf ? 0.0f : m; }
 };
 
-// Steps kFrom .. kTo - 1 of the products q (16 + u) for the 32 keys of block blk of buffer buf.
-template <int D, bool kBf16, int kFrom, int kTo>
-__device__ __forceinline__ void add_products(const RowsLds<D>& lds, int buf, int blk,
-                                             const uint4 (&qf)[D / 16], int lane, v16f& acc) {
+// What a wave reads of a 32-key block (block blk of buffer buf) before its products: the first half
+// of the K operands. The reads run a phase ahead of their use, here and below: two waves a SIMD do not
+// hide an LDS read's latency.
+template <int D>
+struct KeyOps {
+  uint4 k[D / 32];
+};
+template <int D, int kFrom>
+__device__ __forceinline__ KeyOps<D> read_keys(const RowsLds<D>& lds, int buf, int blk, int lane) {
   const int n = lane & 31, half = lane >> 5;
+  KeyOps<D> x;
 #pragma unroll
-  for (int s = kFrom; s < kTo; ++s) {
-    const uint4 kf = *reinterpret_cast<const uint4*>(
-        &lds.k[buf][(32 * blk + n) * kKPitch<D> + 16 * (2 * s + half)]);
-    acc = mfma32<kBf16>(kf, qf[s], acc);
-  }
+  for (int s = 0; s < D / 32; ++s)
+    x.k[s] = *reinterpret_cast<const uint4*>(
+        &lds.k[buf][(32 * blk + n) * kKPitch<D> + 16 * (2 * (kFrom + s) + half)]);
+  return x;
 }
 
-// Which keys of a 32-key block a lane's row sees: [lo, hi) counted from its first key (8 half), and
-// a bit per key whose page is one.
+// V^T operands of step s of a block, channels of chunks 4 d .. 4 d + 3, keys 8 half + 0..7: lane j of 16
+// points at key j / 4, channels 4 (j % 4) and on, and receives channel j of four keys.
+template <int D>
+struct ValueOps {
+  uint4 v[D / 32];
+};
+template <int D>
+__device__ __forceinline__ ValueOps<D> read_values(const RowsLds<D>& lds, int buf, int blk, int s,
+                                                   int lane) {
+  const int j = lane & 15, quad = lane >> 4;
+  const int key = 32 * blk + 16 * s + 8 * (quad >> 1) + (j >> 2);
+  ValueOps<D> x;
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) {
+    const uint32_t chunk = 4 * d + 2 * (quad & 1) + ((j & 3) >> 1);
+    const uint8_t* v = &lds.v[buf][key * kVPitch<D> + 16 * chunk + 8 * (j & 1)];
+    const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)v);
+    const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(v + 4 * kVPitch<D>));
+    const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
+    x.v[d] = {l2.x, l2.y, h2.x, h2.y};
+  }
+  return x;
+}
+
+// Which keys of a 32-key block a lane's row sees: [lo, hi) counted from its first key (8 half).
 struct Seen {
   int lo, hi;
-  uint32_t live;
+  bool pages;  // some page of the workgroup's keys is none of the cache's: `dead` says which keys
 };
 
-// The probabilities of a block as the operands of its two PV steps, from its products x. s_k x +
-// (m_k - 16 s_k) sum(q) - m is a multiplication on the vector unit and two products added to it in f32 on
-// the matrix unit (km, 1) (sum(q), -m). Where a row meets its first keys, or a lane's probabilities pass
-// kPTop, m is raised. The products of the next block (next_blk of next_buf) are under way meanwhile:
-// they are returned.
+// One 32-key block (blk of buf) of a wave, from its products x = q (16 + u): probabilities and the sum
+// over values. s_k x + (m_k - 16 s_k) sum(q) - m is a multiplication on the vector unit and two products
+// added to it in f32 on the matrix unit, (km, 1) (sum(q), -m). Where a row meets its first keys, or a
+// lane's probabilities pass kPTop, m is raised. The products of the next block run among the vector
+// instructions: its first operands are in `keys`, the others' block is next_blk of next_buf; they are
+// returned.
 template <int D, bool kBf16>
-__device__ __forceinline__ v16f probabilities(const RowsLds<D>& lds, int buf, int blk, int next_buf,
-                                              int next_blk, v16f x, const uint4 (&qf)[D / 16],
-                                              bool whole, const Seen& seen, float q_sum, int lane,
-                                              RowSums<D>& r, uint4 (&pf)[2]) {
+__device__ __forceinline__ v16f attend_block(const RowsLds<D>& lds, int buf, int blk, int next_buf,
+                                             int next_blk, v16f x, const uint4 (&qf)[D / 16],
+                                             const KeyOps<D>& keys, bool whole, const Seen& seen,
+                                             float q_sum, int lane, RowSums<D>& r) {
   const int n = lane & 31, half = lane >> 5;
   const float ks = lds.ks[buf][32 * blk + (lane & 7) + 8 * half + 2 * (lane & 8)];
-  const float km = half ? -1.0f : lds.km[buf][32 * blk + swap23(n)];
+  const float kv = lds.km[buf][32 * blk + swap23(n)] + lds.vn[buf][32 * blk + swap23(n)];
+  const KeyOps<D> rest = read_keys<D, D / 32>(lds, next_buf, next_blk, lane);
+  const float km = half ? -1.0f : kv;
+  v16f next = v16f{};
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) next = mfma32<kBf16>(keys.k[s], qf[s], next);
   scale_scores(ks, x);
   v16f y = __builtin_amdgcn_mfma_f32_32x32x2f32(km, half ? r.base() : q_sum, x, 0, 0, 0);
-  v16f next = v16f{};
-  add_products<D, kBf16, 0, D / 32>(lds, next_buf, next_blk, qf, lane, next);
   if (!whole) {
     asm volatile("");  // a branch, not 16 selects in every block
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int k = (i & 7) + 2 * (i & 8);
-      if (k < seen.lo || k >= seen.hi || !((seen.live >> k) & 1)) y[i] = -kInf;
+      if (k < seen.lo || k >= seen.hi) y[i] = -kInf;
+    }
+    if (seen.pages) {
+      asm volatile("");
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (lds.dead[buf][32 * blk + 8 * half + (i & 7) + 2 * (i & 8)]) y[i] = -kInf;
     }
   }
+  const ValueOps<D> v0 = read_values<D>(lds, buf, blk, 0, lane);
   float p[16], ts = 0.0f;
-  add_products<D, kBf16, D / 32, D / 16>(lds, next_buf, next_blk, qf, lane, next);
+#pragma unroll
+  for (int s = 0; s < D / 32; ++s) next = mfma32<kBf16>(rest.k[s], qf[D / 32 + s], next);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     p[i] = __builtin_amdgcn_exp2f(y[i]);
@@ -773,6 +819,7 @@ __device__ __forceinline__ v16f probabilities(const RowsLds<D>& lds, int buf, in
   }
   // Matrix and vector instructions in turn, so that the matrix unit works under the vector ones
   // whatever the SIMD's other wave is at.
+  __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -798,33 +845,18 @@ __device__ __forceinline__ v16f probabilities(const RowsLds<D>& lds, int buf, in
       ts += p[i];
     }
   }
+  const ValueOps<D> v1 = read_values<D>(lds, buf, blk, 1, lane);
   r.l += ts;
+  uint4 pf[2];
 #pragma unroll
   for (int s = 0; s < 2; ++s)
     pf[s] = {narrow2<kBf16>(p[8 * s], p[8 * s + 1]), narrow2<kBf16>(p[8 * s + 2], p[8 * s + 3]),
              narrow2<kBf16>(p[8 * s + 4], p[8 * s + 5]), narrow2<kBf16>(p[8 * s + 6], p[8 * s + 7])};
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) r.o[d] = mfma32<kBf16>(v0.v[d], pf[0], r.o[d]);
+#pragma unroll
+  for (int d = 0; d < D / 32; ++d) r.o[d] = mfma32<kBf16>(v1.v[d], pf[1], r.o[d]);
   return next;
-}
-
-// O^T += V^T P^T for a block. V^T operand of step s and channels 32 d + n: keys 8 half + 0..7 of the
-// step. Lane j of 16 points at key j / 4, channels 4 (j % 4) and on, and receives channel j of four keys.
-template <int D, bool kBf16>
-__device__ __forceinline__ void add_values(const RowsLds<D>& lds, int buf, int blk,
-                                           const uint4 (&pf)[2], int lane, RowSums<D>& r) {
-  const int j = lane & 15, quad = lane >> 4;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int key = 32 * blk + 16 * s + 8 * (quad >> 1) + (j >> 2);
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d) {
-      const uint32_t chunk = 4 * d + 2 * (quad & 1) + ((j & 3) >> 1);
-      const uint8_t* v = &lds.v[buf][key * kVPitch<D> + 16 * chunk + 8 * (j & 1)];
-      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)v);
-      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(v + 4 * kVPitch<D>));
-      const uint2 l2 = __builtin_bit_cast(uint2, lo), h2 = __builtin_bit_cast(uint2, hi);
-      r.o[d] = mfma32<kBf16>(uint4{l2.x, l2.y, h2.x, h2.y}, pf[s], r.o[d]);
-    }
-  }
 }
 
 template <int D, bool kBf16>
@@ -857,7 +889,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   const int from = max(st.first, wave_first.x / kTileKeys);
   const int to = active ? min(st.last, (wave_last.y + kTileKeys - 1) / kTileKeys) : from;
 
-  // Q^T operands: channels 8 (2 s + half) + {0,4,1,5,2,6,3,7}, the order of the codes' pairs.
+  // Q^T operands: chunk 2 s + half's channels, in the order {0,4,1,5,2,6,3,7} of the codes' pairs.
   uint4 qf[kSteps];
   float sum = 0.0f;
 #pragma unroll
@@ -866,7 +898,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
     if (row < rows)
       x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
                                           (size_t)(seq.start + token) * a.q_stride +
-                                          (head * a.group + g) * D + 8 * (2 * s + half));
+                                          (head * a.group + g) * D + 8 * chunk_word<D>(2 * s + half));
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) sum += widen<kBf16>(w[i] & 0xffffu) + widen<kBf16>(w[i] >> 16);
@@ -881,41 +913,51 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   sums.m = row < rows ? -kInf : 0.0f;
   sums.l = 0.0f;
   const int32_t* table = a.table + (size_t)b * a.table_stride;
-  const int at = (int)(threadIdx.x >> 3);
+  const int at = (int)(threadIdx.x >> 2) & 63;
   const Codes codes = make_codes<kBf16>();
 
   Staged<D> staged;
   int page = -1;
+  bool hidden = false;
   if (st.first < st.last) {
-    fetch<D>(a, head, st.first * kTileKeys + at, page_of(a, table, st.first * kTileKeys + at), staged);
-    unpack<D, kBf16>(a, lds, 0, st.first * kTileKeys, key_lo, key_hi, codes, staged);
-    const int key = (st.first + 1) * kTileKeys + at;
+    const int key = st.first * kTileKeys + at;
     fetch<D>(a, head, key, page_of(a, table, key), staged);
     page = page_of(a, table, key + kTileKeys);
-    __syncthreads();
+    for (int k = max(st.first * kTileKeys, key_lo & ~15) + 16 * (int)threadIdx.x;
+         k < min(st.last * kTileKeys, key_hi); k += 16 * kRowsThreads)
+      hidden |= page_of(a, table, k) < 0;
+    unpack<D, kBf16>(a, lds, 0, st.first * kTileKeys, key_lo, key_hi, codes, staged);
+    fetch<D>(a, head, key + kTileKeys, page, staged);
+    page = page_of(a, table, key + 2 * kTileKeys);
   }
+  hidden = __syncthreads_or(hidden);  // some seen key's page is none of the cache's
   // Three buffers and one barrier a tile: while a wave is at tile t, another may still read t - 1's
   // values, and the tile written is t + 1. Tiles past the last are fetched and unpacked like the
   // others (their keys are seen by no row, and page -1 reads page 0), so that the loop has no tail.
   v16f x = v16f{};
+  KeyOps<D> keys;
   int buf = 0;
   for (int step = st.first; step < st.last; ++step) {
     const int next = buf == 2 ? 0 : buf + 1, key0 = step * kTileKeys;
     if (step >= from && step < to) {
-      const uint64_t live = *reinterpret_cast<const uint64_t*>(lds.live[buf]);
-      const bool whole = key0 >= wave_last.x && key0 + kTileKeys <= wave_first.y && live == ~0ull;
-      if (step == from) add_products<D, kBf16, 0, kSteps>(lds, buf, 0, qf, lane, x);
-      Seen see = {seen.x - key0 - 8 * half, seen.y - key0 - 8 * half, (uint32_t)live >> (8 * half)};
-      uint4 pf[2];
-      x = probabilities<D, kBf16>(lds, buf, 0, buf, 1, x, qf, whole, see, q_sum, lane, sums, pf);
-      add_values<D, kBf16>(lds, buf, 0, pf, lane, sums);
+      const bool whole = key0 >= wave_last.x && key0 + kTileKeys <= wave_first.y && !hidden;
+      if (step == from) {
+        const KeyOps<D> k0 = read_keys<D, 0>(lds, buf, 0, lane), k1 = read_keys<D, D / 32>(lds, buf, 0, lane);
+#pragma unroll
+        for (int s = 0; s < kSteps / 2; ++s) x = mfma32<kBf16>(k0.k[s], qf[s], x);
+#pragma unroll
+        for (int s = 0; s < kSteps / 2; ++s) x = mfma32<kBf16>(k1.k[s], qf[kSteps / 2 + s], x);
+      }
+      keys = read_keys<D, 0>(lds, buf, 1, lane);
+      const Seen see = {seen.x - key0 - 8 * half, seen.y - key0 - 8 * half, hidden};
+      x = attend_block<D, kBf16>(lds, buf, 0, buf, 1, x, qf, keys, whole, see, q_sum, lane, sums);
       unpack<D, kBf16>(a, lds, next, key0 + kTileKeys, key_lo, key_hi, codes, staged);
+      __syncthreads();
+      keys = read_keys<D, 0>(lds, next, 0, lane);
       fetch<D>(a, head, key0 + 2 * kTileKeys + at, page, staged);
       page = page_of(a, table, key0 + 3 * kTileKeys + at);
-      __syncthreads();
-      see = {see.lo - 32, see.hi - 32, (uint32_t)(live >> 32) >> (8 * half)};
-      x = probabilities<D, kBf16>(lds, buf, 1, next, 0, x, qf, whole, see, q_sum, lane, sums, pf);
-      add_values<D, kBf16>(lds, buf, 1, pf, lane, sums);
+      x = attend_block<D, kBf16>(lds, buf, 1, next, 0, x, qf, keys, whole,
+                                        {see.lo - 32, see.hi - 32, hidden}, q_sum, lane, sums);
     } else {
       unpack<D, kBf16>(a, lds, next, key0 + kTileKeys, key_lo, key_hi, codes, staged);
       fetch<D>(a, head, key0 + 2 * kTileKeys + at, page, staged);
@@ -926,7 +968,8 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   }
 
   __syncthreads();  // the tiles are done with: LDS is free for the results
-  // Register 4 i + b of block d holds channel 32 d + 8 i + 2 half + {0, 4, 1, 5}[b] of the lane's row.
+  // Register 4 i + b of block d holds channel 8 w + 2 half + {0, 4, 1, 5}[b] of the lane's row, w the
+  // word of chunk 4 d + i.
   if (!active) return;
   const v16f(&o)[kBlocks] = sums.o;
   const float m = sums.m, total = sums.l + __shfl_xor(sums.l, 32);
@@ -940,7 +983,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
       for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float* to = a.part_o + place * D + 32 * d + 8 * i + 2 * half;
+          float* to = a.part_o + place * D + 8 * chunk_word<D>(4 * d + i) + 2 * half;
           *reinterpret_cast<float2*>(to) = {o[d][4 * i], o[d][4 * i + 2]};
           *reinterpret_cast<float2*>(to + 4) = {o[d][4 * i + 1], o[d][4 * i + 3]};
         }
@@ -958,7 +1001,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint8_t* to = rows_lds + n * (2 * D) + 16 * ((4 * d + i) ^ (n & (D / 8 - 1))) + 4 * half;
+      uint8_t* to = rows_lds + n * (2 * D) + 16 * (chunk_word<D>(4 * d + i) ^ (n & (D / 8 - 1))) + 4 * half;
       *reinterpret_cast<uint32_t*>(to) = narrow2<kBf16>(o[d][4 * i] * inv, o[d][4 * i + 2] * inv);
       *reinterpret_cast<uint32_t*>(to + 8) =
           narrow2<kBf16>(o[d][4 * i + 1] * inv, o[d][4 * i + 3] * inv);
