@@ -1148,7 +1148,7 @@ size_t h3_kv4_workspace_bytes(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg*
   if (check_kv4_attention("kv4_workspace_bytes", cfg, attention, batch, q_rows, max_q)) return 0;
   ok();
   return kv4_workspace_bytes(*cfg, *attention, q_rows,
-                             kv4_plan(*cfg, *attention, batch, max_q, device_cus()));
+                             kv4_plan(*cfg, *attention, batch, q_rows, max_q, device_cus()));
 }
 
 int h3_attention_kv4(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attention, uint32_t batch,
@@ -1161,7 +1161,7 @@ int h3_attention_kv4(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attentio
   const uint32_t width = attention->heads * cfg->head_dim;
   const size_t ws = workspace.ptr
                         ? kv4_workspace_bytes(*cfg, *attention, q_rows,
-                                              kv4_plan(*cfg, *attention, batch, max_q, device_cus()))
+                                              kv4_plan(*cfg, *attention, batch, q_rows, max_q, device_cus()))
                         : 0;
   h3_view views[8] = {q, cache, table, lengths, q_starts, out, lse, workspace};
   size_t need[8] = {kv4_rows_bytes(q_rows, attention->q_stride, width), kv4_cache_bytes(*cfg),

@@ -16,6 +16,7 @@
 // A query row is one (token, query head) pair; the G = heads / kv_heads heads of one cache head
 // are rows of the same matrix, row = token * G + g, so that a key is read once for all of them.
 #include <algorithm>
+#include <cmath>
 
 #include "internal.hpp"
 
@@ -232,15 +233,42 @@ __device__ __forceinline__ void load_step(const Args& a, int ids, uint32_t head,
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4s lds_v4s;
 
-// Maximum or sum over the lanes that hold the same rows: the 16 of a group, and the groups whose
-// 4 h % R is the same.
+// Maximum or sum over 16, 32 or 64 lanes, on the vector pipe: quad_perm [1,0,3,2] and [2,3,0,1],
+// row_half_mirror, row_mirror, then the swaps of 16 and of 32 lanes.
+template <bool kMax>
+__device__ __forceinline__ float both(float x, float y) {
+  return kMax ? fmaxf(x, y) : x + y;
+}
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kCtrl, 0xF, 0xF, true));
+}
+template <bool kMax>
+__device__ __forceinline__ float over16(float v) {
+  v = both<kMax>(v, dpp<0xB1>(v));
+  v = both<kMax>(v, dpp<0x4E>(v));
+  v = both<kMax>(v, dpp<0x141>(v));
+  return both<kMax>(v, dpp<0x140>(v));
+}
+template <bool kMax>
+__device__ __forceinline__ float across16(float v) {  // with lane ^ 16
+  const auto r =
+      __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return both<kMax>(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <bool kMax>
+__device__ __forceinline__ float across32(float v) {  // with lane ^ 32
+  const auto r =
+      __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return both<kMax>(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// Over the lanes that hold the same rows: the 16 of a group, and the groups whose 4 h % R is the same.
 template <int R, bool kMax>
 __device__ __forceinline__ float row_lanes(float v) {
-  auto op = [](float x, float y) { return kMax ? fmaxf(x, y) : x + y; };
-#pragma unroll
-  for (int x = 1; x <= 8; x <<= 1) v = op(v, __shfl_xor(v, x));
-  if constexpr (R == 4) v = op(v, __shfl_xor(v, 16));
-  if constexpr (R <= 8) v = op(v, __shfl_xor(v, 32));
+  v = over16<kMax>(v);
+  if constexpr (R == 4) v = across16<kMax>(v);
+  if constexpr (R <= 8) v = across32<kMax>(v);
   return v;
 }
 
@@ -255,27 +283,31 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, h = lane >> 4;
   const uint32_t head = blockIdx.y, b = blockIdx.z, part = blockIdx.x;
+  const int32_t* table = a.table + (size_t)b * a.table_stride;
+  // Step `part` * 4 + wave of the sequence and every 4 * parts-th after it. Without a window the first
+  // is known before the sequence is, and its loads go ahead: where the sequence ends before it, they
+  // read what the table holds, and nothing comes of them.
   const Sequence seq = sequence(a, b);
-  const int group = (int)a.group, rows = seq.rows * group;
+  const int group = (int)a.group, rows = seq.rows * group, stride = (int)a.parts * kWaves;
+  int step = (int)part * kWaves + wave;
+  if (a.window) step += span(a, seq, 0).x / kStepKeys;
+  int ids = page_of(a, table, step * kStepKeys + lane);
+  Step<D, R> next;
+  load_step<D, R>(a, ids, head, step * kStepKeys, n, h, next);
+  ids = page_of(a, table, (step + stride) * kStepKeys + lane);
   if (rows == 0 || !takes(a, rows)) return;
   const int2 first_span = span(a, seq, 0), last_span = span(a, seq, (rows - 1) / group);
   const int key_lo = first_span.x, key_hi = last_span.y;  // seen by some row
   const int all_lo = last_span.x, all_hi = first_span.y;  // seen by every row
-  const Steps st = steps(key_lo, key_hi, a.parts, part, kStepKeys);
+  const int last = (key_hi + kStepKeys - 1) / kStepKeys;
   const uint32_t heads = a.kv_heads * a.group;
-  if (a.parts > 1 && st.first >= st.last && part > 0) {  // no keys: part 0 stands for an empty row
+  if (part > 0 && step - wave >= last) {  // no keys: part 0 stands for an empty row
     if ((int)threadIdx.x < rows) {
       const int token = threadIdx.x / group, g = threadIdx.x - token * group;
       a.part_ml[((size_t)part * a.q_rows + seq.start + token) * heads + head * group + g] = {-kInf, 0};
     }
     return;
   }
-  const int32_t* table = a.table + (size_t)b * a.table_stride;
-  int step = st.first + wave;
-  int ids = page_of(a, table, step * kStepKeys + lane);
-  Step<D, R> next;
-  if (step < st.last) load_step<D, R>(a, ids, head, step * kStepKeys, n, h, next);
-  ids = page_of(a, table, (step + kWaves) * kStepKeys + lane);
 
   // Q operands: channel D/4 h + 8 s + {0,4,1,5,2,6,3,7} in k slot 8 h + 0..7 of step s, the order in
   // which the codes of a word come out in pairs. Rows past the last are zeros.
@@ -302,8 +334,7 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
 #pragma unroll
       for (int u = 0; u < T; ++u) qf[t][u][s] = n / R == u ? x : uint4{0, 0, 0, 0};
     }
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
+    sum = across32<false>(across16<false>(sum));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       q_sum[t][i] = __shfl(sum, (4 * h + i) % R);
@@ -319,13 +350,13 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
   const uint4 one8 = {one2, one2, one2, one2};
   const Codes codes = make_codes<kBf16>();
 
-  for (; step < st.last; step += kWaves) {
+  for (; step < last; step += stride) {
     const Step<D, R> cur = next;
     const int key0 = step * kStepKeys;
-    if (step + kWaves < st.last) {
+    if (step + stride < last) {
       const int now = ids;
-      ids = page_of(a, table, key0 + 2 * kStepKeys * kWaves + lane);
-      load_step<D, R>(a, now, head, key0 + kStepKeys * kWaves, n, h, next);
+      ids = page_of(a, table, key0 + 2 * kStepKeys * stride + lane);
+      load_step<D, R>(a, now, head, key0 + kStepKeys * stride, n, h, next);
     }
     // Scores.
     v4f acc[QT][kTiles];
@@ -404,8 +435,7 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
         float s = vs[0];
 #pragma unroll
         for (int c = 1; c < kTiles; ++c) s = fmaxf(s, vs[c]);
-#pragma unroll
-        for (int w = 32; w >= 1; w >>= 1) s = fmaxf(s, __shfl_xor(s, w));
+        s = across32<true>(across16<true>(over16<true>(s)));
         if (s > s_top) {
           const float up = __uint_as_float((__float_as_uint(s) + 0x7fffffu) & 0x7f800000u);
           ratio = s_top / up;
@@ -830,7 +860,7 @@ __device__ __forceinline__ v16f attend_block(const RowsLds<D>& lds, int buf, int
     float top = y[0];
 #pragma unroll
     for (int i = 1; i < 16; ++i) top = fmaxf(top, y[i]);
-    top = fmaxf(top, __shfl_xor(top, 32)) + (was - kPLog);
+    top = across32<true>(top) + (was - kPLog);
     const float up = fmaxf(r.m, top);
     const float alpha = __builtin_amdgcn_exp2f(r.m - (up == -kInf ? 0.0f : up));
     r.m = up;
@@ -905,7 +935,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
     qf[s] = {(x.x & 0xffffu) | (x.z << 16), (x.x >> 16) | (x.z & 0xffff0000u),
              (x.y & 0xffffu) | (x.w << 16), (x.y >> 16) | (x.w & 0xffff0000u)};
   }
-  const float q_sum = sum + __shfl_xor(sum, 32);
+  const float q_sum = across32<false>(sum);
 
   RowSums<D> sums;
 #pragma unroll
@@ -972,7 +1002,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   // word of chunk 4 d + i.
   if (!active) return;
   const v16f(&o)[kBlocks] = sums.o;
-  const float m = sums.m, total = sums.l + __shfl_xor(sums.l, 32);
+  const float m = sums.m, total = across32<false>(sums.l);
   const bool none = total == 0.0f;
   const size_t q_row = (size_t)(seq.start + token);
   const uint32_t q_head = head * a.group + g;
@@ -1027,6 +1057,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
 // Joins the parts of a row: W waves per (row, query head), wave w the parts w, w + W, ..; lane p of a
 // wave holds part p's weight (kMaxParts lanes at most). A part without keys has no sums to read.
 constexpr uint32_t kMaxParts = 64;
+constexpr uint32_t kFewRows = 32;  // what k_attention_kv4_few holds
 
 template <int D, bool kBf16, int W>
 __global__ __launch_bounds__(kThreads) void k_attention_kv4_join(Args a) {
@@ -1042,13 +1073,9 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_join(Args a) {
   const uint32_t q_head = blockIdx.y * a.group + g;
   const size_t place = q_row * heads + q_head, pitch = (size_t)a.q_rows * heads;
   const float2 ml = lane < (int)a.parts ? a.part_ml[lane * pitch + place] : float2{-kInf, 0.0f};
-  float top = ml.x;
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+  const float top = across32<true>(across16<true>(over16<true>(ml.x)));
   const float f = __builtin_amdgcn_exp2f(ml.x - (top == -kInf ? 0.0f : top));
-  float total = f * ml.y;
-#pragma unroll
-  for (int x = 32; x >= 1; x >>= 1) total += __shfl_xor(total, x);
+  const float total = across32<false>(across16<false>(over16<false>(f * ml.y)));
   // The parts with sums: those with a weight or a NaN.
   uint64_t todo = __ballot(!(ml.y == 0.0f));
   if constexpr (W > 1) {
@@ -1140,32 +1167,67 @@ hipError_t launch_both(const Args& a, uint32_t batch, const Kv4Plan& plan, hipSt
   return e != hipSuccess ? e : launch<D, kBf16>(a, batch, plan.few, stream);
 }
 
-constexpr uint32_t kFewRows = 32;  // what k_attention_kv4_few holds
-
 }  // namespace
 
-// Sequences of up to kFewRows rows are k_attention_kv4_few's, the others k_attention_kv4_rows', a call
-// with both kinds one launch of each (the host knows no sequence's rows, only that none has more than
-// max_q; the workgroups of the other kind leave at once). The keys of a row tile are divided while the
-// chip has room for more workgroups and a part keeps 512 keys.
+// How a call is cut. The host knows no sequence's rows or keys, only that none has more than max_q rows
+// and more keys than the table holds (or a window shows).
+//
+// Which kernel: k_attention_kv4_few up to 32 rows, k_attention_kv4_rows beyond. A call with longer
+// sequences and more than one may hold single tokens too (prompts beside decoding): those go to few,
+// in tiles of the 4, 8, 16 or 32 rows that hold the group's heads, and every other sequence to rows;
+// a launch's workgroups for sequences of the other kind leave at once.
+//
+// Parts: the split of a row tile's keys for which the time estimated from one MI355X's figures is
+// least, in us:
+//   rounds * (start + steps of a workgroup * step) + the join's,
+// few: 6 to start a workgroup and join its waves, 1.2 (4 rows) to 2.7 (32 rows) per 256 keys, which
+// are four waves' step, or what HBM takes for the resident workgroups' bytes where that is more (5.0
+// TB/s, 4.4 with one workgroup a compute unit); rows: 8, and 2.3 per 64 keys. The join is a launch (5 to 6) and writes and reads every
+// part's sums in f32. Timed: 16 groups of 129,024 keys 74, 65 and 68 us in 16, 32 and 64 parts;
+// 128 groups of 32 rows over 4,100 keys 52, 37, 49 and 66 us in 1, 2, 4 and 8; 512 groups of up to
+// 8,192 keys 82, 85, 87 and 98 us; 8 groups of 1,000 keys 10.6, 10.5, 9.4 and 9.0 us, where the second
+// launch costs the host more than the split gains.
 Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
-                 uint32_t max_q, uint32_t cus) {
+                 uint32_t q_rows, uint32_t max_q, uint32_t cus) {
   Kv4Plan p{};
   const uint32_t group = acfg.heads / cfg.kv_heads, rows = max_q * group;
-  const uint64_t most = ((uint64_t)acfg.table_stride * cfg.page_tokens + 511) / 512;
-  auto parts = [&](uint32_t row_tiles, uint32_t resident) {
-    const uint64_t groups = (uint64_t)batch * cfg.kv_heads * row_tiles;
-    const uint64_t room = ((uint64_t)resident * cus + groups - 1) / groups;
-    return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({room, most, kMaxParts}));
+  uint64_t keys = (uint64_t)acfg.table_stride * cfg.page_tokens;
+  if (acfg.window) keys = std::min<uint64_t>(keys, (uint64_t)acfg.window + max_q);
+  const double key_bytes = cfg.head_dim + 8;
+  auto parts = [&](uint64_t groups, uint32_t resident, double start, double step, uint32_t step_keys,
+                   double joined) {
+    uint32_t best = 1;
+    double least = 0;
+    const uint64_t steps = (keys + step_keys - 1) / step_keys;
+    for (uint32_t n = 1; n <= kMaxParts && (n == 1 || n <= steps); ++n) {
+      const double wgs = (double)groups * n, slots = (double)resident * cus;
+      const double each = std::ceil(std::min(wgs, slots) / cus);  // on the fullest compute units
+      const double share = each > 1 ? each * cus : wgs;
+      const double hbm = share * step_keys * key_bytes / (each > 1 ? 5.0e6 : 4.4e6);
+      const double time = std::ceil(wgs / slots) *
+                              (start + (double)((steps + n - 1) / n) * std::max(step, hbm)) +
+                          (n > 1 ? 5 + n * joined * (cfg.head_dim + 2) * 8 / 4e6 : 0);
+      if (n == 1 || time < least) {
+        best = n;
+        least = time;
+      }
+    }
+    return best;
   };
+  uint32_t few = rows;  // rows of the longest sequence that few takes
   if (rows > kFewRows) {
-    p.many = {256, (rows + 255) / 256, 1, kFewRows + 1, rows};
-    p.many.parts = parts(p.many.row_tiles, 1);
+    few = batch > 1 && group <= kFewRows ? group : 0;
+    const uint32_t tiles = (rows + 255) / 256;
+    p.many = {256, tiles, 1, few + 1, rows};
+    const uint64_t total = std::min<uint64_t>((uint64_t)batch * tiles, (uint64_t)q_rows * group / 256 + batch);
+    p.many.parts = parts(total * cfg.kv_heads, 1, 8, 2.3, 64, (double)q_rows * acfg.heads);
   }
-  if (rows <= kFewRows || batch > 1) {
-    const uint32_t few = std::min(rows, kFewRows);
-    p.few = {few <= 4 ? 4u : few <= 8 ? 8u : few <= 16 ? 16u : 32u, 1, 1, 0, few};
-    p.few.parts = parts(1, 4);
+  if (few) {
+    const uint32_t tile = few <= 4 ? 4 : few <= 8 ? 8 : few <= 16 ? 16 : 32;
+    p.few = {tile, 1, 1, 0, few};
+    p.few.parts = parts((uint64_t)batch * cfg.kv_heads, tile == 32 ? 1 : 2, 6,
+                        tile <= 4 ? 1.2 : tile <= 8 ? 1.3 : tile <= 16 ? 1.8 : 2.7, 256,
+                        (double)batch * few * cfg.kv_heads);
   }
   return p;
 }
@@ -1182,7 +1244,7 @@ hipError_t launch_attention_kv4(const h3_kv4_cfg& cfg, const h3_kv4_attention_cf
                                 const void* cache, const int32_t* table, const int32_t* lengths,
                                 const int32_t* q_starts, void* out, float* lse, void* workspace,
                                 hipStream_t stream) {
-  Kv4Plan plan = kv4_plan(cfg, acfg, batch, max_q, device_cus());
+  Kv4Plan plan = kv4_plan(cfg, acfg, batch, q_rows, max_q, device_cus());
   if (!workspace) plan.many.parts = plan.few.parts = 1;
   Args a{};
   a.q = q;

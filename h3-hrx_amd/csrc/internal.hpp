@@ -240,7 +240,7 @@ struct Kv4Plan {
   Kv4Launch many, few;
 };
 Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
-                 uint32_t max_q, uint32_t cus);
+                 uint32_t q_rows, uint32_t max_q, uint32_t cus);
 size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t q_rows,
                            const Kv4Plan& plan);
 hipError_t launch_attention_kv4(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
