@@ -50,10 +50,10 @@ FLAGS = [
 
 # Per-file extras. The attention kernel is checked to a tolerance (never bit-exact) and never
 # sees NaN operands, so it may drop the NaN-quieting canonicalisations IEEE mode otherwise adds
-# to every max; infinities stay honoured (masked keys are -inf). The quantizer files keep full
-# IEEE semantics.
+# to every max; infinities stay honoured (masked keys are -inf). kv4.hip finds NaNs by their bits
+# and keeps them out of its arithmetic. The other quantizer files keep full IEEE semantics.
 EXTRA = {name: ["-fno-honor-nans"]
-         for name in ("attention.hip", "attention_hm.hip", "attention_split.hip")}
+         for name in ("attention.hip", "attention_hm.hip", "attention_split.hip", "kv4.hip")}
 
 
 def _compile(src: pathlib.Path, obj: pathlib.Path) -> None:

@@ -7,9 +7,9 @@
 //   u_c = clamp(rne((x_c - m) / s), 0, 15), 0 where s is 0,
 // and stands for m + s u_c. m is one of the row's own values, so it is held exactly; s is rounded
 // toward zero so that m + 15 s never passes max x (rounded to nearest it can overflow f16, and the
-// top code would read back as infinity). The codes come from an IEEE division in f32, which decides
-// every code as exact arithmetic does wherever x - m is exact; bf16 rows are halved for it, which
-// changes no quotient and keeps max - min below f32's largest. A row that holds a NaN or an infinity
+// top code would read back as infinity). The codes come from a division in f32 that decides every code
+// as exact arithmetic does wherever x - m is exact; bf16 rows are halved for it, which changes no
+// quotient and keeps max - min below f32's largest. A row that holds a NaN or an infinity
 // has m = NaN and reads back as NaN throughout.
 //
 // Layout (h3attn.h): one block per (page, cache head): K codes [page_tokens][D/2] bytes, V codes
@@ -37,22 +37,24 @@ struct RowArgs {
   uint64_t slot_limit;  // slots at or past it name no row
 };
 
-// The lane's place: token, head, and its 8 channels' position in the row.
-template <int D>
+// The lane's places: head, the N tokens kApart from each other, and its 8 channels' position in a row.
+template <int D, int N>
 struct Place {
+  static constexpr uint32_t kLanes = D / 8, kApart = 64 / kLanes;
   uint32_t token, head, lane;
-  bool live;
 };
-template <int D>
-__device__ __forceinline__ Place<D> place(const RowArgs& a) {
-  constexpr uint32_t kLanes = D / 8, kRows = 64 / kLanes;
+template <int D, int N>
+__device__ __forceinline__ Place<D, N> place(const RowArgs& a) {
+  using P = Place<D, N>;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  Place<D> p;
-  p.head = blockIdx.y * kWaves + wave;
-  p.token = blockIdx.x * kRows + lane / kLanes;
-  p.lane = lane % kLanes;
-  p.live = p.head < a.heads && p.token < a.tokens;
-  return p;
+  return {blockIdx.x * (N * P::kApart) + lane / P::kLanes, blockIdx.y * kWaves + wave,
+          lane % P::kLanes};
+}
+
+// The slot of row `token`, or -1 if there is no such row or it names none.
+__device__ __forceinline__ int32_t slot_of(const RowArgs& a, uint32_t token) {
+  const int32_t slot = token < a.tokens ? a.slots[token] : -1;
+  return (uint64_t)(uint32_t)slot < a.slot_limit ? slot : -1;
 }
 
 // Byte offsets of a slot's K codes and K word of one head. `half`: the bytes of a page's K codes.
@@ -106,17 +108,30 @@ __device__ __forceinline__ uint32_t narrow_down(float v) {
   return widen<false>(h) > v ? h - 1 : h;
 }
 
-// The row's word and this lane's eight codes, low nibble first.
+// a / b by r, the reciprocal of b to an ulp or so: q = a r, then q + (a - q b) r. The remainder is exact
+// (b is a short number, or a quotient near a whole one), so the error before the last rounding is some
+// 2^-45 of the quotient: every quotient that 24 bits hold comes out exactly, the borders k + 1/2 of
+// the codes and the values of the element type among them.
+__device__ __forceinline__ float quotient(float a, float b, float r) {
+  const float q = a * r;
+  return fmaf(fmaf(-q, b, a), r, q);
+}
+
+// The row's word and this lane's eight codes, low nibble first. Few vector instructions a channel are
+// what keeps the kernel near HBM's rate: a correctly rounded division by the step for every channel made
+// it 1.8 times as long.
 template <int D, bool kBf16>
 __device__ __forceinline__ uint2 quantize(uint4 raw) {
+  typedef uint16_t v2us __attribute__((ext_vector_type(2)));
+  constexpr uint32_t kTop = kBf16 ? 0x7f80u : 0x7c00u;  // magnitudes from here on are no numbers
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   float x[8];
-  bool bad = false;
+  v2us top = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t h = (w[i / 2] >> (16 * (i & 1))) & 0xffffu;
-    x[i] = widen<kBf16>(h);
-    bad |= (h & 0x7fffu) >= (kBf16 ? 0x7f80u : 0x7c00u);
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = widen<kBf16>(w[i] & 0xffffu);
+    x[2 * i + 1] = kBf16 ? __uint_as_float(w[i] & 0xffff0000u) : widen<kBf16>(w[i] >> 16);
+    top = __builtin_elementwise_max(top, __builtin_bit_cast(v2us, w[i] & 0x7fff7fffu));
   }
   float lo = x[0], hi = x[0];
 #pragma unroll
@@ -124,51 +139,70 @@ __device__ __forceinline__ uint2 quantize(uint4 raw) {
     lo = fminf(lo, x[i]);
     hi = fmaxf(hi, x[i]);
   }
+  // A lane with a NaN or an infinity makes the row's maximum infinite, whatever its others are.
+  if (top[0] >= kTop || top[1] >= kTop) hi = __builtin_inff();
   lo = row_reduce<D, false>(lo);
   hi = row_reduce<D, true>(hi);
-  if (row_reduce<D, true>(bad ? 1.0f : 0.0f) > 0.0f) return {0x7fffu, 0u};
-  constexpr float kPart = kBf16 ? 0.5f : 1.0f;  // exact on every bf16 value, subnormal ones too
-  const float low = lo * kPart;
-  const uint32_t s = narrow_down<kBf16>((hi * kPart - low) / (15.0f * kPart));
-  const float step = widen<kBf16>(s) * kPart;
+  if (__float_as_uint(hi) == 0x7f800000u) return {0x7fffu, 0u};
+  float part = kBf16 ? 0.5f : 1.0f;  // exact on every bf16 value, subnormal ones too
+  const uint32_t s = narrow_down<kBf16>(
+      quotient(hi * part - lo * part, 15.0f * part, (1.0f / 15.0f) / (kBf16 ? 0.5f : 1.0f)));
+  if (kBf16 && widen<kBf16>(s) < 0x1p-60f) part = 0x1p99f;  // the reciprocal stays finite
+  const float low = lo * part, step = widen<kBf16>(s) * part;
   uint32_t codes = 0;
   if (step > 0.0f) {
+    const float r = __builtin_amdgcn_rcpf(step);
+    float u[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float u = fminf(rintf((x[i] * kPart - low) / step), 15.0f);
-      codes |= (uint32_t)u << (4 * i);
-    }
+    for (int i = 0; i < 8; ++i)
+      u[i] = fminf(rintf(quotient(fmaf(x[i], part, -low), step, r)), 15.0f);
+    // Four codes a whole number of 16 bits, exact in f32.
+    const float first = fmaf(fmaf(fmaf(u[3], 16.0f, u[2]), 16.0f, u[1]), 16.0f, u[0]);
+    const float second = fmaf(fmaf(fmaf(u[7], 16.0f, u[6]), 16.0f, u[5]), 16.0f, u[4]);
+    codes = (uint32_t)first | ((uint32_t)second << 16);
   }
   return {narrow<kBf16>(lo) | (s << 16), codes};
 }
 
 // Quantizes rows [tokens][heads][D] of K and V into their slots.
-template <int D, bool kBf16>
+template <int D, bool kBf16, int N>
 __global__ __launch_bounds__(kThreads) void k_kv4_write(RowArgs a) {
-  const Place<D> p = place<D>(a);
-  if (!p.live) return;  // whole rows leave: a row's lanes share token and head
-  const int32_t slot = a.slots[p.token];
-  if (slot < 0 || (uint64_t)slot >= a.slot_limit) return;
+  const Place<D, N> p = place<D, N>(a);
+  if (p.head >= a.heads) return;
   const uint32_t col = p.head * D + 8 * p.lane;
-  const uint4 k = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.k) +
-                                                  (size_t)p.token * a.k_stride + col);
-  const uint4 v = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.v) +
-                                                  (size_t)p.token * a.v_stride + col);
-  const Slot<D> at = slot_at<D>(a, slot, p.head);
-  const uint2 qk = quantize<D, kBf16>(k), qv = quantize<D, kBf16>(v);
-  uint8_t* codes = a.cache + at.codes + 4 * p.lane;
-  *reinterpret_cast<uint32_t*>(codes) = qk.y;
-  *reinterpret_cast<uint32_t*>(codes + at.half) = qv.y;
-  if (p.lane == 0) {
-    uint8_t* words = a.cache + at.words;
-    *reinterpret_cast<uint32_t*>(words) = qk.x;
-    *reinterpret_cast<uint32_t*>(words + 4 * at.tokens) = qv.x;
+  int32_t slot[N];
+  uint4 k[N], v[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t token = p.token + i * p.kApart;
+    slot[i] = slot_of(a, token);
+    // The last row stands for the rows past it: their loads need no branch.
+    const size_t row = min(token, a.tokens - 1);
+    k[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.k) + row * a.k_stride + col);
+    v[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.v) + row * a.v_stride + col);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint2 qk = quantize<D, kBf16>(k[i]), qv = quantize<D, kBf16>(v[i]);
+    if (slot[i] < 0) continue;
+    const Slot<D> at = slot_at<D>(a, slot[i], p.head);
+    uint8_t* codes = a.cache + at.codes + 4 * p.lane;
+    *reinterpret_cast<uint32_t*>(codes) = qk.y;
+    *reinterpret_cast<uint32_t*>(codes + at.half) = qv.y;
+    if (p.lane == 0) {
+      uint8_t* words = a.cache + at.words;
+      *reinterpret_cast<uint32_t*>(words) = qk.x;
+      *reinterpret_cast<uint32_t*>(words + 4 * at.tokens) = qv.x;
+    }
   }
 }
 
-// Eight channels m + s u, rounded to the element type.
+// Eight channels m + s u, rounded to the element type. (NaN by its bits: this file is compiled to
+// assume none in its arithmetic.)
 template <bool kBf16>
 __device__ __forceinline__ uint4 dequantize(uint32_t codes, uint32_t word) {
+  constexpr uint32_t kTop = kBf16 ? 0x7f80u : 0x7c00u;
+  if ((word & kTop) == kTop) return {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
   const float m = widen<kBf16>(word & 0xffffu), s = widen<kBf16>(word >> 16);
   uint32_t out[4];
 #pragma unroll
@@ -181,36 +215,57 @@ __device__ __forceinline__ uint4 dequantize(uint32_t codes, uint32_t word) {
 }
 
 // Reads rows of K and V back from their slots; a slot that names no row gives zeros.
-template <int D, bool kBf16>
+template <int D, bool kBf16, int N>
 __global__ __launch_bounds__(kThreads) void k_kv4_read(RowArgs a) {
-  const Place<D> p = place<D>(a);
-  if (!p.live) return;
-  const int32_t slot = a.slots[p.token];
-  uint4 k = {0, 0, 0, 0}, v = k;
-  if (slot >= 0 && (uint64_t)slot < a.slot_limit) {
-    const Slot<D> at = slot_at<D>(a, slot, p.head);
+  const Place<D, N> p = place<D, N>(a);
+  if (p.head >= a.heads) return;
+  const uint32_t col = p.head * D + 8 * p.lane;
+  int32_t slot[N];
+  uint32_t ck[N], cv[N], wk[N], wv[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) slot[i] = slot_of(a, p.token + i * p.kApart);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const Slot<D> at = slot_at<D>(a, max(slot[i], 0), p.head);  // slot 0 is there to read
     const uint8_t* codes = a.cache + at.codes + 4 * p.lane;
     const uint8_t* words = a.cache + at.words;
-    const uint32_t ck = *reinterpret_cast<const uint32_t*>(codes);
-    const uint32_t cv = *reinterpret_cast<const uint32_t*>(codes + at.half);
-    k = dequantize<kBf16>(ck, *reinterpret_cast<const uint32_t*>(words));
-    v = dequantize<kBf16>(cv, *reinterpret_cast<const uint32_t*>(words + 4 * at.tokens));
+    ck[i] = *reinterpret_cast<const uint32_t*>(codes);
+    cv[i] = *reinterpret_cast<const uint32_t*>(codes + at.half);
+    wk[i] = *reinterpret_cast<const uint32_t*>(words);
+    wv[i] = *reinterpret_cast<const uint32_t*>(words + 4 * at.tokens);
   }
-  const uint32_t col = p.head * D + 8 * p.lane;
-  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(a.k)) +
-                            (size_t)p.token * a.k_stride + col) = k;
-  *reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(a.v)) +
-                            (size_t)p.token * a.v_stride + col) = v;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t token = p.token + i * p.kApart;
+    if (token >= a.tokens) continue;
+    const bool live = slot[i] >= 0;
+    const uint4 k = dequantize<kBf16>(live ? ck[i] : 0u, live ? wk[i] : 0u);
+    const uint4 v = dequantize<kBf16>(live ? cv[i] : 0u, live ? wv[i] : 0u);
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(a.k)) +
+                              (size_t)token * a.k_stride + col) = k;
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(a.v)) +
+                              (size_t)token * a.v_stride + col) = v;
+  }
 }
 
-template <int D, bool kBf16>
+template <int D, bool kBf16, int N>
 hipError_t launch(const RowArgs& a, bool write, hipStream_t stream) {
-  const dim3 grid((a.tokens + 512 / D - 1) / (512 / D), (a.heads + kWaves - 1) / kWaves);
+  constexpr uint32_t kTokens = N * Place<D, N>::kApart;
+  const dim3 grid((a.tokens + kTokens - 1) / kTokens, (a.heads + kWaves - 1) / kWaves);
   if (write)
-    hipLaunchKernelGGL((k_kv4_write<D, kBf16>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_kv4_write<D, kBf16, N>), grid, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((k_kv4_read<D, kBf16>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_kv4_read<D, kBf16, N>), grid, dim3(kThreads), 0, stream, a);
   return hipGetLastError();
+}
+
+// Four rows a lane where that still leaves every compute unit workgroups to choose from (more loads in
+// flight, and a head's parameters of 16 tokens in one line from one wave), one row where it does not.
+template <int D, bool kBf16>
+hipError_t launch_n(const RowArgs& a, bool write, hipStream_t stream) {
+  const uint64_t wgs = (uint64_t)a.tokens * D / 2048 * ((a.heads + kWaves - 1) / kWaves);
+  return wgs >= 4ull * device_cus() ? launch<D, kBf16, 4>(a, write, stream)
+                                    : launch<D, kBf16, 1>(a, write, stream);
 }
 
 hipError_t rows(const h3_kv4_cfg& cfg, uint32_t tokens, uint32_t k_stride, uint32_t v_stride,
@@ -229,8 +284,8 @@ hipError_t rows(const h3_kv4_cfg& cfg, uint32_t tokens, uint32_t k_stride, uint3
   a.slot_limit = (uint64_t)cfg.pages * cfg.page_tokens;
   const bool bf16 = cfg.elem == H3_ELEM_BF16;
   if (cfg.head_dim == 128)
-    return bf16 ? launch<128, true>(a, write, stream) : launch<128, false>(a, write, stream);
-  return bf16 ? launch<64, true>(a, write, stream) : launch<64, false>(a, write, stream);
+    return bf16 ? launch_n<128, true>(a, write, stream) : launch_n<128, false>(a, write, stream);
+  return bf16 ? launch_n<64, true>(a, write, stream) : launch_n<64, false>(a, write, stream);
 }
 
 }  // namespace
