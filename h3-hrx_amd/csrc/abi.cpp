@@ -1147,7 +1147,7 @@ size_t h3_kv4_workspace_bytes(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg*
                               uint32_t batch, uint32_t q_rows, uint32_t max_q) {
   if (check_kv4_attention("kv4_workspace_bytes", cfg, attention, batch, q_rows, max_q)) return 0;
   ok();
-  return kv4_workspace_bytes(*cfg, *attention, q_rows,
+  return kv4_workspace_bytes(*cfg, batch,
                              kv4_plan(*cfg, *attention, batch, q_rows, max_q, device_cus()));
 }
 
@@ -1160,7 +1160,7 @@ int h3_attention_kv4(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attentio
   if (st) return st;
   const uint32_t width = attention->heads * cfg->head_dim;
   const size_t ws = workspace.ptr
-                        ? kv4_workspace_bytes(*cfg, *attention, q_rows,
+                        ? kv4_workspace_bytes(*cfg, batch,
                                               kv4_plan(*cfg, *attention, batch, q_rows, max_q, device_cus()))
                         : 0;
   h3_view views[8] = {q, cache, table, lengths, q_starts, out, lse, workspace};

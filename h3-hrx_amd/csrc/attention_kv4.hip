@@ -41,10 +41,11 @@ struct Args {
   float* lse;  // null: not wanted
   float* part_o;
   float2* part_ml;
+  struct Line* line;
   uint32_t kv_heads, group, q_stride, out_stride, table_stride;
   uint32_t pages, page_shift;
-  uint32_t q_rows, max_q;
-  uint32_t parts, row_tiles;
+  uint32_t batch, q_rows, max_q;
+  uint32_t parts, row_tiles;    // row_tiles: a sequence's at most; of a line, all sequences'
   uint32_t rows_from, rows_to;  // the sequences a launch takes: those of rows_from .. rows_to rows
   uint32_t causal, window;
   float scale;  // the softmax scale times log2(e)
@@ -79,16 +80,10 @@ __device__ __forceinline__ int2 span(const Args& a, const Sequence& s, int i) {
   return {min(lo, hi), hi};
 }
 
-// The steps of `keys` keys that a tile of rows takes, and the ones of them part `part` takes.
+// Steps first .. last - 1 of a row's keys.
 struct Steps {
   int first, last;
 };
-__device__ __forceinline__ Steps steps(int lo, int hi, uint32_t parts, uint32_t part, int keys) {
-  const int t0 = lo / keys, t1 = (hi + keys - 1) / keys;
-  const int n = max(t1 - t0, 0);
-  const int per = (n + (int)parts - 1) / (int)parts;
-  return {t0 + min((int)part * per, n), t0 + min(((int)part + 1) * per, n)};
-}
 
 template <bool kBf16>
 __device__ __forceinline__ float widen(uint32_t bits) {
@@ -272,6 +267,12 @@ __device__ __forceinline__ float row_lanes(float v) {
   return v;
 }
 
+// Where part `part` of a row's keys leaves its sums: row `row` (of at most rows_to) of sequence b.
+__device__ __forceinline__ size_t few_place(const Args& a, uint32_t part, uint32_t b, uint32_t row,
+                                            uint32_t head) {
+  return (((size_t)part * a.batch + b) * a.rows_to + row) * a.kv_heads + head;
+}
+
 template <int D, bool kBf16, int R, int QT>
 __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few(Args a) {
   static_assert(QT == 1 || R == 16, "row tiles of 16");
@@ -302,10 +303,7 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
   const int last = (key_hi + kStepKeys - 1) / kStepKeys;
   const uint32_t heads = a.kv_heads * a.group;
   if (part > 0 && step - wave >= last) {  // no keys: part 0 stands for an empty row
-    if ((int)threadIdx.x < rows) {
-      const int token = threadIdx.x / group, g = threadIdx.x - token * group;
-      a.part_ml[((size_t)part * a.q_rows + seq.start + token) * heads + head * group + g] = {-kInf, 0};
-    }
+    if ((int)threadIdx.x < rows) a.part_ml[few_place(a, part, b, threadIdx.x, head)] = {-kInf, 0};
     return;
   }
 
@@ -587,7 +585,7 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
       const size_t q_row = (size_t)(seq.start + token);
       const uint32_t q_head = head * group + g;
       if (a.parts > 1) {
-        const size_t place = ((size_t)part * a.q_rows + q_row) * heads + q_head;
+        const size_t place = few_place(a, part, b, row, head);
 #pragma unroll
         for (int d = 0; d < kPer; ++d) a.part_o[place * D + ch + d] = sum[d];
         if (ch == 0) a.part_ml[place] = {top, total};
@@ -611,7 +609,7 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
 // operands of the PV product's two steps, as they are. V stays token-major and its operand comes
 // through the transposed LDS read.
 constexpr int kRowsThreads = 512;
-constexpr int kTileKeys = 64;
+constexpr int kTileRows = 256, kTileKeys = 64;
 constexpr float kPTop = 32768.0f;  // a lane's probabilities of 32 keys sum to no more, or m is raised
 constexpr float kPLog = 7.0f;      // the largest score gives p = 2^7: f16 stays normal to 2^-21 of it
 
@@ -889,24 +887,17 @@ __device__ __forceinline__ v16f attend_block(const RowsLds<D>& lds, int buf, int
   return next;
 }
 
+// Steps st (tiles of keys) of rows row0 .. row0 + 255 of sequence b for one cache head. Results go to out
+// and lse, or (slot >= 0) as sums relative to m to that slot of the workspace.
 template <int D, bool kBf16>
-__global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) {
-  constexpr int kRows = 256, kSteps = D / 16, kBlocks = D / 32;
-  __shared__ __attribute__((aligned(16))) RowsLds<D> lds;
+__device__ __forceinline__ void attend_rows(const Args& a, RowsLds<D>& lds, const Sequence& seq,
+                                            uint32_t b, uint32_t head, int row0, Steps st, int slot) {
+  constexpr int kSteps = D / 16, kBlocks = D / 32;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, half = lane >> 5;
-  const uint32_t head = blockIdx.x, b = blockIdx.z;
-  const uint32_t part = blockIdx.y % a.parts;
-  const Sequence seq = sequence(a, b);
-  const int rows = seq.rows * (int)a.group;
-  // The last rows see the most keys: they start first.
-  const int row0 = (int)(a.row_tiles - 1 - blockIdx.y / a.parts) * kRows;
-  if (row0 >= rows || !takes(a, rows)) return;
-  const int group = (int)a.group;
-  const int2 first_span = span(a, seq, row0 / group);
-  const int2 last_span = span(a, seq, (min(row0 + kRows, rows) - 1) / group);
-  const int key_lo = first_span.x, key_hi = last_span.y;
-  const Steps st = steps(key_lo, key_hi, a.parts, part, kTileKeys);
+  const int group = (int)a.group, rows = seq.rows * group;
+  const int key_lo = span(a, seq, row0 / group).x;
+  const int key_hi = span(a, seq, (min(row0 + kTileRows, rows) - 1) / group).y;
   const uint32_t heads = a.kv_heads * a.group;
 
   // The wave's rows, the keys that some and that all of them see, and the tiles it takes.
@@ -1000,15 +991,14 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   __syncthreads();  // the tiles are done with: LDS is free for the results
   // Register 4 i + b of block d holds channel 8 w + 2 half + {0, 4, 1, 5}[b] of the lane's row, w the
   // word of chunk 4 d + i.
-  if (!active) return;
   const v16f(&o)[kBlocks] = sums.o;
   const float m = sums.m, total = across32<false>(sums.l);
   const bool none = total == 0.0f;
   const size_t q_row = (size_t)(seq.start + token);
   const uint32_t q_head = head * a.group + g;
-  if (a.parts > 1) {
+  if (slot >= 0) {
     if (row < rows) {
-      const size_t place = ((size_t)part * a.q_rows + q_row) * heads + q_head;
+      const size_t place = (size_t)slot * kTileRows + (row - row0);
 #pragma unroll
       for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
@@ -1021,6 +1011,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
     }
     return;
   }
+  if (!active) return;
   const float inv = none ? 0.0f : 1.0f / total;
   // Through LDS (each wave its own 32 rows) so that whole rows leave together.
   uint8_t* rows_lds = reinterpret_cast<uint8_t*>(&lds) + wave * 32 * 2 * D;
@@ -1054,24 +1045,214 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
     a.lse[q_row * heads + q_head] = none ? -kInf : (m + __log2f(total)) * kLn2;
 }
 
+// One wave's joined row: D/64 channels a lane.
+template <int D, bool kBf16>
+__device__ __forceinline__ void write_row(const Args& a, size_t q_row, uint32_t q_head, int lane,
+                                          float m, float l, const float (&sum)[D / 64]) {
+  const bool none = l == 0.0f;
+  const float inv = none ? 0.0f : 1.0f / l;
+  uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + lane * (D / 64);
+  if constexpr (D == 128)
+    *reinterpret_cast<uint32_t*>(out) = narrow2<kBf16>(sum[0] * inv, sum[1] * inv);
+  else
+    *out = (uint16_t)narrow<kBf16>(sum[0] * inv);
+  if (a.lse && lane == 0)
+    a.lse[q_row * (a.kv_heads * a.group) + q_head] = none ? -kInf : (m + __log2f(l)) * kLn2;
+}
+
+// The tiles of keys that the rows from row0 on see.
+__device__ __forceinline__ Steps row_steps(const Args& a, const Sequence& seq, int row0) {
+  const int group = (int)a.group, rows = seq.rows * group;
+  const int lo = span(a, seq, row0 / group).x;
+  const int hi = span(a, seq, (min(row0 + kTileRows, rows) - 1) / group).y;
+  return {lo / kTileKeys, max((hi + kTileKeys - 1) / kTileKeys, lo / kTileKeys)};
+}
+
+template <int D, bool kBf16>
+__global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) {
+  __shared__ __attribute__((aligned(16))) RowsLds<D> lds;
+  const Sequence seq = sequence(a, blockIdx.z);
+  const int rows = seq.rows * (int)a.group;
+  // The last rows see the most keys: they start first.
+  const int row0 = (int)(a.row_tiles - 1 - blockIdx.y) * kTileRows;
+  if (row0 >= rows || !takes(a, rows)) return;
+  attend_rows<D, kBf16>(a, lds, seq, blockIdx.z, blockIdx.x, row0, row_steps(a, seq, row0), -1);
+}
+
+// The same row tiles where they would leave the chip partly idle: the tiles of keys of all of them (of
+// every cache head) are one line, of which each workgroup takes an equal range. A range that holds a
+// row tile's keys whole finishes it; one that ends or begins inside leaves its sums in the workspace,
+// in slot 2 w if it is workgroup w's first and 2 w + 1 if its last, for k_attention_kv4_rows_join. Every
+// workgroup finds the line from the sequences by itself (at most kLineTiles row tiles and sequences;
+// rows that q_starts counts twice may have none), and the first leaves it in the workspace for the join.
+constexpr int kLineTiles = 512;  // one per thread
+constexpr int kLeastSteps = 8;   // of a range: a shorter one is mostly start and join
+
+struct Line {
+  int tiles, steps, range;  // row tiles, their steps (of one head), a workgroup's steps
+  int unused;
+  int b[kLineTiles], row0[kLineTiles], first[kLineTiles];
+  int end[kLineTiles];  // of a row tile's steps in the line of one head
+};
+
+// The sum of v over the threads up to this one, of kRowsThreads. `scratch`: eight ints.
+__device__ __forceinline__ int sum_to_here(int v, int* scratch) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int x = __shfl_up(v, d);
+    if (lane >= d) v += x;
+  }
+  if (lane == 63) scratch[wave] = v;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) v += scratch[w];
+  __syncthreads();
+  return v;
+}
+
+__device__ __forceinline__ void make_line(const Args& a, Line& line, int* scratch) {
+  const int t = (int)threadIdx.x;
+  int tiles = 0;
+  if (t < (int)a.batch) {
+    const int rows = sequence(a, t).rows * (int)a.group;
+    if (takes(a, rows)) tiles = (rows + kTileRows - 1) / kTileRows;
+  }
+  const int after = sum_to_here(tiles, scratch);
+  for (int i = 0, at = after - tiles; i < tiles && at < (int)a.row_tiles; ++i, ++at) {
+    line.b[at] = t;
+    line.row0[at] = i * kTileRows;
+  }
+  if (t == kRowsThreads - 1) line.tiles = min(after, (int)a.row_tiles);
+  __syncthreads();
+  int count = 0;
+  if (t < line.tiles) {
+    const Steps st = row_steps(a, sequence(a, line.b[t]), line.row0[t]);
+    line.first[t] = st.first;
+    count = max(st.last - st.first, 1);  // a tile that sees no key still has its rows to write
+  }
+  const int end = sum_to_here(count, scratch);
+  if (t < kLineTiles) line.end[t] = end;
+  if (t == kRowsThreads - 1) {
+    line.steps = end;
+    const int all = end * (int)a.kv_heads;
+    line.range = max((all + (int)gridDim.x - 1) / (int)gridDim.x, kLeastSteps);
+  }
+  __syncthreads();
+}
+
+template <int D, bool kBf16>
+__global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_line(Args a) {
+  __shared__ __attribute__((aligned(16))) RowsLds<D> lds;
+  __shared__ Line line;
+  __shared__ int scratch[8];
+  make_line(a, line, scratch);
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < (int)(sizeof(Line) / 4); i += kRowsThreads)
+      reinterpret_cast<int*>(a.line)[i] = reinterpret_cast<const int*>(&line)[i];
+  const int steps = __builtin_amdgcn_readfirstlane(line.steps);
+  const int range = __builtin_amdgcn_readfirstlane(line.range);
+  const int begin = (int)blockIdx.x * range, stop = min(begin + range, steps * (int)a.kv_heads);
+  for (int at = begin; at < stop;) {
+    const int head = at / steps, off = at - head * steps;
+    int lo = 0, hi = line.tiles - 1;  // the first row tile that ends past off
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (line.end[mid] > off) hi = mid; else lo = mid + 1;
+    }
+    const int tile = __builtin_amdgcn_readfirstlane(lo);
+    const int start = __builtin_amdgcn_readfirstlane(tile ? line.end[tile - 1] : 0);
+    const int count = __builtin_amdgcn_readfirstlane(line.end[tile]) - start;
+    const int first = __builtin_amdgcn_readfirstlane(line.first[tile]);
+    const int b = __builtin_amdgcn_readfirstlane(line.b[tile]);
+    const int row0 = __builtin_amdgcn_readfirstlane(line.row0[tile]);
+    const int s0 = off - start, s1 = min(count, s0 + stop - at);
+    const int slot = s1 - s0 == count ? -1 : 2 * (int)blockIdx.x + (at == begin ? 0 : 1);
+    attend_rows<D, kBf16>(a, lds, sequence(a, b), b, head, row0, {first + s0, first + s1}, slot);
+    __syncthreads();  // LDS is free again
+    at += s1 - s0;
+  }
+}
+
+// Joins the ranges of the row tiles that more than one workgroup took: W waves per row, wave w the ranges
+// w, w + W, ..
+template <int D, bool kBf16, int W>
+__global__ __launch_bounds__(kThreads) void k_attention_kv4_rows_join(Args a) {
+  constexpr int kPer = D / 64, kTileGroups = kTileRows * W / kWaves;
+  __shared__ float lds_sum[W][D];
+  __shared__ float2 lds_ml[W];
+  const Line& line = *a.line;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tile = blockIdx.x / kTileGroups;
+  if (tile >= line.tiles) return;
+  const int start = (int)blockIdx.y * line.steps + (tile ? line.end[tile - 1] : 0);
+  const int end = (int)blockIdx.y * line.steps + line.end[tile];
+  const int w0 = start / line.range, w1 = (end - 1) / line.range;
+  if (w0 == w1) return;
+  const Sequence seq = sequence(a, line.b[tile]);
+  const int in_tile = (int)(blockIdx.x % kTileGroups) * (kWaves / W) + wave / W;
+  const int row = line.row0[tile] + in_tile, group = (int)a.group;
+  if (row >= seq.rows * group) return;  // whole workgroups leave where W waves share a row
+  float m = -kInf, l = 0.0f, sum[kPer];
+#pragma unroll
+  for (int d = 0; d < kPer; ++d) sum[d] = 0.0f;
+  for (int w = w0 + wave % W; w <= w1; w += W) {
+    const size_t place = (size_t)(2 * w + (w * line.range >= start ? 0 : 1)) * kTileRows + in_tile;
+    const float2 ml = a.part_ml[place];
+    const float* x = a.part_o + place * D + lane * kPer;
+    const float up = fmaxf(m, ml.x), base = up == -kInf ? 0.0f : up;
+    const float was = __builtin_amdgcn_exp2f(m - base), f = __builtin_amdgcn_exp2f(ml.x - base);
+    m = up;
+    l = l * was + f * ml.y;
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) sum[d] = sum[d] * was + f * x[d];
+  }
+  if constexpr (W > 1) {
+    if (lane == 0) lds_ml[wave] = {m, l};
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) lds_sum[wave][lane * kPer + d] = sum[d];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < W; ++w) {
+      const float2 ml = lds_ml[w];
+      const float up = fmaxf(m, ml.x), base = up == -kInf ? 0.0f : up;
+      const float was = __builtin_amdgcn_exp2f(m - base), f = __builtin_amdgcn_exp2f(ml.x - base);
+      m = up;
+      l = l * was + f * ml.y;
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) sum[d] = sum[d] * was + f * lds_sum[w][lane * kPer + d];
+    }
+  }
+  const int token = row / group, g = row - token * group;
+  const size_t q_row = (size_t)(seq.start + token);
+  write_row<D, kBf16>(a, q_row, blockIdx.y * a.group + g, lane, m, l, sum);
+}
+
 // Joins the parts of a row: W waves per (row, query head), wave w the parts w, w + W, ..; lane p of a
 // wave holds part p's weight (kMaxParts lanes at most). A part without keys has no sums to read.
 constexpr uint32_t kMaxParts = 64;
 constexpr uint32_t kFewRows = 32;  // what k_attention_kv4_few holds
+
+// At least the row tiles of a call's sequences: a sequence of r rows has r / 256 and a part of one.
+uint32_t line_tiles(uint32_t batch, uint32_t q_rows, uint32_t max_q, uint32_t group) {
+  const uint64_t all = (uint64_t)q_rows * group / kTileRows + batch;
+  const uint64_t each = ((uint64_t)max_q * group + kTileRows - 1) / kTileRows;
+  return (uint32_t)std::min(all, each * batch);
+}
 
 template <int D, bool kBf16, int W>
 __global__ __launch_bounds__(kThreads) void k_attention_kv4_join(Args a) {
   constexpr int kPer = D / 64;
   __shared__ float lds_sum[W == 1 ? 1 : W][D];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t heads = a.kv_heads * a.group;
   const Sequence seq = sequence(a, blockIdx.z);
   const uint32_t row = blockIdx.x * (kWaves / W) + wave / W;
   const uint32_t token = row / a.group, g = row - token * a.group;
   if ((int)token >= seq.rows || !takes(a, seq.rows * (int)a.group)) return;
   const size_t q_row = (size_t)(seq.start + token);
   const uint32_t q_head = blockIdx.y * a.group + g;
-  const size_t place = q_row * heads + q_head, pitch = (size_t)a.q_rows * heads;
+  const size_t place = few_place(a, 0, blockIdx.z, row, blockIdx.y);
+  const size_t pitch = (size_t)a.batch * a.rows_to * a.kv_heads;
   const float2 ml = lane < (int)a.parts ? a.part_ml[lane * pitch + place] : float2{-kInf, 0.0f};
   const float top = across32<true>(across16<true>(over16<true>(ml.x)));
   const float f = __builtin_amdgcn_exp2f(ml.x - (top == -kInf ? 0.0f : top));
@@ -1115,56 +1296,72 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_join(Args a) {
       for (int w = 0; w < W; ++w) sum[d] += lds_sum[w][lane * kPer + d];
     }
   }
-  const bool none = total == 0.0f;
-  const float inv = none ? 0.0f : 1.0f / total;
-  uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + lane * kPer;
-  if constexpr (kPer == 2)
-    *reinterpret_cast<uint32_t*>(out) = narrow2<kBf16>(sum[0] * inv, sum[1] * inv);
-  else
-    *out = (uint16_t)narrow<kBf16>(sum[0] * inv);
-  if (a.lse && lane == 0) a.lse[place] = none ? -kInf : (top + __log2f(total)) * kLn2;
+  write_row<D, kBf16>(a, q_row, q_head, lane, top, total, sum);
 }
 
-// One launch over the sequences of `plan`'s row counts, and the join of its parts.
 template <int D, bool kBf16>
-hipError_t launch(Args a, uint32_t batch, const Kv4Launch& plan, hipStream_t stream) {
+hipError_t launch_few(Args a, const Kv4Launch& plan, hipStream_t stream) {
   if (plan.row_tiles == 0) return hipSuccess;
   a.parts = plan.parts;
-  a.row_tiles = plan.row_tiles;
   a.rows_from = plan.rows_from;
   a.rows_to = plan.rows_to;
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)plan.parts * a.q_rows * a.kv_heads *
-                                                       a.group * D);
-  const uint32_t tiles = plan.row_tiles * plan.parts;
-  const dim3 few(tiles, a.kv_heads, batch);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)plan.parts * a.batch * plan.rows_to *
+                                                       a.kv_heads * D);
+  const dim3 grid(plan.parts, a.kv_heads, a.batch);
   if (plan.tile_rows == 4)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 4, 1>), few, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 4, 1>), grid, dim3(kThreads), 0, stream, a);
   else if (plan.tile_rows == 8)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 8, 1>), few, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 8, 1>), grid, dim3(kThreads), 0, stream, a);
   else if (plan.tile_rows == 16)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16, 1>), few, dim3(kThreads), 0, stream, a);
-  else if (plan.tile_rows == 32)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16, 2>), few, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16, 1>), grid, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((k_attention_kv4_rows<D, kBf16>), dim3(a.kv_heads, tiles, batch),
-                       dim3(kRowsThreads), 0, stream, a);
-  hipError_t e = hipGetLastError();
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16, 2>), grid, dim3(kThreads), 0, stream, a);
+  const hipError_t e = hipGetLastError();
   if (e != hipSuccess || plan.parts == 1) return e;
   const uint32_t rows = std::min(a.max_q * a.group, plan.rows_to);
   if (plan.parts > 8)
-    hipLaunchKernelGGL((k_attention_kv4_join<D, kBf16, kWaves>), dim3(rows, a.kv_heads, batch),
+    hipLaunchKernelGGL((k_attention_kv4_join<D, kBf16, kWaves>), dim3(rows, a.kv_heads, a.batch),
                        dim3(kThreads), 0, stream, a);
   else
     hipLaunchKernelGGL((k_attention_kv4_join<D, kBf16, 1>),
-                       dim3((rows + kWaves - 1) / kWaves, a.kv_heads, batch), dim3(kThreads), 0,
+                       dim3((rows + kWaves - 1) / kWaves, a.kv_heads, a.batch), dim3(kThreads), 0,
                        stream, a);
   return hipGetLastError();
 }
 
 template <int D, bool kBf16>
-hipError_t launch_both(const Args& a, uint32_t batch, const Kv4Plan& plan, hipStream_t stream) {
-  const hipError_t e = launch<D, kBf16>(a, batch, plan.many, stream);
-  return e != hipSuccess ? e : launch<D, kBf16>(a, batch, plan.few, stream);
+hipError_t launch_many(Args a, const Kv4Launch& plan, hipStream_t stream) {
+  if (plan.row_tiles == 0) return hipSuccess;
+  a.row_tiles = plan.row_tiles;
+  a.rows_from = plan.rows_from;
+  a.rows_to = plan.rows_to;
+  if (plan.parts == 1) {
+    hipLaunchKernelGGL((k_attention_kv4_rows<D, kBf16>), dim3(a.kv_heads, plan.row_tiles, a.batch),
+                       dim3(kRowsThreads), 0, stream, a);
+    return hipGetLastError();
+  }
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * plan.parts * kTileRows * D);
+  a.line = reinterpret_cast<Line*>(a.part_ml + (size_t)2 * plan.parts * kTileRows);
+  const uint32_t tiles = line_tiles(a.batch, a.q_rows, a.max_q, a.group);
+  a.row_tiles = tiles;
+  hipLaunchKernelGGL((k_attention_kv4_line<D, kBf16>), dim3(plan.parts), dim3(kRowsThreads), 0, stream,
+                     a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  // A workgroup a row where the rows alone would leave the chip idle.
+  if (tiles * a.kv_heads <= 64)
+    hipLaunchKernelGGL((k_attention_kv4_rows_join<D, kBf16, kWaves>),
+                       dim3(tiles * kTileRows, a.kv_heads), dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((k_attention_kv4_rows_join<D, kBf16, 1>),
+                       dim3(tiles * kTileRows / kWaves, a.kv_heads), dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <int D, bool kBf16>
+hipError_t launch_both(const Args& a, const Kv4Plan& plan, hipStream_t stream) {
+  const hipError_t e = launch_many<D, kBf16>(a, plan.many, stream);
+  return e != hipSuccess ? e : launch_few<D, kBf16>(a, plan.few, stream);
 }
 
 }  // namespace
@@ -1173,70 +1370,81 @@ hipError_t launch_both(const Args& a, uint32_t batch, const Kv4Plan& plan, hipSt
 // and more keys than the table holds (or a window shows).
 //
 // Which kernel: k_attention_kv4_few up to 32 rows, k_attention_kv4_rows beyond. A call with longer
-// sequences and more than one may hold single tokens too (prompts beside decoding): those go to few,
+// sequences that are not all alike may hold single tokens too (prompts beside decoding): those go to few,
 // in tiles of the 4, 8, 16 or 32 rows that hold the group's heads, and every other sequence to rows;
 // a launch's workgroups for sequences of the other kind leave at once.
 //
-// Parts: the split of a row tile's keys for which the time estimated from one MI355X's figures is
-// least, in us:
-//   rounds * (start + steps of a workgroup * step) + the join's,
-// few: 6 to start a workgroup and join its waves, 1.2 (4 rows) to 2.7 (32 rows) per 256 keys, which
-// are four waves' step, or what HBM takes for the resident workgroups' bytes where that is more (5.0
-// TB/s, 4.4 with one workgroup a compute unit); rows: 8, and 2.3 per 64 keys. The join is a launch (5 to 6) and writes and reads every
-// part's sums in f32. Timed: 16 groups of 129,024 keys 74, 65 and 68 us in 16, 32 and 64 parts;
-// 128 groups of 32 rows over 4,100 keys 52, 37, 49 and 66 us in 1, 2, 4 and 8; 512 groups of up to
-// 8,192 keys 82, 85, 87 and 98 us; 8 groups of 1,000 keys 10.6, 10.5, 9.4 and 9.0 us, where the second
-// launch costs the host more than the split gains.
+// few divides a sequence's keys in the number of parts for which the time estimated from one MI355X's
+// figures is least, in us: rounds * (start + steps of a workgroup * step) + the join's, with 6 to start
+// a workgroup and join its waves, 1.2 (4 rows) to 2.7 (32 rows) per 256 keys, which are four waves'
+// step, or what HBM takes for the resident workgroups' bytes where that is more (5.0 TB/s, 4.4 with
+// one workgroup a compute unit). The join is a launch (5) and writes and reads every part's sums in
+// f32. Timed: 16 groups of 129,024 keys 74, 65 and 68 us in 16, 32 and 64 parts; 128 groups of 32 rows
+// over 4,100 keys 52, 37, 49 and 66 us in 1, 2, 4 and 8; 512 groups of up to 8,192 keys 82, 85, 87 and
+// 98 us; 8 groups of 1,000 keys 10.6, 10.5, 9.4 and 9.0 us, where the second launch costs the host more
+// than the split gains.
+//
+// rows takes a workgroup per row tile and cache head, or (parts: how many workgroups) one line of all
+// their keys, as k_attention_kv4_line does, where the workgroups would fill the chip badly: 2.3 us per
+// 64 keys either way, against 12 to find the line and the join's traffic, two row tiles' sums a
+// workgroup.
 Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
                  uint32_t q_rows, uint32_t max_q, uint32_t cus) {
   Kv4Plan p{};
   const uint32_t group = acfg.heads / cfg.kv_heads, rows = max_q * group;
   uint64_t keys = (uint64_t)acfg.table_stride * cfg.page_tokens;
   if (acfg.window) keys = std::min<uint64_t>(keys, (uint64_t)acfg.window + max_q);
-  const double key_bytes = cfg.head_dim + 8;
-  auto parts = [&](uint64_t groups, uint32_t resident, double start, double step, uint32_t step_keys,
-                   double joined) {
-    uint32_t best = 1;
-    double least = 0;
-    const uint64_t steps = (keys + step_keys - 1) / step_keys;
-    for (uint32_t n = 1; n <= kMaxParts && (n == 1 || n <= steps); ++n) {
-      const double wgs = (double)groups * n, slots = (double)resident * cus;
-      const double each = std::ceil(std::min(wgs, slots) / cus);  // on the fullest compute units
-      const double share = each > 1 ? each * cus : wgs;
-      const double hbm = share * step_keys * key_bytes / (each > 1 ? 5.0e6 : 4.4e6);
-      const double time = std::ceil(wgs / slots) *
-                              (start + (double)((steps + n - 1) / n) * std::max(step, hbm)) +
-                          (n > 1 ? 5 + n * joined * (cfg.head_dim + 2) * 8 / 4e6 : 0);
-      if (n == 1 || time < least) {
-        best = n;
-        least = time;
-      }
-    }
-    return best;
-  };
   uint32_t few = rows;  // rows of the longest sequence that few takes
   if (rows > kFewRows) {
-    few = batch > 1 && group <= kFewRows ? group : 0;
-    const uint32_t tiles = (rows + 255) / 256;
-    p.many = {256, tiles, 1, few + 1, rows};
-    const uint64_t total = std::min<uint64_t>((uint64_t)batch * tiles, (uint64_t)q_rows * group / 256 + batch);
-    p.many.parts = parts(total * cfg.kv_heads, 1, 8, 2.3, 64, (double)q_rows * acfg.heads);
+    const bool alike = (uint64_t)batch * max_q == q_rows;  // every sequence has max_q rows
+    few = alike || group > kFewRows ? 0 : group;
+    p.many = {(uint32_t)kTileRows, (rows + kTileRows - 1) / kTileRows, 1, few + 1, rows};
+    const uint32_t tiles = line_tiles(batch, q_rows, max_q, group);
+    const uint64_t most = (keys + kTileKeys - 1) / kTileKeys;  // steps of a row tile
+    if (tiles <= (uint32_t)kLineTiles && batch <= (uint32_t)kLineTiles &&
+        (uint64_t)tiles * most * cfg.kv_heads < (1u << 30)) {
+      // A causal prompt's row tiles see half of its own keys on average.
+      const double mean = acfg.causal && !acfg.window && keys > max_q ? most - max_q / 128.0 : most;
+      const double wgs = std::min<double>((double)tiles, (double)q_rows * group / kTileRows + 1) * cfg.kv_heads;
+      const double all = wgs * std::max(mean, most / 2.0);
+      const double apart = wgs <= cus ? most : std::max<double>(most, all / cus + most * 0.5 * cus / wgs);
+      const double lines = std::min<double>(cus, std::max(1.0, all / kLeastSteps));
+      const double line = all / lines + (12 + 8 + 2 * lines * kTileRows * (cfg.head_dim + 2) * 8 / 4e6) / 2.3;
+      if (line < apart) p.many.parts = std::max(2u, (uint32_t)lines);
+    }
   }
   if (few) {
     const uint32_t tile = few <= 4 ? 4 : few <= 8 ? 8 : few <= 16 ? 16 : 32;
+    const double step = tile <= 4 ? 1.2 : tile <= 8 ? 1.3 : tile <= 16 ? 1.8 : 2.7;
+    const double groups = (double)batch * cfg.kv_heads, slots = (tile == 32 ? 1.0 : 2.0) * cus;
+    const uint64_t steps = (keys + kWaves * kStepKeys - 1) / (kWaves * kStepKeys);
     p.few = {tile, 1, 1, 0, few};
-    p.few.parts = parts((uint64_t)batch * cfg.kv_heads, tile == 32 ? 1 : 2, 6,
-                        tile <= 4 ? 1.2 : tile <= 8 ? 1.3 : tile <= 16 ? 1.8 : 2.7, 256,
-                        (double)batch * few * cfg.kv_heads);
+    double least = 0;
+    for (uint32_t n = 1; n <= kMaxParts && (n == 1 || n <= steps); ++n) {
+      const double wgs = groups * n;
+      const double each = std::ceil(std::min(wgs, slots) / cus);  // on the fullest compute units
+      const double hbm = (each > 1 ? each * cus : wgs) * kWaves * kStepKeys * (cfg.head_dim + 8) /
+                         (each > 1 ? 5.0e6 : 4.4e6);
+      const double time =
+          std::ceil(wgs / slots) * (6 + (double)((steps + n - 1) / n) * std::max(step, hbm)) +
+          (n > 1 ? 5 + wgs * few * (cfg.head_dim + 2) * 8 / 4e6 : 0);
+      if (n == 1 || time < least) {
+        p.few.parts = n;
+        least = time;
+      }
+    }
   }
   return p;
 }
 
-size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t q_rows,
-                           const Kv4Plan& plan) {
-  const uint32_t parts = std::max(plan.many.parts, plan.few.parts);
-  if (parts <= 1) return 0;
-  return (size_t)parts * q_rows * acfg.heads * (cfg.head_dim + 2) * 4;
+size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, uint32_t batch, const Kv4Plan& plan) {
+  const size_t row = (cfg.head_dim + 2) * 4;
+  size_t bytes = 0;
+  if (plan.few.parts > 1)
+    bytes = (size_t)plan.few.parts * batch * plan.few.rows_to * cfg.kv_heads * row;
+  if (plan.many.parts > 1)
+    bytes = std::max(bytes, (size_t)2 * plan.many.parts * kTileRows * row + sizeof(Line));
+  return bytes;
 }
 
 hipError_t launch_attention_kv4(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
@@ -1262,6 +1470,7 @@ hipError_t launch_attention_kv4(const h3_kv4_cfg& cfg, const h3_kv4_attention_cf
   a.table_stride = acfg.table_stride;
   a.pages = cfg.pages;
   a.page_shift = __builtin_ctz(cfg.page_tokens);
+  a.batch = batch;
   a.q_rows = q_rows;
   a.max_q = max_q;
   a.causal = acfg.causal;
@@ -1269,10 +1478,10 @@ hipError_t launch_attention_kv4(const h3_kv4_cfg& cfg, const h3_kv4_attention_cf
   a.scale = acfg.scale * kLog2e;
   const bool bf16 = cfg.elem == H3_ELEM_BF16;
   if (cfg.head_dim == 128)
-    return bf16 ? launch_both<128, true>(a, batch, plan, stream)
-                : launch_both<128, false>(a, batch, plan, stream);
-  return bf16 ? launch_both<64, true>(a, batch, plan, stream)
-              : launch_both<64, false>(a, batch, plan, stream);
+    return bf16 ? launch_both<128, true>(a, plan, stream)
+                : launch_both<128, false>(a, plan, stream);
+  return bf16 ? launch_both<64, true>(a, plan, stream)
+              : launch_both<64, false>(a, plan, stream);
 }
 
 }  // namespace h3

@@ -231,8 +231,9 @@ hipError_t launch_kv4_read(const h3_kv4_cfg& cfg, uint32_t tokens, uint32_t k_st
                            uint32_t v_stride, const int32_t* slots, const void* cache, void* k,
                            void* v, hipStream_t stream);
 // Attention over it (attention_kv4.hip). How a call is cut: a launch for the sequences of many rows
-// and one for those of few (row_tiles 0: none), each in tiles of `tile_rows` rows (a row is a token's
-// query head) with the keys of a tile in `parts`, which need a workspace to be joined.
+// and one for those of few (row_tiles 0: none), each for sequences of rows_from .. rows_to rows, in tiles
+// of `tile_rows` rows (a row is a token's query head). With parts > 1 their keys are divided, those of
+// few in `parts`, those of many over `parts` workgroups, which needs a workspace to be joined.
 struct Kv4Launch {
   uint32_t tile_rows, row_tiles, parts, rows_from, rows_to;
 };
@@ -241,8 +242,7 @@ struct Kv4Plan {
 };
 Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
                  uint32_t q_rows, uint32_t max_q, uint32_t cus);
-size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t q_rows,
-                           const Kv4Plan& plan);
+size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, uint32_t batch, const Kv4Plan& plan);
 hipError_t launch_attention_kv4(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
                                 uint32_t batch, uint32_t q_rows, uint32_t max_q, const void* q,
                                 const void* cache, const int32_t* table, const int32_t* lengths,

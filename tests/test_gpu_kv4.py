@@ -228,6 +228,34 @@ def test_long_keys_in_parts_and_in_one(dev, elem, dim, heads, kv_heads, page, ne
     call.check(workspace=False)
 
 
+@pytest.mark.parametrize("elem,dim,heads,kv_heads,page,new,lengths,causal,window", [
+    (F16, 128, 8, 2, 16, [300, 40, 1, 9], [2000, 40, 700, 1111], 1, 0),  # both kinds of launch
+    (BF16, 128, 4, 1, 64, [513, 257], [600, 3001], 1, 0),                # tiles that end past 256 rows
+    (F16, 64, 6, 3, 32, [100, 0, 100], [4500, 50, 99], 1, 2000),         # a window, rows before any key
+    (BF16, 64, 2, 2, 16, [300], [3900], 0, 0)])
+def test_row_tiles_in_one_line(dev, elem, dim, heads, kv_heads, page, new, lengths, causal, window):
+    """Few long sequences, whose row tiles share one line of keys over the workgroups: the workspace
+    holds its sums, two row tiles a workgroup."""
+    call = Call(dev, elem, dim, heads, kv_heads, page, new, lengths, causal=causal, window=window)
+    need = H.kv4_workspace_bytes(call.cfg, call.acfg, len(new), call.rows, max(new))
+    assert need >= 2 * 2 * 256 * (dim + 2) * 4
+    call.check()
+    call.check(workspace=False)
+
+
+def test_a_line_of_sequences_that_overlap(dev):
+    """q_starts that name rows twice ask for more row tiles than the rows have: nothing is read or
+    written out of bounds, and sequences whose tiles fit are right."""
+    call = Call(dev, F16, 128, 8, 1, 16, [200], [1500])
+    out, lse, out_tol, lse_tol = call.want()
+    call.new, call.lengths = [200] * 4, [1500] * 4
+    call.table = np.repeat(call.table, 4, 0)
+    call.rows = 200
+    got, got_lse = call.run(max_q=200, starts=np.array([0, 200, 0, 200, 0]))
+    P.within(got, out, out_tol)
+    P.within(got_lse, lse, lse_tol)
+
+
 def test_a_table_wider_than_the_sequences(dev):
     """Most parts of a call planned for the table's width have no keys."""
     Call(dev, F16, 128, 4, 2, 16, [1, 1, 2], [3, 0, 40], columns=4000).check()
