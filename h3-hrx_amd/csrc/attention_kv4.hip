@@ -164,57 +164,61 @@ struct Step {
   uint32_t k[4][D / 32];          // key n of each 16: channels D/4 h and on
   uint32_t v[16];                 // keys 32 (e / 8) + 8 h + e % 8: channels D/16 n and on
   uint32_t kw[R / 4], vw[R / 4];  // the words of the lane's key in each score tile
-  uint32_t hidden;                // a bit per 16 keys: their page is none of the cache's
+  uint64_t hidden;                // a bit per key: its page is none of the cache's
 };
 
-// `ids`: lane l's is the page of key `key` + l.
+__device__ __forceinline__ const uint8_t* lane_pointer(const uint8_t* p, int lane) {
+  const uint64_t x = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)x, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(x >> 32), lane);
+  return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
+}
+
+// `ids`: lane l's is the page of key `key` + l. Sixteen keys lie side by side in a page; each lane
+// finds its own key's K codes, and the first lanes of the sixteens lend theirs to all.
 template <int D, int R>
-__device__ __forceinline__ void load_step(const Args& a, int ids, uint32_t head, int key, int n,
-                                          int h, Step<D, R>& s) {
+__device__ __forceinline__ void load_step(const Args& a, int ids, uint32_t head, int key, int lane,
+                                          Step<D, R>& s) {
+  const int n = lane & 15, h = lane >> 4;
   const uint32_t page_tokens = 1u << a.page_shift, mask = page_tokens - 1;
-  const uint32_t block = page_tokens * (D + 8), page_bytes = block * a.kv_heads;
-  const uint8_t* base = a.cache + (uint64_t)head * block;
-  int id[4];
-  s.hidden = 0;
+  const uint32_t block = page_tokens * (D + 8);
+  // Keys of no page are masked; page 0 is there to read.
+  const uint8_t* page = a.cache + (uint64_t)head * block +
+                        (uint64_t)(uint32_t)max(ids, 0) * (block * a.kv_heads);
+  s.hidden = __ballot(ids < 0);
+  const uint8_t* mine = page + (((uint32_t)key + lane) & mask) * (D / 2);
+  const uint8_t* at[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    id[t] = __builtin_amdgcn_readlane(ids, 16 * t);
-    s.hidden |= id[t] < 0 ? 1u << t : 0u;
-    id[t] = max(id[t], 0);  // keys of no page are masked; page 0 is there to read
-  }
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const uint8_t* kc = base + (uint64_t)(uint32_t)id[t] * page_bytes +
-                        (((uint32_t)key + 16 * t) & mask) * (D / 2);
+    at[t] = lane_pointer(mine, 16 * t);
     if constexpr (D == 128) {
-      const uint4 k = *reinterpret_cast<const uint4*>(kc + (n * 64 + 16 * h));
+      const uint4 k = *reinterpret_cast<const uint4*>(at[t] + (n * 64 + 16 * h));
       s.k[t][0] = k.x, s.k[t][1] = k.y, s.k[t][2] = k.z, s.k[t][3] = k.w;
     } else {
-      const uint2 k = *reinterpret_cast<const uint2*>(kc + (n * 32 + 8 * h));
+      const uint2 k = *reinterpret_cast<const uint2*>(at[t] + (n * 32 + 8 * h));
       s.k[t][0] = k.x, s.k[t][1] = k.y;
     }
   }
 #pragma unroll
   for (int c = 0; c < R / 4; ++c) {
-    const int at = 16 * (c * (16 / R) + 4 * h / R);
-    int page;
-    if constexpr (R == 4) page = max(ids, 0);
+    const int t = c * (16 / R) + 4 * h / R;
+    const uint32_t in_page = ((uint32_t)key + 16 * t) & mask;
+    const uint8_t* codes = at[0];
+    if constexpr (R == 4) codes = mine - n * (D / 2);
     if constexpr (R == 8) {
-      const int even = id[2 * c], odd = id[2 * c + 1];
-      page = h >> 1 ? odd : even;
+      const uint8_t *even = at[2 * c], *odd = at[2 * c + 1];
+      codes = h >> 1 ? odd : even;
     }
-    if constexpr (R == 16) page = id[c];
-    const uint8_t* kw = base + (uint64_t)(uint32_t)page * page_bytes + page_tokens * D +
-                        (((uint32_t)key + at + n) & mask) * 4;
+    if constexpr (R == 16) codes = at[c];
+    const uint8_t* kw = codes + (page_tokens * D - in_page * (D / 2 - 4) + 4 * n);
     s.kw[c] = *reinterpret_cast<const uint32_t*>(kw);
     s.vw[c] = *reinterpret_cast<const uint32_t*>(kw + page_tokens * 4);
   }
 #pragma unroll
   for (int st = 0; st < 2; ++st) {
-    const int even = id[2 * st], odd = id[2 * st + 1];
-    const int page = h >> 1 ? odd : even;
-    const uint8_t* vc = base + (uint64_t)(uint32_t)page * page_bytes + page_tokens * (D / 2) +
-                        (((uint32_t)key + 32 * st + 8 * h) & mask) * (D / 2) + n * (D / 32);
+    const uint8_t *even = at[2 * st], *odd = at[2 * st + 1];
+    const uint8_t* vc = (h >> 1 ? odd : even) +
+                        (page_tokens * (D / 2) + 8 * (h & 1) * (D / 2) + n * (D / 32));
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (D == 128)
@@ -293,8 +297,8 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
   int step = (int)part * kWaves + wave;
   if (a.window) step += span(a, seq, 0).x / kStepKeys;
   int ids = page_of(a, table, step * kStepKeys + lane);
-  Step<D, R> next;
-  load_step<D, R>(a, ids, head, step * kStepKeys, n, h, next);
+  Step<D, R> tiles[2];
+  load_step<D, R>(a, ids, head, step * kStepKeys, lane, tiles[0]);
   ids = page_of(a, table, (step + stride) * kStepKeys + lane);
   if (rows == 0 || !takes(a, rows)) return;
   const int2 first_span = span(a, seq, 0), last_span = span(a, seq, (rows - 1) / group);
@@ -348,13 +352,12 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
   const uint4 one8 = {one2, one2, one2, one2};
   const Codes codes = make_codes<kBf16>();
 
-  for (; step < last; step += stride) {
-    const Step<D, R> cur = next;
+  auto attend = [&](const Step<D, R>& cur, Step<D, R>& next) {
     const int key0 = step * kStepKeys;
     if (step + stride < last) {
       const int now = ids;
       ids = page_of(a, table, key0 + 2 * kStepKeys * stride + lane);
-      load_step<D, R>(a, now, head, key0 + kStepKeys * stride, n, h, next);
+      load_step<D, R>(a, now, head, key0 + kStepKeys * stride, lane, next);
     }
     // Scores.
     v4f acc[QT][kTiles];
@@ -388,7 +391,7 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
 #pragma unroll
       for (int c = 0; c < kTiles; ++c) {
         const int sub = c * T + 4 * h / R, key = key0 + 16 * sub + n;
-        const bool none = key < key_lo || key >= key_hi || (cur.hidden >> sub) & 1;
+        const bool none = key < key_lo || key >= key_hi || (cur.hidden >> (16 * sub)) & 1;
         const bool nan = has_nan<kBf16>(cur.vw[c]);
         if (nan) km[c] = __uint_as_float(0x7fc00000u);
         if (none || nan) vs[c] = vm[c] = 0.0f;
@@ -407,7 +410,7 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
 #pragma unroll
       for (int c = 0; c < kTiles; ++c) {
         const int sub = c * T + 4 * h / R, key = key0 + 16 * sub + n;
-        const bool hidden = (cur.hidden >> sub) & 1;
+        const bool hidden = (cur.hidden >> (16 * sub)) & 1;
 #pragma unroll
         for (int t = 0; t < QT; ++t)
 #pragma unroll
@@ -524,6 +527,18 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+  // Two sets of registers in turn, so that the next step's loads land in their place; with 16 rows
+  // and more there are not enough for both, and the loads are moved.
+  for (; step < last; step += stride) {
+    attend(tiles[0], tiles[1]);
+    if constexpr (R <= 8) {
+      step += stride;
+      if (step >= last) break;
+      attend(tiles[1], tiles[0]);
+    } else {
+      tiles[0] = tiles[1];
+    }
   }
 
   // Join the four waves: every wave's sums relative to the common maximum.
