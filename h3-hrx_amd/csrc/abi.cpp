@@ -37,6 +37,19 @@ int ok() {
   return H3_OK;
 }
 
+// The devices of this process, which do not change while it runs: asked once (0.15 us a call).
+struct Devices {
+  int count = 0;
+  hipError_t error;
+  Devices() : error(hipGetDeviceCount(&count)) {
+    if (error != hipSuccess) (void)hipGetLastError();
+  }
+};
+const Devices& devices() {
+  static const Devices d;
+  return d;
+}
+
 // src/dispatch.rs:264-276: every binding must cover the extent the kernel addresses.
 int check_bindings(const char* stage, const h3_view* views, const size_t* need, int n) {
   for (int i = 0; i < n; ++i) {
@@ -50,11 +63,8 @@ int check_bindings(const char* stage, const h3_view* views, const size_t* need, 
   // pointer or another device's buffer handed to a kernel faults the GPU. The HIP runtime knows
   // this process's allocations (device, managed and pinned host memory); anything else it
   // refuses. On a host with no device, device_ready() reports that instead.
-  int devices = 0, current = 0;
-  if (hipGetDeviceCount(&devices) != hipSuccess || devices == 0) {
-    (void)hipGetLastError();
-    return H3_OK;
-  }
+  int current = 0;
+  if (devices().count == 0) return H3_OK;
   if (hipGetDevice(&current) != hipSuccess) {
     (void)hipGetLastError();
     return H3_OK;
@@ -97,10 +107,9 @@ int launched(const char* stage, hipError_t e) {
 }
 
 int device_ready(const char* stage) {
-  int count = 0;
-  hipError_t e = hipGetDeviceCount(&count);
-  if (e != hipSuccess || count == 0)
-    return set_error(H3_ERR_NO_DEVICE, "%s: no HIP device (%s)", stage, hipGetErrorString(e));
+  const Devices& d = devices();
+  if (d.count == 0)
+    return set_error(H3_ERR_NO_DEVICE, "%s: no HIP device (%s)", stage, hipGetErrorString(d.error));
   return H3_OK;
 }
 
@@ -420,6 +429,9 @@ int check_kv4_attention(const char* stage, const h3_kv4_cfg* cfg, const h3_kv4_a
   if (!in_range(q_rows, 1, 16777216) || !in_range(max_q, 1, q_rows))
     return set_error(H3_ERR_ARGUMENT, "%s: q_rows %u outside [1, 2^24] or max_q %u outside [1, q_rows]",
                      stage, q_rows, max_q);
+  if ((uint64_t)max_q * (acfg->heads / cfg->kv_heads) > (1u << 30))
+    return set_error(H3_ERR_ARGUMENT, "%s: max_q %u of %u heads a cache head passes 2^30 rows", stage,
+                     max_q, acfg->heads / cfg->kv_heads);
   return H3_OK;
 }
 

@@ -1088,10 +1088,11 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   __shared__ __attribute__((aligned(16))) RowsLds<D> lds;
   const Sequence seq = sequence(a, blockIdx.z);
   const int rows = seq.rows * (int)a.group;
-  // The last rows see the most keys: they start first.
-  const int row0 = (int)(a.row_tiles - 1 - blockIdx.y) * kTileRows;
+  // A row tile's heads side by side; the last rows see the most keys: they start first.
+  const uint32_t tile = blockIdx.x / a.kv_heads, head = blockIdx.x - tile * a.kv_heads;
+  const int row0 = (int)(a.row_tiles - 1 - tile) * kTileRows;
   if (row0 >= rows || !takes(a, rows)) return;
-  attend_rows<D, kBf16>(a, lds, seq, blockIdx.z, blockIdx.x, row0, row_steps(a, seq, row0), -1);
+  attend_rows<D, kBf16>(a, lds, seq, blockIdx.z, head, row0, row_steps(a, seq, row0), -1);
 }
 
 // The same row tiles where they would leave the chip partly idle: the tiles of keys of all of them (of
@@ -1351,7 +1352,7 @@ hipError_t launch_many(Args a, const Kv4Launch& plan, hipStream_t stream) {
   a.rows_from = plan.rows_from;
   a.rows_to = plan.rows_to;
   if (plan.parts == 1) {
-    hipLaunchKernelGGL((k_attention_kv4_rows<D, kBf16>), dim3(a.kv_heads, plan.row_tiles, a.batch),
+    hipLaunchKernelGGL((k_attention_kv4_rows<D, kBf16>), dim3(a.kv_heads * plan.row_tiles, 1, a.batch),
                        dim3(kRowsThreads), 0, stream, a);
     return hipGetLastError();
   }

@@ -370,11 +370,13 @@ def view(t) -> View:
         return View(None, 0)
     if isinstance(t, View):
         return t
-    if not hasattr(t, "data_ptr"):
-        raise TypeError(f"cannot bind {type(t)}")
-    if not t.is_contiguous():
+    try:
+        contiguous, cuda = t.is_contiguous(), t.is_cuda
+    except AttributeError:
+        raise TypeError(f"cannot bind {type(t)}") from None
+    if not contiguous:
         raise ValueError("bindings must be contiguous")
-    if not t.is_cuda:
+    if not cuda:
         raise ValueError(f"bindings must be GPU tensors, got one on {t.device}")
     torch = _torch or _load_torch()
     if not _one_device and t.device.index != torch.cuda.current_device():

@@ -465,7 +465,8 @@ typedef struct {
  *   q [q_rows][q_stride], out [q_rows][out_stride] (elem, 16-byte aligned), cache, table
  *   [batch][table_stride] i32, lengths [batch] i32, q_starts [batch + 1] i32, lse [q_rows][heads] f32
  *   or an empty view. q_rows in [1, 2^24], batch in [1, 65535], max_q in [1, q_rows]: no sequence
- *   has more rows (of one that has, the rows from max_q on are left as they were).
+ *   has more rows (of one that has, the rows from max_q on are left as they were); max_q * heads /
+ *   kv_heads <= 2^30. bf16 values from 2^100 on pass the range of the f32 sums.
  * The device arrays are read on the device: a call can be captured in a graph and replayed with
  * other lengths, tables and rows. Values outside their ranges read and write nothing out of bounds:
  * a table entry that is no page of the cache hides its keys, a length is cut to table_stride *

@@ -123,6 +123,9 @@ def test_attention_refuses_what_it_cannot_take():
                     (batch, rows, 0), (batch, rows, rows + 1)]:
         assert call_attention(cache_cfg(), attention_cfg(), b, r, m, big) == H.H3_ERR_ARGUMENT
         assert H.kv4_workspace_bytes(cache_cfg(), attention_cfg(), b, r, m) == 0
+    many = H.Kv4AttentionCfg(4096, 2 ** 19, 2 ** 19, 5, 1, 0, 0.1)
+    assert call_attention(cache_cfg(kv_heads=1), many, 1, 2 ** 24, 2 ** 18 + 1,
+                          big) == H.H3_ERR_ARGUMENT and "2^30" in H.last_error()
     assert H.lib().h3_attention_kv4(ctypes.byref(cache_cfg()), None, 1, 1, 1, *big,
                                     None) == H.H3_ERR_ARGUMENT
 
