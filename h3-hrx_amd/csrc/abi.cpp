@@ -1160,7 +1160,7 @@ size_t h3_kv4_workspace_bytes(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg*
   if (check_kv4_attention("kv4_workspace_bytes", cfg, attention, batch, q_rows, max_q)) return 0;
   ok();
   return kv4_workspace_bytes(*cfg, batch,
-                             kv4_plan(*cfg, *attention, batch, q_rows, max_q, device_cus()));
+                             kv4_plan(*cfg, *attention, batch, q_rows, max_q, device_cus(), true));
 }
 
 int h3_attention_kv4(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attention, uint32_t batch,
@@ -1171,10 +1171,9 @@ int h3_attention_kv4(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attentio
   int st = check_kv4_attention(stage, cfg, attention, batch, q_rows, max_q);
   if (st) return st;
   const uint32_t width = attention->heads * cfg->head_dim;
-  const size_t ws = workspace.ptr
-                        ? kv4_workspace_bytes(*cfg, batch,
-                                              kv4_plan(*cfg, *attention, batch, q_rows, max_q, device_cus()))
-                        : 0;
+  const Kv4Plan plan =
+      kv4_plan(*cfg, *attention, batch, q_rows, max_q, device_cus(), workspace.ptr != nullptr);
+  const size_t ws = kv4_workspace_bytes(*cfg, batch, plan);
   h3_view views[8] = {q, cache, table, lengths, q_starts, out, lse, workspace};
   size_t need[8] = {kv4_rows_bytes(q_rows, attention->q_stride, width), kv4_cache_bytes(*cfg),
                     (size_t)batch * attention->table_stride * 4, (size_t)batch * 4,
@@ -1183,8 +1182,8 @@ int h3_attention_kv4(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attentio
   if ((st = check_bindings(stage, views, need, 8))) return st;
   if ((st = check_alignments(stage, views, {16, 16, 4, 4, 4, 16, 4, 16}))) return st;
   if ((st = device_ready(stage))) return st;
-  return launched(stage, launch_attention_kv4(*cfg, *attention, batch, q_rows, max_q, q.ptr,
-                                              cache.ptr, static_cast<const int32_t*>(table.ptr),
+  return launched(stage, launch_attention_kv4(*cfg, *attention, plan, batch, q_rows, max_q,
+                                              q.ptr, cache.ptr, static_cast<const int32_t*>(table.ptr),
                                               static_cast<const int32_t*>(lengths.ptr),
                                               static_cast<const int32_t*>(q_starts.ptr), out.ptr,
                                               static_cast<float*>(lse.ptr), workspace.ptr,

@@ -11,7 +11,8 @@
 // sum of the same rounded p s, which one more MFMA with a row of ones gives, so what p s loses in
 // rounding to 16 bits multiplies u - 8, as in an attention over centred 16-bit values; the second
 // sum is kept in f32. In f16, p s is held relative to the largest scale so far (a power of two,
-// raised as the running maximum is), times 2^14: weights down to 2^-28 of the largest stay normal.
+// raised as the running maximum is), times 2^8: weights down to 2^-22 of the largest stay normal.
+// (With 256 rows to a tile of keys the values are formed once for all of them instead, in LDS.)
 //
 // A query row is one (token, query head) pair; the G = heads / kv_heads heads of one cache head
 // are rows of the same matrix, row = token * G + g, so that a key is read once for all of them.
@@ -145,7 +146,7 @@ __device__ __forceinline__ int page_of(const Args& a, const int32_t* table, int 
   return (uint32_t)id < a.pages ? id : -1;
 }
 
-// Few rows: a workgroup's four waves hold the same R * QT rows of one cache head and take every
+// Up to 16 rows: a workgroup's four waves hold the same R rows of one cache head and take every
 // fourth 64 keys; their results are joined in LDS. Loads of the next 64 keys are in flight over the
 // work on these, so the kernel is bound by HBM as long as that work is short, and most of it is
 // vector instructions: the unpacking of the codes (one shift and one AND-OR a pair, fixed), then the
@@ -277,14 +278,13 @@ __device__ __forceinline__ size_t few_place(const Args& a, uint32_t part, uint32
   return (((size_t)part * a.batch + b) * a.rows_to + row) * a.kv_heads + head;
 }
 
-template <int D, bool kBf16, int R, int QT>
-__global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few(Args a) {
-  static_assert(QT == 1 || R == 16, "row tiles of 16");
-  constexpr int T = 16 / R, kTiles = R / 4, kSteps = D / 32, kDimTiles = D / 16, kRows = R * QT;
-  __shared__ __attribute__((aligned(16))) uint16_t lds_p[kWaves][QT][kStepKeys * R];
+template <int D, bool kBf16, int R>
+__global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
+  constexpr int T = 16 / R, kTiles = R / 4, kSteps = D / 32, kDimTiles = D / 16;
+  __shared__ __attribute__((aligned(16))) uint16_t lds_p[kWaves][kStepKeys * R];
   __shared__ __attribute__((aligned(16))) float lds_o[kWaves][R][D + 4];
-  __shared__ float lds_row[kWaves][kRows];    // a factor per row, from its lanes to its column
-  __shared__ float2 lds_ml[kWaves][kRows];
+  __shared__ float lds_row[kWaves][R];    // a factor per row, from its lanes to its column
+  __shared__ float2 lds_ml[kWaves][R];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, h = lane >> 4;
   const uint32_t head = blockIdx.y, b = blockIdx.z, part = blockIdx.x;
@@ -313,40 +313,35 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
 
   // Q operands: channel D/4 h + 8 s + {0,4,1,5,2,6,3,7} in k slot 8 h + 0..7 of step s, the order in
   // which the codes of a word come out in pairs. Rows past the last are zeros.
-  uint4 qf[QT][T][kSteps];
-  float q_sum[QT][4], m[QT][4], l[QT][4], mid[QT][4];  // row (4 h + i) % R; mid: sum p (m + 8 s)
-  v4f o[QT][kDimTiles], ones[QT];
+  uint4 qf[T][kSteps];
+  float q_sum[4], m[4], l[4], mid[4];  // row (4 h + i) % R; mid: sum p (m + 8 s)
+  v4f o[kDimTiles], ones = {0, 0, 0, 0};
+  const int q_token = n % R / group, q_g = n % R - q_token * group;
+  float q_total = 0.0f;
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const int row = 16 * t + n % R;
-    const int token = row / group, g = row - token * group;
-    float sum = 0.0f;
+  for (int s = 0; s < kSteps; ++s) {
+    uint4 x = {0, 0, 0, 0};
+    if (n % R < rows)
+      x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                          (size_t)(seq.start + q_token) * a.q_stride +
+                                          (head * group + q_g) * D + (D / 4) * h + 8 * s);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      uint4 x = {0, 0, 0, 0};
-      if (row < rows)
-        x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
-                                            (size_t)(seq.start + token) * a.q_stride +
-                                            (head * group + g) * D + (D / 4) * h + 8 * s);
-      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    for (int i = 0; i < 4; ++i) q_total += widen<kBf16>(w[i] & 0xffffu) + widen<kBf16>(w[i] >> 16);
+    x = {(x.x & 0xffffu) | (x.z << 16), (x.x >> 16) | (x.z & 0xffff0000u),
+         (x.y & 0xffffu) | (x.w << 16), (x.y >> 16) | (x.w & 0xffff0000u)};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += widen<kBf16>(w[i] & 0xffffu) + widen<kBf16>(w[i] >> 16);
-      x = {(x.x & 0xffffu) | (x.z << 16), (x.x >> 16) | (x.z & 0xffff0000u),
-           (x.y & 0xffffu) | (x.w << 16), (x.y >> 16) | (x.w & 0xffff0000u)};
-#pragma unroll
-      for (int u = 0; u < T; ++u) qf[t][u][s] = n / R == u ? x : uint4{0, 0, 0, 0};
-    }
-    sum = across32<false>(across16<false>(sum));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      q_sum[t][i] = __shfl(sum, (4 * h + i) % R);
-      m[t][i] = -kInf;
-      l[t][i] = mid[t][i] = 0.0f;
-    }
-#pragma unroll
-    for (int d = 0; d < kDimTiles; ++d) o[t][d] = {0, 0, 0, 0};
-    ones[t] = {0, 0, 0, 0};
+    for (int u = 0; u < T; ++u) qf[u][s] = n / R == u ? x : uint4{0, 0, 0, 0};
   }
+  q_total = across32<false>(across16<false>(q_total));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    q_sum[i] = __shfl(q_total, (4 * h + i) % R);
+    m[i] = -kInf;
+    l[i] = mid[i] = 0.0f;
+  }
+#pragma unroll
+  for (int d = 0; d < kDimTiles; ++d) o[d] = {0, 0, 0, 0};
   float s_top = 0.0f, s_factor = 0.0f;  // f16: a power of two no scale passes, and kHeld over it
   const uint32_t one2 = kBf16 ? 0x3F803F80u : 0x3C003C00u;
   const uint4 one8 = {one2, one2, one2, one2};
@@ -360,11 +355,10 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
       load_step<D, R>(a, now, head, key0 + kStepKeys * stride, lane, next);
     }
     // Scores.
-    v4f acc[QT][kTiles];
+    v4f acc[kTiles];
 #pragma unroll
     for (int c = 0; c < kTiles; ++c) {
-#pragma unroll
-      for (int t = 0; t < QT; ++t) acc[t][c] = {0, 0, 0, 0};
+      acc[c] = {0, 0, 0, 0};
 #pragma unroll
       for (int u = 0; u < T; ++u)
 #pragma unroll
@@ -372,8 +366,7 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
           const uint32_t w = cur.k[c * T + u][s];
           const uint4 kf = {code_pair<kBf16>(w, 0, codes), code_pair<kBf16>(w, 1, codes), code_pair<kBf16>(w, 2, codes),
                             code_pair<kBf16>(w, 3, codes)};
-#pragma unroll
-          for (int t = 0; t < QT; ++t) acc[t][c] = mfma16<kBf16>(qf[t][u][s], kf, acc[t][c]);
+          acc[c] = mfma16<kBf16>(qf[u][s], kf, acc[c]);
         }
     }
     float ks[kTiles], km[kTiles], vs[kTiles], vm[kTiles];
@@ -398,34 +391,28 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
       }
     }
     bool raise = false;
-    float x[QT][kTiles][4];  // scores less m, base 2
+    float x[kTiles][4];  // scores less m, base 2
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
+    for (int c = 0; c < kTiles; ++c)
 #pragma unroll
-      for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          x[t][c][i] = fmaf(ks[c], acc[t][c][i], fmaf(km[c], q_sum[t][i], -m[t][i]));
+      for (int i = 0; i < 4; ++i)
+        x[c][i] = fmaf(ks[c], acc[c][i], fmaf(km[c], q_sum[i], -m[i]));
     if (!whole) {
 #pragma unroll
       for (int c = 0; c < kTiles; ++c) {
         const int sub = c * T + 4 * h / R, key = key0 + 16 * sub + n;
         const bool hidden = (cur.hidden >> (16 * sub)) & 1;
 #pragma unroll
-        for (int t = 0; t < QT; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = 16 * t + (4 * h + i) % R;
-            const int2 seen = row < rows ? span(a, seq, row / group) : int2{0, 0};
-            if (hidden || key < seen.x || key >= seen.y) x[t][c][i] = -kInf;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int row = (4 * h + i) % R;
+          const int2 seen = row < rows ? span(a, seq, row / group) : int2{0, 0};
+          if (hidden || key < seen.x || key >= seen.y) x[c][i] = -kInf;
+        }
       }
     }
 #pragma unroll
-    for (int t = 0; t < QT; ++t)
-#pragma unroll
-      for (int c = 0; c < kTiles; ++c)
-        raise |= fmaxf(fmaxf(x[t][c][0], x[t][c][1]), fmaxf(x[t][c][2], x[t][c][3])) > kRaise;
+    for (int c = 0; c < kTiles; ++c)
+      raise |= fmaxf(fmaxf(x[c][0], x[c][1]), fmaxf(x[c][2], x[c][3])) > kRaise;
     if constexpr (!kBf16) {
 #pragma unroll
       for (int c = 0; c < kTiles; ++c) raise |= vs[c] > s_top;
@@ -445,71 +432,58 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
         }
       }
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
+      for (int i = 0; i < 4; ++i) {
+        // The scores themselves again: x is infinite while m is.
+        float y[kTiles], top = -kInf;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // The scores themselves again: x is infinite while m is.
-          float y[kTiles], top = -kInf;
-#pragma unroll
-          for (int c = 0; c < kTiles; ++c) {
-            y[c] = fmaf(ks[c], acc[t][c][i], km[c] * q_sum[t][i]);
-            if (!whole && x[t][c][i] == -kInf) y[c] = -kInf;
-            top = fmaxf(top, y[c]);
-          }
-          const float up = fmaxf(m[t][i], row_lanes<R, true>(top));
-          const float base = up == -kInf ? 0.0f : up;
-          const float alpha = __builtin_amdgcn_exp2f(m[t][i] - base);
-          m[t][i] = up;
-          l[t][i] *= alpha;
-          mid[t][i] *= alpha;
-          if (n == 0 && 4 * h < R) lds_row[wave][16 * t + 4 * h + i] = alpha * ratio;
-#pragma unroll
-          for (int c = 0; c < kTiles; ++c) x[t][c][i] = y[c] - base;
+        for (int c = 0; c < kTiles; ++c) {
+          y[c] = fmaf(ks[c], acc[c][i], km[c] * q_sum[i]);
+          if (!whole && x[c][i] == -kInf) y[c] = -kInf;
+          top = fmaxf(top, y[c]);
         }
+        const float up = fmaxf(m[i], row_lanes<R, true>(top));
+        const float base = up == -kInf ? 0.0f : up;
+        const float alpha = __builtin_amdgcn_exp2f(m[i] - base);
+        m[i] = up;
+        l[i] *= alpha;
+        mid[i] *= alpha;
+        if (n == 0 && 4 * h < R) lds_row[wave][4 * h + i] = alpha * ratio;
+#pragma unroll
+        for (int c = 0; c < kTiles; ++c) x[c][i] = y[c] - base;
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const float both = lds_row[wave][n % R];
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        const float both = lds_row[wave][16 * t + n % R];
-#pragma unroll
-        for (int d = 0; d < kDimTiles; ++d) o[t][d] *= both;
-        ones[t] *= both;
-      }
+      for (int d = 0; d < kDimTiles; ++d) o[d] *= both;
+      ones *= both;
     }
     // Probabilities, and p s in 16 bits (one rounding, of a weight of u - 8) on their way to columns.
 #pragma unroll
     for (int c = 0; c < kTiles; ++c) {
       const float f = kBf16 ? vs[c] : vs[c] * s_factor;
       const int key = 16 * (c * T + 4 * h / R) + n;
+      float ps[4];
 #pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        float ps[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float p = __builtin_amdgcn_exp2f(x[t][c][i]);
-          l[t][i] += p;
-          mid[t][i] = fmaf(p, vm[c], mid[t][i]);
-          ps[i] = p * f;
-        }
-        *reinterpret_cast<uint2*>(&lds_p[wave][t][key * R + 4 * h % R]) = {
-            narrow2<kBf16>(ps[0], ps[1]), narrow2<kBf16>(ps[2], ps[3])};
+      for (int i = 0; i < 4; ++i) {
+        const float p = __builtin_amdgcn_exp2f(x[c][i]);
+        l[i] += p;
+        mid[i] = fmaf(p, vm[c], mid[i]);
+        ps[i] = p * f;
       }
+      *reinterpret_cast<uint2*>(&lds_p[wave][key * R + 4 * h % R]) = {
+          narrow2<kBf16>(ps[0], ps[1]), narrow2<kBf16>(ps[2], ps[3])};
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     // O^T: dim tile d holds channel D/16 n + d in row n; keys pair up across words.
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      uint4 pf[QT];
       const int at = (32 * s + 8 * h + (n >> 2)) * R + 4 * (n & 3) % R;
-#pragma unroll
-      for (int t = 0; t < QT; ++t) {
-        uint16_t* p = &lds_p[wave][t][at];
-        const v4s p0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p);
-        const v4s p1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 4 * R));
-        const uint2 w0 = __builtin_bit_cast(uint2, p0), w1 = __builtin_bit_cast(uint2, p1);
-        pf[t] = {w0.x, w0.y, w1.x, w1.y};
-        ones[t] = mfma16<kBf16>(one8, pf[t], ones[t]);
-      }
+      uint16_t* p = &lds_p[wave][at];
+      const v4s p0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)p);
+      const v4s p1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 4 * R));
+      const uint2 w0 = __builtin_bit_cast(uint2, p0), w1 = __builtin_bit_cast(uint2, p1);
+      const uint4 pf = {w0.x, w0.y, w1.x, w1.y};
+      ones = mfma16<kBf16>(one8, pf, ones);
       uint32_t lo[4], hi[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -522,14 +496,13 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
         const uint32_t* w = d < 4 ? lo : hi;
         const uint4 vf = {code_pair<kBf16>(w[0], d & 3, codes), code_pair<kBf16>(w[1], d & 3, codes),
                           code_pair<kBf16>(w[2], d & 3, codes), code_pair<kBf16>(w[3], d & 3, codes)};
-#pragma unroll
-        for (int t = 0; t < QT; ++t) o[t][d] = mfma16<kBf16>(vf, pf[t], o[t][d]);
+        o[d] = mfma16<kBf16>(vf, pf, o[d]);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
   // Two sets of registers in turn, so that the next step's loads land in their place; with 16 rows
-  // and more there are not enough for both, and the loads are moved.
+  // there are not enough for both, and the loads are moved.
   for (; step < last; step += stride) {
     attend(tiles[0], tiles[1]);
     if constexpr (R <= 8) {
@@ -544,75 +517,67 @@ __global__ __launch_bounds__(kThreads, QT == 1 ? 2 : 1) void k_attention_kv4_few
   // Join the four waves: every wave's sums relative to the common maximum.
   const float unit = kBf16 ? 1.0f : s_top * (1.0f / kHeld);
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float ls = row_lanes<R, false>(l[t][i]), ms = row_lanes<R, false>(mid[t][i]);
-      if (n == 0 && 4 * h < R) {
-        lds_ml[wave][16 * t + 4 * h + i] = {m[t][i], ls};
-        lds_row[wave][16 * t + 4 * h + i] = ms;
-      }
+  for (int i = 0; i < 4; ++i) {
+    const float ls = row_lanes<R, false>(l[i]), ms = row_lanes<R, false>(mid[i]);
+    if (n == 0 && 4 * h < R) {
+      lds_ml[wave][4 * h + i] = {m[i], ls};
+      lds_row[wave][4 * h + i] = ms;
     }
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const float ms = lds_row[wave][n % R];
+  if (n < R) {
+    // Row i of dim tile d: channel (D/16) (4h + i) + d.
 #pragma unroll
-  for (int t = 0; t < QT; ++t) {
-    const float ms = lds_row[wave][16 * t + n % R];
-    if (t) __syncthreads();
-    if (n < R) {
-      // Row i of dim tile d: channel (D/16) (4h + i) + d.
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int d = 0; d < kDimTiles; d += 4) {
+        float4 f;
+        f.x = fmaf(unit, fmaf(-24.0f, ones[i], o[d][i]), ms);
+        f.y = fmaf(unit, fmaf(-24.0f, ones[i], o[d + 1][i]), ms);
+        f.z = fmaf(unit, fmaf(-24.0f, ones[i], o[d + 2][i]), ms);
+        f.w = fmaf(unit, fmaf(-24.0f, ones[i], o[d + 3][i]), ms);
+        *reinterpret_cast<float4*>(&lds_o[wave][n][kDimTiles * (4 * h + i) + d]) = f;
+      }
+  }
+  __syncthreads();
+  constexpr int kPer = R * D / kThreads;  // channels a thread; 256 / R threads a row
+  const int row = threadIdx.x / (kThreads / R), ch = (threadIdx.x % (kThreads / R)) * kPer;
+  if (row < rows) {
+    float2 ml[kWaves];
+    float top = -kInf;
 #pragma unroll
-        for (int d = 0; d < kDimTiles; d += 4) {
-          float4 f;
-          f.x = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d][i]), ms);
-          f.y = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d + 1][i]), ms);
-          f.z = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d + 2][i]), ms);
-          f.w = fmaf(unit, fmaf(-24.0f, ones[t][i], o[t][d + 3][i]), ms);
-          *reinterpret_cast<float4*>(&lds_o[wave][n][kDimTiles * (4 * h + i) + d]) = f;
-        }
+    for (int w = 0; w < kWaves; ++w) {
+      ml[w] = lds_ml[w][row];
+      top = fmaxf(top, ml[w].x);
     }
-    __syncthreads();
-    constexpr int kPer = R * D / kThreads;  // channels a thread; 256 / R threads a row
-    const int r = threadIdx.x / (kThreads / R), ch = (threadIdx.x % (kThreads / R)) * kPer;
-    const int row = 16 * t + r;
-    if (row < rows) {
-      float2 ml[kWaves];
-      float top = -kInf;
+    const float base = top == -kInf ? 0.0f : top;
+    float total = 0.0f, sum[kPer];
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        ml[w] = lds_ml[w][row];
-        top = fmaxf(top, ml[w].x);
-      }
-      const float base = top == -kInf ? 0.0f : top;
-      float total = 0.0f, sum[kPer];
+    for (int d = 0; d < kPer; ++d) sum[d] = 0.0f;
 #pragma unroll
-      for (int d = 0; d < kPer; ++d) sum[d] = 0.0f;
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(ml[w].x - base);
+      total = fmaf(f, ml[w].y, total);
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = __builtin_amdgcn_exp2f(ml[w].x - base);
-        total = fmaf(f, ml[w].y, total);
+      for (int d = 0; d < kPer; ++d) sum[d] = fmaf(f, lds_o[w][row][ch + d], sum[d]);
+    }
+    const int token = row / group, g = row - token * group;
+    const size_t q_row = (size_t)(seq.start + token);
+    const uint32_t q_head = head * group + g;
+    if (a.parts > 1) {
+      const size_t place = few_place(a, part, b, row, head);
 #pragma unroll
-        for (int d = 0; d < kPer; ++d) sum[d] = fmaf(f, lds_o[w][r][ch + d], sum[d]);
-      }
-      const int token = row / group, g = row - token * group;
-      const size_t q_row = (size_t)(seq.start + token);
-      const uint32_t q_head = head * group + g;
-      if (a.parts > 1) {
-        const size_t place = few_place(a, part, b, row, head);
+      for (int d = 0; d < kPer; ++d) a.part_o[place * D + ch + d] = sum[d];
+      if (ch == 0) a.part_ml[place] = {top, total};
+    } else {
+      const bool none = total == 0.0f;  // a NaN among the scores leaves total NaN
+      const float inv = none ? 0.0f : 1.0f / total;
+      uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + ch;
 #pragma unroll
-        for (int d = 0; d < kPer; ++d) a.part_o[place * D + ch + d] = sum[d];
-        if (ch == 0) a.part_ml[place] = {top, total};
-      } else {
-        const bool none = total == 0.0f;  // a NaN among the scores leaves total NaN
-        const float inv = none ? 0.0f : 1.0f / total;
-        uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + ch;
-#pragma unroll
-        for (int d = 0; d < kPer; ++d) out[d] = (uint16_t)narrow<kBf16>(sum[d] * inv);
-        if (a.lse && ch == 0)
-          a.lse[q_row * heads + q_head] = none ? -kInf : (top + __log2f(total)) * kLn2;
-      }
+      for (int d = 0; d < kPer; ++d) out[d] = (uint16_t)narrow<kBf16>(sum[d] * inv);
+      if (a.lse && ch == 0)
+        a.lse[q_row * heads + q_head] = none ? -kInf : (top + __log2f(total)) * kLn2;
     }
   }
 }
@@ -1060,6 +1025,309 @@ __device__ __forceinline__ void attend_rows(const Args& a, RowsLds<D>& lds, cons
     a.lse[q_row * heads + q_head] = none ? -kInf : (m + __log2f(total)) * kLn2;
 }
 
+// 17 rows and more, in tiles of 32: as k_attention_kv4_few, with score tiles S^T = K Q^T of 32 keys and 32
+// rows (32 x 32 x 16), so that a code unpacked serves 32 rows, and a lane holds 16 keys of one row. K row
+// m of a tile is key swap23(m), so that the score registers (half = lane / 32) are keys 8 half + 0..7 and
+// 16 + 8 half + 0..7, the B operands of O^T = V^T P^T as they are: no probability passes through LDS, and
+// a row's sums and factors stay in its lanes. The keys' factors reach their registers by a broadcast within
+// 16 lanes, lane r holding register r's. Some 325 vector instructions and 19 MFMAs a wave's step of 32
+// keys, where two 16-row tiles of k_attention_kv4_few take 540: 0.92 us a step with one wave a SIMD. 128
+// groups of 25 rows over a window of 4,096 keys 28 us (36 in two tiles of 16 rows); 512 groups of 64 rows
+// over 8,192 keys 251 us (373).
+constexpr int kMidRows = 32, kMidKeys = 32;
+constexpr float kMidTop = 128.0f;  // a lane's 16 probabilities sum to no more, or m is raised
+
+template <int D>
+struct MidStep {
+  uint32_t k[D / 16];  // key swap23(lane % 32): channels D/2 half and on
+  uint32_t v[16];      // keys 16 (e / 8) + 8 half + e % 8: channels D/32 (lane % 32) and on
+  uint32_t kw, ks, vs;  // words: the K word of that key, and K's and V's of register lane % 16's key
+  uint64_t hidden;     // a bit per lane: the key's page is none of the cache's
+};
+
+// `ids`: the page of key `key` + swap23(lane % 32).
+template <int D>
+__device__ __forceinline__ void load_mid(const Args& a, int ids, uint32_t head, int key, int lane,
+                                         MidStep<D>& s) {
+  const uint32_t n = lane & 31, half = lane >> 5;
+  const uint32_t page_tokens = 1u << a.page_shift, mask = page_tokens - 1;
+  const uint32_t block = page_tokens * (D + 8), in_page = ((uint32_t)key + swap23(n)) & mask;
+  // Keys of no page are masked; page 0 is there to read.
+  const uint8_t* page = a.cache + (uint64_t)head * block +
+                        (uint64_t)(uint32_t)max(ids, 0) * (block * a.kv_heads);
+  s.hidden = __ballot(ids < 0);
+  const uint8_t *lo = lane_pointer(page, 0), *hi = lane_pointer(page, 16);  // of each 16 keys
+  const uint8_t* mine = page + (in_page * (D / 2) + half * (D / 4));
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    const uint4 x = *reinterpret_cast<const uint4*>(mine + 16 * i);
+    s.k[4 * i] = x.x, s.k[4 * i + 1] = x.y, s.k[4 * i + 2] = x.z, s.k[4 * i + 3] = x.w;
+  }
+  s.kw = *reinterpret_cast<const uint32_t*>(page + (page_tokens * D + 4 * in_page));
+  const uint32_t at[2] = {(uint32_t)key & mask, ((uint32_t)key + 16) & mask};
+  const uint8_t* words = lane & 8 ? hi + 4 * at[1] : lo + 4 * at[0];
+  words += page_tokens * D + 4 * ((lane & 7) + 8 * half);
+  s.ks = *reinterpret_cast<const uint32_t*>(words);
+  s.vs = *reinterpret_cast<const uint32_t*>(words + page_tokens * 4);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const uint8_t* v = (t ? hi : lo) + (page_tokens + at[t]) * (D / 2) + (8 * half * (D / 2) + n * (D / 64));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (D == 128)
+        s.v[8 * t + e] = *reinterpret_cast<const uint16_t*>(v + e * 64);
+      else
+        s.v[8 * t + e] = v[e * 32];
+    }
+  }
+}
+
+// ps: p times its key's f, and sum: the products of p with its key's `add`, added up. (As an instruction of
+// its own: the compiler broadcasts `add` to a register first.)
+template <int R = 0>
+__device__ __forceinline__ void weigh(float f, float add, const float (&p)[16], float (&ps)[16],
+                                      float& sum) {
+  if constexpr (R < 16) {
+    ps[R] = p[R] * spread<R>(f);
+    asm("v_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf"
+        : "+v"(sum) : "v"(add), "v"(p[R]), "n"(R));
+    weigh<R + 1>(f, add, p, ps, sum);
+  }
+}
+
+template <int D, bool kBf16>
+__global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
+  constexpr int kSteps = D / 16, kBlocks = D / 32;
+  __shared__ __attribute__((aligned(16))) float lds_o[kWaves][kMidRows][D + 4];
+  __shared__ float2 lds_ml[kWaves][kMidRows];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 31, half = lane >> 5;
+  const uint32_t tile = blockIdx.y / a.kv_heads, head = blockIdx.y - tile * a.kv_heads;
+  const uint32_t b = blockIdx.z, part = blockIdx.x;
+  const int32_t* table = a.table + (size_t)b * a.table_stride;
+  const Sequence seq = sequence(a, b);
+  const int group = (int)a.group, rows = seq.rows * group, stride = (int)a.parts * kWaves;
+  const int row0 = (int)tile * kMidRows, mine = (int)swap23(n);
+  int step = (int)part * kWaves + wave;
+  if (a.window) step += span(a, seq, row0 / group).x / kMidKeys;
+  int ids = page_of(a, table, step * kMidKeys + mine);
+  MidStep<D> tiles[2];
+  load_mid<D>(a, ids, head, step * kMidKeys, lane, tiles[0]);
+  ids = page_of(a, table, (step + stride) * kMidKeys + mine);
+  if (row0 >= rows || !takes(a, rows)) return;
+  const int2 first_span = span(a, seq, row0 / group);
+  const int2 last_span = span(a, seq, (min(row0 + kMidRows, rows) - 1) / group);
+  const int key_lo = first_span.x, key_hi = last_span.y;  // seen by some row
+  const int all_lo = last_span.x, all_hi = first_span.y;  // seen by every row
+  const int last = (key_hi + kMidKeys - 1) / kMidKeys;
+  const uint32_t heads = a.kv_heads * a.group;
+  const int row = row0 + n, token = row / group, g = row - token * group;
+  if (part > 0 && step - wave >= last) {  // no keys: part 0 stands for an empty row
+    if (threadIdx.x < kMidRows && row < rows) a.part_ml[few_place(a, part, b, row, head)] = {-kInf, 0};
+    return;
+  }
+
+  // Q operands: channels D/2 half + 8 s + {0,4,1,5,2,6,3,7}. Rows past the last are zeros.
+  uint4 qf[kSteps];
+  float sum = 0.0f;
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    uint4 x = {0, 0, 0, 0};
+    if (row < rows)
+      x = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) +
+                                          (size_t)(seq.start + token) * a.q_stride +
+                                          (head * group + g) * D + (D / 2) * half + 8 * s);
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += widen<kBf16>(w[i] & 0xffffu) + widen<kBf16>(w[i] >> 16);
+    qf[s] = {(x.x & 0xffffu) | (x.z << 16), (x.x >> 16) | (x.z & 0xffff0000u),
+             (x.y & 0xffffu) | (x.w << 16), (x.y >> 16) | (x.w & 0xffff0000u)};
+  }
+  const float q_sum = across32<false>(sum);
+  const int2 seen = row < rows ? span(a, seq, token) : int2{0, 0};
+
+  RowSums<D> r;
+#pragma unroll
+  for (int d = 0; d < kBlocks; ++d) r.o[d] = v16f{};
+  r.m = row < rows ? -kInf : 0.0f;
+  r.l = 0.0f;
+  float mid = 0.0f;                    // sum p (m + 8 s)
+  float s_top = 0.0f, s_factor = 0.0f;  // f16: a power of two no scale passes, and kHeld over it
+  // The sum of a row's p s, by a 16 x 16 x 32 product of the same operands: its columns are rows n % 16,
+  // lanes 16 and on of each half bringing the keys of rows 16 and on, and its rows 4 (lane / 16) and on
+  // take the ones of the lane's own kind.
+  v4f ones = {0, 0, 0, 0};
+  const uint32_t one2 = ((lane >> 2) & 1) == ((lane >> 4) & 1) ? (kBf16 ? 0x3F803F80u : 0x3C003C00u) : 0u;
+  const uint4 one8 = {one2, one2, one2, one2};
+  const Codes codes = make_codes<kBf16>();
+
+  auto attend = [&](const MidStep<D>& cur, MidStep<D>& next) {
+    const int key0 = step * kMidKeys;
+    if (step + stride < last) {
+      const int now = ids;
+      ids = page_of(a, table, key0 + 2 * kMidKeys * stride + mine);
+      load_mid<D>(a, now, head, key0 + kMidKeys * stride, lane, next);
+    }
+    v16f x = v16f{};
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      const uint4 kf = {code_pair<kBf16>(cur.k[s], 0, codes), code_pair<kBf16>(cur.k[s], 1, codes),
+                        code_pair<kBf16>(cur.k[s], 2, codes), code_pair<kBf16>(cur.k[s], 3, codes)};
+      x = mfma32<kBf16>(kf, qf[s], x);
+    }
+    const float ks = widen<kBf16>(cur.ks >> 16) * a.scale;
+    float km = widen<kBf16>(cur.kw & 0xffffu) * a.scale;
+    km = fmaf(-16.0f, widen<kBf16>(cur.kw >> 16) * a.scale, km);
+    float vs = widen<kBf16>(cur.vs >> 16), vm = fmaf(8.0f, vs, widen<kBf16>(cur.vs & 0xffffu));
+    const bool whole = key0 >= all_lo && key0 + kMidKeys <= all_hi && cur.hidden == 0;
+    if (!whole) {
+      // A key whose V words hold a NaN gives NaN through its score, where only the rows that see it
+      // look; the words of keys that no row sees may hold anything.
+      const bool nan = has_nan<kBf16>(cur.vs);
+      const uint64_t nans = __ballot(nan);  // of register lane % 16's keys
+      if ((nans >> ((mine & 7) | (mine & 8) << 2 | (mine & 16) >> 1)) & 1) km = __uint_as_float(0x7fc00000u);
+      const int key = key0 + (lane & 7) + 8 * half + 2 * (lane & 8);
+      const bool none = key < key_lo || key >= key_hi || (cur.hidden >> (2 * (lane & 8))) & 1;
+      if (none || nan) vs = vm = 0.0f;
+    }
+    scale_scores(ks, x);
+    const v16f y = [&] {
+      v16f y = __builtin_amdgcn_mfma_f32_32x32x2f32(half ? -1.0f : km, half ? r.base() : q_sum, x, 0, 0, 0);
+      if (!whole) {
+        asm volatile("");  // a branch, not 16 selects in every step
+        const int lo = seen.x - key0 - 8 * half, hi = seen.y - key0 - 8 * half;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int k = (i & 7) + 2 * (i & 8);
+          if (k < lo || k >= hi || (cur.hidden >> (2 * (i & 8))) & 1) y[i] = -kInf;
+        }
+      }
+      return y;
+    }();
+    float p[16], ts = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p[i] = __builtin_amdgcn_exp2f(y[i]);
+      ts += p[i];
+    }
+    bool raise = !(ts <= kMidTop) || r.m == -kInf;
+    if constexpr (!kBf16) raise |= vs > s_top;
+    if (__any(raise)) {
+      float ratio = 1.0f;
+      if constexpr (!kBf16) {
+        const float s = across32<true>(across16<true>(over16<true>(vs)));
+        if (s > s_top) {
+          const float up = __uint_as_float((__float_as_uint(s) + 0x7fffffu) & 0x7f800000u);
+          ratio = s_top / up;
+          s_top = up;
+          s_factor = kHeld / up;
+        }
+      }
+      const float was = r.base();
+      float top = y[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, y[i]);
+      top = across32<true>(top) + was;
+      const float up = fmaxf(r.m, top);
+      const float alpha = __builtin_amdgcn_exp2f(r.m - (up == -kInf ? 0.0f : up));
+      r.m = up;
+      const float by = was - r.base();
+      r.l *= alpha;
+      mid *= alpha;
+      ones *= alpha * ratio;
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d) r.o[d] *= alpha * ratio;
+      ts = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        p[i] = __builtin_amdgcn_exp2f(y[i] + by);
+        ts += p[i];
+      }
+    }
+    r.l += ts;
+    float ps[16];
+    asm("s_nop 1" : "+v"(vm));  // between its writing and a broadcast
+    weigh(kBf16 ? vs : vs * s_factor, vm, p, ps, mid);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float* w = ps + 8 * t;
+      const uint4 pf = {narrow2<kBf16>(w[0], w[1]), narrow2<kBf16>(w[2], w[3]), narrow2<kBf16>(w[4], w[5]),
+                        narrow2<kBf16>(w[6], w[7])};
+      ones = mfma16<kBf16>(one8, pf, ones);
+      uint32_t v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = cur.v[8 * t + 2 * i] | (cur.v[8 * t + 2 * i + 1] << 16);
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d)
+        r.o[d] = mfma32<kBf16>({code_pair<kBf16>(v[0], d, codes), code_pair<kBf16>(v[1], d, codes),
+                                code_pair<kBf16>(v[2], d, codes), code_pair<kBf16>(v[3], d, codes)},
+                               pf, r.o[d]);
+    }
+  };
+  for (; step < last; step += stride) {
+    attend(tiles[0], tiles[1]);
+    step += stride;
+    if (step >= last) break;
+    attend(tiles[1], tiles[0]);
+  }
+
+  // Join the four waves. Register i of block d holds channel (D/32) (8 (i / 4) + 4 half + i % 4) + d.
+  const float unit = kBf16 ? 1.0f : s_top * (1.0f / kHeld);
+  const float l = across32<false>(r.l), add = across32<false>(mid);
+  if (half == 0) lds_ml[wave][n] = {r.m, l};
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float* to = &lds_o[wave][n][kBlocks * (8 * (i / 4) + 4 * half + i % 4)];
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d) to[d] = fmaf(unit, fmaf(-24.0f, ones[0], r.o[d][i]), add);
+  }
+  __syncthreads();
+  const int at = (int)threadIdx.x / 8, ch = 4 * ((int)threadIdx.x % 8);  // channels ch + 32 j + 0..3
+  const int out_row = row0 + at;
+  if (out_row >= rows) return;
+  float2 ml[kWaves];
+  float top = -kInf, total = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    ml[w] = lds_ml[w][at];
+    top = fmaxf(top, ml[w].x);
+  }
+  const float base = top == -kInf ? 0.0f : top;
+  float4 sums[kBlocks];
+#pragma unroll
+  for (int j = 0; j < kBlocks; ++j) sums[j] = {0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float f = __builtin_amdgcn_exp2f(ml[w].x - base);
+    total = fmaf(f, ml[w].y, total);
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j) {
+      const float4 x = *reinterpret_cast<const float4*>(&lds_o[w][at][ch + 32 * j]);
+      sums[j] = {fmaf(f, x.x, sums[j].x), fmaf(f, x.y, sums[j].y), fmaf(f, x.z, sums[j].z),
+                 fmaf(f, x.w, sums[j].w)};
+    }
+  }
+  const int out_token = out_row / group, out_g = out_row - out_token * group;
+  const size_t q_row = (size_t)(seq.start + out_token);
+  const uint32_t q_head = head * group + out_g;
+  if (a.parts > 1) {
+    const size_t place = few_place(a, part, b, out_row, head);
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j)
+      *reinterpret_cast<float4*>(a.part_o + place * D + ch + 32 * j) = sums[j];
+    if (ch == 0) a.part_ml[place] = {top, total};
+  } else {
+    const bool none = total == 0.0f;  // a NaN among the scores leaves total NaN
+    const float inv = none ? 0.0f : 1.0f / total;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + ch;
+#pragma unroll
+    for (int j = 0; j < kBlocks; ++j)
+      *reinterpret_cast<uint2*>(out + 32 * j) = {narrow2<kBf16>(sums[j].x * inv, sums[j].y * inv),
+                                                 narrow2<kBf16>(sums[j].z * inv, sums[j].w * inv)};
+    if (a.lse && ch == 0) a.lse[q_row * heads + q_head] = none ? -kInf : (top + __log2f(total)) * kLn2;
+  }
+}
+
 // One wave's joined row: D/64 channels a lane.
 template <int D, bool kBf16>
 __device__ __forceinline__ void write_row(const Args& a, size_t q_row, uint32_t q_head, int lane,
@@ -1247,7 +1515,9 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_rows_join(Args a) {
 // Joins the parts of a row: W waves per (row, query head), wave w the parts w, w + W, ..; lane p of a
 // wave holds part p's weight (kMaxParts lanes at most). A part without keys has no sums to read.
 constexpr uint32_t kMaxParts = 64;
-constexpr uint32_t kFewRows = 32;  // what k_attention_kv4_few holds
+constexpr uint32_t kFewRows = 32;    // rows in one tile of k_attention_kv4_few or _mid
+constexpr uint32_t kFewMost = 4096;  // rows of a sequence that they take
+constexpr double kFewBytes = 64e6;   // of their parts' sums
 
 // At least the row tiles of a call's sequences: a sequence of r rows has r / 256 and a part of one.
 uint32_t line_tiles(uint32_t batch, uint32_t q_rows, uint32_t max_q, uint32_t group) {
@@ -1323,15 +1593,15 @@ hipError_t launch_few(Args a, const Kv4Launch& plan, hipStream_t stream) {
   a.rows_to = plan.rows_to;
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)plan.parts * a.batch * plan.rows_to *
                                                        a.kv_heads * D);
-  const dim3 grid(plan.parts, a.kv_heads, a.batch);
+  const dim3 grid(plan.parts, a.kv_heads * plan.row_tiles, a.batch);
   if (plan.tile_rows == 4)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 4, 1>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 4>), grid, dim3(kThreads), 0, stream, a);
   else if (plan.tile_rows == 8)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 8, 1>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 8>), grid, dim3(kThreads), 0, stream, a);
   else if (plan.tile_rows == 16)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16, 1>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16>), grid, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16, 2>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_attention_kv4_mid<D, kBf16>), grid, dim3(kThreads), 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || plan.parts == 1) return e;
   const uint32_t rows = std::min(a.max_q * a.group, plan.rows_to);
@@ -1383,73 +1653,127 @@ hipError_t launch_both(const Args& a, const Kv4Plan& plan, hipStream_t stream) {
 }  // namespace
 
 // How a call is cut. The host knows no sequence's rows or keys, only that none has more than max_q rows
-// and more keys than the table holds (or a window shows).
+// and more keys than the table holds (or a window shows); it estimates times, in us from one MI355X's
+// figures, and takes the least.
 //
-// Which kernel: k_attention_kv4_few up to 32 rows, k_attention_kv4_rows beyond. A call with longer
-// sequences that are not all alike may hold single tokens too (prompts beside decoding): those go to few,
-// in tiles of the 4, 8, 16 or 32 rows that hold the group's heads, and every other sequence to rows;
-// a launch's workgroups for sequences of the other kind leave at once.
-//
-// few divides a sequence's keys in the number of parts for which the time estimated from one MI355X's
-// figures is least, in us: rounds * (start + steps of a workgroup * step) + the join's, with 6 to start
-// a workgroup and join its waves, 1.2 (4 rows) to 2.7 (32 rows) per 256 keys, which are four waves'
-// step, or what HBM takes for the resident workgroups' bytes where that is more (5.0 TB/s, 4.4 with
-// one workgroup a compute unit). The join is a launch (5) and writes and reads every part's sums in
-// f32. Timed: 16 groups of 129,024 keys 74, 65 and 68 us in 16, 32 and 64 parts; 128 groups of 32 rows
-// over 4,100 keys 52, 37, 49 and 66 us in 1, 2, 4 and 8; 512 groups of up to 8,192 keys 82, 85, 87 and
-// 98 us; 8 groups of 1,000 keys 10.6, 10.5, 9.4 and 9.0 us, where the second launch costs the host more
+// The kernel: up to 32 rows a sequence k_attention_kv4_few or _mid, in tiles of 4, 8, 16 or 32 rows. Beyond,
+// tiles of 32 rows there or of 256 in k_attention_kv4_rows: the small ones fill the chip and divide the
+// keys where the large ones would leave it idle, the large ones unpack a key once for 256 rows. In us,
+// small and large, 4 query heads to each of 8 cache heads: one sequence of 1,000 keys 12 and 26 (64 rows),
+// 12 and 39 (256 rows); 64 sequences of 5,000 keys 163 and 253 (48 rows), 630 and 400 (256 rows).
+// A call with longer sequences that are not all alike may hold single tokens too (prompts beside
+// decoding): the large tiles leave those to the small ones; a launch's workgroups for sequences of the
+// other kind leave at once.
+namespace {
+
+// k_attention_kv4_few or _mid for sequences of up to `rows` rows, and its time (all_rows: of all
+// sequences; keys: of a tile, of which its rows see the part `seen` on average). The keys are divided in
+// the number of parts for which that is least: rounds * (start + steps of a workgroup * step) + the
+// join's, with 6 or 7 to start a workgroup and join its waves; per four waves' step 1.2 to 1.8 (256 keys,
+// 4 to 16 rows), or 0.95 for each workgroup on a compute unit (128 keys, 32 rows), or what HBM takes for
+// the resident workgroups' bytes where that is more (5.0 TB/s, 4.4 with one workgroup a compute unit). The
+// join is a launch (5) and writes and reads every part's sums in f32.
+// Timed: 16 groups of 129,024 keys 74, 65 and 68 us in 16, 32 and 64 parts; 128 groups of 25 rows over a
+// window of 4,096 keys 41, 30, 31 and 29 us in 1, 2, 3 and 4; 512 groups of up to 8,192 keys 82, 85, 87
+// and 98 us; 8 groups of 1,000 keys 10.6, 10.5, 9.4 and 9.0 us, where the second launch costs the host more
 // than the split gains.
-//
-// rows takes a workgroup per row tile and cache head, or (parts: how many workgroups) one line of all
-// their keys, as k_attention_kv4_line does, where the workgroups would fill the chip badly: 2.3 us per
-// 64 keys either way, against 12 to find the line and the join's traffic, two row tiles' sums a
-// workgroup.
+Kv4Launch plan_few(const h3_kv4_cfg& cfg, uint32_t rows, uint32_t batch, double all_rows, uint64_t keys,
+                   double seen, uint32_t cus, bool divide, double* time) {
+  const uint32_t tile = rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : kMidRows;
+  const uint32_t tiles = (rows + tile - 1) / tile;
+  const int step_keys = kWaves * (tile == kMidRows ? kMidKeys : kStepKeys);
+  const double step = tile <= 4 ? 1.2 : tile <= 8 ? 1.3 : tile <= 16 ? 1.8 : 0.95;
+  const double groups = cfg.kv_heads * std::min((double)batch * tiles, all_rows / tile + batch);
+  const double slots = 2.0 * cus, start = tile == kMidRows ? 7 : 6;
+  const uint64_t steps = (keys + step_keys - 1) / step_keys;
+  Kv4Launch p = {tile, tiles, 1, 0, rows};
+  const double part_bytes = (double)batch * rows * cfg.kv_heads * (cfg.head_dim + 2) * 4;
+  for (uint32_t n = 1; n <= (divide ? kMaxParts : 1) && (n == 1 || n <= steps); ++n) {
+    if (n > 1 && n * part_bytes > kFewBytes) break;
+    const double wgs = groups * n;
+    const double each = std::ceil(std::min(wgs, slots) / cus);  // on the fullest compute units
+    const double hbm = (each > 1 ? each * cus : wgs) * step_keys * (cfg.head_dim + 8) /
+                       (each > 1 ? 5.0e6 : 4.4e6);
+    const double one = std::max(tile == kMidRows ? step * each : step, hbm);
+    const double longest = (double)((steps + n - 1) / n), usual = longest * seen;
+    const double t = std::max(std::ceil(wgs / slots) * (start + usual * one), start + longest * one) +
+                     (n > 1 ? 5 + wgs * std::min(rows, tile) * (cfg.head_dim + 2) * 8 / 4e6 : 0);
+    if (n == 1 || t < *time) {
+      p.parts = n;
+      *time = t;
+    }
+  }
+  return p;
+}
+
+// k_attention_kv4_rows or _line for sequences of up to `rows` rows, and its time: a workgroup per row tile
+// and cache head, or (parts: how many workgroups) one line of all their keys where the workgroups would
+// fill the chip badly: 1.1 us (one wave with rows) to 2.3 (eight) per 64 keys and 8 to start a row tile,
+// and for the line 12 to find it, a tenth more a step, and the join's traffic, two row tiles' sums a
+// workgroup. In us, apart and along a line, 4 query heads to each of 8 cache heads: 1,025 tokens of 8,192
+// keys 255 and 200; 512 of 65,536 1,950 and 640; 8,192 of 8,192 620 and 820; 12 times 700 of 5,000 784
+// and 787.
+Kv4Launch plan_many(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t rows, uint32_t batch,
+                    uint32_t q_rows, uint32_t max_q, uint64_t keys, double seen, uint32_t cus,
+                    bool divide, double* time) {
+  const uint32_t group = acfg.heads / cfg.kv_heads;
+  Kv4Launch p = {(uint32_t)kTileRows, (rows + kTileRows - 1) / kTileRows, 1, 1, rows};
+  const double step = 0.9 + 0.175 * std::min(8u, (rows + 31) / 32);  // by the waves that have rows
+  const uint32_t tiles = line_tiles(batch, q_rows, max_q, group);
+  const double most = (double)((keys + kTileKeys - 1) / kTileKeys);  // steps of a row tile
+  const bool alike = (uint64_t)batch * max_q == q_rows;
+  const double wgs =
+      cfg.kv_heads * (alike ? tiles : std::min<double>(tiles, (double)q_rows * group / kTileRows + 1));
+  const double all = wgs * most * seen;
+  const double apart = wgs <= cus ? most : std::max<double>(most, all / cus + most * 0.5 * cus / wgs);
+  *time = 4 + 8 * std::max(1.0, wgs / cus) + apart * step;
+  if (divide && tiles <= (uint32_t)kLineTiles && batch <= (uint32_t)kLineTiles &&
+      tiles * (most + 2) * cfg.kv_heads < (1u << 30)) {
+    const double lines = std::min<double>(cus, std::max(1.0, all / kLeastSteps));
+    const double sums = 2 * lines * std::min(rows, (uint32_t)kTileRows) * (cfg.head_dim + 2) * 4;
+    const double line = 12 + 8 * (wgs / lines + 1) + 1.1 * all / lines * step + 2 * sums / 4e6;
+    if (line < *time) {
+      p.parts = std::max(2u, (uint32_t)lines);
+      *time = line;
+    }
+  }
+  return p;
+}
+
+}  // namespace
+
 Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
-                 uint32_t q_rows, uint32_t max_q, uint32_t cus) {
-  Kv4Plan p{};
+                 uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide) {
   const uint32_t group = acfg.heads / cfg.kv_heads, rows = max_q * group;
-  uint64_t keys = (uint64_t)acfg.table_stride * cfg.page_tokens;
-  if (acfg.window) keys = std::min<uint64_t>(keys, (uint64_t)acfg.window + max_q);
-  uint32_t few = rows;  // rows of the longest sequence that few takes
+  const bool alike = (uint64_t)batch * max_q == q_rows;  // every sequence has max_q rows
+  const uint64_t all_keys = (uint64_t)acfg.table_stride * cfg.page_tokens;
+  const auto tile_keys = [&](uint32_t tile) {  // what the rows of a tile see at most
+    return acfg.window ? std::min<uint64_t>(all_keys, (uint64_t)acfg.window + tile / group + 1)
+                       : all_keys;
+  };
+  // A causal prompt's rows see half of its own keys on average.
+  const double seen =
+      acfg.causal && !acfg.window ? 1 - std::min<uint64_t>(all_keys, max_q) / 2.0 / all_keys : 1;
+  Kv4Plan p{};
+  double all_few = 1e30, many = 0, singles = 0;
+  Kv4Launch to_few{}, to_singles{};
+  if (rows <= kFewMost)
+    to_few = plan_few(cfg, rows, batch, (double)q_rows * group, tile_keys(kMidRows), seen, cus, divide,
+                      &all_few);
   if (rows > kFewRows) {
-    const bool alike = (uint64_t)batch * max_q == q_rows;  // every sequence has max_q rows
-    few = alike || group > kFewRows ? 0 : group;
-    p.many = {(uint32_t)kTileRows, (rows + kTileRows - 1) / kTileRows, 1, few + 1, rows};
-    const uint32_t tiles = line_tiles(batch, q_rows, max_q, group);
-    const uint64_t most = (keys + kTileKeys - 1) / kTileKeys;  // steps of a row tile
-    if (tiles <= (uint32_t)kLineTiles && batch <= (uint32_t)kLineTiles &&
-        (uint64_t)tiles * most * cfg.kv_heads < (1u << 30)) {
-      // A causal prompt's row tiles see half of its own keys on average.
-      const double mean = acfg.causal && !acfg.window && keys > max_q ? most - max_q / 128.0 : most;
-      const double wgs = std::min<double>((double)tiles, (double)q_rows * group / kTileRows + 1) * cfg.kv_heads;
-      const double all = wgs * std::max(mean, most / 2.0);
-      const double apart = wgs <= cus ? most : std::max<double>(most, all / cus + most * 0.5 * cus / wgs);
-      const double lines = std::min<double>(cus, std::max(1.0, all / kLeastSteps));
-      const double line = all / lines + (12 + 8 + 2 * lines * kTileRows * (cfg.head_dim + 2) * 8 / 4e6) / 2.3;
-      if (line < apart) p.many.parts = std::max(2u, (uint32_t)lines);
+    p.many = plan_many(cfg, acfg, rows, batch, q_rows, max_q, tile_keys(kTileRows), seen, cus, divide,
+                       &many);
+    if (!alike && group <= kFewRows)
+      to_singles = plan_few(cfg, group, batch, (double)batch * group, tile_keys(0), 1, cus, divide,
+                            &singles);
+    if (many + singles < all_few) {
+      p.few = to_singles;
+      if (p.few.parts) p.many.rows_from = p.few.rows_to + 1;
+      return p;
     }
   }
-  if (few) {
-    const uint32_t tile = few <= 4 ? 4 : few <= 8 ? 8 : few <= 16 ? 16 : 32;
-    const double step = tile <= 4 ? 1.2 : tile <= 8 ? 1.3 : tile <= 16 ? 1.8 : 2.7;
-    const double groups = (double)batch * cfg.kv_heads, slots = (tile == 32 ? 1.0 : 2.0) * cus;
-    const uint64_t steps = (keys + kWaves * kStepKeys - 1) / (kWaves * kStepKeys);
-    p.few = {tile, 1, 1, 0, few};
-    double least = 0;
-    for (uint32_t n = 1; n <= kMaxParts && (n == 1 || n <= steps); ++n) {
-      const double wgs = groups * n;
-      const double each = std::ceil(std::min(wgs, slots) / cus);  // on the fullest compute units
-      const double hbm = (each > 1 ? each * cus : wgs) * kWaves * kStepKeys * (cfg.head_dim + 8) /
-                         (each > 1 ? 5.0e6 : 4.4e6);
-      const double time =
-          std::ceil(wgs / slots) * (6 + (double)((steps + n - 1) / n) * std::max(step, hbm)) +
-          (n > 1 ? 5 + wgs * few * (cfg.head_dim + 2) * 8 / 4e6 : 0);
-      if (n == 1 || time < least) {
-        p.few.parts = n;
-        least = time;
-      }
-    }
-  }
+  p.many = Kv4Launch{};
+  p.few = to_few;
   return p;
 }
 
@@ -1464,12 +1788,11 @@ size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, uint32_t batch, const Kv4Plan&
 }
 
 hipError_t launch_attention_kv4(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
-                                uint32_t batch, uint32_t q_rows, uint32_t max_q, const void* q,
-                                const void* cache, const int32_t* table, const int32_t* lengths,
+                                const Kv4Plan& plan, uint32_t batch, uint32_t q_rows,
+                                uint32_t max_q, const void* q, const void* cache,
+                                const int32_t* table, const int32_t* lengths,
                                 const int32_t* q_starts, void* out, float* lse, void* workspace,
                                 hipStream_t stream) {
-  Kv4Plan plan = kv4_plan(cfg, acfg, batch, q_rows, max_q, device_cus());
-  if (!workspace) plan.many.parts = plan.few.parts = 1;
   Args a{};
   a.q = q;
   a.cache = static_cast<const uint8_t*>(cache);

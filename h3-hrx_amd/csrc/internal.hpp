@@ -241,11 +241,12 @@ struct Kv4Plan {
   Kv4Launch many, few;
 };
 Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
-                 uint32_t q_rows, uint32_t max_q, uint32_t cus);
+                 uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide);
 size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, uint32_t batch, const Kv4Plan& plan);
 hipError_t launch_attention_kv4(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
-                                uint32_t batch, uint32_t q_rows, uint32_t max_q, const void* q,
-                                const void* cache, const int32_t* table, const int32_t* lengths,
+                                const Kv4Plan& plan, uint32_t batch, uint32_t q_rows,
+                                uint32_t max_q, const void* q, const void* cache,
+                                const int32_t* table, const int32_t* lengths,
                                 const int32_t* q_starts, void* out, float* lse, void* workspace,
                                 hipStream_t stream);
 // VSA operations (vsa.hip)

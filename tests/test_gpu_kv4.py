@@ -229,13 +229,75 @@ def test_long_keys_in_parts_and_in_one(dev, elem, dim, heads, kv_heads, page, ne
 
 
 @pytest.mark.parametrize("elem,dim,heads,kv_heads,page,new,lengths,causal,window", [
+    (F16, 128, 17, 1, 16, [1], [200], 1, 0),                   # a tile of 17 rows
+    (BF16, 128, 31, 1, 64, [1, 1], [31, 32], 1, 0),
+    (F16, 64, 32, 1, 16, [1, 1], [33, 0], 1, 0),
+    (BF16, 64, 33, 1, 32, [1, 2, 3], [127, 128, 129], 1, 0),    # a second tile of one row
+    (BF16, 128, 5, 1, 16, [7, 7], [300, 97], 1, 0),             # a token's heads in two tiles
+    (F16, 128, 4, 2, 64, [20, 20], [1000, 20], 1, 0),
+    (BF16, 64, 10, 2, 16, [13, 13], [400, 13], 1, 50),
+    (F16, 128, 6, 1, 128, [40], [500], 0, 0),
+    (F16, 64, 3, 3, 16, [97, 5], [97, 211], 1, 0),
+    (BF16, 128, 4, 2, 16, [20], [5000], 1, 0),                  # keys in parts
+    (F16, 64, 40, 2, 256, [5, 5, 5], [3000, 2999, 1], 1, 700)])
+def test_tiles_of_32_rows(dev, elem, dim, heads, kv_heads, page, new, lengths, causal, window):
+    call = Call(dev, elem, dim, heads, kv_heads, page, new, lengths, causal=causal, window=window)
+    call.check()
+    call.check(workspace=False)
+
+
+# Sequences of more than 4,096 rows, which only the tiles of 256 take.
+@pytest.mark.parametrize("elem,dim,heads,kv_heads,page,new,lengths,causal,window", [
+    (BF16, 128, 64, 1, 16, [65], [65], 1, 0),
+    (F16, 64, 64, 1, 64, [65], [700], 1, 0),
+    (F16, 128, 64, 1, 16, [70, 1, 0], [900, 300, 50], 1, 0),      # one line of keys
+    (BF16, 128, 32, 1, 16, [140, 1, 9], [1200, 700, 300], 1, 0),  # both kinds of launch
+    (F16, 64, 16, 1, 32, [300, 1, 40], [1500, 600, 40], 1, 0),
+    (BF16, 64, 64, 1, 64, [70], [700], 0, 0),
+    (F16, 128, 64, 1, 64, [70], [700], 1, 100),                   # a window
+    (BF16, 128, 71, 1, 32, [60, 61], [60, 300], 1, 0),            # rows before any key, odd groups
+    (F16, 128, 64, 1, 16, [80, 66], [70, 3], 1, 5)])
+def test_tiles_of_256_rows(dev, elem, dim, heads, kv_heads, page, new, lengths, causal, window):
+    call = Call(dev, elem, dim, heads, kv_heads, page, new, lengths, causal=causal, window=window)
+    call.check()
+    call.check(workspace=False)
+
+
+@pytest.mark.parametrize("elem", [F16, BF16])
+def test_masked_places_of_256_rows(dev, elem):
+    """Pages that are none of the cache's, and a NaN key that the last three tokens see."""
+    call = Call(dev, elem, 128, 64, 1, 16, [70, 66], [150, 66])
+    call.table[0, 3] = -1
+    call.table[1, 0] = call.cfg.pages
+    call.check()
+    at = 150 - 3
+    slot = call.table[0, at // 16] * 16 + at % 16
+    for part in (0, 1):
+        call.plain.words[part, slot] = 0x7fff
+        out, lse, out_tol, lse_tol = call.want()
+        got, got_lse = call.run()
+        P.within(np.delete(got, [67, 68, 69], 0), np.delete(out, [67, 68, 69], 0),
+                 np.delete(out_tol, [67, 68, 69], 0))
+        assert np.isnan(got[67:70]).all() and np.isnan(got_lse[67:70]).all()
+        call.plain.words[part, slot] = 0
+
+
+def test_many_sequences(dev):
+    """More sequences than the tiles' line holds, among them prompts beside single tokens."""
+    new = [1, 3, 0, 2] * 130 + [200]
+    lengths = [5 + i % 23 for i in range(520)] + [260]
+    for i in range(0, 520, 7):
+        lengths[i] = new[i]
+    Call(dev, F16, 64, 32, 1, 16, new, lengths).check()
+
+
+@pytest.mark.parametrize("elem,dim,heads,kv_heads,page,new,lengths,causal,window", [
     (F16, 128, 8, 2, 16, [300, 40, 1, 9], [2000, 40, 700, 1111], 1, 0),  # both kinds of launch
     (BF16, 128, 4, 1, 64, [513, 257], [600, 3001], 1, 0),                # tiles that end past 256 rows
     (F16, 64, 6, 3, 32, [100, 0, 100], [4500, 50, 99], 1, 2000),         # a window, rows before any key
     (BF16, 64, 2, 2, 16, [300], [3900], 0, 0)])
-def test_row_tiles_in_one_line(dev, elem, dim, heads, kv_heads, page, new, lengths, causal, window):
-    """Few long sequences, whose row tiles share one line of keys over the workgroups: the workspace
-    holds its sums, two row tiles a workgroup."""
+def test_long_rows_in_parts_and_in_one(dev, elem, dim, heads, kv_heads, page, new, lengths, causal, window):
+    """Few long sequences, whose keys are divided."""
     call = Call(dev, elem, dim, heads, kv_heads, page, new, lengths, causal=causal, window=window)
     need = H.kv4_workspace_bytes(call.cfg, call.acfg, len(new), call.rows, max(new))
     assert need >= 2 * 2 * 256 * (dim + 2) * 4
@@ -246,14 +308,15 @@ def test_row_tiles_in_one_line(dev, elem, dim, heads, kv_heads, page, new, lengt
 def test_a_line_of_sequences_that_overlap(dev):
     """q_starts that name rows twice ask for more row tiles than the rows have: nothing is read or
     written out of bounds, and sequences whose tiles fit are right."""
-    call = Call(dev, F16, 128, 8, 1, 16, [200], [1500])
-    out, lse, out_tol, lse_tol = call.want()
-    call.new, call.lengths = [200] * 4, [1500] * 4
-    call.table = np.repeat(call.table, 4, 0)
-    call.rows = 200
-    got, got_lse = call.run(max_q=200, starts=np.array([0, 200, 0, 200, 0]))
-    P.within(got, out, out_tol)
-    P.within(got_lse, lse, lse_tol)
+    for heads in (8, 32):  # in tiles of 32 rows, and of 256 along one line
+        call = Call(dev, F16, 128, heads, 1, 16, [200], [1500])
+        out, lse, out_tol, lse_tol = call.want()
+        call.new, call.lengths = [200] * 4, [1500] * 4
+        call.table = np.repeat(call.table, 4, 0)
+        call.rows = 200
+        got, got_lse = call.run(max_q=200, starts=np.array([0, 200, 0, 200, 0]))
+        P.within(got, out, out_tol)
+        P.within(got_lse, lse, lse_tol)
 
 
 def test_a_table_wider_than_the_sequences(dev):
@@ -316,11 +379,11 @@ def test_a_nan_key_reaches_only_the_rows_that_see_it(dev, elem, new):
 
 
 @pytest.mark.parametrize("size", [2.0 ** -13, 2.0 ** 12])
-@pytest.mark.parametrize("new", [1, 100])
-def test_values_far_from_one(dev, size, new):
+@pytest.mark.parametrize("new,heads", [(1, 4), (100, 4), (70, 128)])
+def test_values_far_from_one(dev, size, new, heads):
     """f16 values of any size weigh alike: the probabilities' 16-bit form is relative to the
     values' scale."""
-    call = Call(dev, F16, 128, 4, 2, 16, [new], [new + 700])
+    call = Call(dev, F16, 128, heads, 2, 16, [new], [new + 700])
     # The last keys' values a thousandfold smaller: f16 still holds them.
     j = np.arange(new + 700)
     slots = call.table[0, j // 16] * 16 + j % 16
@@ -334,8 +397,8 @@ def test_values_far_from_one(dev, size, new):
 
 def test_scores_far_apart(dev):
     """One key's score far above the others', late and early, and scores of both signs past e^88."""
-    for late in (False, True):
-        call = Call(dev, F16, 128, 2, 1, 16, [1, 100], [900, 900])
+    for late, heads, new in ((False, 2, [1, 100]), (True, 2, [1, 100]), (True, 64, [1, 100])):
+        call = Call(dev, F16, 128, heads, 1, 16, new, [900, 900])
         for b in (0, 1):
             at = 790 if late else 2
             slot = call.table[b, at // 16] * 16 + at % 16

@@ -140,6 +140,52 @@ def test_a_call_that_leaves_the_chip_idle_asks_for_a_workspace():
     assert H.kv4_workspace_bytes(one, short, 1, 1, 1) == 0
 
 
+class Launch(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("tile", "tiles", "parts", "rows_from", "rows_to")]
+
+
+class Plan(ctypes.Structure):
+    _fields_ = [("many", Launch), ("few", Launch)]
+
+
+def test_every_sequence_has_one_launch():
+    """How calls are cut: every count of rows that a sequence can have belongs to one launch, whose tiles
+    hold it; grids and workspaces stay inside their limits."""
+    plan = H.lib()._ZN2h38kv4_planERK10h3_kv4_cfgRK20h3_kv4_attention_cfgjjjjb
+    plan.restype = Plan
+    plan.argtypes = [ctypes.c_void_p] * 2 + [ctypes.c_uint32] * 4 + [ctypes.c_bool]
+    rng = np.random.default_rng(5)
+    for _ in range(3000):
+        dim, page = int(rng.choice([64, 128])), 16 << int(rng.integers(0, 7))
+        kv_heads = int(2 ** rng.uniform(0, 8))
+        group = min(int(2 ** rng.uniform(0, 7)), 4096 // kv_heads)
+        batch, max_q = int(2 ** rng.uniform(0, 12)), int(2 ** rng.uniform(0, 14))
+        q_rows = min(2 ** 24, int(rng.integers(max_q, batch * max_q + 1)))
+        columns = max(1, int(2 ** rng.uniform(0, 20)) // page)
+        window = int(rng.integers(0, 2)) * int(2 ** rng.uniform(0, 14))
+        cfg = H.Kv4Cfg(kv_heads, dim, page, 1000, 0)
+        width = kv_heads * group * dim
+        acfg = H.Kv4AttentionCfg(kv_heads * group, width, width, columns, 1, window, 0.1)
+        for divide in (True, False):
+            p = plan(ctypes.byref(cfg), ctypes.byref(acfg), batch, q_rows, max_q, 256, divide)
+            taken = [0] * 4
+            counts = [1, group, max_q * group, max(1, max_q // 2) * group]
+            for launch in (p.many, p.few):
+                if not launch.tiles:
+                    continue
+                assert launch.parts >= 1 and (divide or launch.parts == 1)
+                for i, n in enumerate(counts):
+                    if launch.rows_from <= n <= launch.rows_to:
+                        taken[i] += 1
+                        assert n <= launch.tile * launch.tiles
+            assert taken == [1] * 4
+            assert p.few.tiles == 0 or p.few.tile in (4, 8, 16, 32)
+            assert p.few.tile == 32 or p.few.tiles <= 1
+            assert p.few.tiles * kv_heads <= 65535 and p.few.parts <= 64
+        need = H.kv4_workspace_bytes(cfg, acfg, batch, q_rows, max_q)
+        assert need <= 2 ** 28
+
+
 def test_rust_mirrors_have_the_header_fields():
     for c_name, rs_name, py in [("h3_kv4_cfg", "H3Kv4Cfg", H.Kv4Cfg),
                                 ("h3_kv4_attention_cfg", "H3Kv4AttentionCfg", H.Kv4AttentionCfg)]:
