@@ -196,13 +196,10 @@ __device__ __forceinline__ void load_step(const Args& a, int ids, uint32_t head,
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     at[t] = lane_pointer(mine, 16 * t);
-    if constexpr (D == 128) {
-      const uint4 k = *reinterpret_cast<const uint4*>(at[t] + (n * 64 + 16 * h));
-      s.k[t][0] = k.x, s.k[t][1] = k.y, s.k[t][2] = k.z, s.k[t][3] = k.w;
-    } else {
-      const uint2 k = *reinterpret_cast<const uint2*>(at[t] + (n * 32 + 8 * h));
-      s.k[t][0] = k.x, s.k[t][1] = k.y;
-    }
+    typedef uint32_t Row __attribute__((ext_vector_type(D / 32)));
+    const Row k = *reinterpret_cast<const Row*>(at[t] + (n * (D / 2) + (D / 8) * h));
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) s.k[t][i] = k[i];
   }
 #pragma unroll
   for (int c = 0; c < R / 4; ++c) {

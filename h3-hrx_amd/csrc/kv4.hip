@@ -18,9 +18,9 @@
 // Both kernels move every byte once (HBM-bound): D/8 lanes of 8 channels hold a row, so a wave
 // takes 512/D consecutive tokens of one head (their codes are 256 contiguous bytes where the slots
 // are), and the four waves of a workgroup four heads of the same tokens, which lie side by side in
-// the input rows. 129,024 rows of 8 heads of 128 channels are read back in 131 us (669 MB, 5.1 TB/s: what
-// a copy reaches); 31,104 rows are written in 44 us (161 MB, 3.7 TB/s, vector pipe 56 % busy) and read back
-// in 34; one row takes 2.2 us each way, which is a launch.
+// the input rows. 129,024 rows of 8 heads of 128 channels are read back in 123 us (669 MB, 5.4 TB/s: a
+// copy reaches 5.1); 31,104 rows are written in 31 us (161 MB, 5.2 TB/s) and read back in 25; one row takes
+// 2.2 us each way, which is a launch.
 #include "internal.hpp"
 
 namespace h3 {
@@ -119,9 +119,28 @@ __device__ __forceinline__ float quotient(float a, float b, float r) {
   return fmaf(fmaf(-q, b, a), r, q);
 }
 
+// Sixteen bytes of a row in 16 bits. Long calls (kOnce) pass the caches by: such rows are more than L2
+// holds, and what stays there is the codes. 31,104 rows written and read back took 79 us without, 61 with;
+// with the codes past the caches too, 70.
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+template <bool kOnce>
+__device__ __forceinline__ uint4 load_row(const void* rows, size_t at) {
+  const v4u* p = reinterpret_cast<const v4u*>(static_cast<const uint16_t*>(rows) + at);
+  const v4u x = kOnce ? __builtin_nontemporal_load(p) : *p;
+  return {x.x, x.y, x.z, x.w};
+}
+template <bool kOnce>
+__device__ __forceinline__ void store_row(const void* rows, size_t at, uint4 x) {
+  v4u* p = reinterpret_cast<v4u*>(static_cast<uint16_t*>(const_cast<void*>(rows)) + at);
+  if constexpr (kOnce)
+    __builtin_nontemporal_store(v4u{x.x, x.y, x.z, x.w}, p);
+  else
+    *p = {x.x, x.y, x.z, x.w};
+}
+
 // The row's word and this lane's eight codes, low nibble first. Few vector instructions a channel are
 // what keeps the kernel near HBM's rate: with a correctly rounded division by the step for every channel
-// 31,104 rows took 51 us for 44.
+// 31,104 rows took 51 us for 44 (before their loads passed the caches by).
 template <int D, bool kBf16>
 __device__ __forceinline__ uint2 quantize(uint4 raw) {
   typedef uint16_t v2us __attribute__((ext_vector_type(2)));
@@ -180,8 +199,8 @@ __global__ __launch_bounds__(kThreads) void k_kv4_write(RowArgs a) {
     slot[i] = slot_of(a, token);
     // The last row stands for the rows past it: their loads need no branch.
     const size_t row = min(token, a.tokens - 1);
-    k[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.k) + row * a.k_stride + col);
-    v[i] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.v) + row * a.v_stride + col);
+    k[i] = load_row<(N > 1)>(a.k, row * a.k_stride + col);
+    v[i] = load_row<(N > 1)>(a.v, row * a.v_stride + col);
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -243,10 +262,8 @@ __global__ __launch_bounds__(kThreads) void k_kv4_read(RowArgs a) {
     const bool live = slot[i] >= 0;
     const uint4 k = dequantize<kBf16>(live ? ck[i] : 0u, live ? wk[i] : 0u);
     const uint4 v = dequantize<kBf16>(live ? cv[i] : 0u, live ? wv[i] : 0u);
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(a.k)) +
-                              (size_t)token * a.k_stride + col) = k;
-    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(const_cast<void*>(a.v)) +
-                              (size_t)token * a.v_stride + col) = v;
+    store_row<(N > 1)>(a.k, (size_t)token * a.k_stride + col, k);
+    store_row<(N > 1)>(a.v, (size_t)token * a.v_stride + col, v);
   }
 }
 
@@ -261,14 +278,17 @@ hipError_t launch(const RowArgs& a, bool write, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Four rows a lane where that still leaves every compute unit workgroups to choose from (more loads in
-// flight, and a head's parameters of 16 tokens in one line from one wave: 31,104 rows in 51 us for 63),
-// one row where it does not (256 rows in 2.7 us).
+// One row a lane where the rows are few (256 in 2.7 us); more, and past the caches, where that still leaves
+// every compute unit workgroups to choose from: more loads in flight, and a head's parameters of 8 or 16
+// tokens in one line from one wave. Two or four, written and read back: 10,000 rows 23.6 and 24.6 us, 31,104
+// 57 and 60, 100,000 199 and 192 (219 with one).
 template <int D, bool kBf16>
 hipError_t launch_n(const RowArgs& a, bool write, hipStream_t stream) {
-  const uint64_t wgs = (uint64_t)a.tokens * D / 2048 * ((a.heads + kWaves - 1) / kWaves);
-  return wgs >= 4ull * device_cus() ? launch<D, kBf16, 4>(a, write, stream)
-                                    : launch<D, kBf16, 1>(a, write, stream);
+  const uint64_t fours = (uint64_t)a.tokens * D / 2048 * ((a.heads + kWaves - 1) / kWaves);
+  const uint64_t cus = device_cus();
+  return fours >= 32 * cus  ? launch<D, kBf16, 4>(a, write, stream)
+         : fours >= 4 * cus ? launch<D, kBf16, 2>(a, write, stream)
+                            : launch<D, kBf16, 1>(a, write, stream);
 }
 
 hipError_t rows(const h3_kv4_cfg& cfg, uint32_t tokens, uint32_t k_stride, uint32_t v_stride,

@@ -23,7 +23,9 @@ def poisoned(cfg, dev):
 
 @pytest.mark.parametrize("elem,dim,heads,page,tokens,pad", [
     (F16, 128, 8, 16, 1, 0), (BF16, 128, 8, 64, 37, 0), (F16, 64, 3, 32, 130, 24),
-    (BF16, 64, 1, 16, 7, 8), (F16, 128, 5, 256, 300, 1024), (BF16, 128, 2, 1024, 515, 8)])
+    (BF16, 64, 1, 16, 7, 8), (F16, 128, 5, 256, 300, 1024), (BF16, 128, 2, 1024, 515, 8),
+    (F16, 128, 1, 32, 20011, 16), (BF16, 64, 3, 16, 40003, 0),        # two rows a lane
+    (BF16, 128, 1, 64, 131111, 8), (F16, 64, 5, 128, 131079, 0)])
 def test_write_and_read_match_the_definition(dev, elem, dim, heads, page, tokens, pad):
     rng = np.random.default_rng(dim * tokens + heads)
     pages = tokens // page + 3
