@@ -179,9 +179,16 @@ __device__ __forceinline__ const uint8_t* lane_pointer(const uint8_t* p, int lan
   return reinterpret_cast<const uint8_t*>((uint64_t)hi << 32 | lo);
 }
 
+// A load of codes; kOnce: past the caches, where they would not be met again (see reads_once).
+template <bool kOnce, typename T>
+__device__ __forceinline__ T load_codes(const uint8_t* p) {
+  const T* from = reinterpret_cast<const T*>(p);
+  return kOnce ? __builtin_nontemporal_load(from) : *from;
+}
+
 // `ids`: lane l's is the page of key `key` + l. Sixteen keys lie side by side in a page; each lane
 // finds its own key's K codes, and the first lanes of the sixteens lend theirs to all.
-template <int D, int R>
+template <int D, int R, bool kOnce>
 __device__ __forceinline__ void load_step(const Args& a, int ids, uint32_t head, int key, int lane,
                                           Step<D, R>& s) {
   const int n = lane & 15, h = lane >> 4;
@@ -197,7 +204,7 @@ __device__ __forceinline__ void load_step(const Args& a, int ids, uint32_t head,
   for (int t = 0; t < 4; ++t) {
     at[t] = lane_pointer(mine, 16 * t);
     typedef uint32_t Row __attribute__((ext_vector_type(D / 32)));
-    const Row k = *reinterpret_cast<const Row*>(at[t] + (n * (D / 2) + (D / 8) * h));
+    const Row k = load_codes<kOnce, Row>(at[t] + (n * (D / 2) + (D / 8) * h));
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) s.k[t][i] = k[i];
   }
@@ -224,9 +231,9 @@ __device__ __forceinline__ void load_step(const Args& a, int ids, uint32_t head,
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (D == 128)
-        s.v[8 * st + e] = *reinterpret_cast<const uint32_t*>(vc + e * 64);
+        s.v[8 * st + e] = load_codes<kOnce, uint32_t>(vc + e * 64);
       else
-        s.v[8 * st + e] = *reinterpret_cast<const uint16_t*>(vc + e * 32);
+        s.v[8 * st + e] = load_codes<kOnce, uint16_t>(vc + e * 32);
     }
   }
 }
@@ -279,7 +286,7 @@ __device__ __forceinline__ size_t few_place(const Args& a, uint32_t part, uint32
   return (((size_t)part * a.batch + b) * a.rows_to + row) * a.kv_heads + head;
 }
 
-template <int D, bool kBf16, int R>
+template <int D, bool kBf16, int R, bool kOnce>
 __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
   constexpr int T = 16 / R, kTiles = R / 4, kSteps = D / 32, kDimTiles = D / 16;
   __shared__ __attribute__((aligned(16))) uint16_t lds_p[kWaves][kStepKeys * R];
@@ -299,7 +306,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
   if (a.window) step += span(a, seq, 0).x / kStepKeys;
   int ids = page_of(a, table, step * kStepKeys + lane);
   Step<D, R> tiles[2];
-  load_step<D, R>(a, ids, head, step * kStepKeys, lane, tiles[0]);
+  load_step<D, R, kOnce>(a, ids, head, step * kStepKeys, lane, tiles[0]);
   ids = page_of(a, table, (step + stride) * kStepKeys + lane);
   if (rows == 0 || !takes(a, rows)) return;
   const int2 first_span = span(a, seq, 0), last_span = span(a, seq, (rows - 1) / group);
@@ -353,7 +360,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
     if (step + stride < last) {
       const int now = ids;
       ids = page_of(a, table, key0 + 2 * kStepKeys * stride + lane);
-      load_step<D, R>(a, now, head, key0 + kStepKeys * stride, lane, next);
+      load_step<D, R, kOnce>(a, now, head, key0 + kStepKeys * stride, lane, next);
     }
     // Scores.
     v4f acc[kTiles];
@@ -1049,7 +1056,7 @@ struct MidStep {
 };
 
 // `ids`: the page of key `key` + swap23(lane % 32).
-template <int D>
+template <int D, bool kOnce>
 __device__ __forceinline__ void load_mid(const Args& a, int ids, uint32_t head, int key, int lane,
                                          MidStep<D>& s) {
   const uint32_t n = lane & 31, half = lane >> 5;
@@ -1063,7 +1070,8 @@ __device__ __forceinline__ void load_mid(const Args& a, int ids, uint32_t head, 
   const uint8_t* mine = page + (in_page * (D / 2) + half * (D / 4));
 #pragma unroll
   for (int i = 0; i < D / 64; ++i) {
-    const uint4 x = *reinterpret_cast<const uint4*>(mine + 16 * i);
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    const Words x = load_codes<kOnce, Words>(mine + 16 * i);
     s.k[4 * i] = x.x, s.k[4 * i + 1] = x.y, s.k[4 * i + 2] = x.z, s.k[4 * i + 3] = x.w;
   }
   s.kw = *reinterpret_cast<const uint32_t*>(page + (page_tokens * D + 4 * in_page));
@@ -1078,7 +1086,7 @@ __device__ __forceinline__ void load_mid(const Args& a, int ids, uint32_t head, 
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (D == 128)
-        s.v[8 * t + e] = *reinterpret_cast<const uint16_t*>(v + e * 64);
+        s.v[8 * t + e] = load_codes<kOnce, uint16_t>(v + e * 64);
       else
         s.v[8 * t + e] = v[e * 32];
     }
@@ -1098,7 +1106,7 @@ __device__ __forceinline__ void weigh(float f, float add, const float (&p)[16], 
   }
 }
 
-template <int D, bool kBf16>
+template <int D, bool kBf16, bool kOnce>
 __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
   constexpr int kSteps = D / 16, kBlocks = D / 32;
   __shared__ __attribute__((aligned(16))) float lds_o[kWaves][kMidRows][D + 4];
@@ -1115,7 +1123,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
   if (a.window) step += span(a, seq, row0 / group).x / kMidKeys;
   int ids = page_of(a, table, step * kMidKeys + mine);
   MidStep<D> tiles[2];
-  load_mid<D>(a, ids, head, step * kMidKeys, lane, tiles[0]);
+  load_mid<D, kOnce>(a, ids, head, step * kMidKeys, lane, tiles[0]);
   ids = page_of(a, table, (step + stride) * kMidKeys + mine);
   if (row0 >= rows || !takes(a, rows)) return;
   const int2 first_span = span(a, seq, row0 / group);
@@ -1169,7 +1177,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
     if (step + stride < last) {
       const int now = ids;
       ids = page_of(a, table, key0 + 2 * kMidKeys * stride + mine);
-      load_mid<D>(a, now, head, key0 + kMidKeys * stride, lane, next);
+      load_mid<D, kOnce>(a, now, head, key0 + kMidKeys * stride, lane, next);
     }
     v16f x = v16f{};
 #pragma unroll
@@ -1589,6 +1597,30 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_join(Args a) {
   write_row<D, kBf16>(a, q_row, q_head, lane, top, total, sum);
 }
 
+template <int D, bool kBf16, bool kOnce>
+void launch_tiles(const Args& a, const Kv4Launch& plan, hipStream_t stream) {
+  const dim3 grid(plan.parts, a.kv_heads * plan.row_tiles, a.batch), block(kThreads);
+  if (plan.tile_rows == 4)
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 4, kOnce>), grid, block, 0, stream, a);
+  else if (plan.tile_rows == 8)
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 8, kOnce>), grid, block, 0, stream, a);
+  else if (plan.tile_rows == 16)
+    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16, kOnce>), grid, block, 0, stream, a);
+  else
+    hipLaunchKernelGGL((k_attention_kv4_mid<D, kBf16, kOnce>), grid, block, 0, stream, a);
+}
+
+// Whether codes go past the caches: where one row tile reads them and the call may read more than half of
+// the 256 MB of the last cache, so that the next call would not meet them there. 32 sequences of 4,096 keys
+// (142 MB, 8 cache heads of 128 channels) 46 us in the caches and 41 past them, two of 129,024 63 and 58;
+// 16 of 4,096, called again and again, 27 and 31. Rows of 64 channels are a quarter of a line each and gain
+// nothing (64 sequences of 8,192 keys 53 and 58 us).
+bool reads_once(const Args& a, const Kv4Launch& plan, int dim) {
+  const double keys = (double)((uint64_t)a.table_stride << a.page_shift);
+  const double seen = a.window ? std::min(keys, (double)a.window + a.max_q) : keys;
+  return dim == 128 && plan.row_tiles == 1 && seen * a.batch * a.kv_heads * (dim + 8) > 128e6;
+}
+
 template <int D, bool kBf16>
 hipError_t launch_few(Args a, const Kv4Launch& plan, hipStream_t stream) {
   if (plan.row_tiles == 0) return hipSuccess;
@@ -1597,15 +1629,14 @@ hipError_t launch_few(Args a, const Kv4Launch& plan, hipStream_t stream) {
   a.rows_to = plan.rows_to;
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)plan.parts * a.batch * plan.rows_to *
                                                        a.kv_heads * D);
-  const dim3 grid(plan.parts, a.kv_heads * plan.row_tiles, a.batch);
-  if (plan.tile_rows == 4)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 4>), grid, dim3(kThreads), 0, stream, a);
-  else if (plan.tile_rows == 8)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 8>), grid, dim3(kThreads), 0, stream, a);
-  else if (plan.tile_rows == 16)
-    hipLaunchKernelGGL((k_attention_kv4_few<D, kBf16, 16>), grid, dim3(kThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((k_attention_kv4_mid<D, kBf16>), grid, dim3(kThreads), 0, stream, a);
+  if constexpr (D == 128) {
+    if (reads_once(a, plan, D))
+      launch_tiles<D, kBf16, true>(a, plan, stream);
+    else
+      launch_tiles<D, kBf16, false>(a, plan, stream);
+  } else {
+    launch_tiles<D, kBf16, false>(a, plan, stream);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || plan.parts == 1) return e;
   const uint32_t rows = std::min(a.max_q * a.group, plan.rows_to);

@@ -326,6 +326,15 @@ def test_a_table_wider_than_the_sequences(dev):
     Call(dev, F16, 128, 4, 2, 16, [1, 1, 2], [3, 0, 40], columns=4000).check()
 
 
+@pytest.mark.parametrize("elem", [F16, BF16])
+@pytest.mark.parametrize("heads", [3, 7, 13, 30])
+def test_a_table_of_more_keys_than_the_caches_hold(dev, elem, heads):
+    """Codes go past the caches then: by the table's width, not by the lengths."""
+    call = Call(dev, elem, 128, heads, 1, 64, [1, 1], [1700, 33], columns=16384)
+    call.check()
+    call.check(workspace=False)
+
+
 def test_entries_that_are_no_page_hide_their_keys(dev):
     call = Call(dev, BF16, 128, 4, 2, 16, [2, 1, 20], [100, 48, 200])
     call.table[0, 2] = -1
