@@ -156,9 +156,9 @@ __device__ __forceinline__ int page_of(const Args& a, const int32_t* table, int 
 // lane (n = lane % 16, h = lane / 16) then has rows (4 h + i) % R of key 16 ((4 h) / R) + n: its
 // own key's factors, and no copies. Probabilities pass through LDS, [key][R] in 16 bits, and come
 // back through the transposed read as the operand of O^T = V^T P^T.
-// 64 sequences of up to 8,192 tokens, 4 query heads to each of 8 cache heads: 353 MB in 79 us, 4.5 TB/s
-// (5.6 while all of them last; the vector pipe is 37 % busy); two of 129,024, 7 to each, in 32 parts: 281 MB
-// in 57 us and 5 for the join. About 6 us go to the launch, the first loads' chain (length, table, codes)
+// 64 sequences of up to 8,192 tokens, 4 query heads to each of 8 cache heads: 353 MB in 76 us, 4.7 TB/s
+// (more while all of them last; the vector pipe is 37 % busy); two of 129,024, 7 to each, in 32 parts: 281
+// MB in 54 us, the join's 5 with it. About 6 us go to the launch, the first loads' chain (length, table, codes)
 // and the join of the waves.
 constexpr int kStepKeys = 64;
 constexpr float kRaise = 7.0f;     // scores may pass m by this (p up to 2^7) before m is raised
@@ -1708,9 +1708,9 @@ namespace {
 // 4 to 16 rows), or 0.95 for each workgroup on a compute unit (128 keys, 32 rows), or what HBM takes for
 // the resident workgroups' bytes where that is more (5.0 TB/s, 4.4 with one workgroup a compute unit). The
 // join is a launch (5) and writes and reads every part's sums in f32.
-// Timed: 16 groups of 129,024 keys 74, 65 and 68 us in 16, 32 and 64 parts; 128 groups of 25 rows over a
-// window of 4,096 keys 41, 30, 31 and 29 us in 1, 2, 3 and 4; 512 groups of up to 8,192 keys 82, 85, 87
-// and 98 us; 8 groups of 1,000 keys 10.6, 10.5, 9.4 and 9.0 us, where the second launch costs the host more
+// Timed: 16 groups of 129,024 keys 73, 58 and 66 us in 16, 32 and 64 parts; 128 groups of 25 rows over a
+// window of 4,096 keys 40, 28, 30 and 28 us in 1, 2, 3 and 4; 512 groups of up to 8,192 keys 78, 83, 84
+// and 86 us; 8 groups of 1,000 keys 10.0, 10.4, 10.5 and 9.1 us, where the second launch costs the host more
 // than the split gains.
 Kv4Launch plan_few(const h3_kv4_cfg& cfg, uint32_t rows, uint32_t batch, double all_rows, uint64_t keys,
                    double seen, uint32_t cus, bool divide, double* time) {
