@@ -1119,6 +1119,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
   const Sequence seq = sequence(a, b);
   const int group = (int)a.group, rows = seq.rows * group, stride = (int)a.parts * kWaves;
   const int row0 = (int)tile * kMidRows, mine = (int)swap23(n);
+  if (tile > 0 && row0 >= rows) return;  // before the loads: most workgroups of a ragged call end here
   int step = (int)part * kWaves + wave;
   if (a.window) step += span(a, seq, row0 / group).x / kMidKeys;
   int ids = page_of(a, table, step * kMidKeys + mine);
@@ -1698,8 +1699,11 @@ hipError_t launch_both(const Args& a, const Kv4Plan& plan, hipStream_t stream) {
 // 12 and 39 (256 rows); 64 sequences of 5,000 keys 163 and 253 (48 rows), 630 and 400 (256 rows).
 // A call with longer sequences that are not all alike may hold single tokens too (prompts beside
 // decoding): the large tiles leave those to the small ones; a launch's workgroups for sequences of the
-// other kind leave at once.
+// other kind leave at once. A prompt of 300 tokens beside single tokens of up to 2,000 keys, in small tiles
+// alone and in both: 33 and 73 us (8 of them), 57 and 76 (32); up to 500 keys, 217 and 95 (512).
 namespace {
+
+constexpr double kLeave = 0.6e-3;  // us for a workgroup that has no rows, where sequences differ in length
 
 // k_attention_kv4_few or _mid for sequences of up to `rows` rows, and its time (all_rows: of all
 // sequences; keys: of a tile, of which its rows see the part `seen` on average). The keys are divided in
@@ -1732,7 +1736,8 @@ Kv4Launch plan_few(const h3_kv4_cfg& cfg, uint32_t rows, uint32_t batch, double 
     const double one = std::max(tile == kMidRows ? step * each : step, hbm);
     const double longest = (double)((steps + n - 1) / n), usual = longest * seen;
     const double t = std::max(std::ceil(wgs / slots) * (start + usual * one), start + longest * one) +
-                     (n > 1 ? 5 + wgs * std::min(rows, tile) * (cfg.head_dim + 2) * 8 / 4e6 : 0);
+                     (n > 1 ? 5 + wgs * std::min(rows, tile) * (cfg.head_dim + 2) * 8 / 4e6 : 0) +
+                     kLeave * n * ((double)cfg.kv_heads * batch * tiles - groups);
     if (n == 1 || t < *time) {
       p.parts = n;
       *time = t;
@@ -1761,7 +1766,8 @@ Kv4Launch plan_many(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uin
       cfg.kv_heads * (alike ? tiles : std::min<double>(tiles, (double)q_rows * group / kTileRows + 1));
   const double all = wgs * most * seen;
   const double apart = wgs <= cus ? most : std::max<double>(most, all / cus + most * 0.5 * cus / wgs);
-  *time = 4 + 8 * std::max(1.0, wgs / cus) + apart * step;
+  *time = 4 + 8 * std::max(1.0, wgs / cus) + apart * step +
+          kLeave * std::max(0.0, (double)cfg.kv_heads * batch * p.row_tiles - wgs);
   if (divide && tiles <= (uint32_t)kLineTiles && batch <= (uint32_t)kLineTiles &&
       tiles * (most + 2) * cfg.kv_heads < (1u << 30)) {
     const double lines = std::min<double>(cus, std::max(1.0, all / kLeastSteps));
