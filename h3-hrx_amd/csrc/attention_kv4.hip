@@ -1093,17 +1093,38 @@ __device__ __forceinline__ void load_mid(const Args& a, int ids, uint32_t head, 
   }
 }
 
-// ps: p times its key's f, and sum: the products of p with its key's `add`, added up. (As an instruction of
-// its own: the compiler broadcasts `add` to a register first.)
+// p times their keys' factors f.
 template <int R = 0>
-__device__ __forceinline__ void weigh(float f, float add, const float (&p)[16], float (&ps)[16],
-                                      float& sum) {
+__device__ __forceinline__ void weigh(float f, const float (&p)[16], float (&ps)[16]) {
   if constexpr (R < 16) {
     ps[R] = p[R] * spread<R>(f);
-    asm("v_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf"
-        : "+v"(sum) : "v"(add), "v"(p[R]), "n"(R));
-    weigh<R + 1>(f, add, p, ps, sum);
+    weigh<R + 1>(f, p, ps);
   }
+}
+// sum plus the products of p with their keys' `add`. One block of instructions: the compiler would move each
+// broadcast to a register first; the wait is what a broadcast's source and p, fresh from exp, ask for.
+__device__ __forceinline__ float add_weighed(float sum, float add, const float (&p)[16]) {
+  asm("s_nop 1\n"
+      "v_fmac_f32_dpp %0, %1, %2 row_newbcast:0 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %3 row_newbcast:1 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %4 row_newbcast:2 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %5 row_newbcast:3 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %6 row_newbcast:4 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %7 row_newbcast:5 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %8 row_newbcast:6 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %9 row_newbcast:7 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %10 row_newbcast:8 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %11 row_newbcast:9 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %12 row_newbcast:10 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %13 row_newbcast:11 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %14 row_newbcast:12 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %15 row_newbcast:13 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %16 row_newbcast:14 row_mask:0xf bank_mask:0xf\n"
+      "v_fmac_f32_dpp %0, %1, %17 row_newbcast:15 row_mask:0xf bank_mask:0xf\n"
+      : "+&v"(sum)
+      : "v"(add), "v"(p[0]), "v"(p[1]), "v"(p[2]), "v"(p[3]), "v"(p[4]), "v"(p[5]), "v"(p[6]), "v"(p[7]),
+        "v"(p[8]), "v"(p[9]), "v"(p[10]), "v"(p[11]), "v"(p[12]), "v"(p[13]), "v"(p[14]), "v"(p[15]));
+  return sum;
 }
 
 template <int D, bool kBf16, bool kOnce>
@@ -1258,8 +1279,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
     }
     r.l += ts;
     float ps[16];
-    asm("s_nop 1" : "+v"(vm));  // between its writing and a broadcast
-    weigh(kBf16 ? vs : vs * s_factor, vm, p, ps, mid);
+    weigh(kBf16 ? vs : vs * s_factor, p, ps);
+    mid = add_weighed(mid, vm, p);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const float* w = ps + 8 * t;
