@@ -1565,44 +1565,45 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_join(Args a) {
   constexpr int kPer = D / 64;
   __shared__ float lds_sum[W == 1 ? 1 : W][D];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const Sequence seq = sequence(a, blockIdx.z);
+  const int parts = (int)a.parts;
   const uint32_t row = blockIdx.x * (kWaves / W) + wave / W;
+  const size_t place = few_place(a, 0, blockIdx.z, min(row, a.rows_to - 1), blockIdx.y);
+  const size_t pitch = (size_t)a.batch * a.rows_to * a.kv_heads;
+  const float* from = a.part_o + place * D + lane * kPer;
+  auto load = [&](int p, float (&x)[4][kPer]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) x[i][d] = p + i * W < parts ? from[(p + i * W) * pitch * D + d] : 0.0f;
+  };
+  // The weights and the first four parts' sums are under way before the row is known to be there.
+  const float2 ml = lane < parts ? a.part_ml[lane * pitch + place] : float2{-kInf, 0.0f};
+  float x[4][kPer], sum[kPer];
+  load(wave % W, x);
+  const Sequence seq = sequence(a, blockIdx.z);
   const uint32_t token = row / a.group, g = row - token * a.group;
   if ((int)token >= seq.rows || !takes(a, seq.rows * (int)a.group)) return;
   const size_t q_row = (size_t)(seq.start + token);
   const uint32_t q_head = blockIdx.y * a.group + g;
-  const size_t place = few_place(a, 0, blockIdx.z, row, blockIdx.y);
-  const size_t pitch = (size_t)a.batch * a.rows_to * a.kv_heads;
-  const float2 ml = lane < (int)a.parts ? a.part_ml[lane * pitch + place] : float2{-kInf, 0.0f};
   const float top = across32<true>(across16<true>(over16<true>(ml.x)));
   const float f = __builtin_amdgcn_exp2f(ml.x - (top == -kInf ? 0.0f : top));
   const float total = across32<false>(across16<false>(over16<false>(f * ml.y)));
-  // The parts with sums: those with a weight or a NaN.
-  uint64_t todo = __ballot(!(ml.y == 0.0f));
-  if constexpr (W > 1) {
-    uint64_t mine = 0;
-#pragma unroll
-    for (int i = 0; i < 64; i += W) mine |= 1ull << i;
-    todo &= mine << (wave % W);
-  }
-  float sum[kPer];
+  const uint64_t live = __ballot(!(ml.y == 0.0f));  // the parts with sums: those with a weight or a NaN
 #pragma unroll
   for (int d = 0; d < kPer; ++d) sum[d] = 0.0f;
-  const float* from = a.part_o + place * D + lane * kPer;
-  while (todo) {
-    float x[4][kPer], w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {  // four loads in flight
-      const int p = todo ? __builtin_ctzll(todo) : 0;
-      w[i] = todo ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), p)) : 0.0f;
-#pragma unroll
-      for (int d = 0; d < kPer; ++d) x[i][d] = todo ? from[p * pitch * D + d] : 0.0f;
-      todo &= todo - 1;
+  for (int p = wave % W; p < parts; p += 4 * W) {
+    if (p >= 4 * W) {
+      if (live >> p == 0) break;
+      load(p, x);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      const int part = p + i * W;
+      if (part >= parts || !((live >> part) & 1)) continue;
+      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), part));
 #pragma unroll
-      for (int d = 0; d < kPer; ++d) sum[d] = fmaf(w[i], x[i][d], sum[d]);
+      for (int d = 0; d < kPer; ++d) sum[d] = fmaf(w, x[i][d], sum[d]);
+    }
   }
   if constexpr (W > 1) {
 #pragma unroll
