@@ -1134,8 +1134,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
   __shared__ float2 lds_ml[kWaves][kMidRows];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, half = lane >> 5;
-  const uint32_t tile = blockIdx.y / a.kv_heads, head = blockIdx.y - tile * a.kv_heads;
-  const uint32_t b = blockIdx.z, part = blockIdx.x;
+  const uint32_t b = blockIdx.z, part = blockIdx.x, at_y = blockIdx.y / a.kv_heads;
+  const uint32_t head = blockIdx.y - at_y * a.kv_heads;
+  // A sequence's tiles begin at a place of its own: with the first tiles, all that short sequences have, a fixed
+  // number of workgroups apart, one shader engine in four would get them (129 sequences, one of them of 30
+  // tokens in four tiles, 102 us for 42).
+  uint32_t tile = at_y + __umulhi(b * 0x9E3779B1u, a.row_tiles);
+  tile -= tile >= a.row_tiles ? a.row_tiles : 0;
   const int32_t* table = a.table + (size_t)b * a.table_stride;
   const Sequence seq = sequence(a, b);
   const int group = (int)a.group, rows = seq.rows * group, stride = (int)a.parts * kWaves;
@@ -1648,6 +1653,7 @@ template <int D, bool kBf16>
 hipError_t launch_few(Args a, const Kv4Launch& plan, hipStream_t stream) {
   if (plan.row_tiles == 0) return hipSuccess;
   a.parts = plan.parts;
+  a.row_tiles = plan.row_tiles;
   a.rows_from = plan.rows_from;
   a.rows_to = plan.rows_to;
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)plan.parts * a.batch * plan.rows_to *
@@ -1720,9 +1726,9 @@ hipError_t launch_both(const Args& a, const Kv4Plan& plan, hipStream_t stream) {
 // small and large, 4 query heads to each of 8 cache heads: one sequence of 1,000 keys 12 and 26 (64 rows),
 // 12 and 39 (256 rows); 64 sequences of 5,000 keys 163 and 253 (48 rows), 630 and 400 (256 rows).
 // A call with longer sequences that are not all alike may hold single tokens too (prompts beside
-// decoding): the large tiles leave those to the small ones; a launch's workgroups for sequences of the
-// other kind leave at once. A prompt of 300 tokens beside single tokens of up to 2,000 keys, in small tiles
-// alone and in both: 33 and 73 us (8 of them), 57 and 76 (32); up to 500 keys, 217 and 95 (512).
+// decoding): beside large tiles those have a launch of their own, in tiles of their heads; a launch's
+// workgroups for sequences of the other kind leave at once. A prompt of 300 tokens beside single tokens of up to 2,000 keys, in small tiles
+// alone and in both: 33 and 74 us (8 of them), 51 and 75 (32); up to 500 keys, 168 and 95 (512).
 namespace {
 
 constexpr double kLeave = 0.6e-3;  // us for a workgroup that has no rows, where sequences differ in length
@@ -1818,25 +1824,27 @@ Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32
   const double seen =
       acfg.causal && !acfg.window ? 1 - std::min<uint64_t>(all_keys, max_q) / 2.0 / all_keys : 1;
   Kv4Plan p{};
-  double all_few = 1e30, many = 0, singles = 0;
-  Kv4Launch to_few{}, to_singles{};
-  if (rows <= kFewMost)
-    to_few = plan_few(cfg, rows, batch, (double)q_rows * group, tile_keys(kMidRows), seen, cus, divide,
-                      &all_few);
-  if (rows > kFewRows) {
-    p.many = plan_many(cfg, acfg, rows, batch, q_rows, max_q, tile_keys(kTileRows), seen, cus, divide,
-                       &many);
-    if (!alike && group <= kFewRows)
-      to_singles = plan_few(cfg, group, batch, (double)batch * group, tile_keys(0), 1, cus, divide,
-                            &singles);
-    if (many + singles < all_few) {
-      p.few = to_singles;
-      if (p.few.parts) p.many.rows_from = p.few.rows_to + 1;
-      return p;
-    }
+  double least = 1e30;
+  const auto take = [&](const Kv4Launch& many, const Kv4Launch& few, double time) {
+    if (time < least) p = {many, few}, least = time;
+  };
+  double small = 0, large = 0, singles = 0;
+  if (rows <= kFewMost) {
+    const Kv4Launch all = plan_few(cfg, rows, batch, (double)q_rows * group, tile_keys(kMidRows), seen, cus,
+                                   divide, &small);
+    take(Kv4Launch{}, all, small);
   }
-  p.many = Kv4Launch{};
-  p.few = to_few;
+  if (rows <= kFewRows) return p;
+  Kv4Launch many = plan_many(cfg, acfg, rows, batch, q_rows, max_q, tile_keys(kTileRows), seen, cus, divide,
+                             &large);
+  if (alike || group > kFewRows) {
+    take(many, Kv4Launch{}, large);
+    return p;
+  }
+  const Kv4Launch few = plan_few(cfg, group, batch, (double)batch * group, tile_keys(0), 1, cus, divide,
+                                 &singles);
+  many.rows_from = group + 1;
+  take(many, few, large + singles);
   return p;
 }
 
