@@ -349,7 +349,7 @@ EXTRA_Q = config_f32(1.0 / math.sqrt(128.0) / 128.0)  # src/stack.rs:622-625
 
 # ------------------------------------------------------------------------- tensor plumbing
 
-_torch = None
+_torch, _one_device = None, False
 
 
 def _load_torch():
@@ -368,20 +368,21 @@ def view(t) -> View:
     live on the current GPU: a host or other-device pointer handed to a kernel faults the GPU."""
     if t is None:
         return View(None, 0)
-    if isinstance(t, View):
-        return t
     try:
         contiguous, cuda = t.is_contiguous(), t.is_cuda
     except AttributeError:
+        if isinstance(t, View):
+            return t
         raise TypeError(f"cannot bind {type(t)}") from None
     if not contiguous:
         raise ValueError("bindings must be contiguous")
     if not cuda:
         raise ValueError(f"bindings must be GPU tensors, got one on {t.device}")
-    torch = _torch or _load_torch()
-    if not _one_device and t.device.index != torch.cuda.current_device():
-        raise ValueError(f"binding on {t.device}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
+    if not _one_device:
+        torch = _torch or _load_torch()
+        if not _one_device and t.device.index != torch.cuda.current_device():
+            raise ValueError(f"binding on {t.device}, the current device is "
+                             f"cuda:{torch.cuda.current_device()}")
     return View(t.data_ptr(), t.nbytes)
 
 
