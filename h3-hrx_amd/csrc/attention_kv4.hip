@@ -671,17 +671,30 @@ __device__ __forceinline__ void fetch(const Args& a, uint32_t head, int key, int
   s.page = page;
 }
 
-// A pair of values m + s u, u as 16 + u in `code`, in the element type. f16: (u - 8) s + (m + 8 s) in
-// packed f16, exact but for the midpoint's rounding and the result's.
+// A key's s and m as its values are made of them: bf16 in f32 (m16: m - 16 s), f16 twice in a pair each.
 template <bool kBf16>
-__device__ __forceinline__ uint32_t value_pair(uint32_t code, float s, float m16, uint32_t s2,
-                                               uint32_t mid2) {
+struct Factors {
+  float s, m16;
+  uint32_t s2, m2;
+};
+template <bool kBf16>
+__device__ __forceinline__ Factors<kBf16> factors(uint32_t word) {
+  const float s = widen<kBf16>(word >> 16);
+  return {s, fmaf(-16.0f, s, widen<kBf16>(word & 0xffffu)), (word >> 16) | (word & 0xffff0000u),
+          (word & 0xffffu) | (word << 16)};
+}
+
+// A pair of values m + s u, u as 16 + u in `code`, rounded once to the element type: in f16 u is exact, and one packed
+// FMA is the value. (Never past the row's own extremes, as m + 15 s is not; a rounded midpoint m + 8 s plus (u - 8) s
+// was infinite for some rows that end near 65504.)
+template <bool kBf16>
+__device__ __forceinline__ uint32_t value_pair(uint32_t code, const Factors<kBf16>& f) {
   if constexpr (kBf16)
-    return narrow2<true>(fmaf(__uint_as_float(code << 16), s, m16),
-                         fmaf(__uint_as_float(code & 0xffff0000u), s, m16));
-  const v2h u = __builtin_bit_cast(v2h, code) - v2h{(_Float16)24.0f, (_Float16)24.0f};
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, __builtin_bit_cast(v2h, s2),
-                                                                __builtin_bit_cast(v2h, mid2)));
+    return narrow2<true>(fmaf(__uint_as_float(code << 16), f.s, f.m16),
+                         fmaf(__uint_as_float(code & 0xffff0000u), f.s, f.m16));
+  const v2h u = __builtin_bit_cast(v2h, code) - v2h{(_Float16)16.0f, (_Float16)16.0f};
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, __builtin_bit_cast(v2h, f.s2),
+                                                                __builtin_bit_cast(v2h, f.m2)));
 }
 
 template <int D, bool kBf16>
@@ -708,18 +721,14 @@ __device__ __forceinline__ void unpack(const Args& a, RowsLds<D>& lds, int buf, 
   const int key = key0 + (int)at;
   const bool nan = has_nan<kBf16>(s.word);
   const bool keep = s.page >= 0 && key >= key_lo && key < key_hi && !nan;
-  const uint32_t word = keep ? s.word : 0u;
-  const float vs = widen<kBf16>(word >> 16), vm = widen<kBf16>(word & 0xffffu);
-  const float m16 = fmaf(-16.0f, vs, vm);
-  const uint32_t s2 = narrow2<kBf16>(vs, vs), mid = narrow<kBf16>(fmaf(8.0f, vs, vm));
-  const uint32_t mid2 = mid | (mid << 16);
+  const Factors<kBf16> f = factors<kBf16>(keep ? s.word : 0u);
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) {
     uint4 x;
-    x.x = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 0, codes), vs, m16, s2, mid2);
-    x.y = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 1, codes), vs, m16, s2, mid2);
-    x.z = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 2, codes), vs, m16, s2, mid2);
-    x.w = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 3, codes), vs, m16, s2, mid2);
+    x.x = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 0, codes), f);
+    x.y = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 1, codes), f);
+    x.z = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 2, codes), f);
+    x.w = value_pair<kBf16>(code_pair<kBf16>(s.codes[i], 3, codes), f);
     *reinterpret_cast<uint4*>(&lds.v[buf][at * kVPitch<D> + 16 * (4 * i + part)]) = x;
   }
   if (part == 0) lds.vn[buf][at] = nan ? __uint_as_float(0x7fc00000u) : 0.0f;

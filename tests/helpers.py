@@ -237,3 +237,37 @@ def vsa_prefix(heads, cubes, blocks, topk, cus=256):
     fn.argtypes, fn.restype = [ctypes.c_uint32] * 5, Prefix
     p = fn(heads, cubes, blocks, topk, cus)
     return p.cubes, p.splits
+
+
+def kv4_plan(cfg, acfg, batch, q_rows, max_q, divide=True, cus=256):
+    """How attention over the 4-bit cache is cut: the launches' (tile rows, row tiles, parts, rows_from, rows_to),
+    that of the 256-row tiles and that of the small ones, None where there is none. In more parts than
+    one the former is the line of all tiles' keys, and `parts` its workgroups."""
+    import ctypes
+
+    import h3attn as H
+
+    class Launch(ctypes.Structure):
+        _fields_ = [(n, ctypes.c_uint32) for n in ("tile", "tiles", "parts", "rows_from", "rows_to")]
+
+    class Plan(ctypes.Structure):
+        _fields_ = [("many", Launch), ("few", Launch)]
+
+    fn = H.lib()._ZN2h38kv4_planERK10h3_kv4_cfgRK20h3_kv4_attention_cfgjjjjb
+    fn.restype = Plan
+    fn.argtypes = [ctypes.c_void_p] * 2 + [ctypes.c_uint32] * 4 + [ctypes.c_bool]
+    p = fn(ctypes.byref(cfg), ctypes.byref(acfg), batch, q_rows, max_q, cus, divide)
+    return tuple(tuple(getattr(x, n) for n, _ in Launch._fields_) if x.tiles else None
+                 for x in (p.many, p.few))
+
+
+def kv4_kernels(cfg, acfg, batch, q_rows, max_q, divide=True):
+    """The names of the kernels that such a call runs."""
+    many, few = kv4_plan(cfg, acfg, batch, q_rows, max_q, divide)
+    names = []
+    if many:
+        names += ["line", "rows_join"] if many[2] > 1 else ["rows"]
+    if few:
+        names.append("mid" if few[0] == 32 else f"few{few[0]}")
+        names += ["join"] if few[2] > 1 else []
+    return names

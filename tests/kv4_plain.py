@@ -139,6 +139,81 @@ def attend(cache, acfg, q, table, new, lengths):
     return out, lse, out_tol, lse_tol
 
 
+def attend_all(cache, acfg, q, table, new, lengths, kernel):
+    """As `attend` over whole matrices, for many rows and heads, with the bounds of one kernel: "few" (tiles
+    of 4 to 32 rows) or "rows" (of 256; along a line too). A row that sees a key whose row of K or of V holds a
+    NaN or an infinity (a word that is none) has NaN in out and lse.
+
+    The bounds, with h a rounding's half step in the element type, w_j a row's weights (they sum to 1),
+    b the largest |v| it sees and n its keys:
+    - scores, sums and lse as in `attend`: (2 delta + 2 sums) 2 b of out;
+    - out once more rounded: h |out|;
+    - few: p s is rounded once, a weight of u - 8: h sum_j w_j s_j |u_j - 8|. In f16 it is held 2^8 / S times, S the
+      power of two from the largest s that any row of the tile has met (at most twice that s), and the largest p of a
+      part is 1 or more: below the normal numbers it is off by 2^-25, n S 2^-33 8 in all. The f32 sums are of
+      p s (16 + u), less 24 p s: 64 sum_j w_j s_j to the terms' roundings;
+    - rows: p and v are rounded once each: 2 h (1 + 2^-8) sum_j w_j |v_j|. In f16, p is off by 2^-25 below the normal
+      numbers, while a row's sum is 2^7 or more: n b 2^-32 in all; and v by 2^-25."""
+    c = cache.cfg
+    group, dim = acfg.heads // c.kv_heads, c.head_dim
+    rows = q.shape[0]
+    out, lse = np.zeros((rows, acfg.heads, dim)), np.full((rows, acfg.heads), -np.inf)
+    out_tol, lse_tol = np.zeros_like(out), np.zeros_like(lse)
+    qd = q.double().numpy()
+    h, f16 = HALF_STEP[c.elem], c.elem == H.H3_ELEM_F16
+    first = 0
+    for b, (n, length) in enumerate(zip(new, lengths)):
+        j = np.arange(length)
+        pages = table[b, j // c.page_tokens].astype(np.int64) if length else np.zeros(0, np.int64)
+        live = (pages >= 0) & (pages < c.pages)
+        slots = np.where(live, pages, 0) * c.page_tokens + j % c.page_tokens
+        spans = [span(n, length, i, acfg.causal, acfg.window) for i in range(n)]
+        seen = np.array([(j >= lo) & (j < hi) for lo, hi in spans], bool).reshape(n, length) & live
+        part = cache.words[:, slots]
+        fields = [from_bits(((part >> s) & 0xffff).astype(np.uint16), c.elem) for s in (0, 16)]
+        bad = ~np.isfinite(fields[0] + fields[1])            # [K, V][keys][heads]
+        m, s = (np.where(bad, 0, x) for x in fields)
+        u = cache.codes[:, slots].astype(np.float64)
+        for g in range(c.kv_heads):
+            k = m[0, :, g, None] + s[0, :, g, None] * u[0, :, g]
+            v = m[1, :, g, None] + s[1, :, g, None] * u[1, :, g]
+            nan = (seen & (bad[0, :, g] | bad[1, :, g])).any(1)
+            heads = slice(g * group, (g + 1) * group)
+            at = slice(first, first + n)
+            x = qd[at, heads].reshape(n * group, dim)
+            mask = np.repeat(seen, group, 0)
+            keys = mask.sum(1)
+            some = keys > 0
+            t = np.where(mask, (x @ k.T) * acfg.scale, -np.inf)
+            top = np.where(some, t.max(1, initial=-np.inf), 0)
+            w = np.exp(t - top[:, None])
+            total = np.where(some, w.sum(1), 1)
+            w /= total[:, None]
+            o = w @ v
+            big = np.where(mask, np.abs(v).max(1, initial=0), 0).max(1, initial=0)
+            ms = np.where(mask, np.abs(m[0, :, g]) + 31 * s[0, :, g], 0).max(1, initial=0)
+            delta = (dim + 8) * F32 * abs(acfg.scale) * np.abs(x).sum(1) * 2 * ms
+            sums = (keys / 8 + 64) * F32
+            if kernel == "few":
+                held = w @ (s[1, :, g, None] * np.abs(u[1, :, g] - 8))
+                more = 64 * (w @ s[1, :, g])
+                unit = 2 * s[1, seen.any(0), g].max(initial=0) * 2.0 ** -30 * keys if f16 else 0 * keys
+            else:
+                held, more = 2 * (1 + 2.0 ** -8) * (w @ np.abs(v)), 0
+                unit = keys * big * 2.0 ** -32 + 2.0 ** -25 if f16 else 0 * keys
+            tol = ((h * held + ((2 * delta + 2 * sums) * 2 * big + sums * more + unit)[:, None]) * (1 + h)
+                   + h * np.abs(o) + (2.0 ** -25 if f16 else 0))
+            log = np.where(some, top + np.log(total), -np.inf)
+            ltol = np.where(some, delta + sums + 4 * F32 * (np.abs(top + np.log(total)) + 1), 0)
+            gone = np.repeat(nan, group)
+            o[~some] = tol[~some] = 0
+            o[gone], log[gone] = np.nan, np.nan
+            out[at, heads], out_tol[at, heads] = (y.reshape(n, group, dim) for y in (o, tol))
+            lse[at, heads], lse_tol[at, heads] = (y.reshape(n, group) for y in (log, ltol))
+        first += n
+    return out, lse, out_tol, lse_tol
+
+
 def rows(rng, shape, elem):
     """Rows whose channels differ in size and offset."""
     dim = shape[-1]
