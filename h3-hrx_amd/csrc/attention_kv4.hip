@@ -280,6 +280,10 @@ __device__ __forceinline__ float row_lanes(float v) {
   return v;
 }
 
+// The sum l of a row's weights: NaN where its sum over values is. A key whose row of V is no number counts as one whose
+// score is none (in blocks at a mask's edge it is made one), so that out and lse say so wherever the key lies.
+__device__ __forceinline__ float or_nan(float l, float sum) { return sum != sum ? sum : l; }
+
 // Where part `part` of a row's keys leaves its sums: row `row` (of at most rows_to) of sequence b.
 __device__ __forceinline__ size_t few_place(const Args& a, uint32_t part, uint32_t b, uint32_t row,
                                             uint32_t head) {
@@ -570,6 +574,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
 #pragma unroll
       for (int d = 0; d < kPer; ++d) sum[d] = fmaf(f, lds_o[w][row][ch + d], sum[d]);
     }
+    total = or_nan(total, sum[0]);
     const int token = row / group, g = row - token * group;
     const size_t q_row = (size_t)(seq.start + token);
     const uint32_t q_head = head * group + g;
@@ -579,7 +584,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
       for (int d = 0; d < kPer; ++d) a.part_o[place * D + ch + d] = sum[d];
       if (ch == 0) a.part_ml[place] = {top, total};
     } else {
-      const bool none = total == 0.0f;  // a NaN among the scores leaves total NaN
+      const bool none = total == 0.0f;  // a NaN among the scores or values leaves total NaN
       const float inv = none ? 0.0f : 1.0f / total;
       uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + ch;
 #pragma unroll
@@ -1354,6 +1359,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
                  fmaf(f, x.w, sums[j].w)};
     }
   }
+  total = or_nan(total, sums[0].x);
   const int out_token = out_row / group, out_g = out_row - out_token * group;
   const size_t q_row = (size_t)(seq.start + out_token);
   const uint32_t q_head = head * group + out_g;
@@ -1364,7 +1370,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
       *reinterpret_cast<float4*>(a.part_o + place * D + ch + 32 * j) = sums[j];
     if (ch == 0) a.part_ml[place] = {top, total};
   } else {
-    const bool none = total == 0.0f;  // a NaN among the scores leaves total NaN
+    const bool none = total == 0.0f;  // a NaN among the scores or values leaves total NaN
     const float inv = none ? 0.0f : 1.0f / total;
     uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + ch;
 #pragma unroll

@@ -461,7 +461,8 @@ typedef struct {
  *   out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j,  lse[r][h] = ln sum_j exp(scale * q . k_j)
  * over the keys that row r sees, k and v as they stand in the cache (not rounded to 16 bits but where
  * noted in the kernels), probabilities and sums in f32. A row that sees no key gets zeros, and -inf
- * as its lse. Rows of q that belong to no sequence are left as they were in out and lse.
+ * as its lse. A key whose row of K or of V holds a NaN or an infinity makes out and lse NaN for every
+ * row that sees it, and for no other. Rows of q that belong to no sequence are left as they were in out and lse.
  *   q [q_rows][q_stride], out [q_rows][out_stride] (elem, 16-byte aligned), cache, table
  *   [batch][table_stride] i32, lengths [batch] i32, q_starts [batch + 1] i32, lse [q_rows][heads] f32
  *   or an empty view. q_rows in [1, 2^24], batch in [1, 65535], max_q in [1, q_rows]: no sequence

@@ -77,3 +77,18 @@ def test_single_values_at_the_end_of_the_range(dev, name, dim):
         x[1::2, :, 0::2], x[1::2, :, 1::2] = -65504, -4212   # s = 4086, m + 8 s = -32816
         call.plain.put(1, slots_of(call, b, keys), x.to(torch.float16))
     check(call, workspace)
+
+
+@pytest.mark.parametrize("elem", [F16, BF16])
+@pytest.mark.parametrize("name", CALLS)
+def test_a_nan_row_of_k_or_of_v_is_one_rule(dev, name, elem):
+    """A key whose row of K or of V is no number makes out and lse NaN for the rows that see it, wherever it lies:
+    in the middle of the keys that all rows see, and at their end, where some rows do not see it."""
+    call, workspace = make(dev, name, elem, 128)
+    for at in (70, call.lengths[0] - 2):
+        for part in (0, 1):
+            slot = slots_of(call, 0, np.array([at]))[0]
+            kept = call.plain.words[part, slot].copy()
+            call.plain.words[part, slot, 0] = 0x7fff
+            check(call, workspace)
+            call.plain.words[part, slot] = kept
