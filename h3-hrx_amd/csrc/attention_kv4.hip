@@ -284,6 +284,22 @@ __device__ __forceinline__ float row_lanes(float v) {
 // score is none (in blocks at a mask's edge it is made one), so that out and lse say so wherever the key lies.
 __device__ __forceinline__ float or_nan(float l, float sum) { return sum != sum ? sum : l; }
 
+// A row's results in the element type, from its sums and the sum of its weights. In f16 they are means of finite
+// values: rounding the weights to 16 bits (2^-11) may carry a mean of values near 65504 past it, and is not to make it
+// infinite. A row whose l is NaN stays NaN.
+struct Mean {
+  float inv, most;
+};
+template <bool kBf16>
+__device__ __forceinline__ Mean make_mean(float l) {
+  return {l == 0.0f ? 0.0f : 1.0f / l, or_nan(kBf16 ? kInf : 65504.0f, l)};
+}
+template <bool kBf16>
+__device__ __forceinline__ float mean(float sum, const Mean& m) {
+  const float x = sum * m.inv;
+  return kBf16 ? x : fminf(fmaxf(x, -m.most), m.most);
+}
+
 // Where part `part` of a row's keys leaves its sums: row `row` (of at most rows_to) of sequence b.
 __device__ __forceinline__ size_t few_place(const Args& a, uint32_t part, uint32_t b, uint32_t row,
                                             uint32_t head) {
@@ -585,10 +601,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
       if (ch == 0) a.part_ml[place] = {top, total};
     } else {
       const bool none = total == 0.0f;  // a NaN among the scores or values leaves total NaN
-      const float inv = none ? 0.0f : 1.0f / total;
+      const Mean by = make_mean<kBf16>(total);
       uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + ch;
 #pragma unroll
-      for (int d = 0; d < kPer; ++d) out[d] = (uint16_t)narrow<kBf16>(sum[d] * inv);
+      for (int d = 0; d < kPer; ++d) out[d] = (uint16_t)narrow<kBf16>(mean<kBf16>(sum[d], by));
       if (a.lse && ch == 0)
         a.lse[q_row * heads + q_head] = none ? -kInf : (top + __log2f(total)) * kLn2;
     }
@@ -1016,7 +1032,7 @@ __device__ __forceinline__ void attend_rows(const Args& a, RowsLds<D>& lds, cons
     return;
   }
   if (!active) return;
-  const float inv = none ? 0.0f : 1.0f / total;
+  const Mean by = make_mean<kBf16>(total);
   // Through LDS (each wave its own 32 rows) so that whole rows leave together.
   uint8_t* rows_lds = reinterpret_cast<uint8_t*>(&lds) + wave * 32 * 2 * D;
   static_assert(sizeof(lds.k) + sizeof(lds.v) >= 8 * 32 * 2 * D && offsetof(RowsLds<D>, k) == 0 &&
@@ -1027,9 +1043,10 @@ __device__ __forceinline__ void attend_rows(const Args& a, RowsLds<D>& lds, cons
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       uint8_t* to = rows_lds + n * (2 * D) + 16 * (chunk_word<D>(4 * d + i) ^ (n & (D / 8 - 1))) + 4 * half;
-      *reinterpret_cast<uint32_t*>(to) = narrow2<kBf16>(o[d][4 * i] * inv, o[d][4 * i + 2] * inv);
+      *reinterpret_cast<uint32_t*>(to) =
+          narrow2<kBf16>(mean<kBf16>(o[d][4 * i], by), mean<kBf16>(o[d][4 * i + 2], by));
       *reinterpret_cast<uint32_t*>(to + 8) =
-          narrow2<kBf16>(o[d][4 * i + 1] * inv, o[d][4 * i + 3] * inv);
+          narrow2<kBf16>(mean<kBf16>(o[d][4 * i + 1], by), mean<kBf16>(o[d][4 * i + 3], by));
     }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
@@ -1371,12 +1388,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
     if (ch == 0) a.part_ml[place] = {top, total};
   } else {
     const bool none = total == 0.0f;  // a NaN among the scores or values leaves total NaN
-    const float inv = none ? 0.0f : 1.0f / total;
+    const Mean by = make_mean<kBf16>(total);
     uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + ch;
 #pragma unroll
     for (int j = 0; j < kBlocks; ++j)
-      *reinterpret_cast<uint2*>(out + 32 * j) = {narrow2<kBf16>(sums[j].x * inv, sums[j].y * inv),
-                                                 narrow2<kBf16>(sums[j].z * inv, sums[j].w * inv)};
+      *reinterpret_cast<uint2*>(out + 32 * j) = {
+          narrow2<kBf16>(mean<kBf16>(sums[j].x, by), mean<kBf16>(sums[j].y, by)),
+          narrow2<kBf16>(mean<kBf16>(sums[j].z, by), mean<kBf16>(sums[j].w, by))};
     if (a.lse && ch == 0) a.lse[q_row * heads + q_head] = none ? -kInf : (top + __log2f(total)) * kLn2;
   }
 }
@@ -1386,12 +1404,12 @@ template <int D, bool kBf16>
 __device__ __forceinline__ void write_row(const Args& a, size_t q_row, uint32_t q_head, int lane,
                                           float m, float l, const float (&sum)[D / 64]) {
   const bool none = l == 0.0f;
-  const float inv = none ? 0.0f : 1.0f / l;
+  const Mean by = make_mean<kBf16>(l);
   uint16_t* out = static_cast<uint16_t*>(a.out) + q_row * a.out_stride + q_head * D + lane * (D / 64);
   if constexpr (D == 128)
-    *reinterpret_cast<uint32_t*>(out) = narrow2<kBf16>(sum[0] * inv, sum[1] * inv);
+    *reinterpret_cast<uint32_t*>(out) = narrow2<kBf16>(mean<kBf16>(sum[0], by), mean<kBf16>(sum[1], by));
   else
-    *out = (uint16_t)narrow<kBf16>(sum[0] * inv);
+    *out = (uint16_t)narrow<kBf16>(mean<kBf16>(sum[0], by));
   if (a.lse && lane == 0)
     a.lse[q_row * (a.kv_heads * a.group) + q_head] = none ? -kInf : (m + __log2f(l)) * kLn2;
 }

@@ -79,6 +79,27 @@ def test_single_values_at_the_end_of_the_range(dev, name, dim):
     check(call, workspace)
 
 
+@pytest.mark.parametrize("high", [True, False])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("name", CALLS)
+def test_means_at_the_end_of_the_range(dev, name, dim, high):
+    """f16 rows of V that hold the type's largest (lowest) value in every other channel: a mean of them is that
+    value, and what the weights lose in rounding does not carry it past it."""
+    call, workspace = make(dev, name, F16, dim)
+    kv_heads = call.cfg.kv_heads
+    # constant rows, and rows of the widest range whose ends are both held exactly (s = 8000), under weights of many
+    # keys and of hardly more than one
+    for other, size in (([-54496.0, 17264.0, 65504.0], 1), ([-54496.0], 6)):
+        other = torch.tensor(other) * (1 if high else -1)
+        for b, length in enumerate(call.lengths):
+            x = other[torch.arange(length) % len(other)].view(-1, 1, 1).repeat(1, kv_heads, dim)
+            x[:, :, ::2] = 65504 if high else -65504
+            call.plain.put(1, slots_of(call, b, np.arange(length)), x.to(torch.float16))
+        for _ in range(1 if call.rows > 40 else 8):
+            call.q = torch.from_numpy(size * call.rng.standard_normal(tuple(call.q.shape))).to(torch.float16)
+            check(call, workspace)
+
+
 @pytest.mark.parametrize("elem", [F16, BF16])
 @pytest.mark.parametrize("name", CALLS)
 def test_a_nan_row_of_k_or_of_v_is_one_rule(dev, name, elem):
