@@ -166,8 +166,15 @@ __device__ __forceinline__ uint2 quantize(uint4 raw) {
   hi = row_reduce<D, true>(hi);
   if (__float_as_uint(hi) == 0x7f800000u) return {0x7fffu, 0u};
   float part = kBf16 ? 0.5f : 1.0f;  // exact on every bf16 value, subnormal ones too
-  const uint32_t s = narrow_down<kBf16>(
-      quotient(hi * part - lo * part, 15.0f * part, (1.0f / 15.0f) / (kBf16 ? 0.5f : 1.0f)));
+  const float from = hi * part, less = lo * part, wide = from - less;
+  uint32_t s = narrow_down<kBf16>(quotient(wide, 15.0f * part, (1.0f / 15.0f) / (kBf16 ? 0.5f : 1.0f)));
+  // max - min may have more bits than f32. The scale is another then only where 15 s is what f32 holds of it: there the
+  // sign of the exact rounding error (a two-sum) decides.
+  if (widen<kBf16>(s) * (15.0f * part) == wide) {
+    asm volatile("");  // a branch: one row in some hundred
+    const float back = wide - from;
+    s -= (from - (wide - back)) - (less + back) < 0.0f ? 1 : 0;
+  }
   if (kBf16 && widen<kBf16>(s) < 0x1p-60f) part = 0x1p99f;  // the reciprocal stays finite
   const float low = lo * part, step = widen<kBf16>(s) * part;
   uint32_t codes = 0;

@@ -399,8 +399,8 @@ int h3_attention_i8qkhm_cross(const h3_cross_cfg *cfg, h3_view qi, h3_view qs, h
  *   elem         H3_ELEM_F16 or H3_ELEM_BF16: the rows' type and the parameters'
  * A row is one token's head_dim channels of one head, of K or of V. It is held as m = min x, s =
  * (max x - m) / 15 rounded toward zero to the element type, and 4-bit codes u = clamp(rne((x - m) /
- * s), 0, 15) (0 where s is 0), and stands for m + s * u, which never leaves [min x, max x]. A row
- * that holds a NaN or an infinity stands for NaN throughout.
+ * s), 0, 15) (0 where s is 0; x - m as f32 holds it), and stands for m + s * u, which never leaves
+ * [min x, max x]. A row that holds a NaN or an infinity stands for NaN throughout.
  * Layout: per page, per head, one block of page_tokens * (head_dim + 8) bytes: K codes
  * [page_tokens][head_dim / 2] (low nibble first), V codes the same, K words [page_tokens] and V words
  * [page_tokens], 32 bits each with m low and s high. Slot t is token t % page_tokens of page
