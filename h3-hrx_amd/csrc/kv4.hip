@@ -145,14 +145,20 @@ template <int D, bool kBf16>
 __device__ __forceinline__ uint2 quantize(uint4 raw) {
   typedef uint16_t v2us __attribute__((ext_vector_type(2)));
   constexpr uint32_t kTop = kBf16 ? 0x7f80u : 0x7c00u;  // magnitudes from here on are no numbers
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   float x[8];
   v2us top = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(v2us, w[i] & 0x7fff7fffu));
+  const bool bad = top[0] >= kTop || top[1] >= kTop;
+  if (bad) {  // zeros in their place: no NaN meets the arithmetic, which this file's flags let assume none
+    asm volatile("");
+    w[0] = w[1] = w[2] = w[3] = 0;
+  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     x[2 * i] = widen<kBf16>(w[i] & 0xffffu);
     x[2 * i + 1] = kBf16 ? __uint_as_float(w[i] & 0xffff0000u) : widen<kBf16>(w[i] >> 16);
-    top = __builtin_elementwise_max(top, __builtin_bit_cast(v2us, w[i] & 0x7fff7fffu));
   }
   float lo = x[0], hi = x[0];
 #pragma unroll
@@ -161,7 +167,7 @@ __device__ __forceinline__ uint2 quantize(uint4 raw) {
     hi = fmaxf(hi, x[i]);
   }
   // A lane with a NaN or an infinity makes the row's maximum infinite, whatever its others are.
-  if (top[0] >= kTop || top[1] >= kTop) hi = __builtin_inff();
+  if (bad) hi = __builtin_inff();
   lo = row_reduce<D, false>(lo);
   hi = row_reduce<D, true>(hi);
   if (__float_as_uint(hi) == 0x7f800000u) return {0x7fffu, 0u};
@@ -230,7 +236,8 @@ __global__ __launch_bounds__(kThreads) void k_kv4_write(RowArgs a) {
 template <bool kBf16>
 __device__ __forceinline__ uint4 dequantize(uint32_t codes, uint32_t word) {
   constexpr uint32_t kTop = kBf16 ? 0x7f80u : 0x7c00u;
-  if ((word & kTop) == kTop) return {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+  if ((word & kTop) == kTop || ((word >> 16) & kTop) == kTop)
+    return {0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
   const float m = widen<kBf16>(word & 0xffffu), s = widen<kBf16>(word >> 16);
   uint32_t out[4];
 #pragma unroll

@@ -400,7 +400,8 @@ int h3_attention_i8qkhm_cross(const h3_cross_cfg *cfg, h3_view qi, h3_view qs, h
  * A row is one token's head_dim channels of one head, of K or of V. It is held as m = min x, s =
  * (max x - m) / 15 rounded toward zero to the element type, and 4-bit codes u = clamp(rne((x - m) /
  * s), 0, 15) (0 where s is 0; x - m as f32 holds it), and stands for m + s * u, which never leaves
- * [min x, max x]. A row that holds a NaN or an infinity stands for NaN throughout.
+ * [min x, max x]. A row that holds a NaN or an infinity stands for NaN throughout, and so does a word
+ * whose m or s is none (no written row has an s that is).
  * Layout: per page, per head, one block of page_tokens * (head_dim + 8) bytes: K codes
  * [page_tokens][head_dim / 2] (low nibble first), V codes the same, K words [page_tokens] and V words
  * [page_tokens], 32 bits each with m low and s high. Slot t is token t % page_tokens of page

@@ -74,3 +74,44 @@ def test_scales_are_rounded_toward_zero_from_the_exact_range(dev, elem, dim):
                 for w in (words[i] & 0xffff, words[i] >> 16))
         assert m == Fraction(lo) and m + int(codes[i].max()) * s <= Fraction(hi), (lo, hi)
         assert lo <= float(back[i].double().min()) and float(back[i].double().max()) <= hi, (lo, hi)
+
+
+@pytest.mark.parametrize("elem", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_rows_that_hold_no_number(dev, elem, dim):
+    """Every kind of NaN and infinity, in every lane's channels and several in a row, beside rows of numbers:
+    0x7fff and codes 0, NaN when read back; the other rows as ever."""
+    top = 0x7c00 if elem == F16 else 0x7f80
+    kinds = [top, top | 0x8000, top | 1, top | 0x8001, 0x7fff, 0xffff, (0x7fff + top) // 2 + 1]
+    rng = np.random.default_rng(dim)
+    x = P.rows(rng, (600, dim), elem)
+    bits = x.view(torch.int16).numpy().view(np.uint16)
+    bad = np.arange(600) % 3 == 1
+    for i in np.flatnonzero(bad):
+        for c in rng.choice(dim, 1 + i % 4, replace=False):
+            bits[i, c] = kinds[(i // 3 + c) % len(kinds)]
+    bits[4] = 0xffff
+    words, codes, back = written(dev, elem, x)
+    want, want_codes, near = P.quantize(x, elem)
+    assert (words == want).all() and (words[bad] == 0x7fff).all() and (codes[bad] == 0).all()
+    assert (codes != want_codes).sum() <= near.sum()
+    assert back[bad].isnan().all() and back[~bad].isfinite().all()
+
+
+@pytest.mark.parametrize("elem", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_words_that_are_no_numbers_read_back_as_nan(dev, elem, dim):
+    """Words that no written row has: either half a NaN or an infinity."""
+    one, top = (0x3c00, 0x7c00) if elem == F16 else (0x3f80, 0x7f80)
+    words = [one | (x << 16) for x in (top, top + 1, 0x7fff, 0x8000 | top, 0xffff)]
+    words += [x | (one << 16) for x in (top, top + 1, 0x7fff, 0x8000 | top, 0xffff)] + [one | (one << 16)] * 6
+    cfg = H.Kv4Cfg(1, dim, 16, 1, elem)
+    plain = P.Cache(cfg, np.random.default_rng(1))
+    plain.words[:, :, 0] = np.array(words, np.uint32)
+    slots = torch.arange(16, dtype=torch.int32, device=dev)
+    back = torch.empty(2, 16, dim, dtype=P.DTYPES[elem], device=dev)
+    H.kv4_read(cfg, 16, dim, dim, slots, torch.from_numpy(plain.bytes()).to(dev), back[0], back[1])
+    for part in (0, 1):
+        y = back[part].cpu().double().numpy()
+        assert np.isnan(y[:10]).all()
+        assert (y[10:] == 1 + plain.codes[part, 10:, 0]).all()
