@@ -5,6 +5,7 @@
 // kernel's config.decl ranges bound its specialisation (kernels/*.loom). A failing check
 // returns its status, records a message for h3_last_error(), and launches nothing.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <initializer_list>
@@ -37,17 +38,23 @@ int ok() {
   return H3_OK;
 }
 
-// The devices of this process, which do not change while it runs: asked once (0.15 us a call).
-struct Devices {
-  int count = 0;
-  hipError_t error;
-  Devices() : error(hipGetDeviceCount(&count)) {
-    if (error != hipSuccess) (void)hipGetLastError();
+// The number of this process's devices, as check_bindings last found it on this thread, and the runtime's error where
+// it told none. Once told it does not change and is not asked for again (0.15 us a call); a count that failed is, at the
+// next call: device_ready() goes by what check_bindings found, so that no call whose bindings were not looked up runs.
+thread_local int t_devices = 0;
+thread_local hipError_t t_device_error = hipSuccess;
+
+int devices() {
+  static std::atomic<int> known{0};
+  t_devices = known.load(std::memory_order_relaxed);
+  if (t_devices > 0) return t_devices;
+  t_device_error = hipGetDeviceCount(&t_devices);
+  if (t_device_error != hipSuccess) {
+    (void)hipGetLastError();
+    t_devices = 0;
   }
-};
-const Devices& devices() {
-  static const Devices d;
-  return d;
+  if (t_devices > 0) known.store(t_devices, std::memory_order_relaxed);
+  return t_devices;
 }
 
 // src/dispatch.rs:264-276: every binding must cover the extent the kernel addresses.
@@ -64,7 +71,7 @@ int check_bindings(const char* stage, const h3_view* views, const size_t* need, 
   // this process's allocations (device, managed and pinned host memory); anything else it
   // refuses. On a host with no device, device_ready() reports that instead.
   int current = 0;
-  if (devices().count == 0) return H3_OK;
+  if (devices() == 0) return H3_OK;
   if (hipGetDevice(&current) != hipSuccess) {
     (void)hipGetLastError();
     return H3_OK;
@@ -106,10 +113,10 @@ int launched(const char* stage, hipError_t e) {
   return ok();
 }
 
+// After the call's check_bindings.
 int device_ready(const char* stage) {
-  const Devices& d = devices();
-  if (d.count == 0)
-    return set_error(H3_ERR_NO_DEVICE, "%s: no HIP device (%s)", stage, hipGetErrorString(d.error));
+  if (t_devices == 0)
+    return set_error(H3_ERR_NO_DEVICE, "%s: no HIP device (%s)", stage, hipGetErrorString(t_device_error));
   return H3_OK;
 }
 
