@@ -368,6 +368,8 @@ def view(t) -> View:
     live on the current GPU: a host or other-device pointer handed to a kernel faults the GPU."""
     if t is None:
         return View(None, 0)
+    if type(t) is View:
+        return t
     try:
         contiguous, cuda = t.is_contiguous(), t.is_cuda
     except AttributeError:
