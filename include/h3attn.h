@@ -460,22 +460,32 @@ typedef struct {
  * query rows q_starts[b] .. q_starts[b + 1] - 1 and lengths[b] keys, key j in slot
  * table[b][j / page_tokens] * page_tokens + j % page_tokens:
  *   out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j,  lse[r][h] = ln sum_j exp(scale * q . k_j)
- * over the keys that row r sees, k and v as they stand in the cache (not rounded to 16 bits but where
- * noted in the kernels), probabilities and sums in f32. A row that sees no key gets zeros, and -inf
- * as its lse. A key whose row of K or of V holds a NaN or an infinity makes out and lse NaN for every
- * row that sees it, and for no other. Rows of q that belong to no sequence are left as they were in out and lse.
+ * over the keys that row r sees, k and v as they stand in the cache. A row that sees no key gets
+ * zeros, and -inf as its lse. A key whose row of K or of V holds a NaN or an infinity makes out and
+ * lse NaN for every row that sees it, and for no other. Rows of q that belong to no sequence are left
+ * as they were in out and lse.
  *   q [q_rows][q_stride], out [q_rows][out_stride] (elem, 16-byte aligned), cache, table
- *   [batch][table_stride] i32, lengths [batch] i32, q_starts [batch + 1] i32, lse [q_rows][heads] f32
- *   or an empty view. q_rows in [1, 2^24], batch in [1, 65535], max_q in [1, q_rows]: no sequence
- *   has more rows (of one that has, the rows from max_q on are left as they were); max_q * heads /
- *   kv_heads <= 2^30. bf16 values from 2^100 on pass the range of the f32 sums.
+ *   [batch][table_stride] i32, lengths [batch] i32, q_starts [batch + 1] i32 that do not decrease, lse
+ *   [q_rows][heads] f32 or an empty view. q_rows in [1, 2^24], batch in [1, 65535], max_q in
+ *   [1, q_rows]: no sequence has more rows (of one that has, the rows from max_q on are left as they
+ *   were); max_q * heads / kv_heads <= 2^30.
+ * Precision: scores, the softmax's maxima and sums, lse and the sums over values are f32. The matrix
+ * products over values take 16 bits of the cache's type, each rounded to them once: the probability
+ * times the key's scale where a launch has tiles of 4 to 32 rows, the probability and the value itself
+ * where it has tiles of 256 (out is rounded once more). In f16 the former is held relative to the
+ * largest scale of V among the keys that any row of the tile sees, its own or not: beside one 2^22
+ * times as large a key's weight loses bits, beside one 2^33 times as large all of them. bf16 values
+ * from 2^100 on pass the range of the f32 sums.
  * The device arrays are read on the device: a call can be captured in a graph and replayed with
  * other lengths, tables and rows. Values outside their ranges read and write nothing out of bounds:
  * a table entry that is no page of the cache hides its keys, a length is cut to table_stride *
- * page_tokens, q_starts to [0, q_rows].
+ * page_tokens, q_starts to [0, q_rows]; where q_starts decreases, rows may be left as they were.
  * With a workspace of h3_kv4_workspace_bytes bytes (16-byte aligned) the keys of a call that leaves
  * the chip idle are divided and the parts joined by a second launch; without one (an empty view)
- * each row's keys are one workgroup's. Calls that share a workspace must not overlap. */
+ * each row's keys are one workgroup's. The bytes follow the configs, batch, q_rows and max_q and may
+ * fall where one of them grows; a workspace below them is refused (H3_ERR_BINDING). On 256 compute
+ * units no call needs more than 66 MiB, so that one workspace of that size serves every call. Calls
+ * that share a workspace must not overlap. */
 size_t h3_kv4_workspace_bytes(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention,
                               uint32_t batch, uint32_t q_rows, uint32_t max_q);
 int h3_attention_kv4(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention, uint32_t batch,
