@@ -616,8 +616,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
 // O^T = V^T P^T on 32 x 32 x 16. LDS row m of 32 K rows holds key swap23(m), so the score registers
 // of a lane (one row of q, half = lane / 32) are keys 8 half + 0..7 and 16 + 8 half + 0..7: the B
 // operands of the PV product's two steps, as they are. V stays token-major and its operand comes
-// through the transposed LDS read. 8,192 causal tokens of 32 heads on 8 (128 channels): 600 us, 0.92
-// PFLOP/s of the 1.14 that a library product of 8,192^3 reaches; the matrix pipe is busy for 45 % of the
+// through the transposed LDS read. 8,192 causal tokens of 32 heads on 8 (128 channels): 593 to 621 us, 0.89 to
+// 0.93 PFLOP/s of the 1.14 that a library product of 8,192^3 reaches; the matrix pipe is busy for 45 % of the
 // time and the vector pipe for 50 %.
 constexpr int kRowsThreads = 512;
 constexpr int kTileRows = 256, kTileKeys = 64;
