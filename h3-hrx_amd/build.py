@@ -25,7 +25,8 @@ SOURCES = ["prepare.hip", "plain.hip", "attention.hip", "attention_hm.hip", "att
            "noalloc.hip", "gemm.hip",
            "abi.cpp", "stack.cpp",
            "tables.cpp", "vsa.hip", "vsa_host.cpp", "fp6.hip",
-           "kv4.hip", "attention_kv4.hip"]
+           "kv4.hip", "kv4_advance.hip", "qk_rows.hip", "attention_kv4.hip", "attention_kv4_sinks.hip",
+           "attention_kv4_prefix.hip"]
 ARCH = "gfx950"
 
 

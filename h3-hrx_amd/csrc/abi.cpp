@@ -442,6 +442,90 @@ int check_kv4_attention(const char* stage, const h3_kv4_cfg* cfg, const h3_kv4_a
   return H3_OK;
 }
 
+// The bindings and the launch of an attention over the 4-bit cache, as planned. `front`: bindings between the cache
+// and the table (a prefix's table and length); launch(Kv4Bindings).
+template <typename Launch>
+int attend_kv4(const char* stage, const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
+               uint32_t q_rows, size_t workspace_bytes, h3_view q, h3_view cache,
+               const h3_view (&front)[2], const size_t (&front_need)[2], h3_view table, h3_view lengths,
+               h3_view q_starts, h3_view out, h3_view lse, h3_view workspace, Launch launch) {
+  const uint32_t width = acfg.heads * cfg.head_dim;
+  const int n = front_need[0] ? 2 : 0;  // the bindings of a call are numbered as its arguments are
+  h3_view views[10] = {q, cache, front[0], front[1]};
+  size_t need[10] = {kv4_rows_bytes(q_rows, acfg.q_stride, width), kv4_cache_bytes(cfg), front_need[0],
+                     front_need[1]};
+  const h3_view rest[6] = {table, lengths, q_starts, out, lse, workspace};
+  const size_t rest_need[6] = {(size_t)batch * acfg.table_stride * 4, (size_t)batch * 4,
+                               ((size_t)batch + 1) * 4, kv4_rows_bytes(q_rows, acfg.out_stride, width),
+                               lse.ptr ? (size_t)q_rows * acfg.heads * 4 : 0, workspace_bytes};
+  for (int i = 0; i < 6; ++i) views[2 + n + i] = rest[i], need[2 + n + i] = rest_need[i];
+  int st = check_bindings(stage, views, need, 8 + n);
+  if (st) return st;
+  if ((st = n ? check_alignments(stage, views, {16, 16, 4, 4, 4, 4, 4, 16, 4, 16})
+              : check_alignments(stage, views, {16, 16, 4, 4, 4, 16, 4, 16})))
+    return st;
+  if ((st = device_ready(stage))) return st;
+  return launched(stage, launch(Kv4Bindings{q.ptr, cache.ptr, static_cast<const int32_t*>(table.ptr),
+                                            static_cast<const int32_t*>(lengths.ptr),
+                                            static_cast<const int32_t*>(q_starts.ptr), out.ptr,
+                                            static_cast<float*>(lse.ptr), workspace.ptr,
+                                            static_cast<const int32_t*>(front[0].ptr),
+                                            static_cast<const int32_t*>(front[1].ptr)}));
+}
+
+int check_kv4_sinks(const char* stage, const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* acfg,
+                    uint32_t sinks, uint32_t batch, uint32_t q_rows, uint32_t max_q) {
+  const int st = check_kv4_attention(stage, cfg, acfg, batch, q_rows, max_q);
+  if (st) return st;
+  if (sinks > 16777216) return set_error(H3_ERR_ARGUMENT, "%s: sinks %u past 2^24", stage, sinks);
+  return H3_OK;
+}
+
+// What rows see before the window (0: there is no window, or nothing before it).
+uint32_t kv4_front(const h3_kv4_attention_cfg& acfg, uint32_t sinks) { return acfg.window ? sinks : 0; }
+
+int check_kv4_prefix(const char* stage, const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* acfg,
+                     uint32_t prefix_stride, uint32_t batch, uint32_t q_rows, uint32_t max_q) {
+  const int st = check_kv4_attention(stage, cfg, acfg, batch, q_rows, max_q);
+  if (st) return st;
+  if (acfg->window)
+    return set_error(H3_ERR_CONFIG, "%s: a window (%u) and a prefix", stage, acfg->window);
+  if (prefix_stride < 1 || ((uint64_t)prefix_stride + acfg->table_stride) * cfg->page_tokens > 16777216)
+    return set_error(H3_ERR_ARGUMENT, "%s: prefix_stride %u and table_stride %u of %u-token pages outside [1, 2^24] "
+                     "tokens", stage, prefix_stride, acfg->table_stride, cfg->page_tokens);
+  return H3_OK;
+}
+
+int check_qk_cfg(const char* stage, const h3_qk_cfg* cfg, uint32_t tokens, bool cached) {
+  if (!cfg) return set_error(H3_ERR_ARGUMENT, "%s: null config", stage);
+  if (!in_range(cfg->heads, 1, 4096) || !in_range(cfg->kv_heads, 1, 256))
+    return set_error(H3_ERR_CONFIG, "%s: heads %u outside [1, 4096] or kv_heads %u outside [1, 256]", stage,
+                     cfg->heads, cfg->kv_heads);
+  if (cfg->head_dim != 64 && cfg->head_dim != 128)
+    return set_error(H3_ERR_CONFIG, "%s: head_dim %u is neither 64 nor 128", stage, cfg->head_dim);
+  if (!in_range(cfg->rotary, 0, cfg->head_dim, 16))
+    return set_error(H3_ERR_CONFIG, "%s: rotary %u outside [0, %u] step 16", stage, cfg->rotary,
+                     cfg->head_dim);
+  if (cfg->interleaved > 1 || cfg->norm > 1)
+    return set_error(H3_ERR_CONFIG, "%s: interleaved %u, norm %u", stage, cfg->interleaved, cfg->norm);
+  if (!in_range(cfg->positions, 1, 16777216))
+    return set_error(H3_ERR_CONFIG, "%s: positions %u outside [1, 2^24]", stage, cfg->positions);
+  if (!std::isfinite(cfg->eps) || cfg->eps < 0)
+    return set_error(H3_ERR_CONFIG, "%s: eps is negative or not finite", stage);
+  if (cfg->elem != H3_ELEM_F16 && cfg->elem != H3_ELEM_BF16)
+    return set_error(H3_ERR_CONFIG, "%s: unknown element format %u", stage, cfg->elem);
+  const uint32_t q_width = cfg->heads * cfg->head_dim, width = cfg->kv_heads * cfg->head_dim;
+  if (!in_range(cfg->q_stride, q_width, 1048576, 8) || !in_range(cfg->q_out_stride, q_width, 1048576, 8) ||
+      !in_range(cfg->k_stride, width, 1048576, 8) ||
+      !in_range(cached ? cfg->v_stride : cfg->k_out_stride, width, 1048576, 8))
+    return set_error(H3_ERR_CONFIG, "%s: strides %u, %u, %u, %u, %u below the heads' channels, past 2^20 or no "
+                     "multiples of 8", stage, cfg->q_stride, cfg->k_stride, cfg->v_stride, cfg->q_out_stride,
+                     cfg->k_out_stride);
+  if (!in_range(tokens, 1, 16777216))
+    return set_error(H3_ERR_ARGUMENT, "%s: tokens %u outside [1, 16777216]", stage, tokens);
+  return H3_OK;
+}
+
 // kernels/vsa_ops.loom:3-9 (h3.vsa.*), plus the relations src/vsa/device.rs:63-77 builds the
 // config with: padded = 64 * blocks, width = 128 * heads, prefix <= blocks.
 int check_vsa_cfg(const char* stage, const h3_vsa_cfg* cfg) {
@@ -1177,24 +1261,162 @@ int h3_attention_kv4(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attentio
   const char* stage = "attention_kv4";
   int st = check_kv4_attention(stage, cfg, attention, batch, q_rows, max_q);
   if (st) return st;
-  const uint32_t width = attention->heads * cfg->head_dim;
   const Kv4Plan plan =
       kv4_plan(*cfg, *attention, batch, q_rows, max_q, device_cus(), workspace.ptr != nullptr);
-  const size_t ws = kv4_workspace_bytes(*cfg, batch, plan);
-  h3_view views[8] = {q, cache, table, lengths, q_starts, out, lse, workspace};
-  size_t need[8] = {kv4_rows_bytes(q_rows, attention->q_stride, width), kv4_cache_bytes(*cfg),
-                    (size_t)batch * attention->table_stride * 4, (size_t)batch * 4,
-                    ((size_t)batch + 1) * 4, kv4_rows_bytes(q_rows, attention->out_stride, width),
-                    lse.ptr ? (size_t)q_rows * attention->heads * 4 : 0, ws};
-  if ((st = check_bindings(stage, views, need, 8))) return st;
-  if ((st = check_alignments(stage, views, {16, 16, 4, 4, 4, 16, 4, 16}))) return st;
+  return attend_kv4(stage, *cfg, *attention, batch, q_rows, kv4_workspace_bytes(*cfg, batch, plan), q, cache,
+                    {}, {}, table, lengths, q_starts, out, lse, workspace, [&](const Kv4Bindings& x) {
+                      return launch_attention_kv4(*cfg, *attention, plan, batch, q_rows, max_q, x,
+                                                  reinterpret_cast<hipStream_t>(stream));
+                    });
+}
+
+size_t h3_kv4_sinks_workspace_bytes(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attention,
+                                    uint32_t sinks, uint32_t batch, uint32_t q_rows, uint32_t max_q) {
+  if (check_kv4_sinks("kv4_sinks_workspace_bytes", cfg, attention, sinks, batch, q_rows, max_q)) return 0;
+  ok();
+  return kv4_workspace_bytes(*cfg, batch, kv4_front_plan(*cfg, *attention, kv4_front(*attention, sinks), batch, q_rows,
+                                                         max_q, device_cus(), true));
+}
+
+int h3_attention_kv4_sinks(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attention, uint32_t sinks,
+                           uint32_t batch, uint32_t q_rows, uint32_t max_q, h3_view q, h3_view cache,
+                           h3_view table, h3_view lengths, h3_view q_starts, h3_view out, h3_view lse,
+                           h3_view workspace, h3_stream stream) {
+  const char* stage = "attention_kv4_sinks";
+  const int st = check_kv4_sinks(stage, cfg, attention, sinks, batch, q_rows, max_q);
+  if (st) return st;
+  const uint32_t front = kv4_front(*attention, sinks);
+  const Kv4Plan plan = kv4_front_plan(*cfg, *attention, front, batch, q_rows, max_q, device_cus(),
+                                      workspace.ptr != nullptr);
+  return attend_kv4(stage, *cfg, *attention, batch, q_rows, kv4_workspace_bytes(*cfg, batch, plan), q, cache,
+                    {}, {}, table, lengths, q_starts, out, lse, workspace, [&](const Kv4Bindings& x) {
+                      const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+                      return front ? launch_attention_kv4_sinks(*cfg, *attention, front, plan, batch, q_rows,
+                                                                max_q, x, s)
+                                   : launch_attention_kv4(*cfg, *attention, plan, batch, q_rows, max_q, x, s);
+                    });
+}
+
+size_t h3_kv4_prefix_workspace_bytes(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attention,
+                                     uint32_t prefix_stride, uint32_t batch, uint32_t q_rows, uint32_t max_q) {
+  if (check_kv4_prefix("kv4_prefix_workspace_bytes", cfg, attention, prefix_stride, batch, q_rows, max_q))
+    return 0;
+  ok();
+  return kv4_workspace_bytes(*cfg, batch, kv4_front_plan(*cfg, *attention, (uint64_t)prefix_stride * cfg->page_tokens, batch,
+                                                         q_rows, max_q, device_cus(), true));
+}
+
+int h3_attention_kv4_prefix(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attention,
+                            uint32_t prefix_stride, uint32_t batch, uint32_t q_rows, uint32_t max_q, h3_view q,
+                            h3_view cache, h3_view prefix_table, h3_view prefix_length, h3_view table,
+                            h3_view lengths, h3_view q_starts, h3_view out, h3_view lse, h3_view workspace,
+                            h3_stream stream) {
+  const char* stage = "attention_kv4_prefix";
+  const int st = check_kv4_prefix(stage, cfg, attention, prefix_stride, batch, q_rows, max_q);
+  if (st) return st;
+  const Kv4Plan plan = kv4_front_plan(*cfg, *attention, (uint64_t)prefix_stride * cfg->page_tokens, batch,
+                                      q_rows, max_q, device_cus(), workspace.ptr != nullptr);
+  return attend_kv4(stage, *cfg, *attention, batch, q_rows, kv4_workspace_bytes(*cfg, batch, plan), q, cache,
+                    {prefix_table, prefix_length}, {(size_t)prefix_stride * 4, 4}, table, lengths, q_starts,
+                    out, lse, workspace, [&](const Kv4Bindings& x) {
+                      return launch_attention_kv4_prefix(*cfg, *attention, prefix_stride, plan, batch, q_rows,
+                                                         max_q, x, reinterpret_cast<hipStream_t>(stream));
+                    });
+}
+
+int h3_kv4_advance(const h3_kv4_cfg* cfg, uint32_t batch, uint32_t table_stride, uint32_t rows, h3_view asked,
+                   h3_view lengths, h3_view free_pages, h3_view free_count, h3_view table,
+                   h3_view lengths_out, h3_view free_count_out, h3_view q_starts, h3_view slots,
+                   h3_view positions, h3_view prefix_length, h3_stream stream) {
+  const char* stage = "kv4_advance";
+  int st = check_kv4_cfg(stage, cfg);
+  if (st) return st;
+  if (!in_range(batch, 1, 65535) || !in_range(rows, 1, 16777216))
+    return set_error(H3_ERR_ARGUMENT, "%s: batch %u outside [1, 65535] or rows %u outside [1, 2^24]", stage,
+                     batch, rows);
+  if (table_stride < 1 || (uint64_t)table_stride * cfg->page_tokens > 16777216)
+    return set_error(H3_ERR_ARGUMENT, "%s: table_stride %u of %u-token pages outside [1, 2^24] tokens", stage,
+                     table_stride, cfg->page_tokens);
+  const size_t each = (size_t)batch * 4;
+  h3_view views[11] = {asked, lengths, free_pages, free_count, table, lengths_out, free_count_out, q_starts,
+                       slots, positions, prefix_length};
+  size_t need[11] = {each, each, (size_t)cfg->pages * 4, 4, each * table_stride, each, 4, each + 4,
+                     (size_t)rows * 4, (size_t)rows * 4, prefix_length.ptr ? 4u : 0u};
+  if ((st = check_bindings(stage, views, need, 11))) return st;
+  if ((st = check_alignments(stage, views, {4, 4, 4, 4, 4, 4, 4, 4, 4, 4, 4}))) return st;
   if ((st = device_ready(stage))) return st;
-  return launched(stage, launch_attention_kv4(*cfg, *attention, plan, batch, q_rows, max_q,
-                                              q.ptr, cache.ptr, static_cast<const int32_t*>(table.ptr),
-                                              static_cast<const int32_t*>(lengths.ptr),
-                                              static_cast<const int32_t*>(q_starts.ptr), out.ptr,
-                                              static_cast<float*>(lse.ptr), workspace.ptr,
-                                              reinterpret_cast<hipStream_t>(stream)));
+  int32_t* p[11];
+  for (int i = 0; i < 11; ++i) p[i] = static_cast<int32_t*>(views[i].ptr);
+  return launched(stage, launch_kv4_advance(*cfg, batch, table_stride, rows,
+                                            {p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], p[10]},
+                                            reinterpret_cast<hipStream_t>(stream)));
+}
+
+int h3_qk_norm_rope(const h3_qk_cfg* cfg, uint32_t tokens, h3_view q, h3_view k, h3_view q_weight,
+                    h3_view k_weight, h3_view cos_t, h3_view sin_t, h3_view positions, h3_view q_out,
+                    h3_view k_out, h3_stream stream) {
+  const char* stage = "qk_norm_rope";
+  int st = check_qk_cfg(stage, cfg, tokens, false);
+  if (st) return st;
+  const uint32_t q_width = cfg->heads * cfg->head_dim, width = cfg->kv_heads * cfg->head_dim;
+  const size_t weight = cfg->norm ? (size_t)cfg->head_dim * 4 : 0;
+  const size_t turns = (size_t)cfg->positions * (cfg->rotary / 2) * 4;
+  h3_view views[9] = {q, k, q_weight, k_weight, cos_t, sin_t, positions, q_out, k_out};
+  size_t need[9] = {kv4_rows_bytes(tokens, cfg->q_stride, q_width), kv4_rows_bytes(tokens, cfg->k_stride, width),
+                    weight, weight, turns, turns, (size_t)tokens * 4,
+                    kv4_rows_bytes(tokens, cfg->q_out_stride, q_width),
+                    kv4_rows_bytes(tokens, cfg->k_out_stride, width)};
+  if ((st = check_bindings(stage, views, need, 9))) return st;
+  if ((st = check_alignments(stage, views, {16, 16, 16, 16, 16, 16, 4, 16, 16}))) return st;
+  if ((st = device_ready(stage))) return st;
+  QkBindings x{};
+  x.q = q.ptr;
+  x.k = k.ptr;
+  x.q_weight = static_cast<const float*>(q_weight.ptr);
+  x.k_weight = static_cast<const float*>(k_weight.ptr);
+  x.cos_t = static_cast<const float*>(cos_t.ptr);
+  x.sin_t = static_cast<const float*>(sin_t.ptr);
+  x.positions = static_cast<const int32_t*>(positions.ptr);
+  x.q_out = q_out.ptr;
+  x.k_out = k_out.ptr;
+  return launched(stage, launch_qk_norm_rope(*cfg, nullptr, tokens, x, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int h3_qk_norm_rope_kv4(const h3_qk_cfg* cfg, const h3_kv4_cfg* kv, uint32_t tokens, h3_view q, h3_view k,
+                        h3_view v, h3_view q_weight, h3_view k_weight, h3_view cos_t, h3_view sin_t,
+                        h3_view positions, h3_view slots, h3_view q_out, h3_view cache, h3_stream stream) {
+  const char* stage = "qk_norm_rope_kv4";
+  int st = check_qk_cfg(stage, cfg, tokens, true);
+  if (st) return st;
+  if ((st = check_kv4_cfg(stage, kv))) return st;
+  if (cfg->kv_heads != kv->kv_heads || cfg->head_dim != kv->head_dim || cfg->elem != kv->elem)
+    return set_error(H3_ERR_CONFIG, "%s: rows of %u heads of %u channels (format %u), a cache of %u of %u (%u)",
+                     stage, cfg->kv_heads, cfg->head_dim, cfg->elem, kv->kv_heads, kv->head_dim, kv->elem);
+  const uint32_t q_width = cfg->heads * cfg->head_dim, width = cfg->kv_heads * cfg->head_dim;
+  const size_t weight = cfg->norm ? (size_t)cfg->head_dim * 4 : 0;
+  const size_t turns = (size_t)cfg->positions * (cfg->rotary / 2) * 4;
+  h3_view views[11] = {q, k, v, q_weight, k_weight, cos_t, sin_t, positions, slots, q_out, cache};
+  size_t need[11] = {kv4_rows_bytes(tokens, cfg->q_stride, q_width),
+                     kv4_rows_bytes(tokens, cfg->k_stride, width),
+                     kv4_rows_bytes(tokens, cfg->v_stride, width), weight, weight, turns, turns,
+                     (size_t)tokens * 4, (size_t)tokens * 4,
+                     kv4_rows_bytes(tokens, cfg->q_out_stride, q_width), kv4_cache_bytes(*kv)};
+  if ((st = check_bindings(stage, views, need, 11))) return st;
+  if ((st = check_alignments(stage, views, {16, 16, 16, 16, 16, 16, 16, 4, 4, 16, 16}))) return st;
+  if ((st = device_ready(stage))) return st;
+  QkBindings x{};
+  x.q = q.ptr;
+  x.k = k.ptr;
+  x.v = v.ptr;
+  x.q_weight = static_cast<const float*>(q_weight.ptr);
+  x.k_weight = static_cast<const float*>(k_weight.ptr);
+  x.cos_t = static_cast<const float*>(cos_t.ptr);
+  x.sin_t = static_cast<const float*>(sin_t.ptr);
+  x.positions = static_cast<const int32_t*>(positions.ptr);
+  x.slots = static_cast<const int32_t*>(slots.ptr);
+  x.q_out = q_out.ptr;
+  x.cache = cache.ptr;
+  return launched(stage, launch_qk_norm_rope(*cfg, kv, tokens, x, reinterpret_cast<hipStream_t>(stream)));
 }
 
 int h3_vsa_attention_i8(const h3_attention_cfg* cfg, uint32_t token_count, uint32_t heads,

@@ -242,13 +242,49 @@ struct Kv4Plan {
 };
 Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
                  uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide);
+// front_keys: what rows see before their window (sinks) or their sequence (a prefix).
+Kv4Plan kv4_front_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint64_t front_keys,
+                       uint32_t batch, uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide);
 size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, uint32_t batch, const Kv4Plan& plan);
+struct Kv4Bindings {
+  const void *q, *cache;
+  const int32_t *table, *lengths, *q_starts;
+  void* out;
+  float* lse;
+  void* workspace;
+  const int32_t *prefix_table, *prefix_length;  // of a shared prefix
+};
 hipError_t launch_attention_kv4(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
                                 const Kv4Plan& plan, uint32_t batch, uint32_t q_rows,
-                                uint32_t max_q, const void* q, const void* cache,
-                                const int32_t* table, const int32_t* lengths,
-                                const int32_t* q_starts, void* out, float* lse, void* workspace,
-                                hipStream_t stream);
+                                uint32_t max_q, const Kv4Bindings& x, hipStream_t stream);
+// With the first `sinks` tokens of a sequence seen outside the window (attention_kv4_sinks.hip).
+hipError_t launch_attention_kv4_sinks(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
+                                      uint32_t sinks, const Kv4Plan& plan, uint32_t batch, uint32_t q_rows,
+                                      uint32_t max_q, const Kv4Bindings& x, hipStream_t stream);
+// Behind a prefix that all sequences share (attention_kv4_prefix.hip).
+hipError_t launch_attention_kv4_prefix(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
+                                       uint32_t prefix_stride, const Kv4Plan& plan, uint32_t batch,
+                                       uint32_t q_rows, uint32_t max_q, const Kv4Bindings& x,
+                                       hipStream_t stream);
+// What the next step of every sequence needs (kv4_advance.hip).
+struct AdvanceBindings {
+  const int32_t *asked, *lengths;
+  int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t *table, *lengths_out, *free_count_out, *q_starts, *slots, *positions;
+  const int32_t* prefix_length;  // null: no prefix
+};
+hipError_t launch_kv4_advance(const h3_kv4_cfg& cfg, uint32_t batch, uint32_t table_stride, uint32_t rows,
+                              const AdvanceBindings& x, hipStream_t stream);
+// Norm and rotation of rows of q and k (qk_rows.hip); kv null: k to rows, else k and v into the cache.
+struct QkBindings {
+  const void *q, *k, *v;
+  const float *q_weight, *k_weight, *cos_t, *sin_t;
+  const int32_t *positions, *slots;
+  void *q_out, *k_out, *cache;
+};
+hipError_t launch_qk_norm_rope(const h3_qk_cfg& cfg, const h3_kv4_cfg* kv, uint32_t tokens,
+                               const QkBindings& x, hipStream_t stream);
 // VSA operations (vsa.hip)
 hipError_t launch_vsa_gather(uint32_t tokens, uint32_t padded, uint32_t width, const int32_t* src,
                              const uint16_t* x, uint16_t* y, hipStream_t stream);

@@ -1,0 +1,273 @@
+// The per-head norm and rotation of a decoder's queries and keys on gfx950, to rows in 16 bits or with the keys and
+// values into the 4-bit cache of kv4.hip.
+//
+// Per row and head, x of D channels, with norm: y = x r w, r = 1 / sqrt(mean(x^2) + eps). Then the pairs (a, b)
+// of the first `rotary` channels, (c, c + rotary / 2) or interleaved (2 c, 2 c + 1), turn by the row's
+// position: (a cos - b sin, b cos + a sin). With x' the other channel of a pair, w' its weight and s = -sin for
+// the first and sin for the second channel of one, the result is r (x (w cos) + x' (w' s)): the two factors are a
+// token's for all its heads, and what passes between lanes is x as it was read, two channels to a register.
+//
+// Queries are computed in f32 and rounded once. Keys are computed in f64, so that the 16 bits that they are rounded to
+// are the definition's, whatever the order of its sums: a bit of one of them is a step of a code or of a whole row's
+// scale in the cache. It costs nothing that is seen: there are few key heads and memory bounds the kernel.
+//
+// D/8 lanes of 8 channels hold a row, so a wave holds one head of 512/D tokens and takes `per` heads of the same
+// tokens one after the other.
+#include "kv4_row.hpp"
+
+namespace h3 {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+
+struct QkArgs {
+  const void *q, *k, *v;
+  const float *q_weight, *k_weight, *cos_t, *sin_t;
+  const int32_t *positions, *slots;
+  void *q_out, *k_out;
+  uint8_t* cache;
+  uint32_t tokens, heads, kv_heads, rotary, position_limit;
+  uint32_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride;
+  uint32_t page_shift;
+  uint32_t units, per;  // heads of q, of k and (cached) of v, one after the other; how many a wave takes
+  uint64_t slot_limit;
+  float eps;
+};
+
+// The lane's place: its token's row, and 8 channels of every head.
+struct Lane {
+  uint32_t token, first;   // first of the channels
+  int32_t position, slot;  // -1: none
+  int other;               // the lane that holds the pairs' other channels, in bytes for a permutation
+};
+
+__device__ __forceinline__ float channel(const uint32_t (&w)[4], int i, bool bf16) {
+  const uint32_t bits = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu;
+  return bf16 ? widen<true>(bits) : widen<false>(bits);
+}
+
+// Eight channels and their pairs' others: [..][i] belongs to channel i.
+template <bool kPairs>
+__device__ __forceinline__ void others(const uint32_t (&w)[4], int lane, uint32_t (&o)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    o[i] = kPairs ? (w[i] >> 16) | (w[i] << 16) : (uint32_t)__builtin_amdgcn_ds_bpermute(lane, (int)w[i]);
+}
+
+template <int kCtrl>
+__device__ __forceinline__ double dpp64(double v) {
+  const uint2 x = __builtin_bit_cast(uint2, v);
+  const uint2 y = {(uint32_t)__builtin_amdgcn_mov_dpp((int)x.x, kCtrl, 0xF, 0xF, true),
+                   (uint32_t)__builtin_amdgcn_mov_dpp((int)x.y, kCtrl, 0xF, 0xF, true)};
+  return __builtin_bit_cast(double, y);
+}
+// The sum over the D/8 lanes of a row.
+template <int D>
+__device__ __forceinline__ float row_sum(float v) {
+  v += dpp<0xB1>(v);
+  v += dpp<0x4E>(v);
+  v += dpp<0x141>(v);
+  if constexpr (D == 128) v += dpp<0x140>(v);
+  return v;
+}
+template <int D>
+__device__ __forceinline__ double row_sum(double v) {
+  v += dpp64<0xB1>(v);
+  v += dpp64<0x4E>(v);
+  v += dpp64<0x141>(v);
+  if constexpr (D == 128) v += dpp64<0x140>(v);
+  return v;
+}
+
+// An f64 value rounded once to the element type: to odd in f32 first (toward zero, the last bit set where that lost
+// something), which the second rounding, of at least two bits fewer, cannot mistake for a tie.
+template <bool kBf16>
+__device__ __forceinline__ uint32_t narrow64(double x) {
+  const float f = (float)x;
+  const double back = f;
+  uint32_t bits = __float_as_uint(f);
+  if (back != x) bits = (bits - (fabs(back) > fabs(x) ? 1u : 0u)) | 1u;
+  return narrow<kBf16>(__uint_as_float(bits));
+}
+
+// What a token's rows of one weight are multiplied by: own = w cos, other = w' (-sin or sin); past the rotated
+// channels w and 0.
+template <typename T>
+struct Factors {
+  T own[8], other[8];
+};
+template <bool kPairs, typename T>
+__device__ __forceinline__ Factors<T> factors(const QkArgs& a, const Lane& l, const float* weight) {
+  Factors<T> f;
+  const uint32_t half = a.rotary / 2;
+  const bool turned = l.first < a.rotary, second = !kPairs && l.first >= half;
+  const uint32_t pair = kPairs ? l.first / 2 : second ? l.first - half : l.first;
+  const size_t at = (size_t)(uint32_t)max(l.position, 0) * half + pair;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t c = l.first + i;
+    const uint32_t o = kPairs ? c ^ 1 : second ? c - half : c + half;
+    const T w = weight ? (T)weight[c] : (T)1;
+    f.own[i] = w;
+    f.other[i] = 0;
+    if (turned) {
+      const T cos_i = a.cos_t[at + (kPairs ? i / 2 : i)], sin_i = a.sin_t[at + (kPairs ? i / 2 : i)];
+      const T v = weight ? (T)weight[o] : (T)1;
+      f.own[i] = w * cos_i;
+      f.other[i] = v * ((kPairs ? i & 1 : second) ? sin_i : -sin_i);
+    }
+  }
+  return f;
+}
+
+// A row's eight channels in 16 bits.
+template <int D, bool kBf16, bool kPairs, bool kNorm, typename T>
+__device__ __forceinline__ uint4 turn(const QkArgs& a, const Lane& l, const Factors<T>& f, uint4 raw) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  uint32_t o[4];
+  others<kPairs>(w, l.other, o);
+  T r = 1;
+  if constexpr (kNorm) {
+    T sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const T x = channel(w, i, kBf16);
+      sum = fma(x, x, sum);
+    }
+    sum = row_sum<D>(sum);
+    if constexpr (sizeof(T) == 8)
+      r = 1.0 / sqrt(sum / D + (double)a.eps);
+    else
+      r = 1.0f / sqrtf(sum / D + a.eps);
+  }
+  uint32_t out[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const T y = fma((T)channel(w, i, kBf16), f.own[i], (T)channel(o, i, kBf16) * f.other[i]) * r;
+    if constexpr (sizeof(T) == 8)
+      out[i] = narrow64<kBf16>(y);
+    else
+      out[i] = narrow<kBf16>(y);
+  }
+  return {out[0] | out[1] << 16, out[2] | out[3] << 16, out[4] | out[5] << 16, out[6] | out[7] << 16};
+}
+
+// Eight channels of a row of K (part 0) or V into their slot.
+template <int D, bool kBf16>
+__device__ __forceinline__ void put(const QkArgs& a, const Lane& l, uint32_t head, uint32_t part, uint4 x) {
+  const uint2 row = quantize<D, kBf16>(x);
+  if (l.slot < 0) return;
+  const Slot<D> at = slot_at<D>(a.page_shift, a.kv_heads, (uint32_t)l.slot, head);
+  *reinterpret_cast<uint32_t*>(a.cache + at.codes + part * at.half + l.first / 2) = row.y;
+  if (l.first == 0) *reinterpret_cast<uint32_t*>(a.cache + at.words + part * 4 * at.tokens) = row.x;
+}
+
+template <int D, bool kBf16, bool kPairs, bool kNorm, bool kCached>
+__global__ __launch_bounds__(kThreads) void k_qk_norm_rope(QkArgs a) {
+  constexpr uint32_t kLanes = D / 8, kTokens = 64 / kLanes;
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t from = (blockIdx.y * kWaves + wave) * a.per, to = min(from + a.per, a.units);
+  if (from >= a.units) return;
+  Lane l;
+  const uint32_t at = blockIdx.x * kTokens + lane / kLanes;
+  l.token = min(at, a.tokens - 1);  // the last row stands for the rows past it: their loads need no branch
+  l.first = lane % kLanes * 8;
+  const int32_t position = at < a.tokens ? a.positions[at] : -1;
+  l.position = (uint32_t)position < a.position_limit ? position : -1;
+  l.slot = -1;
+  if constexpr (kCached) {
+    const int32_t slot = a.slots[l.token];
+    if (l.position >= 0 && (uint64_t)(uint32_t)slot < a.slot_limit) l.slot = slot;
+  }
+  const uint32_t half = a.rotary / 16;  // lanes of the pairs' first channels
+  const uint32_t in_row = lane % kLanes;
+  l.other = 4 * (int)(in_row < half ? lane + half : in_row < 2 * half ? lane - half : lane);
+
+  if (from < a.heads) {
+    const Factors<float> f = factors<kPairs, float>(a, l, kNorm ? a.q_weight : nullptr);
+    for (uint32_t u = from; u < min(to, a.heads); ++u) {
+      const uint4 x = load_row<false>(a.q, (size_t)l.token * a.q_stride + u * D + l.first);
+      const uint4 y = turn<D, kBf16, kPairs, kNorm>(a, l, f, x);
+      if (l.position >= 0) store_row<false>(a.q_out, (size_t)l.token * a.q_out_stride + u * D + l.first, y);
+    }
+  }
+  const uint32_t k_end = a.heads + a.kv_heads;
+  if (from < k_end && to > a.heads) {
+    const Factors<double> f = factors<kPairs, double>(a, l, kNorm ? a.k_weight : nullptr);
+    for (uint32_t u = max(from, a.heads); u < min(to, k_end); ++u) {
+      const uint32_t head = u - a.heads;
+      const uint4 x = load_row<false>(a.k, (size_t)l.token * a.k_stride + head * D + l.first);
+      const uint4 y = turn<D, kBf16, kPairs, kNorm>(a, l, f, x);
+      if constexpr (kCached)
+        put<D, kBf16>(a, l, head, 0, y);
+      else if (l.position >= 0)
+        store_row<false>(a.k_out, (size_t)l.token * a.k_out_stride + head * D + l.first, y);
+    }
+  }
+  if constexpr (kCached)
+    for (uint32_t u = max(from, k_end); u < to; ++u) {
+      const uint32_t head = u - k_end;
+      put<D, kBf16>(a, l, head, 1, load_row<false>(a.v, (size_t)l.token * a.v_stride + head * D + l.first));
+    }
+}
+
+template <int D, bool kBf16, bool kPairs, bool kNorm>
+hipError_t launch(const QkArgs& a, hipStream_t stream) {
+  constexpr uint32_t kTokens = 512 / D;
+  const dim3 grid((a.tokens + kTokens - 1) / kTokens, (a.units + kWaves * a.per - 1) / (kWaves * a.per));
+  if (a.cache)
+    hipLaunchKernelGGL((k_qk_norm_rope<D, kBf16, kPairs, kNorm, true>), grid, dim3(kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((k_qk_norm_rope<D, kBf16, kPairs, kNorm, false>), grid, dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+template <int D, bool kBf16>
+hipError_t launch_kind(const QkArgs& a, const h3_qk_cfg& cfg, hipStream_t stream) {
+  if (cfg.interleaved)
+    return cfg.norm ? launch<D, kBf16, true, true>(a, stream) : launch<D, kBf16, true, false>(a, stream);
+  return cfg.norm ? launch<D, kBf16, false, true>(a, stream) : launch<D, kBf16, false, false>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_qk_norm_rope(const h3_qk_cfg& cfg, const h3_kv4_cfg* kv, uint32_t tokens,
+                               const QkBindings& x, hipStream_t stream) {
+  QkArgs a{};
+  a.q = x.q;
+  a.k = x.k;
+  a.v = x.v;
+  a.q_weight = x.q_weight;
+  a.k_weight = x.k_weight;
+  a.cos_t = x.cos_t;
+  a.sin_t = x.sin_t;
+  a.positions = x.positions;
+  a.slots = x.slots;
+  a.q_out = x.q_out;
+  a.k_out = x.k_out;
+  a.tokens = tokens;
+  a.heads = cfg.heads;
+  a.kv_heads = cfg.kv_heads;
+  a.rotary = cfg.rotary;
+  a.position_limit = cfg.positions;
+  a.q_stride = cfg.q_stride;
+  a.k_stride = cfg.k_stride;
+  a.v_stride = cfg.v_stride;
+  a.q_out_stride = cfg.q_out_stride;
+  a.k_out_stride = cfg.k_out_stride;
+  a.eps = cfg.eps;
+  a.units = cfg.heads + cfg.kv_heads * (kv ? 2 : 1);
+  a.per = 1;
+  if (kv) {
+    a.cache = static_cast<uint8_t*>(x.cache);
+    a.page_shift = __builtin_ctz(kv->page_tokens);
+    a.slot_limit = (uint64_t)kv->pages * kv->page_tokens;
+  }
+  const bool bf16 = cfg.elem == H3_ELEM_BF16;
+  if (cfg.head_dim == 128)
+    return bf16 ? launch_kind<128, true>(a, cfg, stream) : launch_kind<128, false>(a, cfg, stream);
+  return bf16 ? launch_kind<64, true>(a, cfg, stream) : launch_kind<64, false>(a, cfg, stream);
+}
+
+}  // namespace h3

@@ -147,6 +147,26 @@ pub struct H3Kv4AttentionCfg {
     pub scale: f32,
 }
 
+/// Rows of queries and keys to norm and rotate.
+#[repr(C)]
+#[derive(Clone, Copy, Debug, Default)]
+pub struct H3QkCfg {
+    pub heads: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub rotary: u32,
+    pub interleaved: u32,
+    pub norm: u32,
+    pub positions: u32,
+    pub eps: f32,
+    pub elem: u32,
+    pub q_stride: u32,
+    pub k_stride: u32,
+    pub v_stride: u32,
+    pub q_out_stride: u32,
+    pub k_out_stride: u32,
+}
+
 #[repr(C)]
 #[derive(Clone, Copy, Debug, Default)]
 pub struct H3VsaCfg {
@@ -328,6 +348,36 @@ extern "C" {
                             q_rows: u32, max_q: u32, q: H3View, cache: H3View, table: H3View,
                             lengths: H3View, q_starts: H3View, out: H3View, lse: H3View,
                             workspace: H3View, stream: H3Stream) -> c_int;
+
+    pub fn h3_kv4_sinks_workspace_bytes(cfg: *const H3Kv4Cfg, attention: *const H3Kv4AttentionCfg,
+                                        sinks: u32, batch: u32, q_rows: u32, max_q: u32) -> usize;
+    pub fn h3_attention_kv4_sinks(cfg: *const H3Kv4Cfg, attention: *const H3Kv4AttentionCfg,
+                                  sinks: u32, batch: u32, q_rows: u32, max_q: u32, q: H3View,
+                                  cache: H3View, table: H3View, lengths: H3View, q_starts: H3View,
+                                  out: H3View, lse: H3View, workspace: H3View,
+                                  stream: H3Stream) -> c_int;
+    pub fn h3_kv4_prefix_workspace_bytes(cfg: *const H3Kv4Cfg, attention: *const H3Kv4AttentionCfg,
+                                         prefix_stride: u32, batch: u32, q_rows: u32,
+                                         max_q: u32) -> usize;
+    pub fn h3_attention_kv4_prefix(cfg: *const H3Kv4Cfg, attention: *const H3Kv4AttentionCfg,
+                                   prefix_stride: u32, batch: u32, q_rows: u32, max_q: u32,
+                                   q: H3View, cache: H3View, prefix_table: H3View,
+                                   prefix_length: H3View, table: H3View, lengths: H3View,
+                                   q_starts: H3View, out: H3View, lse: H3View, workspace: H3View,
+                                   stream: H3Stream) -> c_int;
+    pub fn h3_kv4_advance(cfg: *const H3Kv4Cfg, batch: u32, table_stride: u32, rows: u32,
+                          asked: H3View, lengths: H3View, free_pages: H3View, free_count: H3View,
+                          table: H3View, lengths_out: H3View, free_count_out: H3View,
+                          q_starts: H3View, slots: H3View, positions: H3View,
+                          prefix_length: H3View, stream: H3Stream) -> c_int;
+    pub fn h3_qk_norm_rope(cfg: *const H3QkCfg, tokens: u32, q: H3View, k: H3View,
+                           q_weight: H3View, k_weight: H3View, cos_t: H3View, sin_t: H3View,
+                           positions: H3View, q_out: H3View, k_out: H3View,
+                           stream: H3Stream) -> c_int;
+    pub fn h3_qk_norm_rope_kv4(cfg: *const H3QkCfg, kv: *const H3Kv4Cfg, tokens: u32, q: H3View,
+                               k: H3View, v: H3View, q_weight: H3View, k_weight: H3View,
+                               cos_t: H3View, sin_t: H3View, positions: H3View, slots: H3View,
+                               q_out: H3View, cache: H3View, stream: H3Stream) -> c_int;
 
     // VSA block-sparse attention
     pub fn h3_vsa_gather(cfg: *const H3VsaCfg, src: H3View, x: H3View, y: H3View,

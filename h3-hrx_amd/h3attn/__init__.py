@@ -145,6 +145,14 @@ class Kv4AttentionCfg(ctypes.Structure):
         ("scale", ctypes.c_float)]
 
 
+class QkCfg(ctypes.Structure):
+    """Rows of queries and keys to norm and rotate (h3_qk_cfg)."""
+    _fields_ = [(name, ctypes.c_uint32) for name in (
+        "heads", "kv_heads", "head_dim", "rotary", "interleaved", "norm", "positions")] + [
+        ("eps", ctypes.c_float)] + [(name, ctypes.c_uint32) for name in (
+            "elem", "q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride")]
+
+
 class VsaCfg(ctypes.Structure):
     """h3.vsa.* (kernels/vsa_ops.loom:3-9)."""
     _fields_ = [
@@ -232,6 +240,28 @@ SIGNATURES = {
     "h3_attention_kv4": (
         [_P(Kv4Cfg), _P(Kv4AttentionCfg), ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, View,
          View, View, View, View, View, View, View, _S], ctypes.c_int),
+    "h3_kv4_sinks_workspace_bytes": (
+        [_P(Kv4Cfg), _P(Kv4AttentionCfg), ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
+         ctypes.c_uint32], ctypes.c_size_t),
+    "h3_attention_kv4_sinks": (
+        [_P(Kv4Cfg), _P(Kv4AttentionCfg), ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
+         ctypes.c_uint32, View, View, View, View, View, View, View, View, _S], ctypes.c_int),
+    "h3_kv4_prefix_workspace_bytes": (
+        [_P(Kv4Cfg), _P(Kv4AttentionCfg), ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
+         ctypes.c_uint32], ctypes.c_size_t),
+    "h3_attention_kv4_prefix": (
+        [_P(Kv4Cfg), _P(Kv4AttentionCfg), ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32,
+         ctypes.c_uint32, View, View, View, View, View, View, View, View, View, View, _S],
+        ctypes.c_int),
+    "h3_kv4_advance": (
+        [_P(Kv4Cfg), ctypes.c_uint32, ctypes.c_uint32, ctypes.c_uint32, View, View, View, View, View,
+         View, View, View, View, View, View, _S], ctypes.c_int),
+    "h3_qk_norm_rope": (
+        [_P(QkCfg), ctypes.c_uint32, View, View, View, View, View, View, View, View, View, _S],
+        ctypes.c_int),
+    "h3_qk_norm_rope_kv4": (
+        [_P(QkCfg), _P(Kv4Cfg), ctypes.c_uint32, View, View, View, View, View, View, View, View, View,
+         View, View, _S], ctypes.c_int),
     "h3_vsa_gather": ([_P(VsaCfg), View, View, View, _S], ctypes.c_int),
     "h3_vsa_scatter": ([_P(VsaCfg), View, View, View, _S], ctypes.c_int),
     "h3_vsa_pool": ([_P(VsaCfg), View, View, View, _S], ctypes.c_int),
@@ -615,6 +645,69 @@ def attention_kv4(cfg: Kv4Cfg, acfg: Kv4AttentionCfg, batch: int, q_rows: int, m
     check(lib().h3_attention_kv4(ctypes.byref(cfg), ctypes.byref(acfg), batch, q_rows, max_q,
                                  view(q), view(cache), view(table), view(lengths), view(q_starts),
                                  view(out), view(lse), view(workspace), stream_ptr(stream)))
+
+
+def kv4_sinks_workspace_bytes(cfg: Kv4Cfg, acfg: Kv4AttentionCfg, sinks: int, batch: int, q_rows: int,
+                              max_q: int) -> int:
+    """Bytes of the workspace with which attention_kv4_sinks divides such a call's keys."""
+    return int(lib().h3_kv4_sinks_workspace_bytes(ctypes.byref(cfg), ctypes.byref(acfg), sinks, batch,
+                                                  q_rows, max_q))
+
+
+def attention_kv4_sinks(cfg: Kv4Cfg, acfg: Kv4AttentionCfg, sinks: int, batch: int, q_rows: int,
+                        max_q: int, q, cache, table, lengths, q_starts, out, lse=None, workspace=None,
+                        stream=None) -> None:
+    """attention_kv4 with each sequence's first `sinks` tokens seen beside the window."""
+    check(lib().h3_attention_kv4_sinks(ctypes.byref(cfg), ctypes.byref(acfg), sinks, batch, q_rows, max_q,
+                                       view(q), view(cache), view(table), view(lengths), view(q_starts),
+                                       view(out), view(lse), view(workspace), stream_ptr(stream)))
+
+
+def kv4_prefix_workspace_bytes(cfg: Kv4Cfg, acfg: Kv4AttentionCfg, prefix_stride: int, batch: int,
+                               q_rows: int, max_q: int) -> int:
+    """Bytes of the workspace with which attention_kv4_prefix divides such a call's keys."""
+    return int(lib().h3_kv4_prefix_workspace_bytes(ctypes.byref(cfg), ctypes.byref(acfg), prefix_stride,
+                                                   batch, q_rows, max_q))
+
+
+def attention_kv4_prefix(cfg: Kv4Cfg, acfg: Kv4AttentionCfg, prefix_stride: int, batch: int, q_rows: int,
+                         max_q: int, q, cache, prefix_table, prefix_length, table, lengths, q_starts, out,
+                         lse=None, workspace=None, stream=None) -> None:
+    """attention_kv4 of sequences that continue one prefix, whose pages are prefix_table's: every row sees
+    all of it and its own sequence's keys."""
+    check(lib().h3_attention_kv4_prefix(ctypes.byref(cfg), ctypes.byref(acfg), prefix_stride, batch,
+                                        q_rows, max_q, view(q), view(cache), view(prefix_table),
+                                        view(prefix_length), view(table), view(lengths), view(q_starts),
+                                        view(out), view(lse), view(workspace), stream_ptr(stream)))
+
+
+def kv4_advance(cfg: Kv4Cfg, batch: int, table_stride: int, rows: int, asked, lengths, free_pages,
+                free_count, table, lengths_out, free_count_out, q_starts, slots, positions,
+                prefix_length=None, stream=None) -> None:
+    """The page table, lengths, row starts, slots and positions of the next step of `batch` sequences, from
+    the rows that each asks for (below 0: it ends). lengths_out may be lengths, free_count_out free_count."""
+    check(lib().h3_kv4_advance(ctypes.byref(cfg), batch, table_stride, rows, view(asked), view(lengths),
+                               view(free_pages), view(free_count), view(table), view(lengths_out),
+                               view(free_count_out), view(q_starts), view(slots), view(positions),
+                               view(prefix_length), stream_ptr(stream)))
+
+
+def qk_norm_rope(cfg: QkCfg, tokens: int, q, k, q_weight, k_weight, cos, sin, positions, q_out, k_out,
+                 stream=None) -> None:
+    """Rows of q and k normed per head and rotated by their positions, into q_out and k_out (which may be q
+    and k)."""
+    check(lib().h3_qk_norm_rope(ctypes.byref(cfg), tokens, view(q), view(k), view(q_weight),
+                                view(k_weight), view(cos), view(sin), view(positions), view(q_out),
+                                view(k_out), stream_ptr(stream)))
+
+
+def qk_norm_rope_kv4(cfg: QkCfg, kv: Kv4Cfg, tokens: int, q, k, v, q_weight, k_weight, cos, sin, positions,
+                     slots, q_out, cache, stream=None) -> None:
+    """qk_norm_rope with the rows of k, and of v as they are, into the cache's slots instead."""
+    check(lib().h3_qk_norm_rope_kv4(ctypes.byref(cfg), ctypes.byref(kv), tokens, view(q), view(k), view(v),
+                                    view(q_weight), view(k_weight), view(cos), view(sin),
+                                    view(positions), view(slots), view(q_out), view(cache),
+                                    stream_ptr(stream)))
 
 
 # ------------------------------------------------------------------------- VSA (src/vsa.rs)

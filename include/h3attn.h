@@ -493,6 +493,107 @@ int h3_attention_kv4(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attentio
                      h3_view lengths, h3_view q_starts, h3_view out, h3_view lse, h3_view workspace,
                      h3_stream stream);
 
+/* h3_attention_kv4_sinks: h3_attention_kv4 with the sequence's first `sinks` tokens seen outside the window
+ * too: row i of a sequence's n rows, at position p = length - n + i, sees the keys j <= p with j > p - window or
+ * j < sinks. The bindings, the precision and the workspace's rules are h3_attention_kv4's; without a window (or
+ * without sinks) it is that call. Pages of the table between the first tokens and the window of every row are not
+ * read: their entries may be anything. sinks in [0, 2^24]. */
+size_t h3_kv4_sinks_workspace_bytes(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention,
+                                    uint32_t sinks, uint32_t batch, uint32_t q_rows, uint32_t max_q);
+int h3_attention_kv4_sinks(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention, uint32_t sinks,
+                           uint32_t batch, uint32_t q_rows, uint32_t max_q, h3_view q, h3_view cache,
+                           h3_view table, h3_view lengths, h3_view q_starts, h3_view out, h3_view lse,
+                           h3_view workspace, h3_stream stream);
+
+/* h3_attention_kv4_prefix: h3_attention_kv4 of sequences that continue one prefix. Every row sees the
+ * prefix's prefix_length[0] keys, key j in slot prefix_table[j / page_tokens] * page_tokens + j %
+ * page_tokens, and of its own sequence's lengths[b] keys (table, counted from the prefix's end) those that
+ * h3_attention_kv4 gives it. The softmax and lse are over both.
+ *   prefix_stride  pages that prefix_table holds, (prefix_stride + table_stride) * page_tokens <= 2^24
+ *   prefix_table [prefix_stride] i32, prefix_length [1] i32 (cut to [0, prefix_stride * page_tokens]), read on
+ *   the device as the others are; the config's window is 0.
+ * The other bindings, the precision and the workspace's rules are h3_attention_kv4's. */
+size_t h3_kv4_prefix_workspace_bytes(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention,
+                                     uint32_t prefix_stride, uint32_t batch, uint32_t q_rows, uint32_t max_q);
+int h3_attention_kv4_prefix(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention,
+                            uint32_t prefix_stride, uint32_t batch, uint32_t q_rows, uint32_t max_q, h3_view q,
+                            h3_view cache, h3_view prefix_table, h3_view prefix_length, h3_view table,
+                            h3_view lengths, h3_view q_starts, h3_view out, h3_view lse, h3_view workspace,
+                            h3_stream stream);
+
+/* h3_kv4_advance: what the next step of `batch` sequences needs, from the rows that each asks for. Sequence b
+ * has lengths[b] tokens in ceil(lengths[b] / page_tokens) pages, the first entries of its row of the table.
+ *   asked[b] < 0: the sequence ends. Its pages go on the stack of free pages, free_pages[0 .. free_count - 1],
+ *     before any are taken, in order of sequences and of columns; lengths_out[b] = 0, no rows.
+ *   asked[b] >= 0: so many rows are appended, if the sequence is granted them; all or none. It is refused where
+ *     its tokens would pass the table's row; where it needs pages and those that it and the sequences before it
+ *     ask for (refused or not, but for the first reason) are more than are free; and where the rows that it and
+ *     the sequences before it ask for are more than `rows`. A refused sequence keeps its tokens and pages, and
+ *     shows in q_starts: it has no rows.
+ * Pages are taken from the top of the stack, in order of sequences and columns, into the table. Sequence b's
+ * rows are q_starts[b] .. q_starts[b + 1] - 1; row i of them has positions = prefix + lengths[b] + i and the slot
+ * of that token for h3_kv4_write; lengths_out is for h3_attention_kv4. Rows from q_starts[batch] on carry -1 in slots and
+ * positions. Table entries that are not taken, and the stack above the pushed pages, keep their values.
+ *   asked [batch], lengths [batch], free_pages [cfg->pages], free_count [1], table [batch][table_stride],
+ *   lengths_out [batch] (may be lengths), free_count_out [1] (may be free_count), q_starts [batch + 1], slots
+ *   [rows], positions [rows], prefix_length [1] or an empty view (prefix 0), all i32. batch in [1, 65535], rows in
+ *   [1, 2^24], table_stride * page_tokens <= 2^24; of cfg only page_tokens and pages matter.
+ * All are read on the device. Values outside their ranges read and write nothing out of bounds: lengths
+ * are cut to the table's row, free_count to [0, pages], pages pushed past the stack's end are dropped, a row on a
+ * page that is none of the cache's has slot -1. The same values give the same pages. */
+int h3_kv4_advance(const h3_kv4_cfg *cfg, uint32_t batch, uint32_t table_stride, uint32_t rows, h3_view asked,
+                   h3_view lengths, h3_view free_pages, h3_view free_count, h3_view table,
+                   h3_view lengths_out, h3_view free_count_out, h3_view q_starts, h3_view slots,
+                   h3_view positions, h3_view prefix_length, h3_stream stream);
+
+/* Config of h3_qk_norm_rope and h3_qk_norm_rope_kv4:
+ *   heads, kv_heads  query heads in [1, 4096], key/value heads in [1, 256]
+ *   head_dim     64 or 128
+ *   rotary       channels that are rotated, a multiple of 16 in [0, head_dim]
+ *   interleaved  0: pairs (c, c + rotary / 2); 1: pairs (2 c, 2 c + 1)
+ *   norm         1: RMSNorm per head first; 0: none
+ *   positions    rows of cos and sin, in [1, 2^24]
+ *   eps          finite, >= 0
+ *   elem         H3_ELEM_F16 or H3_ELEM_BF16
+ *   q_stride, k_stride, v_stride, q_out_stride, k_out_stride  elements per row, multiples of 8 from the heads'
+ *                channels to 2^20, so that columns of a fused projection are views into its rows (v_stride is
+ *                read by h3_qk_norm_rope_kv4 alone, k_out_stride by h3_qk_norm_rope alone) */
+typedef struct {
+  uint32_t heads;
+  uint32_t kv_heads;
+  uint32_t head_dim;
+  uint32_t rotary;
+  uint32_t interleaved;
+  uint32_t norm;
+  uint32_t positions;
+  float eps;
+  uint32_t elem;
+  uint32_t q_stride;
+  uint32_t k_stride;
+  uint32_t v_stride;
+  uint32_t q_out_stride;
+  uint32_t k_out_stride;
+} h3_qk_cfg;
+
+/* h3_qk_norm_rope: per row i < tokens and head, y = x / sqrt(mean(x^2) + eps) * weight (norm 1), then each pair
+ * (a, b) of the first `rotary` channels turned by the row's position, (a cos - b sin, b cos + a sin) with
+ * cos[positions[i]][pair] and sin likewise; rounded once to the element type. A row whose position is outside
+ * [0, cfg->positions) is none: q_out and k_out keep theirs (padding rows carry -1).
+ *   q [tokens][q_stride], k [tokens][k_stride], q_out [tokens][q_out_stride], k_out [tokens][k_out_stride]
+ *   (elem, 16-byte aligned; q_out may be q and k_out k, each with one stride), q_weight and k_weight [head_dim] f32
+ *   (empty views where norm is 0), cos and sin [positions][rotary / 2] f32 (empty where rotary is 0; these four
+ *   16-byte aligned), positions [tokens] i32. tokens in [1, 2^24].
+ * Precision: queries in f32 and rounded once; keys as computed in f64 and rounded once to the element type.
+ * h3_qk_norm_rope_kv4: the same, with k and v (v [tokens][v_stride], as it is) into slots[i] of the cache: the
+ * bytes that h3_kv4_write of k_out and v would leave. The cache's kv_heads, head_dim and elem are cfg's. A row that
+ * is none, and one whose slot is outside the cache, is not written there. */
+int h3_qk_norm_rope(const h3_qk_cfg *cfg, uint32_t tokens, h3_view q, h3_view k, h3_view q_weight,
+                    h3_view k_weight, h3_view cos_t, h3_view sin_t, h3_view positions, h3_view q_out,
+                    h3_view k_out, h3_stream stream);
+int h3_qk_norm_rope_kv4(const h3_qk_cfg *cfg, const h3_kv4_cfg *kv, uint32_t tokens, h3_view q, h3_view k,
+                        h3_view v, h3_view q_weight, h3_view k_weight, h3_view cos_t, h3_view sin_t,
+                        h3_view positions, h3_view slots, h3_view q_out, h3_view cache, h3_stream stream);
+
 /* ------------------------------------------------------------------ VSA (video sparse attention) */
 
 /* Config of h3.vsa.* (kernels/vsa_ops.loom:3-9), as src/vsa/device.rs:63-77 builds it:
