@@ -13,6 +13,9 @@
 //
 // D/8 lanes of 8 channels hold a row, so a wave holds one head of 512/D tokens and takes `per` heads of the same
 // tokens one after the other.
+#include <algorithm>
+#include <type_traits>
+
 #include "kv4_row.hpp"
 
 namespace h3 {
@@ -47,7 +50,7 @@ __device__ __forceinline__ float channel(const uint32_t (&w)[4], int i, bool bf1
   return bf16 ? widen<true>(bits) : widen<false>(bits);
 }
 
-// Eight channels and their pairs' others: [..][i] belongs to channel i.
+// The other channels of the pairs that eight channels belong to.
 template <bool kPairs>
 __device__ __forceinline__ void others(const uint32_t (&w)[4], int lane, uint32_t (&o)[4]) {
 #pragma unroll
@@ -80,6 +83,16 @@ __device__ __forceinline__ double row_sum(double v) {
   return v;
 }
 
+// 1 / sqrt(x): the instruction's, to an ulp; in f64 with two steps of Newton's from its 2^-23 or so.
+__device__ __forceinline__ float inverse_root(float x) { return __builtin_amdgcn_rsqf(x); }
+__device__ __forceinline__ double inverse_root(double x) {
+  const double first = __builtin_amdgcn_rsq(x);
+  double r = first;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) r = fma(r * 0.5, fma(-x * r, r, 1.0), r);
+  return first == 0.0 ? 0.0 : r;  // x infinite
+}
+
 // An f64 value rounded once to the element type: to odd in f32 first (toward zero, the last bit set where that lost
 // something), which the second rounding, of at least two bits fewer, cannot mistake for a tie.
 template <bool kBf16>
@@ -91,32 +104,51 @@ __device__ __forceinline__ uint32_t narrow64(double x) {
   return narrow<kBf16>(__uint_as_float(bits));
 }
 
+// Eight f32, 32 bytes on: of a weight, or of a token's cos or sin.
+struct Eight {
+  float v[8];
+};
+__device__ __forceinline__ Eight eight(const float* p) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  return {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+
 // What a token's rows of one weight are multiplied by: own = w cos, other = w' (-sin or sin); past the rotated
 // channels w and 0.
 template <typename T>
 struct Factors {
   T own[8], other[8];
 };
-template <bool kPairs, typename T>
+template <bool kPairs, bool kNorm, typename T>
 __device__ __forceinline__ Factors<T> factors(const QkArgs& a, const Lane& l, const float* weight) {
   Factors<T> f;
   const uint32_t half = a.rotary / 2;
-  const bool turned = l.first < a.rotary, second = !kPairs && l.first >= half;
-  const uint32_t pair = kPairs ? l.first / 2 : second ? l.first - half : l.first;
-  const size_t at = (size_t)(uint32_t)max(l.position, 0) * half + pair;
+  const bool turned = l.first < a.rotary, second = !kPairs && turned && l.first >= half;
+  Eight w, v;
+  if constexpr (kNorm) {
+    w = eight(weight + l.first);
+    v = kPairs || !turned ? w : eight(weight + (second ? l.first - half : l.first + half));
+  }
+  const size_t at = (size_t)(uint32_t)max(l.position, 0) * half;
+  Eight c = {}, s = {};
+  if constexpr (kPairs) {
+    if (turned) {
+      const float4 x = *reinterpret_cast<const float4*>(a.cos_t + at + l.first / 2);
+      const float4 y = *reinterpret_cast<const float4*>(a.sin_t + at + l.first / 2);
+      c = {x.x, x.x, x.y, x.y, x.z, x.z, x.w, x.w};
+      s = {-y.x, y.x, -y.y, y.y, -y.z, y.z, -y.w, y.w};
+    }
+  } else if (turned) {
+    c = eight(a.cos_t + at + (second ? l.first - half : l.first));
+    s = eight(a.sin_t + at + (second ? l.first - half : l.first));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s.v[i] = second ? s.v[i] : -s.v[i];
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const uint32_t c = l.first + i;
-    const uint32_t o = kPairs ? c ^ 1 : second ? c - half : c + half;
-    const T w = weight ? (T)weight[c] : (T)1;
-    f.own[i] = w;
-    f.other[i] = 0;
-    if (turned) {
-      const T cos_i = a.cos_t[at + (kPairs ? i / 2 : i)], sin_i = a.sin_t[at + (kPairs ? i / 2 : i)];
-      const T v = weight ? (T)weight[o] : (T)1;
-      f.own[i] = w * cos_i;
-      f.other[i] = v * ((kPairs ? i & 1 : second) ? sin_i : -sin_i);
-    }
+    const T x = kNorm ? (T)w.v[i] : (T)1, y = kNorm ? (T)v.v[kPairs ? i ^ 1 : i] : (T)1;
+    f.own[i] = turned ? x * (T)c.v[i] : x;
+    f.other[i] = turned ? y * (T)s.v[i] : (T)0;
   }
   return f;
 }
@@ -136,10 +168,7 @@ __device__ __forceinline__ uint4 turn(const QkArgs& a, const Lane& l, const Fact
       sum = fma(x, x, sum);
     }
     sum = row_sum<D>(sum);
-    if constexpr (sizeof(T) == 8)
-      r = 1.0 / sqrt(sum / D + (double)a.eps);
-    else
-      r = 1.0f / sqrtf(sum / D + a.eps);
+    r = inverse_root(fma(sum, (T)(1.0 / D), (T)a.eps));
   }
   uint32_t out[8];
 #pragma unroll
@@ -163,7 +192,48 @@ __device__ __forceinline__ void put(const QkArgs& a, const Lane& l, uint32_t hea
   if (l.first == 0) *reinterpret_cast<uint32_t*>(a.cache + at.words + part * 4 * at.tokens) = row.x;
 }
 
-template <int D, bool kBf16, bool kPairs, bool kNorm, bool kCached>
+// Heads from .. to - 1 (to may be less) of the token's queries, keys or values, kHeads at a time: the next ones' rows are
+// under way while these are computed.
+enum Kind { kQuery, kKey, kValue };
+constexpr uint32_t kHeads = 4;
+template <int D, bool kBf16, bool kPairs, bool kNorm, bool kCached, bool kOnce, Kind kKind>
+__device__ __forceinline__ void units(const QkArgs& a, const Lane& l, uint32_t from, uint32_t to) {
+  if ((int)from >= (int)to) return;
+  const void* rows = kKind == kQuery ? a.q : kKind == kKey ? a.k : a.v;
+  const uint32_t stride = kKind == kQuery ? a.q_stride : kKind == kKey ? a.k_stride : a.v_stride;
+  const size_t row = (size_t)l.token * stride + l.first;
+  uint4 x[kHeads], next[kHeads];
+  const auto load = [&](uint32_t u, uint4 (&to_x)[kHeads]) {
+#pragma unroll
+    for (uint32_t i = 0; i < kHeads; ++i) to_x[i] = load_row<kOnce>(rows, row + min(u + i, to - 1) * D);
+  };
+  load(from, x);
+  using T = std::conditional_t<kKind == kKey, double, float>;
+  Factors<T> f;
+  if constexpr (kKind != kValue)
+    f = factors<kPairs, kNorm, T>(a, l, kKind == kQuery ? a.q_weight : a.k_weight);
+  for (uint32_t u = from; u < to; u += kHeads) {
+    if (u + kHeads < to) load(u + kHeads, next);
+#pragma unroll
+    for (uint32_t i = 0; i < kHeads; ++i) {
+      if (u + i >= to) break;
+      uint4 y = x[i];
+      if constexpr (kKind != kValue) y = turn<D, kBf16, kPairs, kNorm>(a, l, f, y);
+      const uint32_t head = u + i;
+      if constexpr (kKind == kQuery) {
+        if (l.position >= 0) store_row<kOnce>(a.q_out, (size_t)l.token * a.q_out_stride + head * D + l.first, y);
+      } else if constexpr (kCached) {
+        put<D, kBf16>(a, l, head, kKind == kKey ? 0 : 1, y);
+      } else {
+        if (l.position >= 0) store_row<kOnce>(a.k_out, (size_t)l.token * a.k_out_stride + head * D + l.first, y);
+      }
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kHeads; ++i) x[i] = next[i];
+  }
+}
+
+template <int D, bool kBf16, bool kPairs, bool kNorm, bool kCached, bool kOnce>
 __global__ __launch_bounds__(kThreads) void k_qk_norm_rope(QkArgs a) {
   constexpr uint32_t kLanes = D / 8, kTokens = 64 / kLanes;
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -184,42 +254,38 @@ __global__ __launch_bounds__(kThreads) void k_qk_norm_rope(QkArgs a) {
   const uint32_t in_row = lane % kLanes;
   l.other = 4 * (int)(in_row < half ? lane + half : in_row < 2 * half ? lane - half : lane);
 
-  if (from < a.heads) {
-    const Factors<float> f = factors<kPairs, float>(a, l, kNorm ? a.q_weight : nullptr);
-    for (uint32_t u = from; u < min(to, a.heads); ++u) {
-      const uint4 x = load_row<false>(a.q, (size_t)l.token * a.q_stride + u * D + l.first);
-      const uint4 y = turn<D, kBf16, kPairs, kNorm>(a, l, f, x);
-      if (l.position >= 0) store_row<false>(a.q_out, (size_t)l.token * a.q_out_stride + u * D + l.first, y);
-    }
-  }
   const uint32_t k_end = a.heads + a.kv_heads;
-  if (from < k_end && to > a.heads) {
-    const Factors<double> f = factors<kPairs, double>(a, l, kNorm ? a.k_weight : nullptr);
-    for (uint32_t u = max(from, a.heads); u < min(to, k_end); ++u) {
-      const uint32_t head = u - a.heads;
-      const uint4 x = load_row<false>(a.k, (size_t)l.token * a.k_stride + head * D + l.first);
-      const uint4 y = turn<D, kBf16, kPairs, kNorm>(a, l, f, x);
-      if constexpr (kCached)
-        put<D, kBf16>(a, l, head, 0, y);
-      else if (l.position >= 0)
-        store_row<false>(a.k_out, (size_t)l.token * a.k_out_stride + head * D + l.first, y);
-    }
-  }
+  units<D, kBf16, kPairs, kNorm, kCached, kOnce, kQuery>(a, l, from, min(to, a.heads));
+  units<D, kBf16, kPairs, kNorm, kCached, kOnce, kKey>(a, l, max(from, a.heads) - a.heads, min(to, k_end) - a.heads);
   if constexpr (kCached)
-    for (uint32_t u = max(from, k_end); u < to; ++u) {
-      const uint32_t head = u - k_end;
-      put<D, kBf16>(a, l, head, 1, load_row<false>(a.v, (size_t)l.token * a.v_stride + head * D + l.first));
-    }
+    units<D, kBf16, kPairs, kNorm, kCached, kOnce, kValue>(a, l, max(from, k_end) - k_end, to - k_end);
 }
 
-template <int D, bool kBf16, bool kPairs, bool kNorm>
-hipError_t launch(const QkArgs& a, hipStream_t stream) {
-  constexpr uint32_t kTokens = 512 / D;
-  const dim3 grid((a.tokens + kTokens - 1) / kTokens, (a.units + kWaves * a.per - 1) / (kWaves * a.per));
+template <int D, bool kBf16, bool kPairs, bool kNorm, bool kOnce>
+void launch_once(const QkArgs& a, dim3 grid, hipStream_t stream) {
   if (a.cache)
-    hipLaunchKernelGGL((k_qk_norm_rope<D, kBf16, kPairs, kNorm, true>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_qk_norm_rope<D, kBf16, kPairs, kNorm, true, kOnce>), grid, dim3(kThreads), 0, stream, a);
   else
-    hipLaunchKernelGGL((k_qk_norm_rope<D, kBf16, kPairs, kNorm, false>), grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL((k_qk_norm_rope<D, kBf16, kPairs, kNorm, false, kOnce>), grid, dim3(kThreads), 0, stream, a);
+}
+
+// As many heads a wave as leave 16 waves to each compute unit: a token's factors and position serve them all, and their
+// rows are under way together, while few rows want all the waves that there are. One head, as many, and a
+// quarter of a token's (32 + 8 + 8 heads of 128 channels, into the cache): 256 tokens 4.3, 4.3 and 9.6 us,
+// 1,024 9.2, 7.7 and 10.4, 4,096 31, 20 and 20, 31,104 311, 118 and 118 (705 MB: 6.0 TB/s, where a copy reaches 5.2).
+// More than one: long calls, past the caches (31,104 tokens 118 us, and 132 through them; 8,192 38 and 42).
+template <int D, bool kBf16, bool kPairs, bool kNorm>
+hipError_t launch(QkArgs a, hipStream_t stream) {
+  constexpr uint32_t kTokens = 512 / D;
+  const uint32_t groups = (a.tokens + kTokens - 1) / kTokens;
+  const uint64_t waves = (uint64_t)groups * a.units;  // if each took one head
+  a.per = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(waves / (16 * device_cus()), 1),
+                                       (a.units + kWaves - 1) / kWaves);
+  const dim3 grid(groups, (a.units + kWaves * a.per - 1) / (kWaves * a.per));
+  if (a.per > 1)
+    launch_once<D, kBf16, kPairs, kNorm, true>(a, grid, stream);
+  else
+    launch_once<D, kBf16, kPairs, kNorm, false>(a, grid, stream);
   return hipGetLastError();
 }
 
@@ -258,7 +324,6 @@ hipError_t launch_qk_norm_rope(const h3_qk_cfg& cfg, const h3_kv4_cfg* kv, uint3
   a.k_out_stride = cfg.k_out_stride;
   a.eps = cfg.eps;
   a.units = cfg.heads + cfg.kv_heads * (kv ? 2 : 1);
-  a.per = 1;
   if (kv) {
     a.cache = static_cast<uint8_t*>(x.cache);
     a.page_shift = __builtin_ctz(kv->page_tokens);
