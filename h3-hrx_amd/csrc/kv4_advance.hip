@@ -7,16 +7,15 @@
 // granted; of those granted, whose page is which and whose rows are where. No atomics: the same numbers give the
 // same pages.
 //
-// One workgroup makes the sums, 1,024 sequences at a time, and hands out pages by their number in the step (a search
-// in the sums per page: a prompt's hundreds are as quick as a token's one). Rows are slots and positions by
-// the same search.
+// One workgroup makes the sums, a sequence to a thread, and hands out pages by their number in the step (a search in
+// the sums per page: a prompt's hundreds are as quick as a token's one). Where nobody asks for more than one row a
+// thread finishes its own sequence. Long calls' slots and positions are a launch of their own.
 #include "internal.hpp"
 
 namespace h3 {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWaves = kThreads / 64;
+constexpr uint32_t kRowsApart = 2048;  // more rows than this have a launch of their own
 constexpr uint32_t kMost = 1u << 30;  // sums stop here: past every number of rows or pages that can be granted
 
 struct AdvanceArgs {
@@ -30,29 +29,47 @@ struct Two {
 };
 __device__ __forceinline__ uint32_t add(uint32_t x, uint32_t y) { return min(x + y, kMost); }
 
-// The sums over the threads up to this one. `scratch`: a Two per wave.
-__device__ __forceinline__ Two sum_to_here(Two v, Two* scratch) {
+// The sum of v over the wave's lanes up to this one, on the vector pipe: row_shr by 1, 2, 4 and 8, then the last lane
+// of 16 (row_bcast15) and of 32 (row_bcast31) to the lanes after them.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ uint32_t add_from(uint32_t v) {
+  return add(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xF, false));
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+  v = add_from<0x111, 0xF>(v);
+  v = add_from<0x112, 0xF>(v);
+  v = add_from<0x114, 0xF>(v);
+  v = add_from<0x118, 0xF>(v);
+  v = add_from<0x142, 0xA>(v);
+  return add_from<0x143, 0xC>(v);
+}
+
+// The sums over the workgroup's threads up to this one, and over all of them. `scratch`: a Two per wave.
+template <int kThreads>
+__device__ __forceinline__ Two sum_to_here(Two v, Two* scratch, Two* all) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const Two x = {__shfl_up(v.a, d), __shfl_up(v.b, d)};
-    if (lane >= d) v = {add(v.a, x.a), add(v.b, x.b)};
-  }
+  v = {wave_sum(v.a), wave_sum(v.b)};
   __syncthreads();  // the scratch of the call before is read
   if (lane == 63) scratch[wave] = v;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) v = {add(v.a, scratch[w].a), add(v.b, scratch[w].b)};
-  return v;
+  Two before = {0, 0}, sum = {0, 0};
+#pragma unroll
+  for (int w = 0; w < kThreads / 64; ++w) {
+    if (w == wave) before = sum;
+    sum = {add(sum.a, scratch[w].a), add(sum.b, scratch[w].b)};
+  }
+  *all = sum;
+  return {add(v.a, before.a), add(v.b, before.b)};
 }
 
-// The first of n sums, which do not decrease, that is past i.
-__device__ __forceinline__ int find(const uint32_t* sums, int n, uint32_t i) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (sums[mid] > i) hi = mid; else lo = mid + 1;
-  }
-  return lo;
+// The first of kN sums (a power of two, of which none is below the one before it) that is past i; the last one if
+// none is.
+template <int kN>
+__device__ __forceinline__ uint32_t find(const uint32_t* sums, uint32_t i) {
+  uint32_t at = 0;
+#pragma unroll
+  for (uint32_t step = kN / 2; step; step /= 2) at += sums[at + step - 1] <= i ? step : 0;
+  return at;
 }
 
 __device__ __forceinline__ uint32_t tokens_of(const AdvanceArgs& a, uint32_t b) {
@@ -63,10 +80,25 @@ __device__ __forceinline__ int slot_of(const AdvanceArgs& a, int page, uint32_t 
   return (uint32_t)page < a.pages ? (page << a.page_shift) + (int)(position & ((1u << a.page_shift) - 1)) : -1;
 }
 
-__global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a) {
-  __shared__ Two scratch[kWaves];
+// take(i) and then put(i, what it gave) for i in t, t + kThreads, .. below n: four under way at a time.
+template <int kThreads, typename Take, typename Put>
+__device__ __forceinline__ void each(uint32_t t, uint32_t n, Take take, Put put) {
+  for (uint32_t i = t; i < n; i += 4 * kThreads) {
+    decltype(take(i)) got[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      if (i + k * kThreads < n) got[k] = take(i + k * kThreads);
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      if (i + k * kThreads < n) put(i + k * kThreads, got[k]);
+  }
+}
+
+// places: whether slots and positions are written here.
+template <int kThreads>
+__global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a, bool places) {
+  __shared__ Two scratch[kThreads / 64];
   __shared__ uint32_t page_sums[kThreads], row_sums[kThreads], first_column[kThreads], first_token[kThreads];
-  __shared__ Two carry_s, granted_s;
   const uint32_t t = threadIdx.x, up = (1u << a.page_shift) - 1;
   const uint32_t before = (uint32_t)min(max(*a.x.free_count, 0), (int)a.pages);
   const uint32_t prefix = a.x.prefix_length ? (uint32_t)max(*a.x.prefix_length, 0) : 0;
@@ -77,16 +109,19 @@ __global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a) {
     const uint32_t b = b0 + t;
     uint32_t held = 0;
     if (b < a.batch && a.x.asked[b] < 0) held = (tokens_of(a, b) + up) >> a.page_shift;
-    const Two sums = sum_to_here({held, 0}, scratch);
-    page_sums[t] = sums.a;
+    if (!__syncthreads_or(held != 0)) continue;
+    Two all;
+    page_sums[t] = sum_to_here<kThreads>({held, 0}, scratch, &all).a;
     __syncthreads();
-    const uint32_t all = page_sums[kThreads - 1];
-    for (uint32_t i = t; i < all; i += kThreads) {
-      const int s = find(page_sums, kThreads, i);
-      const uint32_t column = i - (s ? page_sums[s - 1] : 0);
-      if (count + i < a.pages) a.x.free_pages[count + i] = a.x.table[(size_t)(b0 + s) * a.columns + column];
-    }
-    count = min(count + all, a.pages);
+    each<kThreads>(t, all.a,
+                   [&](uint32_t i) {
+                     const uint32_t s = find<kThreads>(page_sums, i);
+                     return a.x.table[(size_t)(b0 + s) * a.columns + i - (s ? page_sums[s - 1] : 0)];
+                   },
+                   [&](uint32_t i, int page) {
+                     if (count + i < a.pages) a.x.free_pages[count + i] = page;
+                   });
+    count = min(count + all.a, a.pages);
   }
   __syncthreads();
 
@@ -96,6 +131,7 @@ __global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a) {
   for (uint32_t b0 = 0; b0 < a.batch; b0 += kThreads) {
     const uint32_t b = b0 + t;
     uint32_t have = 0, rows = 0, held = 0, need = 0;
+    int last_page = -1;  // where a single row goes if it needs no page
     if (b < a.batch) {
       const int n = a.x.asked[b];
       if (n >= 0) {
@@ -103,44 +139,113 @@ __global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a) {
         if ((uint64_t)have + (uint32_t)n <= (uint64_t)a.columns << a.page_shift) rows = (uint32_t)n;
         held = (have + up) >> a.page_shift;
         need = ((have + rows + up) >> a.page_shift) - held;
+        if (held) last_page = a.x.table[(size_t)b * a.columns + held - 1];
       }
     }
-    Two sums = sum_to_here({need, rows}, scratch);
-    sums = {add(sums.a, asked.a), add(sums.b, asked.b)};
-    if ((need != 0 && sums.a > count) || sums.b > a.rows) rows = need = 0;
-    const Two mine = sum_to_here({need, rows}, scratch);
-    page_sums[t] = mine.a;
-    row_sums[t] = mine.b;
-    first_column[t] = held;
-    first_token[t] = have;
-    if (t == kThreads - 1) {
-      carry_s = sums;
-      granted_s = mine;
-    }
-    __syncthreads();
-    asked = carry_s;
-    const Two all = granted_s;
-    for (uint32_t i = t; i < all.a; i += kThreads) {
-      const int s = find(page_sums, kThreads, i);
-      const uint32_t column = first_column[s] + i - (s ? page_sums[s - 1] : 0);
-      a.x.table[(size_t)(b0 + s) * a.columns + column] = a.x.free_pages[count - 1 - (granted.a + i)];
+    Two all;
+    Two mine = sum_to_here<kThreads>({need, rows}, scratch, &all);
+    const Two sums = {add(mine.a, asked.a), add(mine.b, asked.b)};
+    asked = {add(asked.a, all.a), add(asked.b, all.b)};
+    const bool refused = (need != 0 && sums.a > count) || sums.b > a.rows;
+    if (__syncthreads_or(refused)) {
+      if (refused) rows = need = 0;
+      mine = sum_to_here<kThreads>({need, rows}, scratch, &all);
     }
     if (b < a.batch) {
       a.x.lengths_out[b] = (int)(have + rows);
       a.x.q_starts[b + 1] = (int)(granted.b + mine.b);
     }
-    __syncthreads();
-    for (uint32_t i = t; i < all.b; i += kThreads) {
-      const int s = find(row_sums, kThreads, i);
-      const uint32_t position = first_token[s] + i - (s ? row_sums[s - 1] : 0);
-      const int page = a.x.table[(size_t)(b0 + s) * a.columns + (position >> a.page_shift)];
-      a.x.slots[granted.b + i] = slot_of(a, page, position);
-      a.x.positions[granted.b + i] = (int)(prefix + position);
+    if (!__syncthreads_or(rows > 1)) {
+      const uint32_t at = granted.b + mine.b - 1;
+      if (rows) {
+        if (need) {
+          last_page = a.x.free_pages[count - granted.a - mine.a];
+          a.x.table[(size_t)b * a.columns + held] = last_page;
+        }
+        if (places) {
+          a.x.slots[at] = slot_of(a, last_page, have);
+          a.x.positions[at] = (int)(prefix + have);
+        }
+      }
+    } else {
+      page_sums[t] = mine.a;
+      row_sums[t] = mine.b;
+      first_column[t] = held;
+      first_token[t] = have;
+      __syncthreads();
+      each<kThreads>(t, all.a,
+                     [&](uint32_t i) { return a.x.free_pages[count - 1 - (granted.a + i)]; },
+                     [&](uint32_t i, int page) {
+                       const uint32_t s = find<kThreads>(page_sums, i);
+                       const uint32_t column = first_column[s] + i - (s ? page_sums[s - 1] : 0);
+                       a.x.table[(size_t)(b0 + s) * a.columns + column] = page;
+                     });
+      if (places) {
+        __syncthreads();
+        const auto position = [&](uint32_t i, uint32_t s) { return first_token[s] + i - (s ? row_sums[s - 1] : 0); };
+        each<kThreads>(t, all.b,
+                       [&](uint32_t i) {
+                         const uint32_t s = find<kThreads>(row_sums, i), at = position(i, s);
+                         const int page = a.x.table[(size_t)(b0 + s) * a.columns + (at >> a.page_shift)];
+                         return int2{slot_of(a, page, at), (int)(prefix + at)};
+                       },
+                       [&](uint32_t i, int2 place) {
+                         a.x.slots[granted.b + i] = place.x;
+                         a.x.positions[granted.b + i] = place.y;
+                       });
+      }
     }
     granted = {granted.a + all.a, granted.b + all.b};
   }
-  for (uint32_t i = granted.b + t; i < a.rows; i += kThreads) a.x.slots[i] = a.x.positions[i] = -1;
+  if (places)
+    for (uint32_t i = granted.b + t; i < a.rows; i += kThreads) a.x.slots[i] = a.x.positions[i] = -1;
   if (t == 0) *a.x.free_count_out = (int)(count - granted.a);
+}
+
+// Slots and positions from q_starts, lengths_out and the table: four rows a thread. Where the starts fit LDS the search
+// for the first row's sequence is there.
+constexpr int kPlaceThreads = 256, kPlaceRows = 4, kPlaceStarts = 2048;
+__global__ __launch_bounds__(kPlaceThreads) void k_kv4_places(AdvanceArgs a) {
+  __shared__ uint32_t ends[kPlaceStarts];
+  const uint32_t first = (blockIdx.x * kPlaceThreads + threadIdx.x) * kPlaceRows;
+  const int* starts = a.x.q_starts;
+  const uint32_t prefix = a.x.prefix_length ? (uint32_t)max(*a.x.prefix_length, 0) : 0;
+  uint32_t b = 0;  // the first sequence whose end is past the row
+  if (a.batch < kPlaceStarts) {
+    for (uint32_t i = threadIdx.x; i < kPlaceStarts; i += kPlaceThreads)
+      ends[i] = i < a.batch ? (uint32_t)starts[i + 1] : ~0u;
+    __syncthreads();
+    b = find<kPlaceStarts>(ends, first);
+  } else {
+    for (uint32_t hi = a.batch; b < hi;) {
+      const uint32_t mid = (b + hi) / 2;
+      if ((uint32_t)starts[mid + 1] > first) hi = mid; else b = mid + 1;
+    }
+  }
+  uint32_t end = 0, length = 0;
+  if (b < a.batch) end = (uint32_t)starts[b + 1], length = (uint32_t)a.x.lengths_out[b];
+  int slot[kPlaceRows], position[kPlaceRows];
+#pragma unroll
+  for (uint32_t i = 0; i < kPlaceRows; ++i) {
+    const uint32_t row = first + i;
+    while (b < a.batch && row >= end) {
+      if (++b == a.batch) break;
+      end = (uint32_t)starts[b + 1];
+      length = (uint32_t)a.x.lengths_out[b];
+    }
+    slot[i] = position[i] = -1;
+    if (b < a.batch) {
+      const uint32_t at = length - (end - row);
+      slot[i] = slot_of(a, a.x.table[(size_t)b * a.columns + (at >> a.page_shift)], at);
+      position[i] = (int)(prefix + at);
+    }
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < kPlaceRows; ++i)
+    if (first + i < a.rows) {
+      a.x.slots[first + i] = slot[i];
+      a.x.positions[first + i] = position[i];
+    }
 }
 
 }  // namespace
@@ -148,7 +253,15 @@ __global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a) {
 hipError_t launch_kv4_advance(const h3_kv4_cfg& cfg, uint32_t batch, uint32_t table_stride, uint32_t rows,
                               const AdvanceBindings& x, hipStream_t stream) {
   AdvanceArgs a{x, batch, table_stride, rows, cfg.pages, (uint32_t)__builtin_ctz(cfg.page_tokens)};
-  hipLaunchKernelGGL(k_kv4_advance, dim3(1), dim3(kThreads), 0, stream, a);
+  const bool apart = rows > kRowsApart;
+  if (batch <= 64)
+    hipLaunchKernelGGL(k_kv4_advance<256>, dim3(1), dim3(256), 0, stream, a, !apart);
+  else
+    hipLaunchKernelGGL(k_kv4_advance<1024>, dim3(1), dim3(1024), 0, stream, a, !apart);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || !apart) return e;
+  constexpr uint32_t kRows = kPlaceThreads * kPlaceRows;
+  hipLaunchKernelGGL(k_kv4_places, dim3((rows + kRows - 1) / kRows), dim3(kPlaceThreads), 0, stream, a);
   return hipGetLastError();
 }
 
