@@ -1302,8 +1302,9 @@ size_t h3_kv4_prefix_workspace_bytes(const h3_kv4_cfg* cfg, const h3_kv4_attenti
   if (check_kv4_prefix("kv4_prefix_workspace_bytes", cfg, attention, prefix_stride, batch, q_rows, max_q))
     return 0;
   ok();
-  return kv4_workspace_bytes(*cfg, batch, kv4_front_plan(*cfg, *attention, (uint64_t)prefix_stride * cfg->page_tokens, batch,
-                                                         q_rows, max_q, device_cus(), true));
+  return kv4_prefix_workspace_bytes(*cfg, *attention, batch, q_rows,
+                                    kv4_prefix_plan(*cfg, *attention, prefix_stride, batch, q_rows, max_q,
+                                                    device_cus(), true));
 }
 
 int h3_attention_kv4_prefix(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* attention,
@@ -1314,9 +1315,10 @@ int h3_attention_kv4_prefix(const h3_kv4_cfg* cfg, const h3_kv4_attention_cfg* a
   const char* stage = "attention_kv4_prefix";
   const int st = check_kv4_prefix(stage, cfg, attention, prefix_stride, batch, q_rows, max_q);
   if (st) return st;
-  const Kv4Plan plan = kv4_front_plan(*cfg, *attention, (uint64_t)prefix_stride * cfg->page_tokens, batch,
-                                      q_rows, max_q, device_cus(), workspace.ptr != nullptr);
-  return attend_kv4(stage, *cfg, *attention, batch, q_rows, kv4_workspace_bytes(*cfg, batch, plan), q, cache,
+  const Kv4PrefixPlan plan = kv4_prefix_plan(*cfg, *attention, prefix_stride, batch, q_rows, max_q,
+                                             device_cus(), workspace.ptr != nullptr);
+  return attend_kv4(stage, *cfg, *attention, batch, q_rows,
+                    kv4_prefix_workspace_bytes(*cfg, *attention, batch, q_rows, plan), q, cache,
                     {prefix_table, prefix_length}, {(size_t)prefix_stride * 4, 4}, table, lengths, q_starts,
                     out, lse, workspace, [&](const Kv4Bindings& x) {
                       return launch_attention_kv4_prefix(*cfg, *attention, prefix_stride, plan, batch, q_rows,

@@ -105,7 +105,8 @@ Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32
 }
 
 Kv4Plan kv4_front_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint64_t front_keys,
-                       uint32_t batch, uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide) {
+                       uint32_t batch, uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide,
+                       double* time) {
   const uint32_t group = acfg.heads / cfg.kv_heads, rows = max_q * group;
   const bool alike = (uint64_t)batch * max_q == q_rows;  // every sequence has max_q rows
   const uint64_t all_keys = (uint64_t)acfg.table_stride * cfg.page_tokens + (acfg.window ? 0 : front_keys);
@@ -118,8 +119,9 @@ Kv4Plan kv4_front_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, 
       acfg.causal && !acfg.window ? 1 - std::min<uint64_t>(all_keys, max_q) / 2.0 / all_keys : 1;
   Kv4Plan p{};
   double least = 1e30;
-  const auto take = [&](const Kv4Launch& many, const Kv4Launch& few, double time) {
-    if (time < least) p = {many, few}, least = time;
+  const auto take = [&](const Kv4Launch& many, const Kv4Launch& few, double t) {
+    if (t < least) p = {many, few}, least = t;
+    if (time) *time = least;
   };
   double small = 0, large = 0, singles = 0;
   if (rows <= kFewMost) {
@@ -139,6 +141,106 @@ Kv4Plan kv4_front_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, 
   many.rows_from = group + 1;
   take(many, few, large + singles);
   return p;
+}
+
+namespace {
+
+constexpr uint32_t kJoinParts = 64;     // lanes of the join's wave
+constexpr double kSharedBytes = 200e6;  // of the sums of a shared call
+
+// Workgroups of k_attention_kv4_few or _mid with `steps` of their four waves' steps each, over keys that many of them
+// share: us alone on a compute unit, and of one of 512 beside another (`each`: its part of the launch's time). Per step 1.2
+// alone and 2.3 beside another (4 rows, 256 keys), 1.0 and 1.4 (32 rows, 128 keys).
+struct Work {
+  double alone, each;
+};
+Work few_work(uint32_t tile, double steps, uint32_t cus) {
+  const double one = tile <= 4 ? 1.2 : tile <= 8 ? 1.3 : tile <= 16 ? 1.8 : 1.03;
+  const double two = tile <= 4 ? 2.3 : tile <= 8 ? 2.5 : tile <= 16 ? 3.4 : 1.4;
+  return tile == kMidRows ? Work{7 + steps * one, (3 + steps * two) / (2 * cus)}
+                          : Work{5 + steps * one, (4 + steps * two) / (2 * cus)};
+}
+double few_steps(uint32_t tile, double keys) { return keys / (kWaves * (tile == kMidRows ? kMidKeys : kStepKeys)); }
+
+}  // namespace
+
+// Estimated as above, by the workgroups' work rather than HBM's rate, since the prefix comes from the caches. In us, in
+// one pass, shared in tiles of 32 (in parts) and along a line of tiles of 256, 4 query heads to each of 8 cache heads:
+//   rows (sequences x new tokens)     keys: prefix, own   one pass   tiles of 32    of 256
+//   64 x 1                            8,192, 700 at most   81         34 (4)         59
+//   16 x 1                            2,000, 300           18         12.5 (8)       29
+//   64 x 1                            1,000, 700           22         23 (4)         49
+//   32 x 1                            30,000, 300          132        41 (16)        56
+//   400 x 1                           3,000, 300           180        79 (1)         110
+//   32 x 9                            10,000, 500          134        94 (4)         114
+//   4 x 130                           20,000, 130          306        306            254
+//   8 x 257                           31,104, 257          1,415                     1,215
+//   8 x 257                           2,000, 257           166                       171
+Kv4PrefixPlan kv4_prefix_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t prefix_stride,
+                              uint32_t batch, uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide) {
+  const uint64_t prefix = (uint64_t)prefix_stride * cfg.page_tokens;
+  const uint64_t own_keys = (uint64_t)acfg.table_stride * cfg.page_tokens;
+  const uint32_t group = acfg.heads / cfg.kv_heads;
+  const uint64_t rows = (uint64_t)q_rows * group;  // of a cache head
+  Kv4PrefixPlan p{};
+  double least = 0, own_time = 0;
+  p.one = kv4_front_plan(cfg, acfg, prefix, batch, q_rows, max_q, cus, divide, &least);
+  const double row_bytes = (double)rows * cfg.kv_heads * (cfg.head_dim + 2) * 4;
+  if (!divide || row_bytes > kSharedBytes) return p;
+  const auto groups_of = [&](const Kv4Launch& few) {  // workgroups of a part of few rows
+    return cfg.kv_heads * std::min((double)batch * few.row_tiles, (double)rows / few.tile_rows + batch);
+  };
+  const auto join = [&](uint32_t parts) { return 3.5 + 0.15 * parts + parts * row_bytes * 2 / 4e6; };
+  if (p.one.many.row_tiles == 0) {
+    const Kv4Launch& few = p.one.few;
+    const Work w = few_work(few.tile_rows, few_steps(few.tile_rows, (double)(prefix + own_keys)) / few.parts, cus);
+    const double wgs = groups_of(few) * few.parts;
+    least = (wgs <= cus ? w.alone : std::max(w.alone, 2 + wgs * w.each)) + (few.parts > 1 ? join(few.parts) : 0);
+  }
+  p.own = kv4_front_plan(cfg, acfg, 0, batch, q_rows, max_q, cus, false, &own_time);
+  const bool small = p.own.many.row_tiles == 0;
+  const Work own = few_work(p.own.few.tile_rows, few_steps(p.own.few.tile_rows, (double)own_keys), cus);
+  const double own_each = small ? groups_of(p.own.few) * own.each : 0;
+  if (small) own_time = std::max(own.alone, 2 + own_each);
+  const auto take = [&](double time, uint32_t front_parts, uint32_t front_groups, uint32_t parts) {
+    if (parts > kJoinParts || parts * row_bytes > kSharedBytes || time >= least) return;
+    least = time;
+    p.shared = true;
+    p.front_parts = front_parts;
+    p.front_groups = front_groups;
+    p.parts = parts;
+  };
+  // Tiles of 32 rows, in one launch with the sequences' own where those are few.
+  if (rows <= kFewMost && small) {
+    const uint32_t tiles = (uint32_t)(rows + kMidRows - 1) / kMidRows * cfg.kv_heads;
+    const double steps = std::max(1.0, few_steps(kMidRows, (double)prefix));
+    for (uint32_t n = 1; n <= steps && n < kJoinParts; ++n) {
+      const Work w = few_work(kMidRows, steps / n, cus);
+      // One of them to a compute unit runs beside the sequences' own, two beside each other.
+      const double longest = 7 + steps / n * (tiles * n <= cus ? 1.37 : 2.05);
+      // More of them than find room: the last ones leave the chip partly idle.
+      const double tail = tiles * n > 2 * cus ? 0.25 * w.each * 2 * cus : 0;
+      take(std::max({longest, own.alone, 6 + (double)tiles * n * w.each + own_each + tail}) + join(1 + n), n,
+           n * tiles, 1 + n);
+    }
+  }
+  // Tiles of 256 rows along one line.
+  const uint64_t tiles = (rows + kTileRows - 1) / kTileRows * cfg.kv_heads;
+  const double steps = (double)((prefix + kTileKeys - 1) / kTileKeys), all = tiles * steps;
+  if (all < (1u << 30)) {
+    const uint32_t groups = (uint32_t)std::min<double>(cus, std::max(1.0, all / kLeastSteps));
+    const uint32_t pieces = (uint32_t)((groups + tiles - 1) / tiles) + 1;
+    const double step = 0.9 + 0.175 * std::min<double>(8, (rows + 31) / 32);
+    take(own_time + 12 + 8 * (tiles / (double)groups + 1) + all / groups * step + join(1 + pieces), 0, groups,
+         1 + pieces);
+  }
+  return p;
+}
+
+size_t kv4_prefix_workspace_bytes(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
+                                  uint32_t q_rows, const Kv4PrefixPlan& plan) {
+  if (!plan.shared) return kv4_workspace_bytes(cfg, batch, plan.one);
+  return (size_t)plan.parts * q_rows * acfg.heads * (cfg.head_dim + 2) * 4;
 }
 
 size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, uint32_t batch, const Kv4Plan& plan) {

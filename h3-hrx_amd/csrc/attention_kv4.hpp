@@ -34,16 +34,19 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_inff();
 
-// The keys of a launch's rows beside those of their own sequence: none; the sequence's first tokens, seen
-// outside the window too; or the tokens of a prefix that all sequences share.
-enum Keys { kOwn, kSinks, kPrefix };
+// The keys that a launch's rows see: their own sequence's; with its first tokens outside the window too; behind a
+// prefix that all sequences share; their own sequence's alone, or that prefix alone, of all rows of the call as
+// one sequence's, their sums left in the workspace for the join of the two.
+enum Keys { kOwn, kSinks, kPrefix, kOwnPart, kFrontPart };
+template <Keys K> constexpr bool kPart = K == kOwnPart || K == kFrontPart;
+template <Keys K> constexpr bool kPlain = K != kSinks && K != kPrefix;  // nothing lies before span(i)
 
 struct Args {
   const void* q;
   const uint8_t* cache;
   const int32_t* table;
   const int32_t* prefix_table;   // kPrefix
-  const int32_t* prefix_length;  // kPrefix: one
+  const int32_t* prefix_length;  // kPrefix, kFrontPart: one
   const int32_t* lengths;
   const int32_t* q_starts;
   void* out;
@@ -59,6 +62,9 @@ struct Args {
   uint32_t causal, window;
   uint32_t sinks;          // kSinks: the first tokens
   uint32_t prefix_stride;  // kPrefix: pages that prefix_table holds
+  uint32_t part0, part_rows;  // kPart: the launch's first part, and the call's rows (tokens times group)
+  uint32_t front_parts;  // kPart: the parts that the prefix's sums are in (0: pieces of a line, front_groups long)
+  uint32_t front_groups;
   float scale;  // the softmax scale times log2(e)
 };
 
@@ -76,6 +82,12 @@ template <Keys K>
 __device__ __forceinline__ Sequence sequence(const Args& a, uint32_t b) {
   Sequence s;
   s.front = s.base = 0;
+  if constexpr (K == kFrontPart) {
+    s.start = 0;
+    s.n = s.rows = (int)a.q_rows;
+    s.length = min(max(*a.prefix_length, 0), (int)(a.table_stride << a.page_shift));
+    return s;
+  }
   if constexpr (K == kSinks) s.front = (int)a.sinks;
   if constexpr (K == kPrefix) {
     const int unit = max(1 << a.page_shift, kFrontUnit);
@@ -99,7 +111,7 @@ __device__ __forceinline__ bool takes(const Args& a, int rows) {
 template <Keys K>
 __device__ __forceinline__ int2 span(const Args& a, const Sequence& s, int i) {
   const int base = K == kPrefix ? s.base : 0;
-  if (!a.causal) return {base, base + s.length};
+  if (K == kFrontPart || !a.causal) return {base, base + s.length};
   const int p = s.length - s.n + i;
   const int hi = min(max(p + 1, 0), s.length);
   const int lo = a.window ? (int)max((int64_t)p + 1 - a.window, (int64_t)0) : 0;
@@ -109,13 +121,13 @@ __device__ __forceinline__ int2 span(const Args& a, const Sequence& s, int i) {
 // Whether a row that sees [seen.x, seen.y) and what lies below `front` before it does not see key `key`.
 template <Keys K>
 __device__ __forceinline__ bool unseen(const Sequence& s, int2 seen, int key) {
-  if constexpr (K == kOwn) return (key < seen.x) | (key >= seen.y);
+  if constexpr (kPlain<K>) return (key < seen.x) | (key >= seen.y);
   return ((key < seen.x) & (key >= s.front)) | (key >= seen.y);
 }
 // Whether rows of which each sees all of [lo, hi) see all the `keys` keys from key0 on.
 template <Keys K>
 __device__ __forceinline__ bool all_seen(const Sequence& s, int lo, int hi, int key0, int keys) {
-  if constexpr (K == kOwn) return key0 >= lo && key0 + keys <= hi;
+  if constexpr (kPlain<K>) return key0 >= lo && key0 + keys <= hi;
   return (key0 >= lo || key0 + keys <= s.front) && key0 + keys <= hi;
 }
 
@@ -130,14 +142,14 @@ template <Keys K, int kKeys>
 struct Walk {
   int front, gap, first, last;
   __device__ __forceinline__ int key(int v) const {
-    if constexpr (K == kOwn) return v * kKeys;
+    if constexpr (kPlain<K>) return v * kKeys;
     return (v < front ? v : v + gap) * kKeys;
   }
 };
 template <Keys K, int kKeys>
 __device__ __forceinline__ Walk<K, kKeys> walk(const Sequence& s, int lo, int hi) {
   const int first = lo / kKeys, end = (hi + kKeys - 1) / kKeys;
-  if constexpr (K == kOwn) return {0, 0, first, end};
+  if constexpr (kPlain<K>) return {0, 0, first, end};
   const int front = (min(s.front, hi) + kKeys - 1) / kKeys, gap = max(first - front, 0);
   return {front, gap, 0, max(end - gap, front)};
 }
@@ -364,21 +376,32 @@ __device__ __forceinline__ float mean(float sum, const Mean& m) {
 }
 
 // Where part `part` of a row's keys leaves its sums: row `row` (of at most rows_to) of sequence b.
-__device__ __forceinline__ size_t few_place(const Args& a, uint32_t part, uint32_t b, uint32_t row,
-                                            uint32_t head) {
+template <Keys K>
+__device__ __forceinline__ size_t few_place(const Args& a, const Sequence& s, uint32_t part, uint32_t b,
+                                            uint32_t row, uint32_t head) {
+  if constexpr (kPart<K>)
+    return ((size_t)(a.part0 + part) * a.part_rows + (uint32_t)s.start * a.group + row) * a.kv_heads + head;
   return (((size_t)part * a.batch + b) * a.rows_to + row) * a.kv_heads + head;
 }
 
+template <int D, int R>
+struct FewLds {
+  __attribute__((aligned(16))) uint16_t p[kWaves][kStepKeys * R];
+  __attribute__((aligned(16))) float o[kWaves][R][D + 4];
+  float row[kWaves][R];  // a factor per row, from its lanes to its column
+  float2 ml[kWaves][R];
+};
+
 template <int D, bool kBf16, int R, bool kOnce, Keys K>
-__global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
+__device__ __forceinline__ void attend_few(const Args& a, FewLds<D, R>& lds, uint32_t part, uint32_t head,
+                                           uint32_t b) {
   constexpr int T = 16 / R, kTiles = R / 4, kSteps = D / 32, kDimTiles = D / 16;
-  __shared__ __attribute__((aligned(16))) uint16_t lds_p[kWaves][kStepKeys * R];
-  __shared__ __attribute__((aligned(16))) float lds_o[kWaves][R][D + 4];
-  __shared__ float lds_row[kWaves][R];    // a factor per row, from its lanes to its column
-  __shared__ float2 lds_ml[kWaves][R];
+  auto &lds_p = lds.p;
+  auto &lds_o = lds.o;
+  auto &lds_row = lds.row;
+  auto &lds_ml = lds.ml;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, h = lane >> 4;
-  const uint32_t head = blockIdx.y, b = blockIdx.z, part = blockIdx.x;
   const int32_t* table = a.table + (size_t)b * a.table_stride;
   // Step `part` * 4 + wave of the sequence and every 4 * parts-th after it. Without a window the first
   // is known before the sequence is, and its loads go ahead: where the sequence ends before it, they
@@ -387,7 +410,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
   const int group = (int)a.group, rows = seq.rows * group, stride = (int)a.parts * kWaves;
   int step = (int)part * kWaves + wave;
   Walk<K, kStepKeys> way{};
-  if constexpr (K == kOwn) {
+  if constexpr (kPlain<K>) {
     if (a.window) step += span<K>(a, seq, 0).x / kStepKeys;
   } else {
     way = walk<K, kStepKeys>(seq, span<K>(a, seq, 0).x, span<K>(a, seq, (rows - 1) / group).y);
@@ -400,10 +423,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
   const int2 first_span = span<K>(a, seq, 0), last_span = span<K>(a, seq, (rows - 1) / group);
   const int key_lo = first_span.x, key_hi = last_span.y;  // seen by some row
   const int all_lo = last_span.x, all_hi = first_span.y;  // seen by every row
-  const int last = K == kOwn ? (key_hi + kStepKeys - 1) / kStepKeys : way.last;
+  const int last = kPlain<K> ? (key_hi + kStepKeys - 1) / kStepKeys : way.last;
   const uint32_t heads = a.kv_heads * a.group;
   if (part > 0 && step - wave >= last) {  // no keys: part 0 stands for an empty row
-    if ((int)threadIdx.x < rows) a.part_ml[few_place(a, part, b, threadIdx.x, head)] = {-kInf, 0};
+    if ((int)threadIdx.x < rows) a.part_ml[few_place<K>(a, seq, part, b, threadIdx.x, head)] = {-kInf, 0};
     return;
   }
 
@@ -447,8 +470,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
     const int key0 = way.key(step);
     if (step + stride < last) {
       const int now = ids;
-      ids = page_of<K>(a, table, seq, (K == kOwn ? key0 + 2 * kStepKeys * stride : way.key(step + 2 * stride)) + lane);
-      load_step<D, R, kOnce>(a, now, head, K == kOwn ? key0 + kStepKeys * stride : way.key(step + stride), lane, next);
+      ids = page_of<K>(a, table, seq, (kPlain<K> ? key0 + 2 * kStepKeys * stride : way.key(step + 2 * stride)) + lane);
+      load_step<D, R, kOnce>(a, now, head, kPlain<K> ? key0 + kStepKeys * stride : way.key(step + stride), lane, next);
     }
     // Scores.
     v4f acc[kTiles];
@@ -662,8 +685,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
     const int token = row / group, g = row - token * group;
     const size_t q_row = (size_t)(seq.start + token);
     const uint32_t q_head = head * group + g;
-    if (a.parts > 1) {
-      const size_t place = few_place(a, part, b, row, head);
+    if (kPart<K> || a.parts > 1) {
+      const size_t place = few_place<K>(a, seq, part, b, row, head);
 #pragma unroll
       for (int d = 0; d < kPer; ++d) a.part_o[place * D + ch + d] = sum[d];
       if (ch == 0) a.part_ml[place] = {top, total};
@@ -677,6 +700,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
         a.lse[q_row * heads + q_head] = none ? -kInf : (top + __log2f(total)) * kLn2;
     }
   }
+}
+
+template <int D, bool kBf16, int R, bool kOnce, Keys K>
+__global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
+  __shared__ FewLds<D, R> lds;
+  attend_few<D, kBf16, R, kOnce, K>(a, lds, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 // Many rows: eight waves of 32 rows share tiles of 64 keys in LDS, unpacked once for all of them:
@@ -916,7 +945,7 @@ __device__ __forceinline__ v16f attend_block(const RowsLds<D>& lds, int buf, int
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int k = (i & 7) + 2 * (i & 8);
-      if ((k < seen.lo && (K == kOwn || k >= seen.front)) || k >= seen.hi) y[i] = -kInf;
+      if ((k < seen.lo && (kPlain<K> || k >= seen.front)) || k >= seen.hi) y[i] = -kInf;
     }
     if (seen.pages) {
       asm volatile("");
@@ -1034,7 +1063,7 @@ __device__ __forceinline__ void attend_rows(const Args& a, RowsLds<D>& lds, cons
     const int key = way.key(st.first) + at;
     fetch<D>(a, head, key, page_of<K>(a, table, seq, key), staged);
     page = page_of<K>(a, table, seq, way.key(st.first + 1) + at);
-    if constexpr (K == kOwn) {
+    if constexpr (kPlain<K>) {
       for (int k = max(st.first * kTileKeys, key_lo & ~15) + 16 * (int)threadIdx.x;
            k < min(st.last * kTileKeys, key_hi); k += 16 * kRowsThreads)
         hidden |= page_of<K>(a, table, seq, k) < 0;
@@ -1058,14 +1087,14 @@ __device__ __forceinline__ void attend_rows(const Args& a, RowsLds<D>& lds, cons
   bool under_way = false;  // x holds this tile's first products
   for (int step = st.first; step < st.last; ++step) {
     const int next = buf == 2 ? 0 : buf + 1, key0 = way.key(step), key1 = way.key(step + 1);
-    const bool takes_tile = K == kOwn ? step >= from && step < to
+    const bool takes_tile = kPlain<K> ? step >= from && step < to
                                       : active && key0 < wave_last.y &&
                                             (key0 < seq.front || key0 + kTileKeys > wave_first.x);
     if (takes_tile) {
       const bool whole = all_seen<K>(seq, wave_last.x, wave_first.y, key0, kTileKeys) && !hidden;
-      if (K == kOwn ? step == from : !under_way) {
+      if (kPlain<K> ? step == from : !under_way) {
         const KeyOps<D> k0 = read_keys<D, 0>(lds, buf, 0, lane), k1 = read_keys<D, D / 32>(lds, buf, 0, lane);
-        if constexpr (K != kOwn) x = v16f{};  // between the front's tiles and its own the wave let some pass
+        if constexpr (!kPlain<K>) x = v16f{};  // between the front's tiles and its own the wave let some pass
 #pragma unroll
         for (int s = 0; s < kSteps / 2; ++s) x = mfma32<kBf16>(k0.k[s], qf[s], x);
 #pragma unroll
@@ -1073,7 +1102,7 @@ __device__ __forceinline__ void attend_rows(const Args& a, RowsLds<D>& lds, cons
       }
       keys = read_keys<D, 0>(lds, buf, 1, lane);
       const Seen see = {seen.x - key0 - 8 * half, seen.y - key0 - 8 * half,
-                        K == kOwn ? 0 : seq.front - key0 - 8 * half, hidden};
+                        kPlain<K> ? 0 : seq.front - key0 - 8 * half, hidden};
       x = attend_block<D, kBf16, K>(lds, buf, 0, buf, 1, x, qf, keys, whole, see, q_sum, lane, sums);
       unpack<D, kBf16, K>(a, lds, next, key1, seq, key_lo, key_hi, codes, staged);
       __syncthreads();
@@ -1102,7 +1131,8 @@ __device__ __forceinline__ void attend_rows(const Args& a, RowsLds<D>& lds, cons
   const uint32_t q_head = head * a.group + g;
   if (slot >= 0) {
     if (row < rows) {
-      const size_t place = (size_t)slot * kTileRows + (row - row0);
+      const size_t place = kPart<K> ? few_place<K>(a, seq, (uint32_t)slot, b, (uint32_t)row, head)
+                                    : (size_t)slot * kTileRows + (row - row0);
 #pragma unroll
       for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
@@ -1242,15 +1272,20 @@ __device__ __forceinline__ float add_weighed(float sum, float add, const float (
   return sum;
 }
 
+template <int D>
+struct MidLds {
+  __attribute__((aligned(16))) float o[kWaves][kMidRows][D + 4];
+  float2 ml[kWaves][kMidRows];
+};
+
 template <int D, bool kBf16, bool kOnce, Keys K>
-__global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
+__device__ __forceinline__ void attend_mid(const Args& a, MidLds<D>& lds, uint32_t part, uint32_t y, uint32_t b) {
   constexpr int kSteps = D / 16, kBlocks = D / 32;
-  __shared__ __attribute__((aligned(16))) float lds_o[kWaves][kMidRows][D + 4];
-  __shared__ float2 lds_ml[kWaves][kMidRows];
+  auto &lds_o = lds.o;
+  auto &lds_ml = lds.ml;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, half = lane >> 5;
-  const uint32_t b = blockIdx.z, part = blockIdx.x, at_y = blockIdx.y / a.kv_heads;
-  const uint32_t head = blockIdx.y - at_y * a.kv_heads;
+  const uint32_t at_y = y / a.kv_heads, head = y - at_y * a.kv_heads;
   // A sequence's tiles begin at a place of its own: with the first tiles, all that short sequences have, a fixed
   // number of workgroups apart, one shader engine in four would get them (129 sequences, one of them of 30
   // tokens in four tiles, 102 us for 42).
@@ -1263,7 +1298,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
   if (tile > 0 && row0 >= rows) return;  // before the loads: most workgroups of a ragged call end here
   int step = (int)part * kWaves + wave;
   Walk<K, kMidKeys> way{};
-  if constexpr (K == kOwn) {
+  if constexpr (kPlain<K>) {
     if (a.window) step += span<K>(a, seq, row0 / group).x / kMidKeys;
   } else {
     way = walk<K, kMidKeys>(seq, span<K>(a, seq, row0 / group).x,
@@ -1278,11 +1313,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
   const int2 last_span = span<K>(a, seq, (min(row0 + kMidRows, rows) - 1) / group);
   const int key_lo = first_span.x, key_hi = last_span.y;  // seen by some row
   const int all_lo = last_span.x, all_hi = first_span.y;  // seen by every row
-  const int last = K == kOwn ? (key_hi + kMidKeys - 1) / kMidKeys : way.last;
+  const int last = kPlain<K> ? (key_hi + kMidKeys - 1) / kMidKeys : way.last;
   const uint32_t heads = a.kv_heads * a.group;
   const int row = row0 + n, token = row / group, g = row - token * group;
   if (part > 0 && step - wave >= last) {  // no keys: part 0 stands for an empty row
-    if (threadIdx.x < kMidRows && row < rows) a.part_ml[few_place(a, part, b, row, head)] = {-kInf, 0};
+    if (threadIdx.x < kMidRows && row < rows) a.part_ml[few_place<K>(a, seq, part, b, row, head)] = {-kInf, 0};
     return;
   }
 
@@ -1324,8 +1359,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
     const int key0 = way.key(step);
     if (step + stride < last) {
       const int now = ids;
-      ids = page_of<K>(a, table, seq, (K == kOwn ? key0 + 2 * kMidKeys * stride : way.key(step + 2 * stride)) + mine);
-      load_mid<D, kOnce>(a, now, head, K == kOwn ? key0 + kMidKeys * stride : way.key(step + stride), lane, next);
+      ids = page_of<K>(a, table, seq, (kPlain<K> ? key0 + 2 * kMidKeys * stride : way.key(step + 2 * stride)) + mine);
+      load_mid<D, kOnce>(a, now, head, kPlain<K> ? key0 + kMidKeys * stride : way.key(step + stride), lane, next);
     }
     v16f x = v16f{};
 #pragma unroll
@@ -1355,11 +1390,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
       if (!whole) {
         asm volatile("");  // a branch, not 16 selects in every step
         const int lo = seen.x - key0 - 8 * half, hi = seen.y - key0 - 8 * half;
-        const int front = K == kOwn ? 0 : seq.front - key0 - 8 * half;
+        const int front = kPlain<K> ? 0 : seq.front - key0 - 8 * half;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int k = (i & 7) + 2 * (i & 8);
-          if ((k < lo && (K == kOwn || k >= front)) || k >= hi || (cur.hidden >> (2 * (i & 8))) & 1)
+          if ((k < lo && (kPlain<K> || k >= front)) || k >= hi || (cur.hidden >> (2 * (i & 8))) & 1)
             y[i] = -kInf;
         }
       }
@@ -1472,8 +1507,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
   const int out_token = out_row / group, out_g = out_row - out_token * group;
   const size_t q_row = (size_t)(seq.start + out_token);
   const uint32_t q_head = head * group + out_g;
-  if (a.parts > 1) {
-    const size_t place = few_place(a, part, b, out_row, head);
+  if (kPart<K> || a.parts > 1) {
+    const size_t place = few_place<K>(a, seq, part, b, out_row, head);
 #pragma unroll
     for (int j = 0; j < kBlocks; ++j)
       *reinterpret_cast<float4*>(a.part_o + place * D + ch + 32 * j) = sums[j];
@@ -1489,6 +1524,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
           narrow2<kBf16>(mean<kBf16>(sums[j].z, by), mean<kBf16>(sums[j].w, by))};
     if (a.lse && ch == 0) a.lse[q_row * heads + q_head] = none ? -kInf : (top + __log2f(total)) * kLn2;
   }
+}
+
+template <int D, bool kBf16, bool kOnce, Keys K>
+__global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_mid(Args a) {
+  __shared__ MidLds<D> lds;
+  attend_mid<D, kBf16, kOnce, K>(a, lds, blockIdx.x, blockIdx.y, blockIdx.z);
 }
 
 // One wave's joined row: D/64 channels a lane.
@@ -1525,7 +1566,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
   const uint32_t tile = blockIdx.x / a.kv_heads, head = blockIdx.x - tile * a.kv_heads;
   const int row0 = (int)(a.row_tiles - 1 - tile) * kTileRows;
   if (row0 >= rows || !takes(a, rows)) return;
-  attend_rows<D, kBf16, K>(a, lds, seq, blockIdx.z, head, row0, row_steps<K>(a, seq, row0), -1);
+  attend_rows<D, kBf16, K>(a, lds, seq, blockIdx.z, head, row0, row_steps<K>(a, seq, row0), kPart<K> ? 0 : -1);
 }
 
 // The same row tiles where they would leave the chip partly idle: the tiles of keys of all of them (of
@@ -1700,7 +1741,7 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_join(Args a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int parts = (int)a.parts;
   const uint32_t row = blockIdx.x * (kWaves / W) + wave / W;
-  const size_t place = few_place(a, 0, blockIdx.z, min(row, a.rows_to - 1), blockIdx.y);
+  const size_t place = few_place<kOwn>(a, {}, 0, blockIdx.z, min(row, a.rows_to - 1), blockIdx.y);
   const size_t pitch = (size_t)a.batch * a.rows_to * a.kv_heads;
   const float* from = a.part_o + place * D + lane * kPer;
   auto load = [&](int p, float (&x)[4][kPer]) {

@@ -1,16 +1,208 @@
-// Attention over the 4-bit cache behind a prefix that all sequences share: the kernels of attention_kv4.hpp over
-// the prefix's keys and then the sequence's own.
+// Attention over the 4-bit cache behind a prefix that all sequences share, out of the kernels of attention_kv4.hpp.
+//
+// The softmax over a row's keys, the prefix's F and its own O, is that of two partial ones: with m the largest
+// score, l = sum e^(s - m) and o = sum e^(s - m) v over each,
+//   out = (e^(m_F - m) o_F + e^(m_O - m) o_O) / (e^(m_F - m) l_F + e^(m_O - m) l_O),  m = max(m_F, m_O).
+// Where sequences have few rows, all rows of the call are one matrix against the prefix (F), in tiles of 32 rows
+// or of 256, so that each of its keys is unpacked once for as many rows; their own keys (O) are
+// attention_kv4's. Both leave m, l and o in the workspace and a join ends the rows. Calls that gain nothing by that (few
+// rows in all, or sequences that fill tiles by themselves) take every row over F and then O in one pass.
 #include "attention_kv4.hpp"
 
 namespace h3 {
+namespace {
+
+// All rows over the prefix in tiles of 256: the tiles' steps of every cache head are one line, as
+// k_attention_kv4_line's, of which each workgroup takes an equal range. The tiles are alike, so that a tile's pieces
+// follow from its number: piece i of it is part part0 + i.
+struct FrontLine {
+  int steps, range;  // of a tile; of a workgroup
+};
+__device__ __forceinline__ FrontLine front_line(const Args& a, int length, int tiles) {
+  const int steps = max((length + kTileKeys - 1) / kTileKeys, 1);
+  return {steps, max((steps * tiles + (int)a.front_groups - 1) / (int)a.front_groups, kLeastSteps)};
+}
+
+template <int D, bool kBf16>
+__global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_front(Args a) {
+  __shared__ __attribute__((aligned(16))) RowsLds<D> lds;
+  const Sequence seq = sequence<kFrontPart>(a, 0);
+  const int each = (int)a.row_tiles, tiles = each * (int)a.kv_heads;
+  const FrontLine line = front_line(a, seq.length, tiles);
+  const int begin = (int)blockIdx.x * line.range, stop = min(begin + line.range, line.steps * tiles);
+  for (int at = begin; at < stop;) {
+    const int tile = at / line.steps, start = tile * line.steps, first = at - start;
+    const int last = min(line.steps, first + stop - at);
+    const int head = tile / each, piece = (int)blockIdx.x - start / line.range;
+    attend_rows<D, kBf16, kFrontPart>(a, lds, seq, 0, head, (tile - head * each) * kTileRows, {first, last}, piece);
+    __syncthreads();  // LDS is free again
+    at += last - first;
+  }
+}
+
+// The first workgroups take all rows over the prefix in tiles of 32, the others the sequences' own keys, in
+// tiles of R rows or (0) of 32.
+template <int D, bool kBf16, int R>
+__global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_shared(Args own, Args front) {
+  union Lds {
+    MidLds<D> mid;
+    FewLds<D, R ? R : 4> few;
+  };
+  __shared__ Lds lds;
+  uint32_t x = blockIdx.x;
+  if (x < front.front_groups) {
+    const uint32_t y = x / front.parts;
+    attend_mid<D, kBf16, false, kFrontPart>(front, lds.mid, x - y * front.parts, y, 0);
+    return;
+  }
+  x -= front.front_groups;
+  const uint32_t y = x / own.parts, part = x - y * own.parts, tiles = own.kv_heads * own.row_tiles, b = y / tiles;
+  if constexpr (R == 0)
+    attend_mid<D, kBf16, false, kOwnPart>(own, lds.mid, part, y - b * tiles, b);
+  else
+    attend_few<D, kBf16, R, false, kOwnPart>(own, lds.few, part, y - b * tiles, b);
+}
+
+// Joins a row's parts, its own first: W waves per (row, query head), wave w the parts w, w + W, ..; lane p of a wave
+// holds part p's weight. rows_to: sequences of more rows have one part.
+template <int D, bool kBf16, int W>
+__global__ __launch_bounds__(kThreads) void k_attention_kv4_shared_join(Args a) {
+  constexpr int kPer = D / 64;
+  __shared__ float lds_sum[W == 1 ? 1 : W][D];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t row = blockIdx.x * (kWaves / W) + wave / W;
+  const Sequence seq = sequence<kOwn>(a, blockIdx.z);
+  const uint32_t token = row / a.group, g = row - token * a.group;
+  if ((int)token >= seq.rows) return;
+  const uint32_t at = (uint32_t)seq.start * a.group + row;
+  const int own = seq.rows * (int)a.group <= (int)a.rows_to ? (int)a.parts : 1;
+  int front = (int)a.front_parts;
+  if (front == 0) {
+    const int each = (int)a.row_tiles, tile = (int)blockIdx.y * each + (int)at / kTileRows;
+    const int length = min(max(*a.prefix_length, 0), (int)(a.prefix_stride << a.page_shift));
+    const FrontLine line = front_line(a, length, each * (int)a.kv_heads);
+    front = (tile * line.steps + line.steps - 1) / line.range - tile * line.steps / line.range + 1;
+  }
+  const int parts = own + front;
+  const auto part_of = [&](int p) { return p < own ? p : (int)a.part0 + p - own; };
+  const size_t place = (size_t)at * a.kv_heads + blockIdx.y, pitch = (size_t)a.part_rows * a.kv_heads;
+  const float2 ml = lane < parts ? a.part_ml[part_of(lane) * pitch + place] : float2{-kInf, 0.0f};
+  const float* from = a.part_o + place * D + lane * kPer;
+  const float top = across32<true>(across16<true>(over16<true>(ml.x)));
+  const float f = __builtin_amdgcn_exp2f(ml.x - (top == -kInf ? 0.0f : top));
+  const float total = across32<false>(across16<false>(over16<false>(f * ml.y)));
+  const uint64_t live = __ballot(!(ml.y == 0.0f));  // the parts with sums: those with a weight or a NaN
+  float sum[kPer];
+#pragma unroll
+  for (int d = 0; d < kPer; ++d) sum[d] = 0.0f;
+  for (int p0 = wave % W; p0 < parts; p0 += 4 * W) {
+    float x[4][kPer];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + i * W;
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) x[i][d] = p < parts ? from[part_of(p) * pitch * D + d] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = p0 + i * W;
+      if (p >= parts || !((live >> p) & 1)) continue;
+      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), p));
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) sum[d] = fmaf(w, x[i][d], sum[d]);
+    }
+  }
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) lds_sum[wave][lane * kPer + d] = sum[d];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int d = 0; d < kPer; ++d) {
+      sum[d] = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) sum[d] += lds_sum[w][lane * kPer + d];
+    }
+  }
+  write_row<D, kBf16>(a, (size_t)seq.start + token, blockIdx.y * a.group + g, lane, top, total, sum);
+}
+
+template <int D, bool kBf16>
+hipError_t launch_shared(const Args& all, const Kv4PrefixPlan& plan, hipStream_t stream) {
+  const uint32_t rows = all.q_rows * all.group;
+  Args own = all;  // part_ml is the same for every launch: behind all parts' sums
+  own.part_rows = rows;
+  own.part_ml = reinterpret_cast<float2*>(all.part_o + (size_t)plan.parts * rows * all.kv_heads * D);
+  own.parts = std::max(plan.own.few.parts, 1u);
+  Args front = own;
+  front.batch = 1;
+  front.max_q = front.q_rows;
+  front.table = all.prefix_table;
+  front.table_stride = all.prefix_stride;
+  front.part0 = own.parts;
+  front.parts = plan.front_parts;
+  front.front_groups = plan.front_groups;
+  front.rows_from = 0;
+  front.rows_to = rows;
+  Args few = own;
+  few.row_tiles = plan.own.few.row_tiles;
+  few.rows_from = plan.own.few.rows_from;
+  few.rows_to = plan.own.few.rows_to;
+  const dim3 block(kThreads);
+  if (plan.front_parts) {
+    front.row_tiles = (rows + kMidRows - 1) / kMidRows;
+    const dim3 grid(front.front_groups + own.parts * all.kv_heads * few.row_tiles * all.batch);
+    switch (plan.own.few.tile_rows) {
+      case 4: hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, 4>), grid, block, 0, stream, few, front); break;
+      case 8: hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, 8>), grid, block, 0, stream, few, front); break;
+      case 16: hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, 16>), grid, block, 0, stream, few, front); break;
+      default: hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, 0>), grid, block, 0, stream, few, front);
+    }
+  } else {
+    front.row_tiles = (rows + kTileRows - 1) / kTileRows;
+    hipLaunchKernelGGL((k_attention_kv4_front<D, kBf16>), dim3(front.front_groups), dim3(kRowsThreads), 0, stream,
+                       front);
+    if (plan.own.many.row_tiles) {
+      Args many = own;
+      many.row_tiles = plan.own.many.row_tiles;
+      many.rows_from = plan.own.many.rows_from;
+      many.rows_to = plan.own.many.rows_to;
+      hipLaunchKernelGGL((k_attention_kv4_rows<D, kBf16, kOwnPart>), dim3(all.kv_heads * many.row_tiles, 1, all.batch),
+                         dim3(kRowsThreads), 0, stream, many);
+    }
+    if (few.row_tiles) launch_tiles<D, kBf16, false, kOwnPart>(few, plan.own.few, stream);
+  }
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  Args join = own;
+  join.rows_to = plan.own.few.row_tiles ? plan.own.few.rows_to : 0;
+  join.part0 = own.parts;
+  join.front_parts = plan.front_parts;
+  join.front_groups = plan.front_groups;
+  join.row_tiles = front.row_tiles;
+  const uint32_t most = all.max_q * all.group;
+  if (plan.parts > 8)
+    hipLaunchKernelGGL((k_attention_kv4_shared_join<D, kBf16, kWaves>), dim3(most, all.kv_heads, all.batch), block, 0,
+                       stream, join);
+  else
+    hipLaunchKernelGGL((k_attention_kv4_shared_join<D, kBf16, 1>),
+                       dim3((most + kWaves - 1) / kWaves, all.kv_heads, all.batch), block, 0, stream, join);
+  return hipGetLastError();
+}
+
+}  // namespace
 
 hipError_t launch_attention_kv4_prefix(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
-                                       uint32_t prefix_stride, const Kv4Plan& plan, uint32_t batch,
+                                       uint32_t prefix_stride, const Kv4PrefixPlan& plan, uint32_t batch,
                                        uint32_t q_rows, uint32_t max_q, const Kv4Bindings& x,
                                        hipStream_t stream) {
   Args a = make_args(cfg, acfg, batch, q_rows, max_q, x);
   a.prefix_stride = prefix_stride;
-  return launch_keys<kPrefix>(cfg, a, plan, stream);
+  if (!plan.shared) return launch_keys<kPrefix>(cfg, a, plan.one, stream);
+  const bool bf16 = cfg.elem == H3_ELEM_BF16;
+  if (cfg.head_dim == 128)
+    return bf16 ? launch_shared<128, true>(a, plan, stream) : launch_shared<128, false>(a, plan, stream);
+  return bf16 ? launch_shared<64, true>(a, plan, stream) : launch_shared<64, false>(a, plan, stream);
 }
 
 }  // namespace h3

@@ -244,7 +244,8 @@ Kv4Plan kv4_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32
                  uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide);
 // front_keys: what rows see before their window (sinks) or their sequence (a prefix).
 Kv4Plan kv4_front_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint64_t front_keys,
-                       uint32_t batch, uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide);
+                       uint32_t batch, uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide,
+                       double* time = nullptr);
 size_t kv4_workspace_bytes(const h3_kv4_cfg& cfg, uint32_t batch, const Kv4Plan& plan);
 struct Kv4Bindings {
   const void *q, *cache;
@@ -262,8 +263,20 @@ hipError_t launch_attention_kv4_sinks(const h3_kv4_cfg& cfg, const h3_kv4_attent
                                       uint32_t sinks, const Kv4Plan& plan, uint32_t batch, uint32_t q_rows,
                                       uint32_t max_q, const Kv4Bindings& x, hipStream_t stream);
 // Behind a prefix that all sequences share (attention_kv4_prefix.hip).
+// How such a call is cut: in one pass of every row over the prefix and its own keys (`one`), or (shared) all rows over
+// the prefix as one matrix, in `front_parts` parts in tiles of 32 rows or, in tiles of 256, along one line over
+// `front_groups` workgroups, and over their own keys as `own` says, each leaving `parts` sums in all to be joined.
+struct Kv4PrefixPlan {
+  bool shared;
+  Kv4Plan one, own;
+  uint32_t front_parts, front_groups, parts;
+};
+Kv4PrefixPlan kv4_prefix_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t prefix_stride,
+                              uint32_t batch, uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide);
+size_t kv4_prefix_workspace_bytes(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t batch,
+                                  uint32_t q_rows, const Kv4PrefixPlan& plan);
 hipError_t launch_attention_kv4_prefix(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg,
-                                       uint32_t prefix_stride, const Kv4Plan& plan, uint32_t batch,
+                                       uint32_t prefix_stride, const Kv4PrefixPlan& plan, uint32_t batch,
                                        uint32_t q_rows, uint32_t max_q, const Kv4Bindings& x,
                                        hipStream_t stream);
 // What the next step of every sequence needs (kv4_advance.hip).

@@ -8,6 +8,7 @@ import h3attn as H
 import kv4_plain as P
 import kv4_step_plain as S
 from test_gpu_kv4 import STALE, Call
+from test_kv4_step_host import prefix_plan
 
 pytestmark = pytest.mark.gpu
 
@@ -298,3 +299,38 @@ def test_calls_repeat_bit_for_bit_and_on_another_stream(dev, kind):
         first = call.run()
         again = call.run(stream=torch.cuda.Stream())
         assert all(np.array_equal(x, y) for x, y in zip(first, again))
+
+
+# Calls that are cut in each way: all rows over the prefix in tiles of 32 beside the sequences' own tiles of 4 to 32
+# rows, or along a line of tiles of 256.
+@pytest.mark.parametrize("cut,elem,dim,heads,kv_heads,page,new,most,prefix", [
+    (4, F16, 128, 8, 2, 16, [1] * 64, 200, 5003),
+    (4, BF16, 64, 12, 4, 64, [1] * 60 + [0], 90, 9001),
+    (8, BF16, 128, 14, 2, 32, [1] * 90, 150, 6000),
+    (8, F16, 64, 8, 2, 16, [2, 1] * 20, 130, 7777),
+    (16, F16, 128, 32, 2, 16, [1] * 60, 100, 7000),
+    (16, BF16, 64, 8, 2, 128, [4, 3, 0, 1] * 9, 333, 5000),
+    (32, BF16, 128, 20, 4, 64, [5] * 30, 150, 8000),
+    (32, F16, 64, 4, 1, 16, [17, 30, 1, 20] * 5, 99, 12000),
+    ("line", F16, 64, 4, 1, 16, [1] * 1100, 20, 3001),
+    ("line", BF16, 128, 64, 2, 64, [65] * 6, 300, 5000),                  # own keys in tiles of 32
+    ("line", F16, 128, 64, 2, 16, [66, 1, 1, 90] * 4, 250, 9000),         # of 32 and of 256
+    ("line", BF16, 64, 64, 2, 32, [1] * 60 + [140], 120, 9000)])
+def test_calls_behind_a_prefix_cut_in_every_way(dev, cut, elem, dim, heads, kv_heads, page, new, most, prefix):
+    rng = np.random.default_rng(len(new) + prefix)
+    lengths = [n + int(m) for n, m in zip(new, rng.integers(0, most, len(new)))]
+    lengths[0] = max(0, new[0] - 1)  # its first row sees no key of its own
+    call = Front(dev, elem, dim, heads, kv_heads, page, new, lengths, prefix=prefix)
+    plan = prefix_plan(call.cfg, call.acfg, len(call.prefix_table), len(new), call.rows, max(new))
+    assert plan.shared
+    if cut == "line":
+        assert plan.front_parts == 0
+    else:
+        assert plan.front_parts > 0 and plan.own.few.tile == cut
+    call.check()
+    # replays of what the workspace held before do no harm, nor do a length and starts that changed
+    call.lengths[1] = max(0, call.lengths[1] - 1)
+    call.check()
+    for length in (0, 1, prefix // 2):
+        call.prefix = call.prefix_length = length
+        call.check()

@@ -1,6 +1,7 @@
 """What the operators of a serving step refuse, before any device work. No kernel is launched here."""
 import ctypes
 
+import numpy as np
 import pytest
 
 import h3attn as H
@@ -162,3 +163,75 @@ def test_rows_and_their_cache_are_of_one_kind():
 def test_rust_mirror_has_the_header_fields():
     fields = header_struct_fields("h3_qk_cfg")
     assert fields == rust_struct_fields("H3QkCfg") == [f for f, _ in H.QkCfg._fields_]
+
+
+# ---------------------------------------------------------------- how a call behind a prefix is cut
+
+class Launch(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_uint32) for n in ("tile", "tiles", "parts", "rows_from", "rows_to")]
+
+
+class Plan(ctypes.Structure):
+    _fields_ = [("many", Launch), ("few", Launch)]
+
+
+class PrefixPlan(ctypes.Structure):
+    _fields_ = [("shared", ctypes.c_bool), ("one", Plan), ("own", Plan), ("front_parts", ctypes.c_uint32),
+                ("front_groups", ctypes.c_uint32), ("parts", ctypes.c_uint32)]
+
+
+def prefix_plan(cfg, acfg, stride, batch, q_rows, max_q, divide=True):
+    call = H.lib()._ZN2h315kv4_prefix_planERK10h3_kv4_cfgRK20h3_kv4_attention_cfgjjjjjb
+    call.restype = PrefixPlan
+    call.argtypes = [ctypes.c_void_p] * 2 + [ctypes.c_uint32] * 5 + [ctypes.c_bool]
+    return call(ctypes.byref(cfg), ctypes.byref(acfg), stride, batch, q_rows, max_q, 256, divide)
+
+
+def test_every_row_behind_a_prefix_has_its_launches():
+    """Every count of rows that a sequence can have belongs to one launch of its own keys; the parts fit the join's
+    wave and the workspace, the pieces of a line the parts; grids stay inside their limits."""
+    rng = np.random.default_rng(6)
+    kinds = set()
+    for _ in range(3000):
+        dim, page = int(rng.choice([64, 128])), 16 << int(rng.integers(0, 7))
+        kv_heads = int(2 ** rng.uniform(0, 8))
+        group = min(int(2 ** rng.uniform(0, 7)), 4096 // kv_heads)
+        batch, max_q = int(2 ** rng.uniform(0, 12)), int(2 ** rng.uniform(0, 12))
+        q_rows = min(2 ** 24, int(rng.integers(max_q, batch * max_q + 1)))
+        columns = max(1, int(2 ** rng.uniform(0, 16)) // page)
+        stride = max(1, int(2 ** rng.uniform(0, 20)) // page)
+        cfg = H.Kv4Cfg(kv_heads, dim, page, 1000, 0)
+        width = kv_heads * group * dim
+        acfg = H.Kv4AttentionCfg(kv_heads * group, width, width, columns, 1, 0, 0.1)
+        assert not prefix_plan(cfg, acfg, stride, batch, q_rows, max_q, False).shared
+        p = prefix_plan(cfg, acfg, stride, batch, q_rows, max_q)
+        need = H.kv4_prefix_workspace_bytes(cfg, acfg, stride, batch, q_rows, max_q)
+        rows = q_rows * group
+        if not p.shared:
+            kinds.add("one")
+            assert need <= 2 ** 28
+            continue
+        own = max(1, p.own.few.parts)
+        assert own == 1 and p.parts <= 64 and need == p.parts * rows * kv_heads * (dim + 2) * 4 <= 200e6
+        for n in (1, group, max_q * group, max(1, max_q // 2) * group):
+            taken = [x for x in (p.own.many, p.own.few) if x.tiles and x.rows_from <= n <= x.rows_to]
+            assert len(taken) == 1 and n <= taken[0].tile * taken[0].tiles
+        if p.front_parts:
+            kinds.add(("tiles of 32", p.own.few.tile))
+            tiles = -(-rows // 32) * kv_heads
+            assert p.own.many.tiles == 0 and p.parts == own + p.front_parts
+            assert p.front_groups == tiles * p.front_parts
+            assert p.front_groups + kv_heads * p.own.few.tiles * batch < 2 ** 31
+            assert p.own.few.tile in (4, 8, 16, 32)
+        else:
+            kinds.add(("line", bool(p.own.many.tiles), bool(p.own.few.tiles)))
+            tiles = -(-rows // 256) * kv_heads
+            for length in {1, 64, stride * page // 2 + 1, stride * page}:
+                steps = max(1, -(-length // 64))
+                each = max(8, -(-steps * tiles // p.front_groups))
+                assert steps * tiles < 2 ** 30 and each * p.front_groups >= steps * tiles
+                first = np.arange(tiles, dtype=np.int64) * steps
+                pieces = (first + steps - 1) // each - first // each + 1
+                assert pieces.max() <= p.parts - own
+    assert kinds >= {"one", ("tiles of 32", 4), ("tiles of 32", 8), ("tiles of 32", 16), ("tiles of 32", 32),
+                     ("line", False, True), ("line", True, False), ("line", True, True)}, kinds
