@@ -954,6 +954,9 @@ __device__ __forceinline__ v16f attend_block(const RowsLds<D>& lds, int buf, int
         if (lds.dead[buf][32 * blk + 8 * half + (i & 7) + 2 * (i & 8)]) y[i] = -kInf;
     }
   }
+  // The softmax goes before the SIMD's other wave's products, which wait for nothing: 8,224 rows behind a prefix of
+  // 31,104 keys 1,194 us with this priority and 1,236 without.
+  __builtin_amdgcn_s_setprio(1);
   const ValueOps<D> v0 = read_values<D>(lds, buf, blk, 0, lane);
   float p[16], ts = 0.0f;
 #pragma unroll
@@ -998,6 +1001,7 @@ __device__ __forceinline__ v16f attend_block(const RowsLds<D>& lds, int buf, int
   for (int s = 0; s < 2; ++s)
     pf[s] = {narrow2<kBf16>(p[8 * s], p[8 * s + 1]), narrow2<kBf16>(p[8 * s + 2], p[8 * s + 3]),
              narrow2<kBf16>(p[8 * s + 4], p[8 * s + 5]), narrow2<kBf16>(p[8 * s + 6], p[8 * s + 7])};
+  __builtin_amdgcn_s_setprio(0);
 #pragma unroll
   for (int d = 0; d < D / 32; ++d) r.o[d] = mfma32<kBf16>(v0.v[d], pf[0], r.o[d]);
 #pragma unroll
