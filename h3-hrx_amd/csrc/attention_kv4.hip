@@ -202,10 +202,11 @@ Kv4PrefixPlan kv4_prefix_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg&
   const Work own = few_work(p.own.few.tile_rows, few_steps(p.own.few.tile_rows, (double)own_keys), cus);
   const double own_each = small ? groups_of(p.own.few) * own.each : 0;
   if (small) own_time = std::max(own.alone, 2 + own_each);
-  const auto take = [&](double time, uint32_t front_parts, uint32_t front_groups, uint32_t parts) {
+  const auto take = [&](double time, uint32_t front_parts, uint32_t front_groups, uint32_t parts, bool apart) {
     if (parts > kJoinParts || parts * row_bytes > kSharedBytes || time >= least) return;
     least = time;
     p.shared = true;
+    p.heads_apart = apart;
     p.front_parts = front_parts;
     p.front_groups = front_groups;
     p.parts = parts;
@@ -214,14 +215,21 @@ Kv4PrefixPlan kv4_prefix_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg&
   if (rows <= kFewMost && small) {
     const uint32_t tiles = (uint32_t)(rows + kMidRows - 1) / kMidRows * cfg.kv_heads;
     const double steps = std::max(1.0, few_steps(kMidRows, (double)prefix));
+    // Own keys of a head by one wave: a workgroup for four heads, each step of which takes four times as long.
+    const double each_keys = few_steps(p.own.few.tile_rows, (double)own_keys) * kWaves;
+    const Work wide = few_work(p.own.few.tile_rows, each_keys, cus);
+    const double wide_each = (double)batch * ((cfg.kv_heads + kWaves - 1) / kWaves) * wide.each;
     for (uint32_t n = 1; n <= steps && n < kJoinParts; ++n) {
       const Work w = few_work(kMidRows, steps / n, cus);
       // One of them to a compute unit runs beside the sequences' own, two beside each other.
       const double longest = 7 + steps / n * (tiles * n <= cus ? 1.37 : 2.05);
       // More of them than find room: the last ones leave the chip partly idle.
-      const double tail = tiles * n > 2 * cus ? 0.25 * w.each * 2 * cus : 0;
-      take(std::max({longest, own.alone, 6 + (double)tiles * n * w.each + own_each + tail}) + join(1 + n), n,
-           n * tiles, 1 + n);
+      const double tail = tiles * n > 2 * cus ? 0.4 * w.each * 2 * cus : 0;
+      const double front = 6 + (double)tiles * n * w.each + tail;
+      take(std::max({longest, own.alone, front + own_each}) + join(1 + n), n, n * tiles, 1 + n, false);
+      if (p.own.few.tile_rows < kMidRows)
+        take(std::max({longest, 5 + wide.each * 2 * cus, front + wide_each}) + 2 + join(1 + n), n, n * tiles, 1 + n,
+             true);
     }
   }
   // Tiles of 256 rows along one line.
@@ -232,7 +240,7 @@ Kv4PrefixPlan kv4_prefix_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg&
     const uint32_t pieces = (uint32_t)((groups + tiles - 1) / tiles) + 1;
     const double step = 0.9 + 0.175 * std::min<double>(8, (rows + 31) / 32);
     take(own_time + 12 + 8 * (tiles / (double)groups + 1) + all / groups * step + join(1 + pieces), 0, groups,
-         1 + pieces);
+         1 + pieces, false);
   }
   return p;
 }

@@ -392,7 +392,8 @@ struct FewLds {
   float2 ml[kWaves][R];
 };
 
-template <int D, bool kBf16, int R, bool kOnce, Keys K>
+// kShare: the waves that share a head's keys, all four or (1) each wave a head of its own.
+template <int D, bool kBf16, int R, bool kOnce, Keys K, int kShare = kWaves>
 __device__ __forceinline__ void attend_few(const Args& a, FewLds<D, R>& lds, uint32_t part, uint32_t head,
                                            uint32_t b) {
   constexpr int T = 16 / R, kTiles = R / 4, kSteps = D / 32, kDimTiles = D / 16;
@@ -407,8 +408,9 @@ __device__ __forceinline__ void attend_few(const Args& a, FewLds<D, R>& lds, uin
   // is known before the sequence is, and its loads go ahead: where the sequence ends before it, they
   // read what the table holds, and nothing comes of them.
   const Sequence seq = sequence<K>(a, b);
-  const int group = (int)a.group, rows = seq.rows * group, stride = (int)a.parts * kWaves;
-  int step = (int)part * kWaves + wave;
+  const int group = (int)a.group, rows = seq.rows * group, stride = (int)a.parts * kShare;
+  const int mine = kShare == kWaves ? wave : 0, thread = kShare == kWaves ? (int)threadIdx.x : lane;
+  int step = (int)part * kShare + mine;
   Walk<K, kStepKeys> way{};
   if constexpr (kPlain<K>) {
     if (a.window) step += span<K>(a, seq, 0).x / kStepKeys;
@@ -425,8 +427,8 @@ __device__ __forceinline__ void attend_few(const Args& a, FewLds<D, R>& lds, uin
   const int all_lo = last_span.x, all_hi = first_span.y;  // seen by every row
   const int last = kPlain<K> ? (key_hi + kStepKeys - 1) / kStepKeys : way.last;
   const uint32_t heads = a.kv_heads * a.group;
-  if (part > 0 && step - wave >= last) {  // no keys: part 0 stands for an empty row
-    if ((int)threadIdx.x < rows) a.part_ml[few_place<K>(a, seq, part, b, threadIdx.x, head)] = {-kInf, 0};
+  if (part > 0 && step - mine >= last) {  // no keys: part 0 stands for an empty row
+    if (thread < rows) a.part_ml[few_place<K>(a, seq, part, b, thread, head)] = {-kInf, 0};
     return;
   }
 
@@ -659,15 +661,20 @@ __device__ __forceinline__ void attend_few(const Args& a, FewLds<D, R>& lds, uin
         *reinterpret_cast<float4*>(&lds_o[wave][n][kDimTiles * (4 * h + i) + d]) = f;
       }
   }
-  __syncthreads();
-  constexpr int kPer = R * D / kThreads;  // channels a thread; 256 / R threads a row
-  const int row = threadIdx.x / (kThreads / R), ch = (threadIdx.x % (kThreads / R)) * kPer;
+  if constexpr (kShare == kWaves) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+  }
+  constexpr int kJoiners = kShare * 64, kPer = R * D / kJoiners;  // channels a thread; kJoiners / R threads a row
+  const int row = thread / (kJoiners / R), ch = (thread % (kJoiners / R)) * kPer, wave0 = wave - mine;
   if (row < rows) {
-    float2 ml[kWaves];
+    float2 ml[kShare];
     float top = -kInf;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      ml[w] = lds_ml[w][row];
+    for (int w = 0; w < kShare; ++w) {
+      ml[w] = lds_ml[wave0 + w][row];
       top = fmaxf(top, ml[w].x);
     }
     const float base = top == -kInf ? 0.0f : top;
@@ -675,11 +682,11 @@ __device__ __forceinline__ void attend_few(const Args& a, FewLds<D, R>& lds, uin
 #pragma unroll
     for (int d = 0; d < kPer; ++d) sum[d] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
+    for (int w = 0; w < kShare; ++w) {
       const float f = __builtin_amdgcn_exp2f(ml[w].x - base);
       total = fmaf(f, ml[w].y, total);
 #pragma unroll
-      for (int d = 0; d < kPer; ++d) sum[d] = fmaf(f, lds_o[w][row][ch + d], sum[d]);
+      for (int d = 0; d < kPer; ++d) sum[d] = fmaf(f, lds_o[wave0 + w][row][ch + d], sum[d]);
     }
     total = or_nan(total, sum[0]);
     const int token = row / group, g = row - token * group;

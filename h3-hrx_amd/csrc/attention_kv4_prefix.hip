@@ -41,8 +41,8 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_front(Args a)
 }
 
 // The first workgroups take all rows over the prefix in tiles of 32, the others the sequences' own keys, in
-// tiles of R rows or (0) of 32.
-template <int D, bool kBf16, int R>
+// tiles of R rows or (0) of 32; kShare: see attend_few.
+template <int D, bool kBf16, int R, int kShare>
 __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_shared(Args own, Args front) {
   union Lds {
     MidLds<D> mid;
@@ -56,11 +56,31 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_shared(Args own, 
     return;
   }
   x -= front.front_groups;
+  if constexpr (kShare == 1) {  // one part
+    const uint32_t each = (own.kv_heads + kWaves - 1) / kWaves, b = x / each;
+    const uint32_t head = (x - b * each) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (head < own.kv_heads) attend_few<D, kBf16, R, false, kOwnPart, 1>(own, lds.few, 0, head, b);
+    return;
+  }
   const uint32_t y = x / own.parts, part = x - y * own.parts, tiles = own.kv_heads * own.row_tiles, b = y / tiles;
   if constexpr (R == 0)
     attend_mid<D, kBf16, false, kOwnPart>(own, lds.mid, part, y - b * tiles, b);
   else
     attend_few<D, kBf16, R, false, kOwnPart>(own, lds.few, part, y - b * tiles, b);
+}
+
+template <int D, bool kBf16, int R>
+void launch_tiles_shared(const Args& own, const Args& front, bool heads_apart, hipStream_t stream) {
+  if constexpr (R != 0) {
+    if (heads_apart) {
+      const uint32_t groups = front.front_groups + (own.kv_heads + kWaves - 1) / kWaves * own.batch;
+      hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, R, 1>), dim3(groups), dim3(kThreads), 0, stream, own, front);
+      return;
+    }
+  }
+  const uint32_t groups = front.front_groups + own.parts * own.kv_heads * own.row_tiles * own.batch;
+  hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, R, kWaves>), dim3(groups), dim3(kThreads), 0, stream, own,
+                     front);
 }
 
 // Joins a row's parts, its own first: W waves per (row, query head), wave w the parts w, w + W, ..; lane p of a wave
@@ -151,12 +171,11 @@ hipError_t launch_shared(const Args& all, const Kv4PrefixPlan& plan, hipStream_t
   const dim3 block(kThreads);
   if (plan.front_parts) {
     front.row_tiles = (rows + kMidRows - 1) / kMidRows;
-    const dim3 grid(front.front_groups + own.parts * all.kv_heads * few.row_tiles * all.batch);
     switch (plan.own.few.tile_rows) {
-      case 4: hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, 4>), grid, block, 0, stream, few, front); break;
-      case 8: hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, 8>), grid, block, 0, stream, few, front); break;
-      case 16: hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, 16>), grid, block, 0, stream, few, front); break;
-      default: hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, 0>), grid, block, 0, stream, few, front);
+      case 4: launch_tiles_shared<D, kBf16, 4>(few, front, plan.heads_apart, stream); break;
+      case 8: launch_tiles_shared<D, kBf16, 8>(few, front, plan.heads_apart, stream); break;
+      case 16: launch_tiles_shared<D, kBf16, 16>(few, front, plan.heads_apart, stream); break;
+      default: launch_tiles_shared<D, kBf16, 0>(few, front, false, stream);
     }
   } else {
     front.row_tiles = (rows + kTileRows - 1) / kTileRows;

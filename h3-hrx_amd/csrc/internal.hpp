@@ -266,8 +266,9 @@ hipError_t launch_attention_kv4_sinks(const h3_kv4_cfg& cfg, const h3_kv4_attent
 // How such a call is cut: in one pass of every row over the prefix and its own keys (`one`), or (shared) all rows over
 // the prefix as one matrix, in `front_parts` parts in tiles of 32 rows or, in tiles of 256, along one line over
 // `front_groups` workgroups, and over their own keys as `own` says, each leaving `parts` sums in all to be joined.
+// heads_apart: own tiles of up to 16 rows, each wave a cache head's.
 struct Kv4PrefixPlan {
-  bool shared;
+  bool shared, heads_apart;
   Kv4Plan one, own;
   uint32_t front_parts, front_groups, parts;
 };

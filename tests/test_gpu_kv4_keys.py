@@ -312,6 +312,10 @@ def test_calls_repeat_bit_for_bit_and_on_another_stream(dev, kind):
     (16, BF16, 64, 8, 2, 128, [4, 3, 0, 1] * 9, 333, 5000),
     (32, BF16, 128, 20, 4, 64, [5] * 30, 150, 8000),
     (32, F16, 64, 4, 1, 16, [17, 30, 1, 20] * 5, 99, 12000),
+    ("apart", F16, 128, 12, 3, 16, [1] * 500, 70, 2000),                  # a wave to a cache head
+    ("apart", BF16, 64, 30, 6, 64, [1] * 300 + [0], 90, 1500),
+    ("apart", F16, 64, 10, 5, 32, [3, 1, 0, 2] * 80, 130, 1200),
+    ("apart", BF16, 64, 45, 5, 32, [1] * 200, 60, 2000),
     ("line", F16, 64, 4, 1, 16, [1] * 1100, 20, 3001),
     ("line", BF16, 128, 64, 2, 64, [65] * 6, 300, 5000),                  # own keys in tiles of 32
     ("line", F16, 128, 64, 2, 16, [66, 1, 1, 90] * 4, 250, 9000),         # of 32 and of 256
@@ -326,7 +330,7 @@ def test_calls_behind_a_prefix_cut_in_every_way(dev, cut, elem, dim, heads, kv_h
     if cut == "line":
         assert plan.front_parts == 0
     else:
-        assert plan.front_parts > 0 and plan.own.few.tile == cut
+        assert plan.front_parts > 0 and (plan.heads_apart if cut == "apart" else plan.own.few.tile == cut)
     call.check()
     # replays of what the workspace held before do no harm, nor do a length and starts that changed
     call.lengths[1] = max(0, call.lengths[1] - 1)
