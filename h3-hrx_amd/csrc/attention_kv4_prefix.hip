@@ -56,17 +56,17 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_shared(Args own, 
     return;
   }
   x -= front.front_groups;
-  if constexpr (kShare == 1) {  // one part
+  if constexpr (kShare == 1) {
     const uint32_t each = (own.kv_heads + kWaves - 1) / kWaves, b = x / each;
     const uint32_t head = (x - b * each) * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (head < own.kv_heads) attend_few<D, kBf16, R, false, kOwnPart, 1>(own, lds.few, 0, head, b);
     return;
   }
-  const uint32_t y = x / own.parts, part = x - y * own.parts, tiles = own.kv_heads * own.row_tiles, b = y / tiles;
+  const uint32_t tiles = own.kv_heads * own.row_tiles, b = x / tiles;
   if constexpr (R == 0)
-    attend_mid<D, kBf16, false, kOwnPart>(own, lds.mid, part, y - b * tiles, b);
+    attend_mid<D, kBf16, false, kOwnPart>(own, lds.mid, 0, x - b * tiles, b);
   else
-    attend_few<D, kBf16, R, false, kOwnPart>(own, lds.few, part, y - b * tiles, b);
+    attend_few<D, kBf16, R, false, kOwnPart>(own, lds.few, 0, x - b * tiles, b);
 }
 
 template <int D, bool kBf16, int R>
@@ -78,24 +78,41 @@ void launch_tiles_shared(const Args& own, const Args& front, bool heads_apart, h
       return;
     }
   }
-  const uint32_t groups = front.front_groups + own.parts * own.kv_heads * own.row_tiles * own.batch;
+  const uint32_t groups = front.front_groups + own.kv_heads * own.row_tiles * own.batch;
   hipLaunchKernelGGL((k_attention_kv4_shared<D, kBf16, R, kWaves>), dim3(groups), dim3(kThreads), 0, stream, own,
                      front);
 }
 
-// Joins a row's parts, its own first: W waves per (row, query head), wave w the parts w, w + W, ..; lane p of a wave
-// holds part p's weight. rows_to: sequences of more rows have one part.
+// Whether a token's row is one that its sequence takes. 64 ends at a time, a lane each: the first past the token is the
+// sequence's.
+__device__ __forceinline__ bool taken(const Args& a, int token, int lane) {
+  int b = 0;
+  for (int span = (int)a.batch; span > 0;) {  // the sequence is one of b .. b + span - 1, or there is none
+    const int each = (span + 63) / 64, last = min(b + (lane + 1) * each, b + span) - 1;
+    const uint64_t past = __ballot(a.q_starts[last + 1] > token);
+    if (past == 0) return false;
+    const int chunk = __builtin_ctzll(past) * each;
+    if (each == 1) {
+      b += chunk;
+      break;
+    }
+    span = min(each, span - chunk);
+    b += chunk;
+  }
+  const int start = max(a.q_starts[b], 0);
+  return token >= start && token - start < (int)a.max_q;
+}
+
+// Joins a row's parts, its own and then the prefix's: W waves per (row, query head), wave w the parts w, w + W, ..; lane p
+// of a wave holds part p's weight.
 template <int D, bool kBf16, int W>
 __global__ __launch_bounds__(kThreads) void k_attention_kv4_shared_join(Args a) {
   constexpr int kPer = D / 64;
   __shared__ float lds_sum[W == 1 ? 1 : W][D];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t row = blockIdx.x * (kWaves / W) + wave / W;
-  const Sequence seq = sequence<kOwn>(a, blockIdx.z);
-  const uint32_t token = row / a.group, g = row - token * a.group;
-  if ((int)token >= seq.rows) return;
-  const uint32_t at = (uint32_t)seq.start * a.group + row;
-  const int own = seq.rows * (int)a.group <= (int)a.rows_to ? (int)a.parts : 1;
+  const uint32_t at = blockIdx.x * (kWaves / W) + wave / W;
+  if (at >= a.part_rows) return;
+  const uint32_t token = at / a.group, g = at - token * a.group;
   int front = (int)a.front_parts;
   if (front == 0) {
     const int each = (int)a.row_tiles, tile = (int)blockIdx.y * each + (int)at / kTileRows;
@@ -103,11 +120,19 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_shared_join(Args a) 
     const FrontLine line = front_line(a, length, each * (int)a.kv_heads);
     front = (tile * line.steps + line.steps - 1) / line.range - tile * line.steps / line.range + 1;
   }
-  const int parts = own + front;
-  const auto part_of = [&](int p) { return p < own ? p : (int)a.part0 + p - own; };
+  const int parts = 1 + front;
   const size_t place = (size_t)at * a.kv_heads + blockIdx.y, pitch = (size_t)a.part_rows * a.kv_heads;
-  const float2 ml = lane < parts ? a.part_ml[part_of(lane) * pitch + place] : float2{-kInf, 0.0f};
+  const float2 ml = lane < parts ? a.part_ml[lane * pitch + place] : float2{-kInf, 0.0f};
   const float* from = a.part_o + place * D + lane * kPer;
+  float x[4][kPer];
+  const auto load = [&](int p0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int d = 0; d < kPer; ++d) x[i][d] = p0 + i * W < parts ? from[(p0 + i * W) * pitch * D + d] : 0.0f;
+  };
+  load(wave % W);  // under way before the row is known to be one
+  if (!taken(a, (int)token, lane)) return;  // whole workgroups where W waves share a row
   const float top = across32<true>(across16<true>(over16<true>(ml.x)));
   const float f = __builtin_amdgcn_exp2f(ml.x - (top == -kInf ? 0.0f : top));
   const float total = across32<false>(across16<false>(over16<false>(f * ml.y)));
@@ -116,13 +141,7 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_shared_join(Args a) 
 #pragma unroll
   for (int d = 0; d < kPer; ++d) sum[d] = 0.0f;
   for (int p0 = wave % W; p0 < parts; p0 += 4 * W) {
-    float x[4][kPer];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int p = p0 + i * W;
-#pragma unroll
-      for (int d = 0; d < kPer; ++d) x[i][d] = p < parts ? from[part_of(p) * pitch * D + d] : 0.0f;
-    }
+    if (p0 >= 4 * W) load(p0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int p = p0 + i * W;
@@ -144,7 +163,7 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_shared_join(Args a) 
       for (int w = 0; w < W; ++w) sum[d] += lds_sum[w][lane * kPer + d];
     }
   }
-  write_row<D, kBf16>(a, (size_t)seq.start + token, blockIdx.y * a.group + g, lane, top, total, sum);
+  write_row<D, kBf16>(a, token, blockIdx.y * a.group + g, lane, top, total, sum);
 }
 
 template <int D, bool kBf16>
@@ -153,13 +172,13 @@ hipError_t launch_shared(const Args& all, const Kv4PrefixPlan& plan, hipStream_t
   Args own = all;  // part_ml is the same for every launch: behind all parts' sums
   own.part_rows = rows;
   own.part_ml = reinterpret_cast<float2*>(all.part_o + (size_t)plan.parts * rows * all.kv_heads * D);
-  own.parts = std::max(plan.own.few.parts, 1u);
+  own.parts = 1;
   Args front = own;
   front.batch = 1;
   front.max_q = front.q_rows;
   front.table = all.prefix_table;
   front.table_stride = all.prefix_stride;
-  front.part0 = own.parts;
+  front.part0 = 1;
   front.parts = plan.front_parts;
   front.front_groups = plan.front_groups;
   front.rows_from = 0;
@@ -194,18 +213,15 @@ hipError_t launch_shared(const Args& all, const Kv4PrefixPlan& plan, hipStream_t
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   Args join = own;
-  join.rows_to = plan.own.few.row_tiles ? plan.own.few.rows_to : 0;
-  join.part0 = own.parts;
   join.front_parts = plan.front_parts;
   join.front_groups = plan.front_groups;
   join.row_tiles = front.row_tiles;
-  const uint32_t most = all.max_q * all.group;
   if (plan.parts > 8)
-    hipLaunchKernelGGL((k_attention_kv4_shared_join<D, kBf16, kWaves>), dim3(most, all.kv_heads, all.batch), block, 0,
-                       stream, join);
+    hipLaunchKernelGGL((k_attention_kv4_shared_join<D, kBf16, kWaves>), dim3(rows, all.kv_heads), block, 0, stream,
+                       join);
   else
-    hipLaunchKernelGGL((k_attention_kv4_shared_join<D, kBf16, 1>),
-                       dim3((most + kWaves - 1) / kWaves, all.kv_heads, all.batch), block, 0, stream, join);
+    hipLaunchKernelGGL((k_attention_kv4_shared_join<D, kBf16, 1>), dim3((rows + kWaves - 1) / kWaves, all.kv_heads),
+                       block, 0, stream, join);
   return hipGetLastError();
 }
 
