@@ -720,8 +720,8 @@ __global__ __launch_bounds__(kThreads, 2) void k_attention_kv4_few(Args a) {
 // O^T = V^T P^T on 32 x 32 x 16. LDS row m of 32 K rows holds key swap23(m), so the score registers
 // of a lane (one row of q, half = lane / 32) are keys 8 half + 0..7 and 16 + 8 half + 0..7: the B
 // operands of the PV product's two steps, as they are. V stays token-major and its operand comes
-// through the transposed LDS read. 8,192 causal tokens of 32 heads on 8 (128 channels): 593 to 621 us, 0.89 to
-// 0.93 PFLOP/s of the 1.14 that a library product of 8,192^3 reaches; the matrix pipe is busy for 45 % of the
+// through the transposed LDS read. 8,192 causal tokens of 32 heads on 8 (128 channels): 599 to 605 us, 0.91 to
+// 0.92 PFLOP/s of the 1.14 to 1.32 that a library product of 8,192^3 reaches; the matrix pipe is busy for 45 % of the
 // time and the vector pipe for 50 %.
 constexpr int kRowsThreads = 512;
 constexpr int kTileRows = 256, kTileKeys = 64;
@@ -1586,7 +1586,7 @@ __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_rows(Args a) 
 // in slot 2 w if it is workgroup w's first and 2 w + 1 if its last, for k_attention_kv4_rows_join. Every
 // workgroup finds the line from the sequences by itself (at most kLineTiles row tiles and sequences;
 // rows that q_starts counts twice may have none), and the first leaves it in the workspace for the join.
-// 1,025 tokens of 32 heads on 8 over 8,192 keys: 178 us and 15 for the join, 255 apart.
+// 1,025 tokens of 32 heads on 8 over 8,192 keys: 172 us and 15 for the join, 255 apart.
 constexpr int kLineTiles = 512;  // one per thread
 constexpr int kLeastSteps = 8;   // of a range: a shorter one is mostly start and join
 

@@ -7,6 +7,11 @@
 // or of 256, so that each of its keys is unpacked once for as many rows; their own keys (O) are
 // attention_kv4's. Both leave m, l and o in the workspace and a join ends the rows. Calls that gain nothing by that (few
 // rows in all, or sequences that fill tiles by themselves) take every row over F and then O in one pass.
+//
+// 4 query heads to each of 8 cache heads of 128 channels: 64 sequences of up to 700 keys of their own behind 8,192, 28
+// us and 4 for the join (70 in one pass), bound by what starts a workgroup and by vector issue beside the products (44 and 15 %
+// busy); 8 times 257 rows behind 31,104, 1,102 us, 39 for their own keys and 28 for the join (1,392), bound as
+// k_attention_kv4_rows is, whose loop it runs (vector pipe 53 and matrix pipe 48 % busy).
 #include "attention_kv4.hpp"
 
 namespace h3 {

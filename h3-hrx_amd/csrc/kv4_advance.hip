@@ -9,7 +9,9 @@
 //
 // One workgroup makes the sums, a sequence to a thread, and hands out pages by their number in the step (a search in
 // the sums per page: a prompt's hundreds are as quick as a token's one). Where nobody asks for more than one row a
-// thread finishes its own sequence. Long calls' slots and positions are a launch of their own.
+// thread finishes its own sequence. Long calls' slots and positions are a launch of their own. Latency bounds
+// both: 64 sequences of a token each, of which three end, 4.9 us (one alone 3.5); 512 with prompts among them, 129,024 rows,
+// 6.8 and 4.9 (61 with the rows in the first, a search after another).
 #include "internal.hpp"
 
 namespace h3 {

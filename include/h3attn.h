@@ -512,7 +512,10 @@ int h3_attention_kv4_sinks(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *at
  *   prefix_stride  pages that prefix_table holds, (prefix_stride + table_stride) * page_tokens <= 2^24
  *   prefix_table [prefix_stride] i32, prefix_length [1] i32 (cut to [0, prefix_stride * page_tokens]), read on
  *   the device as the others are; the config's window is 0.
- * The other bindings, the precision and the workspace's rules are h3_attention_kv4's. */
+ * The other bindings, the precision and the workspace's rules are h3_attention_kv4's, but for the size (200 MB at
+ * most): with a workspace, rows of sequences that have few are taken over the prefix together, and their sums over the
+ * two kinds of keys joined, where that is estimated to be faster; a row's sums are then of parts that follow from the
+ * call's sizes, not from its values. Rows that q_starts names twice may be of either sequence, or of both. */
 size_t h3_kv4_prefix_workspace_bytes(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention,
                                      uint32_t prefix_stride, uint32_t batch, uint32_t q_rows, uint32_t max_q);
 int h3_attention_kv4_prefix(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention,
@@ -583,7 +586,8 @@ typedef struct {
  *   (elem, 16-byte aligned; q_out may be q and k_out k, each with one stride), q_weight and k_weight [head_dim] f32
  *   (empty views where norm is 0), cos and sin [positions][rotary / 2] f32 (empty where rotary is 0; these four
  *   16-byte aligned), positions [tokens] i32. tokens in [1, 2^24].
- * Precision: queries in f32 and rounded once; keys as computed in f64 and rounded once to the element type.
+ * Precision: queries in f32 and rounded once (those whose squares pass f32's range give zeros); keys in f64 and
+ * rounded once to the element type. A row with a NaN or an infinity has NaN in the channels that it reaches.
  * h3_qk_norm_rope_kv4: the same, with k and v (v [tokens][v_stride], as it is) into slots[i] of the cache: the
  * bytes that h3_kv4_write of k_out and v would leave. The cache's kv_heads, head_dim and elem are cfg's. A row that
  * is none, and one whose slot is outside the cache, is not written there. */
