@@ -114,16 +114,18 @@ __device__ __forceinline__ Eight eight(const float* p) {
 }
 
 // What a token's rows of one weight are multiplied by: own = w cos, other = w' (-sin or sin); past the rotated
-// channels w and 0.
+// channels w and -0, which the other channel is not to meet (an infinity would make a NaN of it): adding
+// 0 times -0 changes nothing, not a zero's sign either.
 template <typename T>
 struct Factors {
   T own[8], other[8];
+  bool turned;
 };
 template <bool kPairs, bool kNorm, typename T>
 __device__ __forceinline__ Factors<T> factors(const QkArgs& a, const Lane& l, const float* weight) {
   Factors<T> f;
   const uint32_t half = a.rotary / 2;
-  const bool turned = l.first < a.rotary, second = !kPairs && turned && l.first >= half;
+  const bool turned = f.turned = l.first < a.rotary, second = !kPairs && turned && l.first >= half;
   Eight w, v;
   if constexpr (kNorm) {
     w = eight(weight + l.first);
@@ -148,7 +150,7 @@ __device__ __forceinline__ Factors<T> factors(const QkArgs& a, const Lane& l, co
   for (int i = 0; i < 8; ++i) {
     const T x = kNorm ? (T)w.v[i] : (T)1, y = kNorm ? (T)v.v[kPairs ? i ^ 1 : i] : (T)1;
     f.own[i] = turned ? x * (T)c.v[i] : x;
-    f.other[i] = turned ? y * (T)s.v[i] : (T)0;
+    f.other[i] = turned ? y * (T)s.v[i] : (T)-0.0f;
   }
   return f;
 }
@@ -159,6 +161,8 @@ __device__ __forceinline__ uint4 turn(const QkArgs& a, const Lane& l, const Fact
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
   uint32_t o[4];
   others<kPairs>(w, l.other, o);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = f.turned ? o[i] : 0;
   T r = 1;
   if constexpr (kNorm) {
     T sum = 0;

@@ -162,6 +162,33 @@ def test_rows_of_extreme_values(dev, elem, norm):
             assert not torch.isfinite(k_out[t, h]).all()
 
 
+@pytest.mark.parametrize("elem", [F16, BF16])
+@pytest.mark.parametrize("interleaved", [0, 1])
+@pytest.mark.parametrize("rotary", [0, 32])
+def test_no_number_stays_in_its_pair(dev, elem, interleaved, rotary):
+    """Without a norm an infinity or a NaN reaches its own channel and its pair's other; the channels that are not rotated
+    are copies, signs of zeros included."""
+    rows = Rows(dev, elem, 64, 2, 2, 9, rotary, interleaved, 0, skip=0)
+    for x in (rows.q, rows.k):
+        x[0, 0, 40], x[1, 0, 41], x[2, 1, 63] = float("inf"), float("nan"), -float("inf")
+        x[3, :, 33:50] = -0.0
+        x[4, 1, 3] = float("inf")
+        x[5, 0, 17] = float("nan")
+    rows.fused[:, :rows.q_width + rows.width] = torch.cat([rows.q.flatten(1), rows.k.flatten(1)], 1)
+    q_out, k_out = rows.run()
+    for x, got in ((rows.q, q_out), (rows.k, k_out)):
+        assert torch.equal(got[..., rotary:].contiguous().view(torch.int16), x[..., rotary:].contiguous().view(torch.int16))
+    if rotary:
+        other = 2 if interleaved else 3 + 16
+        pair17 = {17, 16 if interleaved else 1}
+        for got in (q_out, k_out):
+            bad = ~torch.isfinite(got[..., :rotary].float())
+            assert set(bad[4, 1].nonzero().flatten().tolist()) == {3, other}
+            assert set(bad[5, 0].nonzero().flatten().tolist()) == pair17
+            bad[4, 1], bad[5, 0] = False, False
+            assert not bad.any()
+
+
 @pytest.mark.parametrize("elem,dim,heads,kv_heads,page,tokens,interleaved,norm", [
     (F16, 128, 32, 8, 16, 1, 0, 1), (BF16, 128, 4, 2, 64, 37, 1, 1), (F16, 64, 6, 3, 32, 130, 0, 0),
     (BF16, 64, 5, 5, 256, 700, 0, 1), (F16, 128, 2, 1, 16, 4003, 1, 1), (BF16, 128, 32, 8, 64, 3001, 0, 1),
