@@ -219,7 +219,7 @@ Kv4PrefixPlan kv4_prefix_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg&
     const double each_keys = few_steps(p.own.few.tile_rows, (double)own_keys) * kWaves;
     const Work wide = few_work(p.own.few.tile_rows, each_keys, cus);
     const double wide_each = (double)batch * ((cfg.kv_heads + kWaves - 1) / kWaves) * wide.each;
-    for (uint32_t n = 1; n <= steps && n < kJoinParts; ++n) {
+    for (uint32_t n = 1; n <= steps && n < kJoinParts; n += 1 + n / 8) {  // (the estimate is flat between)
       const Work w = few_work(kMidRows, steps / n, cus);
       // One of them to a compute unit runs beside the sequences' own, two beside each other.
       const double longest = 7 + steps / n * (tiles * n <= cus ? 1.37 : 2.05);

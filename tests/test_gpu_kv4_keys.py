@@ -338,3 +338,15 @@ def test_calls_behind_a_prefix_cut_in_every_way(dev, cut, elem, dim, heads, kv_h
     for length in (0, 1, prefix // 2):
         call.prefix = call.prefix_length = length
         call.check()
+    if max(new) > 1:  # a bound below a sequence's rows: the rows past it are left
+        out, lse, out_tol, lse_tol = call.want()
+        got, got_lse = call.run(max_q=max(new) - 1)
+        last = np.cumsum(new)[np.array(new) == max(new)] - 1
+        some = np.setdiff1d(np.arange(call.rows), last)
+        P.within(got[some], out[some], out_tol[some])
+        P.within(got_lse[some], lse[some], lse_tol[some])
+        assert (got[last] == 5.0).all() and (got_lse[last] == 9.0).all()
+    call.prefix = call.prefix_length = prefix
+    call.plain.words[1, call.prefix_table[0] * page + 9] = 0x7fff  # a key that every row sees
+    out, lse = call.run()
+    assert np.isnan(out).all() and np.isnan(lse).all()
