@@ -221,15 +221,19 @@ Kv4PrefixPlan kv4_prefix_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg&
     const double wide_each = (double)batch * ((cfg.kv_heads + kWaves - 1) / kWaves) * wide.each;
     for (uint32_t n = 1; n <= steps && n < kJoinParts; n += 1 + n / 8) {  // (the estimate is flat between)
       const Work w = few_work(kMidRows, steps / n, cus);
-      // One of them to a compute unit runs beside the sequences' own, two beside each other.
-      const double longest = 7 + steps / n * (tiles * n <= cus ? 1.37 : 2.05);
       // More of them than find room: the last ones leave the chip partly idle.
       const double tail = tiles * n > 2 * cus ? 0.4 * w.each * 2 * cus : 0;
       const double front = 6 + (double)tiles * n * w.each + tail;
-      take(std::max({longest, own.alone, front + own_each}) + join(1 + n), n, n * tiles, 1 + n, false);
+      // The longest of them, one to a compute unit slower by a third while `beside` us of the sequences' own run there
+      // too, or two beside each other.
+      const auto longest = [&](double beside) {
+        const double walk = steps / n * 1.03;
+        return 7 + (tiles * n <= cus ? walk + 0.33 * std::min(walk, beside) : 2 * walk);
+      };
+      take(std::max({longest(2 * own_each), own.alone, front + own_each}) + join(1 + n), n, n * tiles, 1 + n, false);
       if (p.own.few.tile_rows < kMidRows)
-        take(std::max({longest, 5 + wide.each * 2 * cus, front + wide_each}) + 2 + join(1 + n), n, n * tiles, 1 + n,
-             true);
+        take(std::max({longest(2 * wide_each), 5 + wide.each * 2 * cus, front + wide_each}) + join(1 + n), n,
+             n * tiles, 1 + n, true);
     }
   }
   // Tiles of 256 rows along one line.
