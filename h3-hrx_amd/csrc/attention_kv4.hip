@@ -149,8 +149,8 @@ constexpr uint32_t kJoinParts = 64;     // lanes of the join's wave
 constexpr double kSharedBytes = 200e6;  // of the sums of a shared call
 
 // Workgroups of k_attention_kv4_few or _mid with `steps` of their four waves' steps each, over keys that many of them
-// share: us alone on a compute unit, and of one of 512 beside another (`each`: its part of the launch's time). Per step 1.2
-// alone and 2.3 beside another (4 rows, 256 keys), 1.0 and 1.4 (32 rows, 128 keys).
+// share: us alone on a compute unit, and of one of 512 beside another (`each`: its part of the launch's time). Per
+// step 1.2 alone and 2.3 beside another (4 rows, 256 keys), 1.0 and 1.4 (32 rows, 128 keys).
 struct Work {
   double alone, each;
 };

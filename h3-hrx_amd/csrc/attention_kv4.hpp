@@ -62,7 +62,7 @@ struct Args {
   uint32_t causal, window;
   uint32_t sinks;          // kSinks: the first tokens
   uint32_t prefix_stride;  // kPrefix: pages that prefix_table holds
-  uint32_t part0, part_rows;  // kPart: the launch's first part (its own keys' is 0), and the call's rows (tokens times group)
+  uint32_t part0, part_rows;  // kPart: the launch's first part (own keys' is 0), the call's rows (tokens times group)
   uint32_t front_parts;  // kPart: the parts that the prefix's sums are in (0: pieces of a line, front_groups long)
   uint32_t front_groups;
   float scale;  // the softmax scale times log2(e)

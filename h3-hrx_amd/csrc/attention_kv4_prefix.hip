@@ -5,13 +5,13 @@
 //   out = (e^(m_F - m) o_F + e^(m_O - m) o_O) / (e^(m_F - m) l_F + e^(m_O - m) l_O),  m = max(m_F, m_O).
 // Where sequences have few rows, all rows of the call are one matrix against the prefix (F), in tiles of 32 rows
 // or of 256, so that each of its keys is unpacked once for as many rows; their own keys (O) are
-// attention_kv4's. Both leave m, l and o in the workspace and a join ends the rows. Calls that gain nothing by that (few
-// rows in all, or sequences that fill tiles by themselves) take every row over F and then O in one pass.
+// attention_kv4's. Both leave m, l and o in the workspace and a join ends the rows. Calls that gain nothing by that
+// (few rows in all, or sequences that fill tiles by themselves) take every row over F and then O in one pass.
 //
-// 4 query heads to each of 8 cache heads of 128 channels: 64 sequences of up to 700 keys of their own behind 8,192, 28
-// us and 4 for the join (70 in one pass), bound by what starts a workgroup and by vector issue beside the products (44 and 15 %
-// busy); 8 times 257 rows behind 31,104, 1,102 us, 39 for their own keys and 28 for the join (1,392), bound as
-// k_attention_kv4_rows is, whose loop it runs (vector pipe 53 and matrix pipe 48 % busy).
+// 4 query heads to each of 8 cache heads of 128 channels: 64 sequences of up to 700 keys of their own behind 8,192,
+// 28 us and 4 for the join (70 in one pass), bound by what starts a workgroup and by vector issue beside the products
+// (44 and 15 % busy); 8 times 257 rows behind 31,104, 1,102 us, 39 for their own keys and 28 for the join (1,392),
+// bound as k_attention_kv4_rows is, whose loop it runs (vector pipe 53 and matrix pipe 48 % busy).
 #include "attention_kv4.hpp"
 
 namespace h3 {
@@ -88,8 +88,8 @@ void launch_tiles_shared(const Args& own, const Args& front, bool heads_apart, h
                      front);
 }
 
-// Whether a token's row is one that its sequence takes. 64 ends at a time, a lane each: the first past the token is the
-// sequence's.
+// Whether a token's row is one that its sequence takes. 64 ends at a time, a lane each: the first past the token is
+// the sequence's.
 __device__ __forceinline__ bool taken(const Args& a, int token, int lane) {
   int b = 0;
   for (int span = (int)a.batch; span > 0;) {  // the sequence is one of b .. b + span - 1, or there is none
@@ -108,8 +108,8 @@ __device__ __forceinline__ bool taken(const Args& a, int token, int lane) {
   return token >= start && token - start < (int)a.max_q;
 }
 
-// Joins a row's parts, its own and then the prefix's: W waves per (row, query head), wave w the parts w, w + W, ..; lane p
-// of a wave holds part p's weight.
+// Joins a row's parts, its own and then the prefix's: W waves per (row, query head), wave w the parts w, w + W, ..;
+// lane p of a wave holds part p's weight.
 template <int D, bool kBf16, int W>
 __global__ __launch_bounds__(kThreads) void k_attention_kv4_shared_join(Args a) {
   constexpr int kPer = D / 64;

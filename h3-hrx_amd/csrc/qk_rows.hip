@@ -196,8 +196,8 @@ __device__ __forceinline__ void put(const QkArgs& a, const Lane& l, uint32_t hea
   if (l.first == 0) *reinterpret_cast<uint32_t*>(a.cache + at.words + part * 4 * at.tokens) = row.x;
 }
 
-// Heads from .. to - 1 (to may be less) of the token's queries, keys or values, kHeads at a time: the next ones' rows are
-// under way while these are computed.
+// Heads from .. to - 1 (to may be less) of the token's queries, keys or values, kHeads at a time: the next ones'
+// rows are under way while these are computed.
 enum Kind { kQuery, kKey, kValue };
 constexpr uint32_t kHeads = 4;
 template <int D, bool kBf16, bool kPairs, bool kNorm, bool kCached, bool kOnce, Kind kKind>

@@ -535,8 +535,8 @@ int h3_attention_kv4_prefix(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *a
  *     shows in q_starts: it has no rows.
  * Pages are taken from the top of the stack, in order of sequences and columns, into the table. Sequence b's
  * rows are q_starts[b] .. q_starts[b + 1] - 1; row i of them has positions = prefix + lengths[b] + i and the slot
- * of that token for h3_kv4_write; lengths_out is for h3_attention_kv4. Rows from q_starts[batch] on carry -1 in slots and
- * positions. Table entries that are not taken, and the stack above the pushed pages, keep their values.
+ * of that token for h3_kv4_write; lengths_out is for h3_attention_kv4. Rows from q_starts[batch] on carry -1 in
+ * slots and positions. Table entries that are not taken, and the stack above the pushed pages, keep their values.
  *   asked [batch], lengths [batch], free_pages [cfg->pages], free_count [1], table [batch][table_stride],
  *   lengths_out [batch] (may be lengths), free_count_out [1] (may be free_count), q_starts [batch + 1], slots
  *   [rows], positions [rows], prefix_length [1] or an empty view (prefix 0), all i32. batch in [1, 65535], rows in

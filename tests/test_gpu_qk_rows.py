@@ -166,8 +166,8 @@ def test_rows_of_extreme_values(dev, elem, norm):
 @pytest.mark.parametrize("interleaved", [0, 1])
 @pytest.mark.parametrize("rotary", [0, 32])
 def test_no_number_stays_in_its_pair(dev, elem, interleaved, rotary):
-    """Without a norm an infinity or a NaN reaches its own channel and its pair's other; the channels that are not rotated
-    are copies, signs of zeros included."""
+    """Without a norm an infinity or a NaN reaches its own channel and its pair's other; the channels that are not
+    rotated are copies, signs of zeros included."""
     rows = Rows(dev, elem, 64, 2, 2, 9, rotary, interleaved, 0, skip=0)
     for x in (rows.q, rows.k):
         x[0, 0, 40], x[1, 0, 41], x[2, 1, 63] = float("inf"), float("nan"), -float("inf")
@@ -177,7 +177,8 @@ def test_no_number_stays_in_its_pair(dev, elem, interleaved, rotary):
     rows.fused[:, :rows.q_width + rows.width] = torch.cat([rows.q.flatten(1), rows.k.flatten(1)], 1)
     q_out, k_out = rows.run()
     for x, got in ((rows.q, q_out), (rows.k, k_out)):
-        assert torch.equal(got[..., rotary:].contiguous().view(torch.int16), x[..., rotary:].contiguous().view(torch.int16))
+        bits = [y[..., rotary:].contiguous().view(torch.int16) for y in (got, x)]
+        assert torch.equal(*bits)
     if rotary:
         other = 2 if interleaved else 3 + 16
         pair17 = {17, 16 if interleaved else 1}

@@ -176,7 +176,8 @@ class Plan(ctypes.Structure):
 
 
 class PrefixPlan(ctypes.Structure):
-    _fields_ = [("shared", ctypes.c_bool), ("heads_apart", ctypes.c_bool), ("one", Plan), ("own", Plan), ("front_parts", ctypes.c_uint32),
+    _fields_ = [("shared", ctypes.c_bool), ("heads_apart", ctypes.c_bool), ("one", Plan), ("own", Plan),
+                ("front_parts", ctypes.c_uint32),
                 ("front_groups", ctypes.c_uint32), ("parts", ctypes.c_uint32)]
 
 
