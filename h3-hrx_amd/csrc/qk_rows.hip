@@ -7,9 +7,10 @@
 // the first and sin for the second channel of one, the result is r (x (w cos) + x' (w' s)): the two factors are a
 // token's for all its heads, and what passes between lanes is x as it was read, two channels to a register.
 //
-// Queries are computed in f32 and rounded once. Keys are computed in f64, so that the 16 bits that they are rounded to
-// are the definition's, whatever the order of its sums: a bit of one of them is a step of a code or of a whole row's
-// scale in the cache. It costs nothing that is seen: there are few key heads and memory bounds the kernel.
+// Queries are computed in f32 and rounded once, but for rows whose squares f32 does not hold, which are as the keys.
+// Keys are computed in f64, so that the 16 bits that they are rounded to are the definition's, whatever the order of
+// its sums: a bit of one of them is a step of a code or of a whole row's scale in the cache. It costs nothing that is
+// seen: there are few key heads and memory bounds the kernel.
 //
 // D/8 lanes of 8 channels hold a row, so a wave holds one head of 512/D tokens and takes `per` heads of the same
 // tokens one after the other.
@@ -155,6 +156,33 @@ __device__ __forceinline__ Factors<T> factors(const QkArgs& a, const Lane& l, co
   return f;
 }
 
+// mean(x^2) + eps of a row, in T.
+template <int D, bool kBf16, typename T>
+__device__ __forceinline__ T mean_square(const uint32_t (&w)[4], float eps) {
+  T sum = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const T x = channel(w, i, kBf16);
+    sum = fma(x, x, sum);
+  }
+  return fma(row_sum<D>(sum), (T)(1.0 / D), (T)eps);
+}
+
+// A channel before its rounding, and rounded.
+template <bool kBf16, typename T, typename F>
+__device__ __forceinline__ uint32_t turned_channel(const uint32_t (&w)[4], const uint32_t (&o)[4], int i,
+                                                   const Factors<F>& f, T r) {
+  const T y = fma((T)channel(w, i, kBf16), (T)f.own[i], (T)channel(o, i, kBf16) * (T)f.other[i]) * r;
+  if constexpr (sizeof(T) == 8)
+    return narrow64<kBf16>(y);
+  else
+    return narrow<kBf16>(y);
+}
+
+// Mean squares that f32's sums are exact enough for: what is lost of smaller squares is below 2^-119, and none of these
+// overflows.
+constexpr float kLeastSquare = 0x1p-80f, kMostSquare = 0x1p120f;
+
 // A row's eight channels in 16 bits.
 template <int D, bool kBf16, bool kPairs, bool kNorm, typename T>
 __device__ __forceinline__ uint4 turn(const QkArgs& a, const Lane& l, const Factors<T>& f, uint4 raw) {
@@ -163,25 +191,20 @@ __device__ __forceinline__ uint4 turn(const QkArgs& a, const Lane& l, const Fact
   others<kPairs>(w, l.other, o);
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = f.turned ? o[i] : 0;
-  T r = 1;
+  T square = 1, r = 1;
   if constexpr (kNorm) {
-    T sum = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const T x = channel(w, i, kBf16);
-      sum = fma(x, x, sum);
-    }
-    sum = row_sum<D>(sum);
-    r = inverse_root(fma(sum, (T)(1.0 / D), (T)a.eps));
+    square = mean_square<D, kBf16, T>(w, a.eps);
+    r = inverse_root(square);
   }
   uint32_t out[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const T y = fma((T)channel(w, i, kBf16), f.own[i], (T)channel(o, i, kBf16) * f.other[i]) * r;
-    if constexpr (sizeof(T) == 8)
-      out[i] = narrow64<kBf16>(y);
-    else
-      out[i] = narrow<kBf16>(y);
+  for (int i = 0; i < 8; ++i) out[i] = turned_channel<kBf16>(w, o, i, f, r);
+  if constexpr (kNorm && kBf16 && sizeof(T) == 4) {
+    if (!(square >= kLeastSquare && square < kMostSquare)) {  // (a row's lanes are of one mind)
+      const double r64 = inverse_root(mean_square<D, kBf16, double>(w, a.eps));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) out[i] = turned_channel<kBf16>(w, o, i, f, r64);
+    }
   }
   return {out[0] | out[1] << 16, out[2] | out[3] << 16, out[4] | out[5] << 16, out[6] | out[7] << 16};
 }

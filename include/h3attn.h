@@ -586,7 +586,7 @@ typedef struct {
  *   (elem, 16-byte aligned; q_out may be q and k_out k, each with one stride), q_weight and k_weight [head_dim] f32
  *   (empty views where norm is 0), cos and sin [positions][rotary / 2] f32 (empty where rotary is 0; these four
  *   16-byte aligned), positions [tokens] i32. tokens in [1, 2^24].
- * Precision: queries in f32 and rounded once (those whose squares pass f32's range give zeros); keys in f64 and
+ * Precision: queries in f32 and rounded once (rows whose squares f32 does not hold in f64); keys in f64 and
  * rounded once to the element type. A row with a NaN or an infinity has NaN in the channels that it reaches.
  * h3_qk_norm_rope_kv4: the same, with k and v (v [tokens][v_stride], as it is) into slots[i] of the cache: the
  * bytes that h3_kv4_write of k_out and v would leave. The cache's kv_heads, head_dim and elem are cfg's. A row that

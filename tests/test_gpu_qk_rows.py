@@ -61,7 +61,7 @@ class Rows:
     def live(self):
         return (self.positions >= 0) & (self.positions < self.cfg.positions)
 
-    def check(self, q_out, k_out):
+    def check(self, q_out, k_out, least=0.0):
         c, live = self.cfg, self.live()
         q, k = (S.norm_rope(c, x, w, self.cos, self.sin, self.positions)
                 for x, w in zip((self.q, self.k), self.weights))
@@ -72,7 +72,7 @@ class Rows:
         other = S.norm_rope(both, self.q.abs(), np.abs(self.weights[0]), np.abs(self.cos), np.abs(self.sin),
                             self.positions)
         size = np.maximum(np.abs(size), np.abs(other))
-        half, tiny = P.HALF_STEP[c.elem], 2.0 ** -25 if c.elem == F16 else 0.0
+        half, tiny = P.HALF_STEP[c.elem], 2.0 ** -25 if c.elem == F16 else least
         tol = half * np.abs(q) * (1 + 2.0 ** -10) + (self.dim / 16 + 24) * P.F32 * size + tiny
         got = q_out.double().numpy()
         P.within(got[live], q[live], tol[live])
@@ -160,6 +160,24 @@ def test_rows_of_extreme_values(dev, elem, norm):
         assert torch.equal(k_out[keep], want[keep])
         for t, h in ((5, 0), (6, 1), (7, 0)):
             assert not torch.isfinite(k_out[t, h]).all()
+
+
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -140, 1e-5, 2.0 ** 127])
+@pytest.mark.parametrize("dim,interleaved", [(64, 0), (128, 1), (128, 0)])
+def test_squares_outside_f32(dev, dim, interleaved, eps):
+    """Rows whose squares f32 does not hold, beside rows whose squares it does."""
+    rows = Rows(dev, BF16, dim, 5, 2, 41, dim, interleaved, 1, skip=0)
+    rows.cfg.eps = eps
+    scale = torch.exp2(torch.from_numpy(rows.rng.integers(-110, 120, (rows.tokens, 5, 1)).astype(np.float32)))
+    scale[::3] = 1.0
+    rows.q = (rows.q.float() * scale).bfloat16()
+    rows.k = (rows.k.float() * scale[:, :2]).bfloat16()
+    rows.fused[:, :rows.q_width + rows.width] = torch.cat([rows.q.flatten(1), rows.k.flatten(1)], 1)
+    assert torch.isfinite(rows.q.float()).all()
+    q_out, k_out = rows.run()
+    if eps == 0:
+        assert (q_out.float().abs().amax(-1) > 0.1).all() and torch.isfinite(q_out.float()).all()
+    rows.check(q_out, k_out, least=2.0 ** -133)  # a step of bf16 below its normal range
 
 
 @pytest.mark.parametrize("elem", [F16, BF16])
