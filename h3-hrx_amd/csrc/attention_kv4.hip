@@ -211,7 +211,9 @@ Kv4PrefixPlan kv4_prefix_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg&
     p.front_groups = front_groups;
     p.parts = parts;
   };
-  // Tiles of 32 rows, in one launch with the sequences' own where those are few.
+  // Tiles of 32 rows, in one launch with the sequences' own where those are few. It has all workgroups in one dimension
+  // of the grid, which holds 2^32 threads at most.
+  const auto fits = [](uint64_t groups) { return groups * kThreads < (1ull << 32); };
   if (rows <= kFewMost && small) {
     const uint32_t tiles = (uint32_t)(rows + kMidRows - 1) / kMidRows * cfg.kv_heads;
     const double steps = std::max(1.0, few_steps(kMidRows, (double)prefix));
@@ -230,8 +232,9 @@ Kv4PrefixPlan kv4_prefix_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg&
         const double walk = steps / n * 1.03;
         return 7 + (tiles * n <= cus ? walk + 0.33 * std::min(walk, beside) : 2 * walk);
       };
-      take(std::max({longest(2 * own_each), own.alone, front + own_each}) + join(1 + n), n, n * tiles, 1 + n, false);
-      if (p.own.few.tile_rows < kMidRows)
+      if (fits((uint64_t)batch * cfg.kv_heads * p.own.few.row_tiles + n * tiles))
+        take(std::max({longest(2 * own_each), own.alone, front + own_each}) + join(1 + n), n, n * tiles, 1 + n, false);
+      if (p.own.few.tile_rows < kMidRows && fits((uint64_t)batch * ((cfg.kv_heads + kWaves - 1) / kWaves) + n * tiles))
         take(std::max({longest(2 * wide_each), 5 + wide.each * 2 * cus, front + wide_each}) + join(1 + n), n,
              n * tiles, 1 + n, true);
     }

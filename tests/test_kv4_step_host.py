@@ -188,6 +188,28 @@ def prefix_plan(cfg, acfg, stride, batch, q_rows, max_q, divide=True):
     return call(ctypes.byref(cfg), ctypes.byref(acfg), stride, batch, q_rows, max_q, 256, divide)
 
 
+def test_grids_of_the_largest_batches():
+    """65,535 sequences, most of them without rows: the launch that holds them all in its first dimension is taken only
+    where it stays below 2^32 threads there."""
+    rng = np.random.default_rng(1)
+    shared = past = 0
+    for _ in range(3000):
+        kv_heads, group = int(rng.choice([64, 128, 200, 255, 256])), int(rng.choice([1, 2, 4, 8, 16]))
+        batch, q_rows = 65535, int(2 ** rng.uniform(0, 13))
+        max_q, dim = max(1, min(q_rows, int(2 ** rng.uniform(0, 12)))), int(rng.choice([64, 128]))
+        cfg = H.Kv4Cfg(kv_heads, dim, 16, 1000, 0)
+        width = kv_heads * group * dim
+        columns, causal = int(2 ** rng.uniform(0, 14)), int(rng.integers(0, 2))
+        acfg = H.Kv4AttentionCfg(kv_heads * group, width, width, columns, causal, 0, 0.1)
+        p = prefix_plan(cfg, acfg, int(2 ** rng.uniform(0, 18)), batch, q_rows, max_q)
+        own = batch * (-(-kv_heads // 4) if p.heads_apart else kv_heads * p.own.few.tiles)
+        past += (kv_heads * p.own.few.tiles * batch + 256) * 256 >= 2 ** 32
+        if p.shared and p.front_parts:
+            shared += 1
+            assert (p.front_groups + own) * 256 < 2 ** 32, (kv_heads, group, q_rows, max_q)
+    assert shared > 100 and past > 100
+
+
 def test_every_row_behind_a_prefix_has_its_launches():
     """Every count of rows that a sequence can have belongs to one launch of its own keys; the parts fit the join's
     wave and the workspace, the pieces of a line the parts; grids stay inside their limits."""
