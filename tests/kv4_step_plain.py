@@ -45,6 +45,8 @@ def attend(cache, acfg, q, table, new, lengths, sinks=0, prefix=None):
     front, front_live = slots_of(shared_pages, shared)
     first = 0
     for b, (n, length) in enumerate(zip(new, lengths)):
+        if n == 0:
+            continue
         own, own_live = slots_of(table[b], length)
         slots, live = np.concatenate([front, own]), np.concatenate([front_live, own_live])
         seen = visible(n, length, acfg.causal, acfg.window, sinks, shared) & live

@@ -350,3 +350,13 @@ def test_calls_behind_a_prefix_cut_in_every_way(dev, cut, elem, dim, heads, kv_h
     call.plain.words[1, call.prefix_table[0] * page + 9] = 0x7fff  # a key that every row sees
     out, lse = call.run()
     assert np.isnan(out).all() and np.isnan(lse).all()
+
+
+@pytest.mark.parametrize("more", [{"prefix": 700}, {"sinks": 9, "window": 100}])
+@pytest.mark.parametrize("kv_heads,batch", [(2, 20001), (20, 65535)])
+def test_batches_of_which_few_sequences_have_rows(dev, more, kv_heads, batch):
+    new, lengths = [0] * batch, [0] * batch
+    for b, n, length in ((5, 1, 300), (4444, 2, 77), (batch - 1, 3, 120)):
+        new[b], lengths[b] = n, length
+    lengths[7] = 40  # keys and no rows
+    Front(dev, F16, 64, kv_heads, kv_heads, 16, new, lengths, **more).both()
