@@ -76,6 +76,15 @@ def test_steps_match_the_definition(dev, batch, page, most, new, ended, free, ro
         both(dev, cfg, columns, rows, asked, lengths, stack, count, table, prefix, in_place)
 
 
+@pytest.mark.parametrize("new,rows", [(1, 2000), (1, 70000), (3, 60000)])
+def test_the_largest_batch(dev, new, rows):
+    rng = np.random.default_rng(rows)
+    cfg, columns, asked, lengths, stack, count, table = state(rng, 65535, 16, 40, new, 0.3, 3000)
+    if rows == 2000:
+        asked[rng.random(len(asked)) < 0.95] = 0  # nearly all idle
+    both(dev, cfg, columns, rows, asked, lengths, stack, count, table, 5, True)
+
+
 def test_a_refused_sequence_keeps_what_it_has(dev):
     cfg = H.Kv4Cfg(1, 64, 16, 12, 0)
     table = np.array([[0, 1, -1], [2, -1, -1], [3, 4, 5], [6, -1, -1]], np.int32)
