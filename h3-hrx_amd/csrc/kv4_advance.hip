@@ -20,6 +20,7 @@ namespace {
 // More rows than this have a launch of their own: 512 sequences with prompts among them, 8.1 us for 2,048 rows in one
 // launch and 11.8 for 2,049 in two, 11.9 for 16,384; in one, 61 for 129,024.
 constexpr uint32_t kRowsApart = 2048;
+constexpr uint32_t kGiven = 4;  // entries of ended sequences under way in a thread
 constexpr uint32_t kMost = 1u << 30;  // sums stop here: past every number of rows or pages that can be granted
 
 struct AdvanceArgs {
@@ -103,12 +104,15 @@ template <int kThreads>
 __global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a, bool places) {
   __shared__ Two scratch[kThreads / 64];
   __shared__ uint32_t page_sums[kThreads], row_sums[kThreads], first_column[kThreads], first_token[kThreads];
+  __shared__ uint32_t some_none[2];
   const uint32_t t = threadIdx.x, up = (1u << a.page_shift) - 1;
   const uint32_t before = (uint32_t)min(max(*a.x.free_count, 0), (int)a.pages);
   const uint32_t prefix = a.x.prefix_length ? (uint32_t)max(*a.x.prefix_length, 0) : 0;
 
-  // The pages of the sequences that end, onto the stack.
-  uint32_t count = before;
+  // The pages of the sequences that end, onto the stack. An entry that is no page (-1 where the program has taken the
+  // page back, as behind a window) is not pushed: it would be granted as one, and what is written there lost.
+  uint32_t count = before, turn = 0;
+  if (t < 2) some_none[t] = 0;
   for (uint32_t b0 = 0; b0 < a.batch; b0 += kThreads) {
     const uint32_t b = b0 + t;
     uint32_t held = 0;
@@ -117,15 +121,34 @@ __global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a, bool pl
     Two all;
     page_sums[t] = sum_to_here<kThreads>({held, 0}, scratch, &all).a;
     __syncthreads();
-    each<kThreads>(t, all.a,
-                   [&](uint32_t i) {
-                     const uint32_t s = find<kThreads>(page_sums, i);
-                     return a.x.table[(size_t)(b0 + s) * a.columns + i - (s ? page_sums[s - 1] : 0)];
-                   },
-                   [&](uint32_t i, int page) {
-                     if (count + i < a.pages) a.x.free_pages[count + i] = page;
-                   });
-    count = min(count + all.a, a.pages);
+    for (uint32_t i0 = 0; i0 < all.a; i0 += kGiven * kThreads, turn ^= 1) {
+      int page[kGiven];
+#pragma unroll
+      for (uint32_t k = 0; k < kGiven; ++k) {
+        const uint32_t i = i0 + k * kThreads + t;
+        page[k] = -1;
+        if (i >= all.a) continue;
+        const uint32_t s = find<kThreads>(page_sums, i);
+        page[k] = a.x.table[(size_t)(b0 + s) * a.columns + i - (s ? page_sums[s - 1] : 0)];
+        if ((uint32_t)page[k] >= a.pages) some_none[turn] = 1;
+      }
+      // Places on the stack by the entries' numbers, or, from a turn with an entry that is no page on, by the pages'
+      // sums. Two flags in turn: a thread that is ahead sets the other one until all have read this.
+      __syncthreads();
+      const bool whole = some_none[turn] == 0;
+#pragma unroll
+      for (uint32_t k = 0; k < kGiven; ++k) {
+        const bool is = (uint32_t)page[k] < a.pages;
+        uint32_t place = t, given = min(all.a - min(i0 + k * kThreads, all.a), (uint32_t)kThreads);
+        if (!whole) {
+          Two sum;
+          place = sum_to_here<kThreads>({is, 0}, scratch, &sum).a - 1;
+          given = sum.a;
+        }
+        if (is && count + place < a.pages) a.x.free_pages[count + place] = page[k];
+        count = min(count + given, a.pages);
+      }
+    }
   }
   __syncthreads();
 

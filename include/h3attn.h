@@ -497,7 +497,8 @@ int h3_attention_kv4(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attentio
  * too: row i of a sequence's n rows, at position p = length - n + i, sees the keys j <= p with j > p - window or
  * j < sinks. The bindings, the precision and the workspace's rules are h3_attention_kv4's; without a window (or
  * without sinks) it is that call. Pages of the table between the first tokens and the window of every row are not
- * read: their entries may be anything. sinks in [0, 2^24]. */
+ * read: their entries may be anything. (h3_kv4_advance keeps a sequence's pages until it ends: a program that gives such
+ * pages back sooner writes -1 into their entries.) sinks in [0, 2^24]. */
 size_t h3_kv4_sinks_workspace_bytes(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention,
                                     uint32_t sinks, uint32_t batch, uint32_t q_rows, uint32_t max_q);
 int h3_attention_kv4_sinks(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *attention, uint32_t sinks,
@@ -527,7 +528,9 @@ int h3_attention_kv4_prefix(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *a
 /* h3_kv4_advance: what the next step of `batch` sequences needs, from the rows that each asks for. Sequence b
  * has lengths[b] tokens in ceil(lengths[b] / page_tokens) pages, the first entries of its row of the table.
  *   asked[b] < 0: the sequence ends. Its pages go on the stack of free pages, free_pages[0 .. free_count - 1],
- *     before any are taken, in order of sequences and of columns; lengths_out[b] = 0, no rows.
+ *     before any are taken, in order of sequences and of columns; lengths_out[b] = 0, no rows. Entries that are no
+ *     page of the cache (-1 where the program has given a page back before) are passed over; a page that is another's
+ *     by now and still stands there would have two owners.
  *   asked[b] >= 0: so many rows are appended, if the sequence is granted them; all or none. It is refused where
  *     its tokens would pass the table's row; where it needs pages and those that it and the sequences before it
  *     ask for (refused or not, but for the first reason) are more than are free; and where the rows that it and

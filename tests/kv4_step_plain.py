@@ -99,7 +99,7 @@ def advance(cfg, table_stride, rows, asked, lengths, free_pages, free_count, tab
     for b, n in enumerate(asked):
         if n < 0:
             for column in range(up(cut[b])):
-                if count < cfg.pages:
+                if 0 <= table[b, column] < cfg.pages and count < cfg.pages:  # an entry that is no page is none
                     free[count] = table[b, column]
                     count += 1
     out, starts = [], [0]
