@@ -145,7 +145,6 @@ Kv4Plan kv4_front_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, 
 
 namespace {
 
-constexpr uint32_t kJoinParts = 64;     // lanes of the join's wave
 constexpr double kSharedBytes = 200e6;  // of the sums of a shared call
 
 // Workgroups of k_attention_kv4_few or _mid with `steps` of their four waves' steps each, over keys that many of them

@@ -19,21 +19,30 @@ namespace {
 
 // All rows over the prefix in tiles of 256: the tiles' steps of every cache head are one line, as
 // k_attention_kv4_line's, of which each workgroup takes an equal range. The tiles are alike, so that a tile's pieces
-// follow from its number: piece i of it is part part0 + i.
+// follow from its number: piece i of it is the prefix's part i. The line is of the rows that there are: where a call has
+// places for more (a captured step's padding) their sums have room for more pieces, and the line is divided
+// as finely: 64 tokens of 2,056 places behind 31,104 keys 99 us (all places' rows multiplied 1,001). A tile of n steps
+// in ranges of n / (most - 1) and more has `most` pieces at most; without padding those of the plan's.
 struct FrontLine {
-  int steps, range;  // of a tile; of a workgroup
+  int rows, each, steps, range;  // of a cache head, its tiles; of a tile; of a workgroup
 };
-__device__ __forceinline__ FrontLine front_line(const Args& a, int length, int tiles) {
+__device__ __forceinline__ FrontLine front_line(const Args& a, int tokens, int length) {
+  const int rows = tokens * (int)a.group, each = (rows + kTileRows - 1) / kTileRows, groups = (int)a.front_groups;
   const int steps = max((length + kTileKeys - 1) / kTileKeys, 1);
-  return {steps, max((steps * tiles + (int)a.front_groups - 1) / (int)a.front_groups, kLeastSteps)};
+  int range = max((steps * each * (int)a.kv_heads + groups - 1) / groups, kLeastSteps);
+  if (rows < (int)a.part_rows) {
+    const int most = (int)min(a.front_places / (uint32_t)max(rows, 1), kJoinParts - 1);
+    range = max(range, (steps + most - 2) / (most - 1));
+  }
+  return {rows, each, steps, range};
 }
 
 template <int D, bool kBf16>
 __global__ __launch_bounds__(kRowsThreads, 2) void k_attention_kv4_front(Args a) {
   __shared__ __attribute__((aligned(16))) RowsLds<D> lds;
   const Sequence seq = sequence<kFrontPart>(a, 0);
-  const int each = (int)a.row_tiles, tiles = each * (int)a.kv_heads;
-  const FrontLine line = front_line(a, seq.length, tiles);
+  const FrontLine line = front_line(a, seq.rows, seq.length);
+  const int each = line.each, tiles = each * (int)a.kv_heads;
   const int begin = (int)blockIdx.x * line.range, stop = min(begin + line.range, line.steps * tiles);
   for (int at = begin; at < stop;) {
     const int tile = at / line.steps, start = tile * line.steps, first = at - start;
@@ -89,8 +98,9 @@ void launch_tiles_shared(const Args& own, const Args& front, bool heads_apart, h
 }
 
 // Whether a token's row is one that its sequence takes. 64 ends at a time, a lane each: the first past the token is
-// the sequence's.
+// the sequence's. (No row from the last sequence's end on has sums over the prefix.)
 __device__ __forceinline__ bool taken(const Args& a, int token, int lane) {
+  const int end = a.q_starts[a.batch];
   int b = 0;
   for (int span = (int)a.batch; span > 0;) {  // the sequence is one of b .. b + span - 1, or there is none
     const int each = (span + 63) / 64, last = min(b + (lane + 1) * each, b + span) - 1;
@@ -105,7 +115,7 @@ __device__ __forceinline__ bool taken(const Args& a, int token, int lane) {
     b += chunk;
   }
   const int start = max(a.q_starts[b], 0);
-  return token >= start && token - start < (int)a.max_q;
+  return token >= start && token - start < (int)a.max_q && token < end;
 }
 
 // Joins a row's parts, its own and then the prefix's: W waves per (row, query head), wave w the parts w, w + W, ..;
@@ -119,22 +129,28 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_shared_join(Args a) 
   if (at >= a.part_rows) return;
   const uint32_t token = at / a.group, g = at - token * a.group;
   int front = (int)a.front_parts;
+  uint32_t pitch = a.part_rows;
   if (front == 0) {
-    const int each = (int)a.row_tiles, tile = (int)blockIdx.y * each + (int)at / kTileRows;
     const int length = min(max(*a.prefix_length, 0), (int)(a.prefix_stride << a.page_shift));
-    const FrontLine line = front_line(a, length, each * (int)a.kv_heads);
+    const FrontLine line = front_line(a, min(max(a.q_starts[a.batch], 0), (int)a.q_rows), length);
+    if ((int)at >= line.rows) return;
+    const int tile = (int)blockIdx.y * line.each + (int)at / kTileRows;
     front = (tile * line.steps + line.steps - 1) / line.range - tile * line.steps / line.range + 1;
+    pitch = (uint32_t)line.rows;
   }
   const int parts = 1 + front;
-  const size_t place = (size_t)at * a.kv_heads + blockIdx.y, pitch = (size_t)a.part_rows * a.kv_heads;
-  const float2 ml = lane < parts ? a.part_ml[lane * pitch + place] : float2{-kInf, 0.0f};
-  const float* from = a.part_o + place * D + lane * kPer;
+  const auto place = [&](int p) {  // of the row's part p
+    return ((p ? a.part_rows + (size_t)(p - 1) * pitch : 0) + at) * a.kv_heads + blockIdx.y;
+  };
+  const float2 ml = lane < parts ? a.part_ml[place(lane)] : float2{-kInf, 0.0f};
   float x[4][kPer];
   const auto load = [&](int p0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+      const float* from = a.part_o + place(p0 + i * W) * D + lane * kPer;
 #pragma unroll
-      for (int d = 0; d < kPer; ++d) x[i][d] = p0 + i * W < parts ? from[(p0 + i * W) * pitch * D + d] : 0.0f;
+      for (int d = 0; d < kPer; ++d) x[i][d] = p0 + i * W < parts ? from[d] : 0.0f;
+    }
   };
   load(wave % W);  // under way before the row is known to be one
   if (!taken(a, (int)token, lane)) return;  // whole workgroups where W waves share a row
@@ -183,9 +199,11 @@ hipError_t launch_shared(const Args& all, const Kv4PrefixPlan& plan, hipStream_t
   front.max_q = front.q_rows;
   front.table = all.prefix_table;
   front.table_stride = all.prefix_stride;
-  front.part0 = 1;
+  front.q_starts = all.q_starts + all.batch;
   front.parts = plan.front_parts;
+  front.front_parts = plan.front_parts;
   front.front_groups = plan.front_groups;
+  front.front_places = (plan.parts - 1) * rows;
   front.rows_from = 0;
   front.rows_to = rows;
   Args few = own;
@@ -202,7 +220,6 @@ hipError_t launch_shared(const Args& all, const Kv4PrefixPlan& plan, hipStream_t
       default: launch_tiles_shared<D, kBf16, 0>(few, front, false, stream);
     }
   } else {
-    front.row_tiles = (rows + kTileRows - 1) / kTileRows;
     hipLaunchKernelGGL((k_attention_kv4_front<D, kBf16>), dim3(front.front_groups), dim3(kRowsThreads), 0, stream,
                        front);
     if (plan.own.many.row_tiles) {
@@ -220,7 +237,7 @@ hipError_t launch_shared(const Args& all, const Kv4PrefixPlan& plan, hipStream_t
   Args join = own;
   join.front_parts = plan.front_parts;
   join.front_groups = plan.front_groups;
-  join.row_tiles = front.row_tiles;
+  join.front_places = front.front_places;
   if (plan.parts > 8)
     hipLaunchKernelGGL((k_attention_kv4_shared_join<D, kBf16, kWaves>), dim3(rows, all.kv_heads), block, 0, stream,
                        join);
