@@ -229,36 +229,44 @@ __global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a, bool pl
   if (t == 0) *a.x.free_count_out = (int)(count - granted.a);
 }
 
-// Slots and positions from q_starts, lengths_out and the table: four rows a thread. Where the starts fit LDS the search
-// for the first row's sequence is there.
+// Slots and positions from q_starts, lengths_out and the table: four rows a thread. Where the starts fit LDS the
+// searches for the rows' sequences are there. A row behind its sequence's end is most often the next one's; if not (idle
+// sequences between them, 65,534 behind the last row at most) it is searched for: the thread's other rows one
+// sequence after another cost 8.3 ms there, 51 us with 411 idle ones.
 constexpr int kPlaceThreads = 256, kPlaceRows = 4, kPlaceStarts = 2048;
 __global__ __launch_bounds__(kPlaceThreads) void k_kv4_places(AdvanceArgs a) {
   __shared__ uint32_t ends[kPlaceStarts];
   const uint32_t first = (blockIdx.x * kPlaceThreads + threadIdx.x) * kPlaceRows;
   const int* starts = a.x.q_starts;
   const uint32_t prefix = a.x.prefix_length ? (uint32_t)max(*a.x.prefix_length, 0) : 0;
-  uint32_t b = 0;  // the first sequence whose end is past the row
-  if (a.batch < kPlaceStarts) {
+  const bool in_lds = a.batch < kPlaceStarts;
+  if (in_lds) {
     for (uint32_t i = threadIdx.x; i < kPlaceStarts; i += kPlaceThreads)
       ends[i] = i < a.batch ? (uint32_t)starts[i + 1] : ~0u;
     __syncthreads();
-    b = find<kPlaceStarts>(ends, first);
-  } else {
-    for (uint32_t hi = a.batch; b < hi;) {
-      const uint32_t mid = (b + hi) / 2;
-      if ((uint32_t)starts[mid + 1] > first) hi = mid; else b = mid + 1;
-    }
   }
-  uint32_t end = 0, length = 0;
-  if (b < a.batch) end = (uint32_t)starts[b + 1], length = (uint32_t)a.x.lengths_out[b];
+  const auto end_of = [&](uint32_t s) { return in_lds ? ends[s] : (uint32_t)starts[s + 1]; };
+  // The first sequence from `from` on whose end is past the row; a.batch if there is none.
+  const auto search = [&](uint32_t from, uint32_t row) {
+    if (in_lds) return find<kPlaceStarts>(ends, row);
+    for (uint32_t hi = a.batch; from < hi;) {
+      const uint32_t mid = (from + hi) / 2;
+      if ((uint32_t)starts[mid + 1] > row) hi = mid; else from = mid + 1;
+    }
+    return from;
+  };
+  uint32_t b = search(0, first), end = 0, length = 0;
+  const auto take = [&] {
+    if (b < a.batch) end = end_of(b), length = (uint32_t)a.x.lengths_out[b];
+  };
+  take();
   int slot[kPlaceRows], position[kPlaceRows];
 #pragma unroll
   for (uint32_t i = 0; i < kPlaceRows; ++i) {
     const uint32_t row = first + i;
-    while (b < a.batch && row >= end) {
-      if (++b == a.batch) break;
-      end = (uint32_t)starts[b + 1];
-      length = (uint32_t)a.x.lengths_out[b];
+    if (b < a.batch && row >= end) {
+      if (++b < a.batch && end_of(b) <= row) b = search(b + 1, row);
+      take();
     }
     slot[i] = position[i] = -1;
     if (b < a.batch) {
