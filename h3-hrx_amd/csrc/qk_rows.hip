@@ -84,8 +84,12 @@ __device__ __forceinline__ double row_sum(double v) {
   return v;
 }
 
-// 1 / sqrt(x): the instruction's, to an ulp; in f64 with two steps of Newton's from its 2^-23 or so.
-__device__ __forceinline__ float inverse_root(float x) { return __builtin_amdgcn_rsqf(x); }
+// 1 / sqrt(x): the instruction's, to an ulp; in f64 with two steps of Newton's from its 2^-23 or so. The f32 one takes
+// subnormal numbers for 0: they count as the least normal one, since such a row is zeros (f16), of which any finite
+// root makes zeros, or is normed again in 64 bits (bf16).
+__device__ __forceinline__ float inverse_root(float x) {
+  return __builtin_amdgcn_rsqf(x > 0.0f ? fmaxf(x, 0x1p-126f) : x);
+}
 __device__ __forceinline__ double inverse_root(double x) {
   const double first = __builtin_amdgcn_rsq(x);
   double r = first;
