@@ -590,7 +590,9 @@ typedef struct {
  *   (empty views where norm is 0), cos and sin [positions][rotary / 2] f32 (empty where rotary is 0; these four
  *   16-byte aligned), positions [tokens] i32. tokens in [1, 2^24].
  * Precision: queries in f32 and rounded once (rows whose squares f32 does not hold in f64); keys in f64 and
- * rounded once to the element type. A row with a NaN or an infinity has NaN in the channels that it reaches.
+ * rounded once to the element type. NaN and infinities follow the formula: with the norm a NaN makes its head's whole row
+ * NaN, an infinity (whose 1 / sqrt is 0) its own channel and its pair's other, beside zeros; without it either stays in its
+ * channel and, where that is rotated, its pair's other (inf * 0 and inf - inf are NaN, other infinities stay).
  * h3_qk_norm_rope_kv4: the same, with k and v (v [tokens][v_stride], as it is) into slots[i] of the cache: the
  * bytes that h3_kv4_write of k_out and v would leave. The cache's kv_heads, head_dim and elem are cfg's. A row that
  * is none, and one whose slot is outside the cache, is not written there. */
