@@ -531,7 +531,8 @@ int h3_attention_kv4_prefix(const h3_kv4_cfg *cfg, const h3_kv4_attention_cfg *a
  *     before any are taken, in order of sequences and of columns; lengths_out[b] = 0, no rows. Entries that are no
  *     page of the cache (-1 where the program has given a page back before) are passed over; a page that is another's
  *     by now and still stands there would have two owners.
- *   asked[b] >= 0: so many rows are appended, if the sequence is granted them; all or none. It is refused where
+ *   asked[b] >= 0: so many rows are appended, if the sequence is granted them; all or none. (More than the max_q of
+ *     the attention that follows are appended too, but that leaves the outputs of those past it.) It is refused where
  *     its tokens would pass the table's row; where it needs pages and those that it and the sequences before it
  *     ask for (refused or not, but for the first reason) are more than are free; and where the rows that it and
  *     the sequences before it ask for are more than `rows`. A refused sequence keeps its tokens and pages, and
