@@ -135,18 +135,22 @@ __global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a, bool pl
       // Places on the stack by the entries' numbers, or, from a turn with an entry that is no page on, by the pages'
       // sums. Two flags in turn: a thread that is ahead sets the other one until all have read this.
       __syncthreads();
-      const bool whole = some_none[turn] == 0;
+      if (some_none[turn] == 0) {
 #pragma unroll
-      for (uint32_t k = 0; k < kGiven; ++k) {
-        const bool is = (uint32_t)page[k] < a.pages;
-        uint32_t place = t, given = min(all.a - min(i0 + k * kThreads, all.a), (uint32_t)kThreads);
-        if (!whole) {
-          Two sum;
-          place = sum_to_here<kThreads>({is, 0}, scratch, &sum).a - 1;
-          given = sum.a;
+        for (uint32_t k = 0; k < kGiven; ++k) {
+          const uint32_t i = k * kThreads + t;
+          if (i0 + i < all.a && count + i < a.pages) a.x.free_pages[count + i] = page[k];
         }
-        if (is && count + place < a.pages) a.x.free_pages[count + place] = page[k];
-        count = min(count + given, a.pages);
+        count = min(count + min(all.a - i0, kGiven * kThreads), a.pages);
+      } else {
+#pragma unroll
+        for (uint32_t k = 0; k < kGiven; ++k) {
+          const bool is = (uint32_t)page[k] < a.pages;
+          Two sum;
+          const uint32_t place = count + sum_to_here<kThreads>({is, 0}, scratch, &sum).a - 1;
+          if (is && place < a.pages) a.x.free_pages[place] = page[k];
+          count = min(count + sum.a, a.pages);
+        }
       }
     }
   }
