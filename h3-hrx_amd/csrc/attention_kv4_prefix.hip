@@ -139,15 +139,16 @@ __global__ __launch_bounds__(kThreads) void k_attention_kv4_shared_join(Args a) 
     pitch = (uint32_t)line.rows;
   }
   const int parts = 1 + front;
-  const auto place = [&](int p) {  // of the row's part p
-    return ((p ? a.part_rows + (size_t)(p - 1) * pitch : 0) + at) * a.kv_heads + blockIdx.y;
-  };
+  // Of the row's part p: in 32 bits, as the workspace is 200 MB at most. Part p - 1 of the prefix's is pitch * (p - 1) on.
+  const uint32_t own = at * a.kv_heads + blockIdx.y, step = pitch * a.kv_heads;
+  const uint32_t behind = own + (a.part_rows - pitch) * a.kv_heads;
+  const auto place = [&](uint32_t p) { return p ? behind + p * step : own; };
   const float2 ml = lane < parts ? a.part_ml[place(lane)] : float2{-kInf, 0.0f};
   float x[4][kPer];
   const auto load = [&](int p0) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float* from = a.part_o + place(p0 + i * W) * D + lane * kPer;
+      const float* from = a.part_o + (size_t)place(p0 + i * W) * D + lane * kPer;
 #pragma unroll
       for (int d = 0; d < kPer; ++d) x[i][d] = p0 + i * W < parts ? from[d] : 0.0f;
     }
