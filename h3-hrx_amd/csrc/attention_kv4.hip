@@ -166,15 +166,21 @@ double few_steps(uint32_t tile, double keys) { return keys / (kWaves * (tile == 
 // Estimated as above, by the workgroups' work rather than HBM's rate, since the prefix comes from the caches. In us, in
 // one pass, shared in tiles of 32 (in parts) and along a line of tiles of 256, 4 query heads to each of 8 cache heads:
 //   rows (sequences x new tokens)     keys: prefix, own   one pass   tiles of 32    of 256
-//   64 x 1                            8,192, 700 at most   81         34 (4)         59
-//   16 x 1                            2,000, 300           18         12.5 (8)       29
-//   64 x 1                            1,000, 700           22         23 (4)         49
-//   32 x 1                            30,000, 300          132        41 (16)        56
-//   400 x 1                           3,000, 300           180        79 (1)         110
-//   32 x 9                            10,000, 500          134        94 (4)         114
-//   4 x 130                           20,000, 130          306        306            254
-//   8 x 257                           31,104, 257          1,415                     1,215
-//   8 x 257                           2,000, 257           166                       171
+//   64 x 1                            8,192, 700 at most   79         33 (4)         54
+//   16 x 1                            2,000, 300           17         12 (8)         30
+//   64 x 1                            1,000, 700           22         22 (1)         49
+//   32 x 1                            30,000, 300          118        39 (16)        59
+//   400 x 1                           3,000, 300           173        70 (1, apart)  112
+//   32 x 9                            10,000, 500          129        92 (4)         112
+//   4 x 130                           20,000, 130          303                       241
+//   8 x 257                           31,104, 257          1,400                     1,149
+//   8 x 257                           2,000, 257           155                       168
+// and with long keys of their own, which a shared call does not divide:
+//   2 x 1                             31,104, 31,104       26         151 (3)        186
+//   8 x 1                             31,104, 8,192        49         47 (8)         82
+//   8 x 1                             8,192, 8,192         27         47 (2)         65
+//   64 x 1                            8,192, 8,192         142        98 (1)         131
+// (a captured run, three caches in turn). It takes the least of a line, or one 2 us from it.
 Kv4PrefixPlan kv4_prefix_plan(const h3_kv4_cfg& cfg, const h3_kv4_attention_cfg& acfg, uint32_t prefix_stride,
                               uint32_t batch, uint32_t q_rows, uint32_t max_q, uint32_t cus, bool divide) {
   const uint64_t prefix = (uint64_t)prefix_stride * cfg.page_tokens;

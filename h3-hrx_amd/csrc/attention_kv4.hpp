@@ -1831,7 +1831,9 @@ void launch_tiles(const Args& a, const Kv4Launch& plan, hipStream_t stream) {
 // the 256 MB of the last cache, so that the next call would not meet them there. 32 sequences of 4,096 keys
 // (142 MB, 8 cache heads of 128 channels) 46 us in the caches and 41 past them, two of 129,024 63 and 58;
 // 16 of 4,096, called again and again, 27 and 31. Rows of 64 channels are a quarter of a line each and gain
-// nothing (64 sequences of 8,192 keys 53 and 58 us).
+// nothing (64 sequences of 8,192 keys 53 and 58 us). In one pass behind a prefix they go through them, since the prefix's
+// come to every sequence and one kernel reads both: 64 sequences of 8,192 keys of their own 86 us behind 64 shared ones
+// (82 past the caches) and 103 behind 2,000 (101).
 bool reads_once(const Args& a, const Kv4Launch& plan, int dim) {
   const double keys = (double)((uint64_t)a.table_stride << a.page_shift);
   const double seen = a.window ? std::min(keys, (double)a.window + a.sinks + a.max_q) : keys;

@@ -9,8 +9,8 @@
 // (few rows in all, or sequences that fill tiles by themselves) take every row over F and then O in one pass.
 //
 // 4 query heads to each of 8 cache heads of 128 channels: 64 sequences of up to 700 keys of their own behind 8,192,
-// 28 us and 4 for the join (70 in one pass), bound by what starts a workgroup and by vector issue beside the products
-// (44 and 15 % busy); 8 times 257 rows behind 31,104, 1,102 us, 39 for their own keys and 28 for the join (1,392),
+// 29 us and 5 for the join (79 in one pass), bound by what starts a workgroup and by vector issue beside the products
+// (43 and 14 % busy); 8 times 257 rows behind 31,104, 1,137 us, 39 for their own keys and 31 for the join (1,400),
 // bound as k_attention_kv4_rows is, whose loop it runs (vector pipe 53 and matrix pipe 48 % busy).
 #include "attention_kv4.hpp"
 

@@ -10,15 +10,15 @@
 // One workgroup makes the sums, a sequence to a thread, and hands out pages by their number in the step (a search in
 // the sums per page: a prompt's hundreds are as quick as a token's one). Where nobody asks for more than one row a
 // thread finishes its own sequence. Long calls' slots and positions are a launch of their own. Latency bounds
-// both: 64 sequences of a token each, of which three end, 4.9 us (one alone 3.5); 512 with prompts among them,
-// 129,024 rows, 6.8 and 4.9 (61 with the rows in the first, a search after another).
+// both: 64 sequences of a token each, of which three end, 5.1 us (one alone 3.4); 512 with prompts among them,
+// 129,024 rows, 6.9 and 5.5 (61 with the rows in the first, a search after another).
 #include "internal.hpp"
 
 namespace h3 {
 namespace {
 
-// More rows than this have a launch of their own: 512 sequences with prompts among them, 8.1 us for 2,048 rows in one
-// launch and 11.8 for 2,049 in two, 11.9 for 16,384; in one, 61 for 129,024.
+// More rows than this have a launch of their own: 512 sequences with prompts among them, 9.0 us for 2,048 rows in one
+// launch and 12.8 for 2,049 in two, 12.8 for 16,384; in one, 61 for 129,024.
 constexpr uint32_t kRowsApart = 2048;
 constexpr uint32_t kGiven = 4;  // entries of ended sequences under way in a thread
 constexpr uint32_t kMost = 1u << 30;  // sums stop here: past every number of rows or pages that can be granted
@@ -235,8 +235,8 @@ __global__ __launch_bounds__(kThreads) void k_kv4_advance(AdvanceArgs a, bool pl
 
 // Slots and positions from q_starts, lengths_out and the table: four rows a thread. Where the starts fit LDS the
 // searches for the rows' sequences are there. A row behind its sequence's end is most often the next one's; if not (idle
-// sequences between them, 65,534 behind the last row at most) it is searched for: the thread's other rows one
-// sequence after another cost 8.3 ms there, 51 us with 411 idle ones.
+// sequences between them, 65,534 behind the last row at most) it is searched for: passing those one after
+// another cost a thread 8.2 ms there, and 51 us where 411 are idle.
 constexpr int kPlaceThreads = 256, kPlaceRows = 4, kPlaceStarts = 2048;
 __global__ __launch_bounds__(kPlaceThreads) void k_kv4_places(AdvanceArgs a) {
   __shared__ uint32_t ends[kPlaceStarts];
