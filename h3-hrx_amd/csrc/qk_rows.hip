@@ -304,7 +304,7 @@ void launch_once(const QkArgs& a, dim3 grid, hipStream_t stream) {
 // rows are under way together, while few rows want all the waves that there are. One head, as many, and a
 // quarter of a token's (32 + 8 + 8 heads of 128 channels, into the cache): 256 tokens 4.3, 4.3 and 9.6 us,
 // 1,024 9.2, 7.7 and 10.4, 4,096 31, 20 and 20, 31,104 311, 118 and 118 (705 MB: 6.0 TB/s, where a copy reaches 5.2).
-// More than one (from 683 tokens of those heads on): past the caches, in which the rows of such a call serve nobody.
+// More than one (from 683 tokens of those heads on): past the caches, where the rows of such a call are seldom met again.
 // Through them and past, alone | behind the write of its rows | and before a prompt's attention that reads q_out: 768
 // tokens 8.1 and 7.4 | 12.5 and 11.7 | 32.8 and 31.9 us; 1,024 9.5 and 9.1 | 14.5 and 13.5 | 42.5 and 41.7; 4,096 21.7
 // and 21.5 | 43.6 and 34.5 | 201 and 200; 8,192 43 and 38 | 83 and 77 | 655 and 655; 31,104 132 and 118. Before the
